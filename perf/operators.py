@@ -1,0 +1,410 @@
+"""Workloads of the 4-bit operators: the linear layer over 4-bit weights and the paged 4-bit key/value cache.
+
+Three operators are run, each as a decoder's step calls it:
+
+  append   kv_append (rotation of q and k by their positions, quantisation, the write into the pages) followed by
+           kv_read of the tokens just written: the outputs are the rotated q and what the cache now holds
+  attend   kv_attention: queries of one or many new tokens a sequence against everything the sequence has in the cache
+  linear   linear_int4: residual + act(x W^T + bias) with W in 4 bits, a scale and a zero point per group
+
+With `own` false each is computed in its plain form, from elementary torch operations; with `own` true by this package.
+Formats: a group of 32 channels of one token and head is held as m + c s, with m the group's minimum and s the largest
+fp16 not above (maximum - minimum) / 15, and c in 0..15; a weight is held as s (c - z), with c and z in 0..15.
+"""
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+GROUP = 32          # channels of a key or value that share a scale
+
+
+# ----------------------------------------------------------------------------------------------------------- cases
+
+def listed():
+    """Shapes are those of the OPT layers this repository benchmarks (hidden 5120 with 40 heads, hidden 7168 and 9216) and
+    of generic layers with shared key/value heads."""
+    return [
+        # one decode step of an OPT-13B layer at batch 8: no rotation, every head has its own keys; latency counts
+        _append("append_decode_mha", B=8, T=1, Hq=40, Hkv=40, D=128, L=700, page=64, rot=0, inter=False, ragged=True),
+        # decode of a busy server: 64 sequences of different lengths, shared heads, rotation on the way
+        _append("append_decode_gqa", B=64, T=1, Hq=64, Hkv=8, D=128, L=2000, page=16, rot=128, inter=False, ragged=True),
+        # prompts of different lengths admitted together, half of every head rotated, neighbouring pairs
+        _append("append_prompts", B=5, T=1900, Hq=32, Hkv=8, D=128, L=2300, page=32, rot=64, inter=True, ragged=True),
+        # a single user, a short context that ends inside a page: the smallest call
+        _attend("attend_single_short", B=1, T=1, Hq=40, Hkv=40, D=128, L=131, page=64, ragged=False),
+        # the decode step of an OPT-13B layer at batch 8
+        _attend("attend_decode_mha", B=8, T=1, Hq=40, Hkv=40, D=128, L=1087, page=64, ragged=True),
+        # a busy server's decode step over contexts of very different lengths, eight queries to a key head
+        _attend("attend_decode_gqa", B=32, T=1, Hq=64, Hkv=8, D=128, L=8191, page=16, ragged=True),
+        # one user far into a very long context: few rows, the work has to be split over the keys
+        _attend("attend_long", B=1, T=1, Hq=32, Hkv=8, D=128, L=262139, page=128, ragged=False),
+        # five drafted tokens a sequence checked at once, heads of 64
+        _attend("attend_drafts", B=6, T=5, Hq=32, Hkv=8, D=64, L=4099, page=32, ragged=True),
+        # a chunk of a prompt against what is already in the cache: bound by arithmetic
+        _attend("attend_chunk", B=2, T=1021, Hq=40, Hkv=40, D=128, L=2043, page=64, ragged=True),
+        # one token through a square projection of an OPT-13B layer
+        _linear("linear_single", M=5120, K=5120, N=1, G=128, bias=True, act=0, res=True),
+        # the first feed-forward matrix at a decode batch of 16, finer groups, ReLU
+        _linear("linear_decode", M=28672, K=7168, N=16, G=64, bias=True, act=1, res=False),
+        # a prompt chunk through the second feed-forward matrix
+        _linear("linear_chunk", M=9216, K=36864, N=509, G=128, bias=True, act=0, res=True),
+    ]
+
+
+def _append(name, **kw):
+    return {"name": name, "op": "append", **kw}
+
+
+def _attend(name, **kw):
+    return {"name": name, "op": "attend", **kw}
+
+
+def _linear(name, **kw):
+    return {"name": name, "op": "linear", **kw}
+
+
+def _log(rng, lo, hi):
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(["append", "attend", "attend", "linear", "linear"])
+    if op == "linear":
+        M, K = 64 * _log(rng, 4, 576), 64 * _log(rng, 4, 576)
+        while M * K > 9216 * 36864:
+            M //= 128
+            M *= 64
+        G = rng.choice([g for g in (32, 64, 128) if K % g == 0])
+        N = rng.choice([_log(rng, 1, 64), _log(rng, 1, 509)])
+        return {"op": op, "M": M, "K": K, "N": N, "G": G, "bias": rng.random() < 0.5, "act": rng.choice([0, 1]),
+                "res": rng.random() < 0.5}
+    Hq, Hkv = rng.choice([(40, 40), (32, 8), (64, 8), (12, 12), (16, 1), (24, 4), (7, 7)])
+    c = {"op": op, "Hq": Hq, "Hkv": Hkv, "D": rng.choice([64, 128, 128]), "page": rng.choice([16, 32, 64, 128]),
+         "ragged": rng.random() < 0.7, "B": _log(rng, 1, 64)}
+    if op == "append":
+        c["T"] = 1 if rng.random() < 0.4 else _log(rng, 1, max(1, min(2048, 9000 // c["B"])))
+        c["L"] = c["T"] + _log(rng, 1, 2000)
+        c["rot"] = rng.choice([0, c["D"], c["D"] // 2])
+        c["inter"] = rng.random() < 0.5
+        return c
+    c["T"] = rng.choice([1, 1, _log(rng, 1, 8), _log(rng, 1, max(1, 1024 // c["B"]))])
+    c["L"] = c["T"] + _log(rng, 1, max(1, min(120000, 1200000 // (c["B"] * Hkv))))
+    while work(c)["flops"] > 3.2e10:
+        c["L"] = c["T"] + (c["L"] - c["T"]) // 2
+        if c["L"] - c["T"] < 64:
+            c["T"] = max(1, c["T"] // 2)
+    return c
+
+
+def _lengths(case):
+    """New tokens and, counting them, tokens in the cache of each sequence: a rule of the case, not of the seed."""
+    B, T, L = case["B"], case["T"], case["L"]
+    if not case["ragged"]:
+        return [T] * B, [L] * B
+    q = [T - (b * 7919) % (T // 2 + 1) for b in range(B)]
+    return q, [max(q[b], L - (b * 104729) % (L // 2 + 1)) for b in range(B)]
+
+
+def work(case):
+    if case["op"] == "linear":
+        M, K, N, G = case["M"], case["K"], case["N"], case["G"]
+        weights = M * K // 2 + M * (K // G) * 2 + M * (K // G) // 2      # codes, fp16 scales, 4-bit zero points
+        return {"bytes": weights + 2 * N * K + 2 * N * M * (2 if case["res"] else 1) + (2 * M if case["bias"] else 0),
+                "flops": 2 * M * N * K}
+    q, lens = _lengths(case)
+    D, Hq, Hkv = case["D"], case["Hq"], case["Hkv"]
+    entry = D // 2 + 4 * D // GROUP                                      # one token of one head: codes, scales, minima
+    if case["op"] == "append":
+        n = sum(q)
+        # k and v in, 4-bit entries out and in again, dense k and v out; q in and out and the angles where there is a rotation
+        b = n * Hkv * (4 * D + 2 * entry + 2 * entry + 4 * D)
+        if case["rot"]:
+            b += n * Hq * D * 4 + 4 * case["rot"] * n
+        return {"bytes": b, "flops": n * (Hkv * D * 10 + (Hq + Hkv) * case["rot"] * 3)}
+    pairs = sum(sum(range(n - t + 1, n + 1)) for t, n in zip(q, lens))   # query t of a sequence sees n - T + t + 1 keys
+    return {"bytes": sum(lens) * Hkv * 2 * entry + sum(q) * Hq * D * 4, "flops": 4 * D * Hq * pairs}
+
+
+# ---------------------------------------------------------------------------------------------------------- inputs
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _kv_like(shape, g):
+    """Keys or values: normal, with some channels of large mean as trained keys have."""
+    x = torch.randn(shape, device="cuda", generator=g)
+    shift = torch.randn(shape[-2:], device="cuda", generator=g)
+    return (x + 3 * shift * (shift.abs() > 1.5)).half()
+
+
+def _cache_inputs(case, seed):
+    g = _gen(seed)
+    B, Hq, Hkv, D, page = case["B"], case["Hq"], case["Hkv"], case["D"], case["page"]
+    q_lens, lens = _lengths(case)
+    per = [-(-n // page) for n in lens]
+    pages = sum(per) + 3
+    order = torch.randperm(pages, device="cuda", generator=g).to(torch.int32)
+    table = torch.full((B, max(per)), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for b, n in enumerate(per):
+        table[b, :n] = order[at:at + n]
+        at += n
+    cu = torch.tensor([0] + list(np.cumsum(q_lens)), dtype=torch.int32, device="cuda")
+    st = {"case": case, "table": table, "pages": pages, "cu": cu, "q_lens": q_lens, "lens_h": lens,
+          "lens": torch.tensor(lens, dtype=torch.int32, device="cuda"), "n": sum(q_lens)}
+    st["q"] = torch.randn((st["n"], Hq, D), device="cuda", generator=g).half()
+    n = st["n"] if case["op"] == "append" else sum(lens)
+    st["k"], st["v"] = _kv_like((n, Hkv, D), g), _kv_like((n, Hkv, D), g)
+    st["cos"] = st["sin"] = None
+    if case.get("rot"):
+        pos = torch.arange(max(lens), device="cuda", dtype=torch.float64)[:, None]
+        f = 10000.0 ** (-torch.arange(0, case["rot"], 2, device="cuda", dtype=torch.float64) / case["rot"])
+        st["cos"], st["sin"] = torch.cos(pos * f).float(), torch.sin(pos * f).float()
+    return st
+
+
+def _linear_inputs(case, seed):
+    g = _gen(seed)
+    M, K, N, G = case["M"], case["K"], case["N"], case["G"]
+    st = {"case": case}
+    st["codes"] = torch.randint(0, 16, (M, K), device="cuda", generator=g, dtype=torch.uint8)
+    st["zeros"] = torch.randint(6, 10, (M, K // G), device="cuda", generator=g, dtype=torch.uint8)
+    st["scales"] = (0.003 + 0.004 * torch.rand((M, K // G), device="cuda", generator=g)).half()
+    st["x"] = torch.randn((N, K), device="cuda", generator=g).half()
+    st["bias"] = (torch.randn(M, device="cuda", generator=g) * 0.5).half() if case["bias"] else None
+    st["residual"] = torch.randn((N, M), device="cuda", generator=g).half() if case["res"] else None
+    return st
+
+
+def prepare(case, seed):
+    if case["op"] == "linear":
+        st = _linear_inputs(case, seed)
+        if own:
+            import spmspm_b200 as sp
+            st["W"] = sp.pack_int4(st["codes"], st["scales"], st["zeros"])
+        else:
+            st["packed"] = st["codes"][:, 0::2] | (st["codes"][:, 1::2] << 4)
+        del st["codes"]
+        return st
+    st = _cache_inputs(case, seed)
+    Hkv, D, page = case["Hkv"], case["D"], case["page"]
+    # attend: everything in the contexts is appended here, as the steps before this one did
+    full_cu = torch.tensor([0] + list(np.cumsum(st["lens_h"])), dtype=torch.int32, device="cuda")
+    if own:
+        import spmspm_b200 as sp
+        st["cache"] = sp.KvCacheInt4(st["pages"], page, Hkv, D, device="cuda")
+        if case["op"] == "attend":
+            sp.kv_append(st["cache"], st["k"], st["v"], st["table"], st["lens"], cu_q=full_cu)
+    else:
+        shape = (st["pages"], page, Hkv, D)
+        st["codes"] = [torch.zeros(shape[:-1] + (D // 2,), dtype=torch.uint8, device="cuda") for _ in range(2)]
+        st["par"] = [torch.zeros(shape[:-1] + (D // GROUP, 2), dtype=torch.float16, device="cuda") for _ in range(2)]
+        if case["op"] == "attend":
+            page_of, off = _slots(st["table"], st["lens_h"], st["lens_h"], page)
+            for i, x in enumerate((st["k"], st["v"])):
+                st["codes"][i][page_of, off], st["par"][i][page_of, off] = _quantise(x)
+    if case["op"] == "attend":
+        del st["k"], st["v"]
+    return st
+
+
+# ------------------------------------------------------------------------------------------------------ plain forms
+
+def _to_half(x):
+    """64-bit values rounded once to fp16: through fp32 rounded to odd, which keeps the second rounding right."""
+    f = x.float()
+    toward = torch.where(f.double().abs() > x.abs(), torch.nextafter(f, torch.zeros_like(f)), f)
+    odd = torch.where(toward.double() != x, (toward.view(torch.int32) | 1).view(torch.float32), toward)
+    return torch.where(torch.isfinite(f), odd, f).half()
+
+
+def _half_down(x):
+    """The largest fp16 not above x >= 0."""
+    h = x.half()
+    return torch.where(h.float() > x, (h.view(torch.int16) - 1).view(torch.float16), h)
+
+
+def _quantise(x):
+    """fp16 [..., D] -> packed codes [..., D/2] and (scale, minimum) [..., D/32, 2]."""
+    g = x.float().unflatten(-1, (-1, GROUP))
+    lo, hi = g.amin(-1), g.amax(-1)
+    s = _half_down((hi - lo) / 15)
+    sf = s.float()[..., None]
+    c = torch.where(sf > 0, torch.round((g - lo[..., None]) / sf), torch.zeros_like(g)).clamp(0, 15).to(torch.uint8).flatten(-2)
+    return c[..., 0::2] | (c[..., 1::2] << 4), torch.stack([s, lo.half()], -1)
+
+
+def _values(codes, par):
+    """What codes and (scale, minimum) stand for, in fp32."""
+    c = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).float().unflatten(-1, (-1, GROUP))
+    return (c * par[..., 0:1].float() + par[..., 1:2].float()).flatten(-2)
+
+
+def _slots(table, lens, counts, page):
+    """Page and place inside it of the last counts[b] of lens[b] tokens of every sequence, one after the other."""
+    row = torch.cat([torch.full((c,), b, dtype=torch.long, device="cuda") for b, c in enumerate(counts)])
+    pos = torch.cat([torch.arange(n - c, n, device="cuda") for n, c in zip(lens, counts)])
+    return table[row, pos // page].long(), pos % page
+
+
+def _rotate(x, cos, sin, rot, inter):
+    """Channels 0..rot-1 turned pair by pair; 64 bits, rounded once."""
+    if not rot:
+        return x
+    d = x[..., :rot].double()
+    a, b = (d[..., 0::2], d[..., 1::2]) if inter else (d[..., :rot // 2], d[..., rot // 2:])
+    c, s = cos[:, None].double(), sin[:, None].double()
+    y = (a * c - b * s, b * c + a * s)
+    y = torch.stack(y, -1).flatten(-2) if inter else torch.cat(y, -1)
+    return torch.cat([_to_half(y), x[..., rot:]], -1)
+
+
+def _plain_append(st):
+    case = st["case"]
+    page_of, off = _slots(st["table"], st["lens_h"], st["q_lens"], case["page"])
+    out = {}
+    k = st["k"]
+    if case["rot"]:
+        pos = torch.cat([torch.arange(n - c, n, device="cuda") for n, c in zip(st["lens_h"], st["q_lens"])])
+        cos, sin = st["cos"][pos], st["sin"][pos]
+        k = _rotate(k, cos, sin, case["rot"], case["inter"])
+        out["q"] = _rotate(st["q"], cos, sin, case["rot"], case["inter"])
+    for i, (name, x) in enumerate((("k", k), ("v", st["v"]))):
+        st["codes"][i][page_of, off], st["par"][i][page_of, off] = _quantise(x)
+        out[name] = _values(st["codes"][i][page_of, off], st["par"][i][page_of, off]).half()
+    return out
+
+
+def _plain_attend(st):
+    case = st["case"]
+    Hq, Hkv, D = case["Hq"], case["Hkv"], case["D"]
+    out = torch.empty((st["n"], Hq, D), dtype=torch.float16, device="cuda")
+    at = 0
+    for b, (t, n) in enumerate(zip(st["q_lens"], st["lens_h"])):
+        pages = st["table"][b, :-(-n // case["page"])].long()
+        k, v = (_values(st["codes"][i][pages].flatten(0, 1)[:n], st["par"][i][pages].flatten(0, 1)[:n]) for i in range(2))
+        q = st["q"][at:at + t].float().view(t, Hkv, Hq // Hkv, D).permute(1, 2, 0, 3).flatten(1, 2)          # [Hkv, g t, D]
+        s = torch.matmul(q, k.permute(1, 2, 0)).mul_(1 / math.sqrt(D))                                       # [Hkv, g t, n]
+        seen = torch.arange(n, device="cuda")[None] <= torch.arange(n - t, n, device="cuda")[:, None]
+        s = s.view(Hkv, Hq // Hkv, t, n).masked_fill_(~seen, float("-inf")).flatten(1, 2)
+        p = torch.exp(s - s.amax(-1, keepdim=True))
+        o = torch.matmul(p, v.permute(1, 0, 2)) / p.sum(-1, keepdim=True)
+        out[at:at + t] = o.view(Hkv, Hq // Hkv, t, D).permute(2, 0, 1, 3).reshape(t, Hq, D).half()
+        at += t
+    return out
+
+
+def _plain_linear(st):
+    codes = torch.stack([st["packed"] & 15, st["packed"] >> 4], -1).flatten(-2).float()
+    w = codes.unflatten(-1, (-1, st["case"]["G"]))
+    w = ((w - st["zeros"][..., None].float()) * st["scales"][..., None].float()).flatten(-2)
+    y = torch.matmul(st["x"].float(), w.t())
+    if st["bias"] is not None:
+        y = y + st["bias"].float()
+    if st["case"]["act"]:
+        y = torch.clamp_min(y, 0)
+    if st["residual"] is not None:
+        y = y + st["residual"].float()
+    return y.half()
+
+
+def run(state):
+    op = state["case"]["op"]
+    if not own:
+        return {"append": _plain_append, "attend": _plain_attend, "linear": _plain_linear}[op](state)
+    import spmspm_b200 as sp
+    if op == "linear":
+        return sp.linear_int4(state["W"], state["x"], bias=state["bias"], residual=state["residual"],
+                              activation=sp.ACT_RELU if state["case"]["act"] else sp.ACT_NONE)
+    if op == "attend":
+        return sp.kv_attention(state["q"], state["cache"], state["table"], state["lens"], cu_q=state["cu"], max_q=max(state["q_lens"]))
+    case, out = state["case"], {}
+    if case["rot"]:
+        out["q"] = sp.kv_append(state["cache"], state["k"], state["v"], state["table"], state["lens"], cu_q=state["cu"],
+                                q=state["q"], cos=state["cos"], sin=state["sin"], interleaved=case["inter"])
+    else:
+        sp.kv_append(state["cache"], state["k"], state["v"], state["table"], state["lens"], cu_q=state["cu"])
+    out["k"], out["v"] = sp.kv_read(state["cache"], state["table"], state["lens"], cu_q=state["cu"], n_tokens=state["n"])
+    return out
+
+
+# -------------------------------------------------------------------------------------------------- 64-bit definition
+
+def _exact_entry(x):
+    """numpy float64 [..., D] of fp16 values -> what the cache holds for them."""
+    g = x.reshape(x.shape[:-1] + (-1, GROUP))
+    lo, span = g.min(-1, keepdims=True), g.max(-1, keepdims=True) - g.min(-1, keepdims=True)
+    s = (span / 15).astype(np.float16)
+    s = np.where(s.astype(np.float64) > span / 15, np.nextafter(s, np.float16(0)), s).astype(np.float64)
+    with np.errstate(divide="ignore", invalid="ignore"):
+        c = np.where(s > 0, np.clip(np.rint((g - lo) / s), 0, 15), 0)
+    return (lo + c * s).reshape(x.shape)
+
+
+def _exact_turn(x, pos, rot, inter, cos, sin):
+    y = x.copy()
+    for i in range(rot // 2):
+        a, b = (2 * i, 2 * i + 1) if inter else (i, i + rot // 2)
+        c, s = cos[pos, i][:, None], sin[pos, i][:, None]
+        y[..., a], y[..., b] = x[..., a] * c - x[..., b] * s, x[..., a] * s + x[..., b] * c
+    return y.astype(np.float16).astype(np.float64)
+
+
+def exact(case, seed):
+    if case["op"] == "linear":
+        st = _linear_inputs(case, seed)
+        M, K, N, G = case["M"], case["K"], case["N"], case["G"]
+        y = torch.empty((N, M), dtype=torch.float64, device="cuda")
+        x = st["x"].double().view(N, K // G, G).transpose(0, 1)                      # [K/G, N, G]
+        for r in range(0, M, 1024):
+            c = st["codes"][r:r + 1024].double().view(-1, K // G, G).permute(1, 2, 0)  # [K/G, G, rows]
+            z, s = st["zeros"][r:r + 1024].double().t(), st["scales"][r:r + 1024].double().t()
+            dots = torch.bmm(x, c) - x.sum(-1, keepdim=True) * z[:, None]            # sum of x (c - z) in each group
+            y[:, r:r + 1024] = (dots * s[:, None]).sum(0)
+        if case["bias"]:
+            y += st["bias"].double()
+        if case["act"]:
+            y = torch.where(y > 0, y, torch.zeros_like(y))
+        if case["res"]:
+            y += st["residual"].double()
+        return y
+    st = _cache_inputs(case, seed)
+    Hq, Hkv, D = case["Hq"], case["Hkv"], case["D"]
+    if case["op"] == "append":
+        host = {n: st[n].cpu().numpy().astype(np.float64) for n in "qkv"}
+        out = {}
+        if case["rot"]:
+            pos = np.concatenate([np.arange(n - c, n) for n, c in zip(st["lens_h"], st["q_lens"])])
+            cos, sin = (st[n].cpu().numpy().astype(np.float64) for n in ("cos", "sin"))
+            for n in "qk":
+                host[n] = _exact_turn(host[n], pos, case["rot"], case["inter"], cos, sin)
+            out["q"] = host["q"]
+        return {**out, "k": _exact_entry(host["k"]), "v": _exact_entry(host["v"])}
+    out = torch.empty((st["n"], Hq, D), dtype=torch.float64, device="cuda")
+    at = first = 0
+    for t, n in zip(st["q_lens"], st["lens_h"]):
+        rows = torch.arange(n - t, n, device="cuda")[:, None]
+        hidden = torch.arange(n, device="cuda")[None] > rows
+        for h in range(Hkv):
+            k, v = (_exact_entry_gpu(st[x][first:first + n, h].double()) for x in "kv")
+            for j in range(h * Hq // Hkv, (h + 1) * Hq // Hkv):
+                z = (st["q"][at:at + t, j].double() @ k.t()) / math.sqrt(D)
+                z[hidden] = -math.inf
+                out[at:at + t, j] = torch.softmax(z, -1) @ v
+        at, first = at + t, first + n
+    return out
+
+
+def _exact_entry_gpu(x):
+    """_exact_entry for a 64-bit tensor on the GPU (long contexts)."""
+    g = x.view(x.shape[0], -1, GROUP)
+    lo = g.min(-1, keepdim=True).values
+    s = (g.max(-1, keepdim=True).values - lo) / 15
+    bits = s.half().view(torch.int16)
+    s = torch.where(s.half().double() > s, (bits - 1).view(torch.float16), s.half()).double()
+    c = torch.where(s > 0, ((g - lo) / s).round().clamp(0, 15), torch.zeros_like(g))
+    return (lo + c * s).view(x.shape)
