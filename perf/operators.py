@@ -223,16 +223,16 @@ def _to_half(x):
 
 
 def _half_down(x):
-    """The largest fp16 not above x >= 0."""
+    """The largest fp16 not above x >= 0 (64 bits)."""
     h = x.half()
-    return torch.where(h.float() > x, (h.view(torch.int16) - 1).view(torch.float16), h)
+    return torch.where(h.double() > x, (h.view(torch.int16) - 1).view(torch.float16), h)
 
 
 def _quantise(x):
     """fp16 [..., D] -> packed codes [..., D/2] and (scale, minimum) [..., D/32, 2]."""
     g = x.float().unflatten(-1, (-1, GROUP))
     lo, hi = g.amin(-1), g.amax(-1)
-    s = _half_down((hi - lo) / 15)
+    s = _half_down((hi.double() - lo.double()) / 15)
     sf = s.float()[..., None]
     c = torch.where(sf > 0, torch.round((g - lo[..., None]) / sf), torch.zeros_like(g)).clamp(0, 15).to(torch.uint8).flatten(-2)
     return c[..., 0::2] | (c[..., 1::2] << 4), torch.stack([s, lo.half()], -1)
