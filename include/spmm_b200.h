@@ -309,6 +309,81 @@ int spb_linear_allreduce_finish(void* stream, uint16_t* C, const uint16_t* parts
                                 int M_Global, int N_Global, const uint16_t* bias, const uint16_t* residual,
                                 int activation);
 
+/* ------------------------------------------------------------------ 4-bit weights */
+
+/*
+ * Linear layer over a dense weight held in 4 bits: the counterpart of spb_linear_bitmap_v3 for weights that are quantised
+ * instead of pruned.  Weight (m, k) is s * (c - z): code c and zero point z in 0..15, scale s fp16, s and z shared by
+ * `group` (32, 64 or 128) consecutive k of a row.  M and K are multiples of 64, K of the group.
+ *   spb_int4_pack    brings codes [M][K] (one per byte), scales [M][K/group] and zero points [M][K/group] (one per byte), as
+ *                    quantisation tools deliver them, into the library's layout (all device pointers);
+ *   spb_int4_encode  makes such codes, scales and zero points from a dense fp16 matrix: per group lo = min(0, min),
+ *                    hi = max(0, max), s = fp16((hi - lo) / 15), z = round(-lo / s), c = clamp(round(x / s) + z, 0, 15);
+ *                    a group with a value that is not finite gets s = NaN;
+ *   spb_int4_decode  the inverse of the layout: dense fp16 s * (c - z), rounded once;
+ *   spb_linear_int4  out[N][M] = residual + act(x W^T + bias), x [N][K]; summed in fp32 and rounded to fp16 once, at the
+ *                    very end (unlike spb_linear_bitmap_v3, which rounds after every step as the kernels it replaces do).
+ *                    bias, residual: as there, or NULL; residual may be out itself.  No workspace; may be captured.
+ */
+size_t spb_int4_codes_bytes(int M, int K);
+size_t spb_int4_params_bytes(int M, int K, int group);
+int spb_int4_pack(void* stream, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int M, int K, int group,
+                  void* packed, void* params);
+int spb_int4_encode(void* stream, const uint16_t* dense, int M, int K, int group, uint8_t* codes, uint16_t* scales,
+                    uint8_t* zeros);
+int spb_int4_decode(void* stream, const void* packed, const void* params, int M, int K, int group, uint16_t* dense);
+int spb_linear_int4(void* stream, const void* packed, const void* params, int M, int K, int group, const uint16_t* x,
+                    uint16_t* out, int N, const uint16_t* bias, const uint16_t* residual, int activation);
+
+/* ------------------------------------------------------------------ 4-bit key/value cache */
+
+/*
+ * Paged key/value cache in 4 bits, and attention over it (the reference leaves both to its caller; in FasterTransformer
+ * the cache is dense fp16).  32 consecutive channels of one token and head are held as m + s * c: m their minimum, s the
+ * largest fp16 not above (max - min) / 15, c in 0..15; a group with a value that is not finite reads back as NaN.  The pool
+ * (spb_kv_cache_bytes bytes, 16-byte aligned) is num_pages pages of page_size tokens (a multiple of 16) for kv_heads
+ * heads of head_dim 64 or 128 channels; its inner layout is the library's own.
+ *
+ * Every call describes a batch the same way:
+ *   page_table  [batch][table_stride] int32: page that holds tokens i * page_size .. of a sequence
+ *   kv_lens     [batch] int32: tokens of the sequence in the cache, those of this call included
+ *   cu_q        [batch + 1] int32: rows cu_q[b] .. cu_q[b + 1] - 1 of the packed inputs are the last tokens of sequence b; NULL:
+ *               every sequence has n_tokens / batch of them.  Rows outside cu_q[0] .. cu_q[batch] - 1 are neither read nor written.
+ * all on the device, so that a captured step keeps working while the contexts grow.  A page number outside
+ * 0 .. num_pages - 1, or a token past the table's width, sets bit 8 of the device status word; the token is then not written,
+ * reads as zeros, and counts as unseen by attention.
+ *
+ *   spb_kv_append     writes the keys and values of the new tokens.  With cos_table / sin_table ([max_pos][rot_dim / 2] fp32)
+ *                     the first rot_dim channels of the keys, and of q if given (result in q_out, [n_tokens][q_heads][head_dim]),
+ *                     are first turned by the angles of the token's position in the cache: pairs (i, i + rot_dim / 2), or
+ *                     (2 i, 2 i + 1) if interleaved; computed in 64 bits, rounded once to fp16.  rot_dim: a multiple of 8.
+ *                     A position that is negative (more new tokens than kv_lens) is skipped; one past max_pos is skipped
+ *                     and sets bit 8.  Two rows of one call must not name the same slot of a page.
+ *   spb_kv_read       k, v [n_tokens][kv_heads][head_dim] fp16: what the cache holds for these tokens.
+ *   spb_kv_attention  out[i] = softmax(scale q[i] K^T) V over the keys of its sequence up to its own position
+ *                     (row cu_q[b + 1] - 1 sees all kv_lens[b]); a row that sees no key gets zeros.  q_heads is a multiple of
+ *                     kv_heads.  max_q: an upper bound of the rows of one sequence; it only chooses the kernel's tiling.
+ *                     workspace: spb_kv_attention_workspace_bytes bytes, 16-byte aligned, need not be cleared; not shared by
+ *                     calls that may run at the same time.
+ * k, v and q are fp16 with contiguous channels; token and head strides in elements, multiples of 4; pointers 8-byte aligned
+ * (out and the workspace 16).  The same bits come out for the same call on the same device.
+ */
+size_t spb_kv_cache_bytes(int num_pages, int page_size, int kv_heads, int head_dim);
+int spb_kv_append(void* stream, void* pool, int num_pages, int page_size, int kv_heads, int head_dim, const int* page_table,
+                  int table_stride, const int* kv_lens, const int* cu_q, int batch, long long n_tokens, const uint16_t* k,
+                  long long k_token_stride, long long k_head_stride, const uint16_t* v, long long v_token_stride,
+                  long long v_head_stride, const uint16_t* q, long long q_token_stride, long long q_head_stride, int q_heads,
+                  uint16_t* q_out, const float* cos_table, const float* sin_table, int max_pos, int rot_dim,
+                  int interleaved);
+int spb_kv_read(void* stream, const void* pool, int num_pages, int page_size, int kv_heads, int head_dim,
+                const int* page_table, int table_stride, const int* kv_lens, const int* cu_q, int batch, long long n_tokens,
+                uint16_t* k, uint16_t* v);
+size_t spb_kv_attention_workspace_bytes(int head_dim, int batch, int q_heads, int kv_heads, int max_q);
+int spb_kv_attention(void* stream, const void* pool, int num_pages, int page_size, int kv_heads, int head_dim,
+                     const int* page_table, int table_stride, const int* kv_lens, const int* cu_q, int batch,
+                     long long n_tokens, const uint16_t* q, long long q_token_stride, long long q_head_stride, int q_heads,
+                     int max_q, float scale, uint16_t* out, void* workspace, size_t workspace_bytes);
+
 /*
  * Status word of the current device: 0 when no kernel of this library has hit a
  * bounded wait that ran out or an inconsistent offset since the last reset.

@@ -14,6 +14,7 @@ _u16p = ctypes.POINTER(ctypes.c_uint16)
 _i32p = ctypes.POINTER(ctypes.c_int)
 _u64p = ctypes.POINTER(ctypes.c_uint64)
 _vp = ctypes.c_void_p
+_ll = ctypes.c_longlong
 
 # name -> (restype, argtypes); every symbol include/spmm_b200.h declares
 SIGNATURES = {
@@ -54,6 +55,20 @@ SIGNATURES = {
                                             _vp, _vp, ctypes.c_int, _vp, ctypes.c_int]),
     "spb_linear_allreduce_finish": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp,
                                                    ctypes.c_int]),
+    "spb_int4_codes_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int]),
+    "spb_int4_params_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "spb_int4_pack": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp]),
+    "spb_int4_encode": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp]),
+    "spb_int4_decode": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp]),
+    "spb_linear_int4": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp, _vp,
+                                       ctypes.c_int]),
+    "spb_kv_cache_bytes": (ctypes.c_size_t, [ctypes.c_int] * 4),
+    "spb_kv_append": (ctypes.c_int, [_vp, _vp] + [ctypes.c_int] * 4 + [_vp, ctypes.c_int, _vp, _vp, ctypes.c_int, _ll]
+                      + [_vp, _ll, _ll] * 3 + [ctypes.c_int, _vp, _vp, _vp] + [ctypes.c_int] * 3),
+    "spb_kv_read": (ctypes.c_int, [_vp, _vp] + [ctypes.c_int] * 4 + [_vp, ctypes.c_int, _vp, _vp, ctypes.c_int, _ll, _vp, _vp]),
+    "spb_kv_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 5),
+    "spb_kv_attention": (ctypes.c_int, [_vp, _vp] + [ctypes.c_int] * 4 + [_vp, ctypes.c_int, _vp, _vp, ctypes.c_int, _ll, _vp, _ll,
+                                        _ll, ctypes.c_int, ctypes.c_int, ctypes.c_float, _vp, _vp, ctypes.c_size_t]),
     "spb_launch_count": (ctypes.c_ulonglong, []),
     "spb_device_status": (ctypes.c_int, [_i32p]),
     "spb_reset_device_status": (ctypes.c_int, []),

@@ -12,6 +12,7 @@ enum DeviceStatus : int {
     kStatusWaitTimeout = 1,    // a bounded mbarrier wait ran out
     kStatusBadOffsets = 2,     // a global-tile chunk was larger than max_nnz_intile allows
     kStatusEncodeOverflow = 4, // encoder: packed values did not fit the caller's buffer
+    kStatusBadCache = 8,       // 4-bit cache: a page number, length or position the tables do not cover
 };
 
 // Address of the calling device's status word (device memory, one int).

@@ -1,0 +1,399 @@
+// Linear layer over 4-bit weights (layout: int4.cuh) for few rows of x, and the kernels that bring weights into the layout.
+//
+//   y[n][m] = residual + act(bias + sum over groups of s (sum_k c x - z sum_k x))      summed in fp32, rounded once
+//
+// int4_small_kernel: bound by the bytes of the codes while N is small.  The codes enter mma.sync.m16n8k16 as they are: a
+// nibble masked out of its word is an fp16 subnormal, c 2^-24 (low nibble of a byte) or c 2^-20 (high), multiplied
+// exactly, so unpacking costs 1.25 instructions per two weights; low and high nibbles are summed apart, and scale and zero
+// point are applied to the fp32 sums of a group, with sum_k x from one more matrix instruction on ones.  No weight is
+// rounded.  The warps of a thread block, and the thread blocks of a cluster, share out K; partial sums meet in shared
+// memory, in a fixed order.  Codes and x go from memory to registers with 16-byte loads, kDepth tiles ahead.
+#include "../../include/spmm_b200.h"
+#include "int4.cuh"
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
+
+namespace spb {
+namespace {
+
+constexpr int kWarps = 8;
+
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 load_stream(const uint4* p)
+{
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// RT row tiles of 16, NT column tiles of 8 rows of x per warp; kGT 64-k tiles per group (2: group 128), or 0: group 32.
+template <int RT, int NT, int kGroup>
+__global__ void __launch_bounds__(32 * kWarps) int4_small_kernel(Int4Args a)
+{
+    constexpr int kDepth = RT == 1 ? 4 : 2;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, t = lane % 4;
+    const int kt_all = a.K / 64, rt_all = a.M / 16, groups = a.K / kGroup;
+    const int parts = gridDim.y * kWarps, part = blockIdx.y * kWarps + warp;
+    // K in pieces of whole groups, as even as they come
+    constexpr int kStep = kGroup == 128 ? 2 : 1;   // 64-k tiles that stay together
+    const int steps = kt_all / kStep;
+    const int kt0 = (int)((long long)steps * part / parts) * kStep, kt1 = (int)((long long)steps * (part + 1) / parts) * kStep;
+    const int rt0 = blockIdx.x * RT, n0 = blockIdx.z * 8 * NT;
+
+    const uint4* code[RT];
+    const __half2* par[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int rt = min(rt0 + r, rt_all - 1);   // past the end: a row tile that is there, its result is not stored
+        code[r] = reinterpret_cast<const uint4*>(a.codes) + (long long)rt * kt_all * 32 + lane;
+        par[r] = a.params + (long long)rt * groups * 16;
+    }
+    const uint16_t* xr[NT];
+    bool have[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        have[nt] = n0 + nt * 8 + g < a.N;
+        xr[nt] = a.x + (long long)(have[nt] ? n0 + nt * 8 + g : 0) * a.K + 8 * t;
+    }
+    float out[RT][NT][4] = {};
+    float low[RT][NT][4] = {}, high[RT][NT][4] = {}, xsum[NT][4] = {};
+    uint4 w[kDepth][RT], xv[kDepth][NT][2];
+    auto fetch = [&](int slot, int kt) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) w[slot][r] = load_stream(code[r] + (long long)kt * 32);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                xv[slot][nt][h] = have[nt] ? *reinterpret_cast<const uint4*>(xr[nt] + kt * 64 + 32 * h) : make_uint4(0, 0, 0, 0);
+    };
+    auto apply = [&](int grp) {   // a group is complete: scale and zero point
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const float2 p0 = __half22float2(par[r][grp * 16 + g]), p1 = __half22float2(par[r][grp * 16 + g + 8]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float dot = fmaf(low[r][nt][i], 16.f, high[r][nt][i]) * 1048576.f;
+                    const float2 p = i < 2 ? p0 : p1;
+                    out[r][nt][i] = fmaf(p.x, fmaf(-p.y, xsum[nt][i & 1], dot), out[r][nt][i]);
+                    low[r][nt][i] = high[r][nt][i] = 0.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) xsum[nt][0] = xsum[nt][1] = xsum[nt][2] = xsum[nt][3] = 0.f;
+    };
+    auto step = [&](const uint4 (&wv)[RT], const uint4 (&xw)[NT][2], int kt) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                mma(xsum[nt], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, xw[nt][h].x, xw[nt][h].y);
+                mma(xsum[nt], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, xw[nt][h].z, xw[nt][h].w);
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const uint32_t u = h ? wv[r].y : wv[r].x, v = h ? wv[r].w : wv[r].z;
+                const uint32_t us = u >> 8, vs = v >> 8;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma(low[r][nt], u & 0x000f000fu, v & 0x000f000fu, us & 0x000f000fu, vs & 0x000f000fu, xw[nt][h].x, xw[nt][h].y);
+                    mma(high[r][nt], u & 0x00f000f0u, v & 0x00f000f0u, us & 0x00f000f0u, vs & 0x00f000f0u, xw[nt][h].z, xw[nt][h].w);
+                }
+            }
+            if constexpr (kGroup == 32) apply(kt * 2 + h);
+        }
+        if constexpr (kGroup == 64) apply(kt);
+        if constexpr (kGroup == 128)
+            if (kt & 1) apply(kt / 2);
+    };
+#pragma unroll
+    for (int i = 0; i < kDepth; ++i)
+        if (kt0 + i < kt1) fetch(i, kt0 + i);
+    int kt = kt0;
+    for (; kt + kDepth <= kt1; kt += kDepth) {
+#pragma unroll
+        for (int i = 0; i < kDepth; ++i) {
+            step(w[i], xv[i], kt + i);
+            if (kt + i + kDepth < kt1) fetch(i, kt + i + kDepth);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kDepth; ++i)
+        if (kt + i < kt1) step(w[i], xv[i], kt + i);
+
+    // sums of the warps, then of the cluster's thread blocks (blockIdx.y), in order
+    __shared__ float part_sum[kWarps][RT * NT * 4][32];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part_sum[warp][(r * NT + nt) * 4 + i][lane] = out[r][nt][i];
+    __syncthreads();
+    constexpr int kVals = RT * NT * 4 * 32;
+    float* flat = &part_sum[0][0][0];
+    for (int v = threadIdx.x; v < kVals; v += 32 * kWarps) {
+        float sum = flat[v];
+#pragma unroll
+        for (int i = 1; i < kWarps; ++i) sum += flat[i * kVals + v];
+        flat[v] = sum;
+    }
+    auto store = [&](int v, float y) {
+        const int l = v & 31, i = (v >> 5) & 3, nt = (v >> 7) % NT, r = (v >> 7) / NT;
+        const int m = (rt0 + r) * 16 + l / 4 + 8 * (i >> 1), n = n0 + nt * 8 + 2 * (l & 3) + (i & 1);
+        if (rt0 + r >= rt_all || n >= a.N) return;
+        if (a.bias) y += __half2float(__ushort_as_half(a.bias[m]));
+        if (a.activation) y = y < 0.f ? 0.f : y;   // NaN stays NaN
+        if (a.residual) y += __half2float(__ushort_as_half(a.residual[(long long)n * a.M + m]));
+        a.out[(long long)n * a.M + m] = __half_as_ushort(__float2half_rn(y));
+    };
+    if (gridDim.y == 1) {
+        for (int v = threadIdx.x; v < kVals; v += 32 * kWarps) store(v, flat[v]);
+        return;
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int ranks = gridDim.y, rank = blockIdx.y;
+    for (int v = rank * (32 * kWarps) + threadIdx.x; v < kVals; v += ranks * 32 * kWarps) {
+        float sum = 0.f;
+        for (int i = 0; i < ranks; ++i) sum += *cluster.map_shared_rank(flat + v, i);
+        store(v, sum);
+    }
+    cluster.sync();   // nobody leaves while its sums are being read
+}
+
+// One thread per word: eight codes of one row.
+template <class F>
+__device__ __forceinline__ void for_word(int K, long long i, F&& f)   // f(word index, row, first k)
+{
+    const int q = (int)(i & 3), lane = (int)(i >> 2 & 31);
+    const long long tile = i >> 7, mt = tile / (K / 64), kt = tile % (K / 64);
+    f(mt * 16 + lane / 4 + 8 * (q >> 1), kt * 64 + 32 * (q & 1) + 8 * (lane & 3));
+}
+__global__ void int4_pack_kernel(const uint8_t* codes, uint32_t* packed, int M, int K)
+{
+    const long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
+    if (i >= (long long)M * K / 8) return;
+    for_word(K, i, [&](long long row, long long k) {
+        const uint2 b = *reinterpret_cast<const uint2*>(codes + row * K + k);
+        uint32_t w = 0;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) w |= ((r < 4 ? b.x >> 8 * r : b.y >> 8 * (r - 4)) & 15u) << 4 * int4_nibble(r);
+        packed[i] = w;
+    });
+}
+__global__ void int4_pack_params_kernel(const uint16_t* scales, const uint8_t* zeros, __half2* params, int M, int groups)
+{
+    const long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
+    if (i >= (long long)M * groups) return;
+    const long long row = i / groups, grp = i % groups;
+    params[(row / 16 * groups + grp) * 16 + row % 16] =
+        __halves2half2(__ushort_as_half(scales[i]), __ushort2half_rn((unsigned short)(zeros[i] & 15)));
+}
+// The value of a weight: s (c - z), rounded once to fp16.
+__global__ void int4_decode_kernel(const uint32_t* packed, const __half2* params, uint16_t* dense, int M, int K, int group)
+{
+    const long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
+    if (i >= (long long)M * K / 8) return;
+    for_word(K, i, [&](long long row, long long k) {
+        const __half2 p = params[(row / 16 * (K / group) + k / group) * 16 + row % 16];
+        const uint32_t w = packed[i];
+        __half y[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            y[r] = __hmul(__hsub(__uint2half_rn(w >> 4 * int4_nibble(r) & 15u), __high2half(p)), __low2half(p));
+        *reinterpret_cast<uint4*>(dense + row * K + k) = *reinterpret_cast<uint4*>(y);
+    });
+}
+// Quantises one group of one row per 8 lanes x (group / 64) values: lo = min(0, min), hi = max(0, max), s = fp16((hi - lo) / 15),
+// z = round(-lo / s), c = clamp(round(x / s) + z, 0, 15).  Zero is always a value of the group, as pruned weights need it.
+__global__ void int4_encode_kernel(const uint16_t* dense, uint8_t* codes, uint16_t* scales, uint8_t* zeros, int M, int K, int group)
+{
+    const long long i = blockIdx.x * (long long)(blockDim.x / 32) + threadIdx.x / 32;   // one warp per group
+    const int lane = threadIdx.x & 31, groups = K / group;
+    if (i >= (long long)M * groups) return;
+    const long long row = i / groups, k0 = (i % groups) * group;
+    float lo = 0.f, hi = 0.f;
+    bool finite = true;
+    for (int k = lane; k < group; k += 32) {
+        const float x = __half2float(__ushort_as_half(dense[row * K + k0 + k]));
+        lo = fminf(lo, x), hi = fmaxf(hi, x);
+        finite = finite && fabsf(x) <= 65504.f;
+    }
+#pragma unroll
+    for (int o = 16; o; o /= 2) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    finite = __all_sync(0xffffffffu, finite);
+    const __half s = finite ? __float2half_rn(__fdiv_rn(hi - lo, 15.f)) : __ushort_as_half((unsigned short)0x7fff);
+    const float sf = __half2float(s);
+    const float z = sf > 0.f ? fminf(rintf(__fdiv_rn(-lo, sf)), 15.f) : 0.f;
+    for (int k = lane; k < group; k += 32) {
+        const float x = __half2float(__ushort_as_half(dense[row * K + k0 + k]));
+        const float c = sf > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x, sf)) + z, 0.f), 15.f) : 0.f;
+        codes[row * K + k0 + k] = (uint8_t)c;
+    }
+    if (lane == 0) {
+        scales[i] = __half_as_ushort(s);
+        zeros[i] = (uint8_t)z;
+    }
+}
+
+int sm_count()
+{
+    static int n[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (!n[dev] && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    return n[dev];
+}
+
+template <int RT, int NT, int kGroup>
+cudaError_t launch_small(cudaStream_t s, const Int4Args& a)
+{
+    const int gx = (a.M / 16 + RT - 1) / RT, gz = (a.N + 8 * NT - 1) / (8 * NT);
+    // thread blocks that share K: enough to put about two on every SM, at least two 128-k steps for every warp
+    int split = 1;
+    while (split < 8 && (long long)gx * gz * split < 2 * sm_count() && a.K / 128 >= 2 * kWarps * 2 * split) split *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(gx, split, gz);
+    cfg.blockDim = dim3(32 * kWarps);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = split;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, int4_small_kernel<RT, NT, kGroup>, a);
+    count_launch();
+    return e;
+}
+template <int kGroup>
+cudaError_t launch_group(cudaStream_t s, const Int4Args& a)
+{
+    const bool many = a.M / 16 >= 8 * sm_count();   // rows enough to fill the device with four row tiles a warp
+    if (a.N <= 8) return many ? launch_small<4, 1, kGroup>(s, a) : launch_small<1, 1, kGroup>(s, a);
+    if (a.N <= 16) return many ? launch_small<4, 2, kGroup>(s, a) : launch_small<2, 2, kGroup>(s, a);
+    return launch_small<2, 4, kGroup>(s, a);
+}
+
+bool check_weight(const char* who, int M, int K, int group)
+{
+    if (M <= 0 || K <= 0 || M % 64 || K % 64) {
+        set_error("%s: M and K must be positive multiples of 64 (M=%d K=%d)", who, M, K);
+        return false;
+    }
+    if ((group != 32 && group != 64 && group != 128) || K % group) {
+        set_error("%s: the group must be 32, 64 or 128 and divide K (group=%d K=%d)", who, group, K);
+        return false;
+    }
+    return true;
+}
+unsigned blocks(long long items, int per) { return (unsigned)((items + per - 1) / per); }
+
+}  // namespace
+
+cudaError_t int4_linear_launch(cudaStream_t s, const Int4Args& a, int* status)
+{
+    (void)status;
+    return a.group == 128 ? launch_group<128>(s, a) : a.group == 64 ? launch_group<64>(s, a) : launch_group<32>(s, a);
+}
+
+}  // namespace spb
+
+extern "C" {
+
+size_t spb_int4_codes_bytes(int M, int K) { return M > 0 && K > 0 ? (size_t)M * K / 2 : 0; }
+size_t spb_int4_params_bytes(int M, int K, int group) { return M > 0 && K > 0 && group > 0 ? (size_t)M * (K / group) * 4 : 0; }
+
+int spb_int4_pack(void* stream, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int M, int K, int group,
+                  void* packed, void* params)
+{
+    using namespace spb;
+    if (!check_weight("int4_pack", M, K, group)) return (int)cudaErrorInvalidValue;
+    if (!codes || !scales || !zeros || !packed || !params || !aligned16(codes) || !aligned16(packed) || !aligned16(params) ||
+        (reinterpret_cast<uintptr_t>(scales) & 1)) {
+        set_error("int4_pack: null or misaligned device pointer (codes, packed and params: 16 bytes)");
+        return (int)cudaErrorInvalidValue;
+    }
+    cudaStream_t s = (cudaStream_t)stream;
+    int4_pack_kernel<<<blocks((long long)M * K / 8, 256), 256, 0, s>>>(codes, (uint32_t*)packed, M, K);
+    int4_pack_params_kernel<<<blocks((long long)M * (K / group), 256), 256, 0, s>>>(scales, zeros, (__half2*)params, M, K / group);
+    count_launch(2);
+    return (int)cudaGetLastError();
+}
+
+int spb_int4_encode(void* stream, const uint16_t* dense, int M, int K, int group, uint8_t* codes, uint16_t* scales, uint8_t* zeros)
+{
+    using namespace spb;
+    if (!check_weight("int4_encode", M, K, group)) return (int)cudaErrorInvalidValue;
+    if (!dense || !codes || !scales || !zeros || ((reinterpret_cast<uintptr_t>(dense) | reinterpret_cast<uintptr_t>(scales)) & 1)) {
+        set_error("int4_encode: null or misaligned device pointer");
+        return (int)cudaErrorInvalidValue;
+    }
+    int4_encode_kernel<<<blocks((long long)M * (K / group), 8), 256, 0, (cudaStream_t)stream>>>(dense, codes, scales, zeros, M, K, group);
+    count_launch();
+    return (int)cudaGetLastError();
+}
+
+int spb_int4_decode(void* stream, const void* packed, const void* params, int M, int K, int group, uint16_t* dense)
+{
+    using namespace spb;
+    if (!check_weight("int4_decode", M, K, group)) return (int)cudaErrorInvalidValue;
+    if (!packed || !params || !dense || !aligned16(packed) || !aligned16(params) || !aligned16(dense)) {
+        set_error("int4_decode: null or misaligned device pointer (16 bytes)");
+        return (int)cudaErrorInvalidValue;
+    }
+    int4_decode_kernel<<<blocks((long long)M * K / 8, 256), 256, 0, (cudaStream_t)stream>>>((const uint32_t*)packed, (const __half2*)params,
+                                                                                              dense, M, K, group);
+    count_launch();
+    return (int)cudaGetLastError();
+}
+
+int spb_linear_int4(void* stream, const void* packed, const void* params, int M, int K, int group, const uint16_t* x, uint16_t* out,
+                    int N, const uint16_t* bias, const uint16_t* residual, int activation)
+{
+    using namespace spb;
+    if (!check_weight("linear_int4", M, K, group)) return (int)cudaErrorInvalidValue;
+    if (N <= 0) {
+        set_error("linear_int4: N must be positive (N=%d)", N);
+        return (int)cudaErrorInvalidValue;
+    }
+    if (activation != 0 && activation != 1) {
+        set_error("linear_int4: activation must be 0 (none) or 1 (ReLU), got %d", activation);
+        return (int)cudaErrorInvalidValue;
+    }
+    if (!packed || !params || !x || !out) {
+        set_error("linear_int4: null device pointer");
+        return (int)cudaErrorInvalidValue;
+    }
+    if (!aligned16(packed) || !aligned16(params) || !aligned16(x) || !aligned16(out) || !aligned16(bias) || !aligned16(residual)) {
+        set_error("linear_int4: codes, parameters, x, out, bias and residual must be 16-byte aligned");
+        return (int)cudaErrorMisalignedAddress;
+    }
+    int* status = nullptr;
+    cudaError_t e = device_status_ptr(&status);
+    if (e != cudaSuccess) return (int)e;
+    Int4Args a;
+    a.codes = (const uint32_t*)packed;
+    a.params = (const __half2*)params;
+    a.M = M, a.K = K, a.group = group;
+    a.x = x, a.bias = bias, a.residual = residual, a.out = out;
+    a.N = N, a.activation = activation;
+    e = int4_linear_launch((cudaStream_t)stream, a, status);
+    if (e != cudaSuccess) set_error("linear_int4: %s", cudaGetErrorString(e));
+    return (int)e;
+}
+
+}  // extern "C"

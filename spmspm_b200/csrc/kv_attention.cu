@@ -1,0 +1,686 @@
+// Attention over the paged 4-bit cache (layout: kv_int4.cuh):  out = softmax(q K^T scale) V  with K = m + s c, V likewise.
+//
+// kv_attention_split_kernel: few query rows a key head (decoding, drafts).  Everything is transposed, keys and channels on
+// the 16-row side of mma.sync.m16n8k16 and query rows on its 8-column side, so that a single row wastes 7/8 of a cheap
+// operand and not of the cache's:
+//
+//   scores   S^T = K Q^T per group of 32 channels: the codes enter the matrix instruction as they are.  A nibble masked out
+//            of its word is an fp16 subnormal, c 2^-24 (low nibble of a byte) or c 2^-20 (high), which the instruction
+//            multiplies exactly; the high nibbles' share of q is divided by 16 beforehand.  Scale and minimum are applied to
+//            the fp32 sum of a group: z = s (q.c) + m sum(q), so keys are never rounded, and the cost is 1.25 instructions
+//            per pair of codes instead of three.  q is first multiplied by a power of two that brings its row's largest
+//            magnitude to [2^8, 2^9): the division by 16 then loses nothing above 2^-25 of that magnitude.
+//   softmax  running maximum and sum in fp32 per row, in base 2.  The accumulators are only rescaled when a maximum grows by more
+//            than 2^8; weights are kept 2^7 too large, so that in fp16 they span 2^-31 .. 1 relative to the largest.
+//   values   O^T += V^T P^T: pairs of codes become fp16 with one AND/OR, one subtraction (exact) and one fused multiply-add
+//            (one rounding, the value that kv_read returns); P^T comes from S^T with two 8 x 8 transposes in registers.
+//
+// Work: the context is cut in units of 64 tokens (four warps, one 16-token block each); all units of all (sequence, key
+// head, row tile) are laid end to end and every thread block takes an equal share, found from the lengths on the device.
+// A share that covers a whole row tile is finished where it is; the others leave fp32 (O, max, sum) in the workspace,
+// two slots a thread block, and kv_attention_join_kernel adds them in order: no atomics, the same bits every time.
+// Every warp streams its own blocks: one bulk copy per block into its own ring, nobody waits for another warp except at
+// the end of a row tile.
+#include "kv_int4.cuh"
+#include <cstdio>
+
+namespace spb {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kStages = 4;                 // 16-token blocks in flight per warp
+constexpr uint32_t kSpin = 1u << 22;       // polls before a wait gives up
+constexpr float kShift = 7.f, kSlack = 8.f;
+constexpr int kUnit = kKvBlock * kWarps;   // tokens a thread block advances per step
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity)
+{
+    for (uint32_t i = 0; i < kSpin; ++i) {
+        uint32_t ok;
+        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+        if (i > 1024) __nanosleep(40);
+    }
+    return false;
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
+
+// Sequence b of the work list.
+struct Seq {
+    int b = 0;
+    int len = 0, qlen = 0, tiles = 0;   // tokens in the cache, new tokens, row tiles
+    long long first = 0;                // first packed row
+    long long units = 0;                // 64-token units of one row tile
+    long long begin = 0, total = 0;     // its range of the list
+};
+template <int ROWS>
+__device__ __forceinline__ void load_seq(Seq& s, const KvView& c, int b, int group)
+{
+    long long first, n;
+    kv_rows(c, b, first, n);
+    s.b = b;
+    s.first = first;
+    s.qlen = (int)n;
+    s.len = max(c.lens[b], 0);
+    s.tiles = (int)((n * group + ROWS - 1) / ROWS);
+    // tokens past the table's width have no page: they are not walked over
+    const long long held = min((long long)s.len, (long long)c.table_stride * c.page_size);
+    s.units = max((held + kUnit - 1) / kUnit, 1ll);
+    s.total = (long long)c.kv_heads * s.tiles * s.units;
+}
+template <int ROWS>
+__device__ __forceinline__ long long list_length(const KvView& c, int group)
+{
+    long long sum = 0;
+    for (int b = threadIdx.x & 31; b < c.B; b += 32) {
+        Seq s;
+        load_seq<ROWS>(s, c, b, group);
+        sum += s.total;
+    }
+#pragma unroll
+    for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+}
+// The sequence that holds unit x of the list (x inside the list); every lane gets the same.
+template <int ROWS>
+__device__ __forceinline__ void find_seq(Seq& s, const KvView& c, int group, long long x)
+{
+    const int lane = threadIdx.x & 31;
+    long long before = 0;
+    for (int b0 = 0; b0 < c.B; b0 += 32) {
+        Seq t;
+        if (b0 + lane < c.B) load_seq<ROWS>(t, c, b0 + lane, group);
+        long long incl = t.total;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, before + incl > x);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            const long long begin = before + __shfl_sync(0xffffffffu, incl - t.total, l);
+            load_seq<ROWS>(s, c, b0 + l, group);
+            s.begin = begin;
+            return;
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+}
+template <int ROWS>
+__device__ __forceinline__ void next_seq(Seq& s, const KvView& c, int group)
+{
+    do {
+        const long long end = s.begin + s.total;
+        load_seq<ROWS>(s, c, s.b + 1, group);
+        s.begin = end;
+    } while (s.total == 0 && s.b + 1 < c.B);
+}
+__device__ __forceinline__ long long share_begin(long long total, int ctas, int i) { return total * i / ctas; }
+// Thread block whose share holds unit x.
+__device__ __forceinline__ int share_of(long long total, int ctas, long long x)
+{
+    int i = (int)(((x + 1) * ctas - 1) / total);
+    while (i > 0 && share_begin(total, ctas, i) > x) --i;
+    while (i + 1 < ctas && share_begin(total, ctas, i + 1) <= x) ++i;
+    return i;
+}
+
+// ws: slot n (two per thread block): [rows][D] sums, then [rows] maxima and [rows] sums of weights
+template <int D, int ROWS>
+__host__ __device__ constexpr size_t slot_floats() { return (size_t)ROWS * (D + 2); }
+
+// Keys that row r of a row tile may see.
+__device__ __forceinline__ int visible_keys(const Seq& s, int row, int group)
+{
+    return max(s.len - s.qlen + row / group + 1, 0);
+}
+
+template <int D, int NT>
+struct Smem {
+    alignas(128) uint8_t ring[kWarps][kStages][KvLayout<D>::kBlockBytes];
+    alignas(16) float merge[kWarps - 1][NT * (D / 16) * 4 * 32 + 4 * NT * 32];
+    uint2 qfrag[NT][D / 16][32];                 // q operand, [row tile of 8][k-step][lane]
+    float qsum[NT][KvLayout<D>::kGroups][8];     // sum of q over a group, in units of the score sums
+    float factor[NT][8];                         // score sums -> base-2 scores
+    uint64_t full[kWarps][kStages];
+    int ok[kWarps][kStages];
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(KvAttnArgs a, int* status)
+{
+    using L = KvLayout<D>;
+    constexpr int G = L::kGroups, KS = D / 16, MT = D / 16, ROWS = 8 * NT;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    Smem<D, NT>& sm = *reinterpret_cast<Smem<D, NT>*>(smem_raw);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, t = lane % 4;
+    const KvView& c = a.c;
+    const int group = a.q_heads / c.kv_heads;
+
+    if (lane == 0) {
+        for (int i = 0; i < kStages; ++i)
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&sm.full[warp][i])) : "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+
+    const long long total = list_length<ROWS>(c, group);
+    const long long lo = share_begin(total, gridDim.x, blockIdx.x), hi = share_begin(total, gridDim.x, blockIdx.x + 1);
+    if (lo >= hi) return;
+
+    // ---- this warp's copies: lane l looks after every 32nd unit of the share
+    Seq ps;   // the lane's own place in the list
+    find_seq<ROWS>(ps, c, group, lo);
+    auto block_of = [&](long long x) -> long long {   // pool offset of this warp's block of unit x; -1: nothing to fetch
+        while (x >= ps.begin + ps.total) next_seq<ROWS>(ps, c, group);
+        const long long r = x - ps.begin, pair = r / ps.units;
+        const int rt = (int)(pair % ps.tiles), h = (int)(pair / ps.tiles);
+        const long long pos = ((r % ps.units) * kWarps + warp) * kKvBlock;
+        const int last_row = min((rt + 1) * ROWS, ps.qlen * group) - 1;
+        if (pos >= visible_keys(ps, last_row, group)) return -1;
+        const long long off = kv_block_offset<D>(c, ps.b, h, pos);
+        if (off < 0) atomicOr(status, kStatusBadCache);
+        return off;
+    };
+    auto issue = [&](int stage, long long off) {   // one lane
+        const uint32_t bar = smem_u32(&sm.full[warp][stage]);
+        sm.ok[warp][stage] = off >= 0;
+        if (off >= 0) {
+            asm volatile("{ .reg .b64 st; mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1; }" ::"r"(bar), "r"(L::kBlockBytes) : "memory");
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                             smem_u32(sm.ring[warp][stage])), "l"(c.pool + off), "r"(L::kBlockBytes), "r"(bar) : "memory");
+        } else {
+            asm volatile("{ .reg .b64 st; mbarrier.arrive.shared::cta.b64 st, [%0]; }" ::"r"(bar) : "memory");
+        }
+    };
+    const int count = (int)min(hi - lo, 0x7fffffffll);
+    int issued = 0;                 // units whose copy is under way or done
+    bool alive = true;              // no wait has run out
+    long long my_off = lane < count ? block_of(lo + lane) : -1;
+    auto refill = [&](int upto) {   // whole warp
+        for (; alive && issued < min(upto, count); ++issued) {
+            if (issued && issued % 32 == 0) my_off = issued + lane < count ? block_of(lo + issued + lane) : -1;
+            if (lane == issued % 32) issue(issued % kStages, my_off);
+        }
+    };
+    refill(kStages);
+
+    // ---- consumer
+    Seq s;
+    find_seq<ROWS>(s, c, group, lo);
+    long long x = lo;
+    int done = 0, waited = 0;       // units passed, units whose copy has been waited for
+    while (x < hi) {
+        while (x >= s.begin + s.total) next_seq<ROWS>(s, c, group);
+        const long long pair = (x - s.begin) / s.units;
+        const int rt = (int)(pair % s.tiles), h = (int)(pair / s.tiles);
+        const long long pair_begin = s.begin + pair * s.units, pair_end = pair_begin + s.units;
+        const long long seg_begin = x, seg_end = min(hi, pair_end);
+        if ((long long)s.len > (long long)c.table_stride * c.page_size && threadIdx.x == 0) atomicOr(status, kStatusBadCache);
+        const int rows = min(ROWS, s.qlen * group - rt * ROWS);   // rows of this tile
+        const int kmin = visible_keys(s, rt * ROWS, group), kmax = visible_keys(s, rt * ROWS + rows - 1, group);
+
+        // q of the tile: warps take the 8-row subtiles in turn
+        __syncthreads();
+        for (int nt = warp; nt < NT; nt += kWarps) {
+            const int row = nt * 8 + g, abs_row = rt * ROWS + row;
+            const bool have = row < rows;
+            const uint16_t* src = a.q + (s.first + (have ? abs_row / group : 0)) * a.q_tok + (h * group + (have ? abs_row % group : 0)) * a.q_head;
+            uint2 raw[KS];
+            float big = 0.f;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+                raw[j] = have ? *reinterpret_cast<const uint2*>(src + 16 * j + 4 * t) : make_uint2(0, 0);
+                const float2 u = __half22float2(as_h2(raw[j].x)), w = __half22float2(as_h2(raw[j].y));
+                big = fmaxf(big, fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(w.x), fabsf(w.y))));
+            }
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            int e = 0;   // q is used as q 2^e, its largest magnitude in [2^8, 2^9)
+            if (big > 0.f && big <= 65504.f) e = 8 - ilogbf(big);
+            const float up = exp2f((float)e);
+            float sum[G] = {};
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+                const float k = up * ((j & 1) ? 0.0625f : 1.f);
+                const float2 u = __half22float2(as_h2(raw[j].x)), w = __half22float2(as_h2(raw[j].y));
+                sum[j / 2] += (u.x + u.y) + (w.x + w.y);
+                sm.qfrag[nt][j][lane] = make_uint2(h2_bits(__floats2half2_rn(u.x * k, u.y * k)), h2_bits(__floats2half2_rn(w.x * k, w.y * k)));
+            }
+#pragma unroll
+            for (int w = 0; w < G; ++w) {
+                sum[w] += __shfl_xor_sync(0xffffffffu, sum[w], 1);
+                sum[w] += __shfl_xor_sync(0xffffffffu, sum[w], 2);
+                if (t == 0) sm.qsum[nt][w][g] = sum[w] * exp2f((float)(e - 24));
+            }
+            if (t == 0) sm.factor[nt][g] = a.scale * 1.4426950408889634f * exp2f((float)(24 - e));
+        }
+        __syncthreads();
+
+        float o[NT][MT][4];
+        float mx[NT][2], sum[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+            mx[nt][0] = mx[nt][1] = -INFINITY;
+            sum[nt][0] = sum[nt][1] = 0.f;
+        }
+
+        for (; x < seg_end; ++x, ++done) {
+            const int stage = done % kStages;
+            if (alive) {
+                alive = wait_full(smem_u32(&sm.full[warp][stage]), (done / kStages) & 1);
+                alive = __all_sync(0xffffffffu, alive);
+                if (alive) ++waited;
+                else if (lane == 0) atomicOr(status, kStatusWaitTimeout);   // the rest counts as unseen
+            }
+            const int pos = (int)(((x - pair_begin) * kWarps + warp) * kKvBlock);
+            if (alive && sm.ok[warp][stage]) {
+                const uint8_t* blk = sm.ring[warp][stage];
+                const bool edge = pos + kKvBlock > kmin;   // some row does not see all of these tokens
+                // keys: one word of codes per group for tokens g and g + 8
+                uint32_t k0[G], k1[G];
+                __half2 p0[G], p1[G];
+                {
+                    const uint32_t* kc = reinterpret_cast<const uint32_t*>(blk + L::kKCodes);
+                    const uint32_t* kp = reinterpret_cast<const uint32_t*>(blk + L::kKParams);
+                    if constexpr (G == 4) {
+                        *reinterpret_cast<uint4*>(k0) = *reinterpret_cast<const uint4*>(kc + g * 16 + t * 4);
+                        *reinterpret_cast<uint4*>(k1) = *reinterpret_cast<const uint4*>(kc + (g + 8) * 16 + t * 4);
+                        *reinterpret_cast<uint4*>(p0) = *reinterpret_cast<const uint4*>(kp + g * 4);
+                        *reinterpret_cast<uint4*>(p1) = *reinterpret_cast<const uint4*>(kp + (g + 8) * 4);
+                    } else {
+                        *reinterpret_cast<uint2*>(k0) = *reinterpret_cast<const uint2*>(kc + g * 8 + t * 2);
+                        *reinterpret_cast<uint2*>(k1) = *reinterpret_cast<const uint2*>(kc + (g + 8) * 8 + t * 2);
+                        *reinterpret_cast<uint2*>(p0) = *reinterpret_cast<const uint2*>(kp + g * 2);
+                        *reinterpret_cast<uint2*>(p1) = *reinterpret_cast<const uint2*>(kp + (g + 8) * 2);
+                    }
+                }
+                float z[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) z[nt][0] = z[nt][1] = z[nt][2] = z[nt][3] = 0.f;
+#pragma unroll
+                for (int w = 0; w < G; ++w) {
+                    const uint32_t h0 = k0[w] >> 8, h1 = k1[w] >> 8;
+                    const uint32_t alow[4] = {k0[w] & 0x000f000fu, k1[w] & 0x000f000fu, h0 & 0x000f000fu, h1 & 0x000f000fu};
+                    const uint32_t ahigh[4] = {k0[w] & 0x00f000f0u, k1[w] & 0x00f000f0u, h0 & 0x00f000f0u, h1 & 0x00f000f0u};
+                    const float2 f0 = __half22float2(p0[w]), f1 = __half22float2(p1[w]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                        const uint2 ql = sm.qfrag[nt][2 * w][lane], qh = sm.qfrag[nt][2 * w + 1][lane];
+                        const float2 qs = *reinterpret_cast<const float2*>(&sm.qsum[nt][w][2 * t]);
+                        mma(acc, alow, ql.x, ql.y);
+                        mma(acc, ahigh, qh.x, qh.y);
+                        z[nt][0] = fmaf(f0.x, acc[0], fmaf(f0.y, qs.x, z[nt][0]));
+                        z[nt][1] = fmaf(f0.x, acc[1], fmaf(f0.y, qs.y, z[nt][1]));
+                        z[nt][2] = fmaf(f1.x, acc[2], fmaf(f1.y, qs.x, z[nt][2]));
+                        z[nt][3] = fmaf(f1.x, acc[3], fmaf(f1.y, qs.y, z[nt][3]));
+                    }
+                }
+                bool grow = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float2 f = *reinterpret_cast<const float2*>(&sm.factor[nt][2 * t]);
+                    z[nt][0] *= f.x, z[nt][2] *= f.x;
+                    z[nt][1] *= f.y, z[nt][3] *= f.y;
+                    if (edge) {
+                        const int row = rt * ROWS + nt * 8 + 2 * t;
+                        const int s0 = visible_keys(s, row, group) - pos, s1 = visible_keys(s, row + 1, group) - pos;
+                        if (g >= s0) z[nt][0] = -INFINITY;
+                        if (g >= s1) z[nt][1] = -INFINITY;
+                        if (g + 8 >= s0) z[nt][2] = -INFINITY;
+                        if (g + 8 >= s1) z[nt][3] = -INFINITY;
+                    }
+                    grow = grow || fmaxf(z[nt][0], z[nt][2]) > mx[nt][0] + kSlack || fmaxf(z[nt][1], z[nt][3]) > mx[nt][1] + kSlack;
+                }
+                if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float n0 = fmaxf(z[nt][0], z[nt][2]), n1 = fmaxf(z[nt][1], z[nt][3]);
+#pragma unroll
+                        for (int d = 4; d < 32; d *= 2) {
+                            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, d));
+                            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, d));
+                        }
+                        n0 = fmaxf(n0, mx[nt][0]), n1 = fmaxf(n1, mx[nt][1]);
+                        const float r0 = mx[nt][0] == -INFINITY ? 0.f : exp2_approx(mx[nt][0] - n0);
+                        const float r1 = mx[nt][1] == -INFINITY ? 0.f : exp2_approx(mx[nt][1] - n1);
+                        mx[nt][0] = n0, mx[nt][1] = n1;
+                        sum[nt][0] *= r0, sum[nt][1] *= r1;
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) o[nt][i][0] *= r0, o[nt][i][1] *= r1, o[nt][i][2] *= r0, o[nt][i][3] *= r1;
+                    }
+                }
+                uint32_t b0[NT], b1[NT];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float m0 = (mx[nt][0] == -INFINITY ? 0.f : mx[nt][0]) - kShift;
+                    const float m1 = (mx[nt][1] == -INFINITY ? 0.f : mx[nt][1]) - kShift;
+                    const float w0 = exp2_approx(z[nt][0] - m0), w1 = exp2_approx(z[nt][1] - m1);
+                    const float w2 = exp2_approx(z[nt][2] - m0), w3 = exp2_approx(z[nt][3] - m1);
+                    sum[nt][0] += w0 + w2;
+                    sum[nt][1] += w1 + w3;
+                    b0[nt] = transpose8x8(h2_bits(__floats2half2_rn(w0, w1)));
+                    b1[nt] = transpose8x8(h2_bits(__floats2half2_rn(w2, w3)));
+                }
+                // values: tokens 2t, 2t+1 (j = 0) and 2t+8, 2t+9 (j = 1), D/8 channels of group vg
+                const int vg = g * G / 8;
+                uint32_t vw[2][D / 32];
+                __half2 vs[2], vm[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint8_t* vc = blk + L::kVCodes + j * 4 * D + lane * (D / 8);
+                    if constexpr (G == 4) *reinterpret_cast<uint4*>(vw[j]) = *reinterpret_cast<const uint4*>(vc);
+                    else *reinterpret_cast<uint2*>(vw[j]) = *reinterpret_cast<const uint2*>(vc);
+                    const uint2 p = *reinterpret_cast<const uint2*>(blk + L::kVParams + ((t + 4 * j) * G + vg) * 8);
+                    vs[j] = as_h2(p.x);
+                    vm[j] = as_h2(p.y);
+                }
+                if (edge) {
+                    // Tokens that no row sees count as zero, whatever the page holds there.  A token that some rows see and
+                    // others do not may be NaN for the first and must not touch the others: it is taken out of the product
+                    // and put back row by row.
+                    uint32_t nan_tokens = 0;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        uint32_t sb = h2_bits(vs[j]), mb = h2_bits(vm[j]);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int tok = 2 * t + 8 * j + e;
+                            const uint32_t keep = e ? 0x0000ffffu : 0xffff0000u;
+                            const bool bad = ((sb >> 16 * e) & 0x7c00u) == 0x7c00u || ((mb >> 16 * e) & 0x7c00u) == 0x7c00u;
+                            const bool unseen = pos + tok >= kmax;
+                            if (bad && !unseen) nan_tokens |= 1u << tok;
+                            if (bad || unseen) sb &= keep, mb &= keep;
+                        }
+                        vs[j] = as_h2(sb), vm[j] = as_h2(mb);
+                    }
+                    if (__any_sync(0xffffffffu, nan_tokens != 0)) {
+                        nan_tokens |= __shfl_xor_sync(0xffffffffu, nan_tokens, 1);   // the quad holds one group's 16 tokens
+                        nan_tokens |= __shfl_xor_sync(0xffffffffu, nan_tokens, 2);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int seen = visible_keys(s, rt * ROWS + nt * 8 + 2 * t + e, group) - pos;
+                                const uint32_t mask = seen >= 16 ? 0xffffu : seen <= 0 ? 0u : (1u << seen) - 1;
+                                if (nan_tokens & mask)
+#pragma unroll
+                                    for (int i = 0; i < MT; ++i) o[nt][i][e] = o[nt][i][2 + e] = __int_as_float(0x7fffffff);
+                            }
+                    }
+                }
+                const __half2 off_low = __half2half2(__ushort_as_half((unsigned short)0x6400));    // 1024: nibble at bit 0
+                const __half2 off_high = __half2half2(__ushort_as_half((unsigned short)0x5400));   // 64: nibble at bit 4
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {   // m-tile 2 k + u
+                        uint32_t av[4];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const uint32_t w = u ? vw[j][k] >> 8 : vw[j][k];
+                            const __half2 lowc = __hsub2(as_h2((w & 0x000f000fu) | 0x64006400u), off_low);
+                            const __half2 highc = __hsub2(as_h2((w & 0x00f000f0u) | 0x54005400u), off_high);
+                            av[2 * j] = h2_bits(__hfma2(lowc, vs[j], vm[j]));
+                            av[2 * j + 1] = h2_bits(__hfma2(highc, vs[j], vm[j]));
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma(o[nt][2 * k + u], av, b0[nt], b1[nt]);
+                    }
+                }
+            }
+            __syncwarp();
+            refill(done + 1 + kStages);
+        }
+
+        // ---- join the four warps
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) sum[nt][e] += __shfl_xor_sync(0xffffffffu, sum[nt][e], d);
+        if (warp) {
+            float* dst = sm.merge[warp - 1];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float4 ms = make_float4(mx[nt][0], mx[nt][1], sum[nt][0], sum[nt][1]);
+                reinterpret_cast<float4*>(dst)[(NT * MT + nt) * 32 + lane] = ms;
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    reinterpret_cast<float4*>(dst)[(nt * MT + i) * 32 + lane] = make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]);
+            }
+        }
+        __syncthreads();
+        if (warp == 0) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float4 ms[kWarps - 1];
+                float n0 = mx[nt][0], n1 = mx[nt][1];
+#pragma unroll
+                for (int w = 0; w < kWarps - 1; ++w) {
+                    ms[w] = reinterpret_cast<const float4*>(sm.merge[w])[(NT * MT + nt) * 32 + lane];
+                    n0 = fmaxf(n0, ms[w].x), n1 = fmaxf(n1, ms[w].y);
+                }
+                const float z0 = n0 == -INFINITY ? 0.f : n0, z1 = n1 == -INFINITY ? 0.f : n1;
+                float r0 = exp2_approx(mx[nt][0] - z0), r1 = exp2_approx(mx[nt][1] - z1);
+                float t0 = sum[nt][0] * r0, t1 = sum[nt][1] * r1;
+#pragma unroll
+                for (int i = 0; i < MT; ++i) o[nt][i][0] *= r0, o[nt][i][1] *= r1, o[nt][i][2] *= r0, o[nt][i][3] *= r1;
+#pragma unroll
+                for (int w = 0; w < kWarps - 1; ++w) {
+                    r0 = exp2_approx(ms[w].x - z0), r1 = exp2_approx(ms[w].y - z1);
+                    t0 = fmaf(ms[w].z, r0, t0), t1 = fmaf(ms[w].w, r1, t1);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        const float4 v = reinterpret_cast<const float4*>(sm.merge[w])[(nt * MT + i) * 32 + lane];
+                        o[nt][i][0] = fmaf(v.x, r0, o[nt][i][0]), o[nt][i][1] = fmaf(v.y, r1, o[nt][i][1]);
+                        o[nt][i][2] = fmaf(v.z, r0, o[nt][i][2]), o[nt][i][3] = fmaf(v.w, r1, o[nt][i][3]);
+                    }
+                }
+                const bool whole = seg_begin == pair_begin && seg_end == pair_end;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = nt * 8 + 2 * t + e;
+                    if (row >= rows) continue;
+                    const float total_w = e ? t1 : t0;
+                    if (whole) {
+                        const float inv = total_w == 0.f ? 0.f : 1.f / total_w;   // no visible key: zeros
+                        const int r = rt * ROWS + row;
+                        uint32_t y[MT];
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) y[i] = h2_bits(__floats2half2_rn(o[nt][i][e] * inv, o[nt][i][2 + e] * inv));
+                        uint4* dst = reinterpret_cast<uint4*>(a.out + ((s.first + r / group) * a.q_heads + h * group + r % group) * D + g * (D / 8));
+#pragma unroll
+                        for (int i = 0; i < MT / 4; ++i) dst[i] = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                    } else {
+                        float* slot = a.ws + (2 * (size_t)blockIdx.x + (seg_begin == pair_begin)) * slot_floats<D, ROWS>();
+                        float4* dst = reinterpret_cast<float4*>(slot + row * D + g * (D / 8));
+#pragma unroll
+                        for (int i = 0; i < MT / 2; ++i)
+                            dst[i] = make_float4(o[nt][2 * i][e], o[nt][2 * i][2 + e], o[nt][2 * i + 1][e], o[nt][2 * i + 1][2 + e]);
+                        if (g == 0) {
+                            slot[ROWS * D + row] = e ? n1 : n0;
+                            slot[ROWS * D + ROWS + row] = total_w;
+                        }
+                    }
+                }
+            }
+        }
+    }
+    // only after a wait that ran out: give the copies still under way one more bounded wait before the memory goes away
+    for (; waited < issued; ++waited) wait_full(smem_u32(&sm.full[warp][waited % kStages]), (waited / kStages) & 1);
+}
+
+// Adds the parts of the row tiles that were cut between thread blocks; one thread block per (key head and row tile,
+// sequence), one warp per row in turn.
+template <int D, int NT>
+__global__ void __launch_bounds__(128) kv_attention_join_kernel(KvAttnArgs a, int ctas)
+{
+    constexpr int ROWS = 8 * NT, V = D / 32;
+    const KvView& c = a.c;
+    const int group = a.q_heads / c.kv_heads, lane = threadIdx.x & 31;
+    const long long total = list_length<ROWS>(c, group);
+    if (total == 0) return;
+    Seq s;
+    load_seq<ROWS>(s, c, blockIdx.y, group);
+    long long begin = 0;
+    for (int b = lane; b < (int)blockIdx.y; b += 32) {
+        Seq o;
+        load_seq<ROWS>(o, c, b, group);
+        begin += o.total;
+    }
+#pragma unroll
+    for (int o = 16; o; o /= 2) begin += __shfl_xor_sync(0xffffffffu, begin, o);
+    for (long long pair = blockIdx.x; pair < (long long)c.kv_heads * s.tiles; pair += gridDim.x) {
+        const int rt = (int)(pair % s.tiles), h = (int)(pair / s.tiles);
+        const long long p0 = begin + pair * s.units, p1 = p0 + s.units;
+        const int c0 = share_of(total, ctas, p0), c1 = share_of(total, ctas, p1 - 1);
+        if (c0 == c1) continue;
+        const int rows = min(ROWS, s.qlen * group - rt * ROWS);
+        for (int row = threadIdx.x / 32; row < rows; row += 4) {
+            auto slot = [&](int i) { return a.ws + (2 * (size_t)i + (share_begin(total, ctas, i) <= p0)) * slot_floats<D, ROWS>(); };
+            auto empty = [&](int i) { return share_begin(total, ctas, i) >= share_begin(total, ctas, i + 1); };
+            float m = -INFINITY;
+            for (int i = c0 + lane; i <= c1; i += 32)
+                if (!empty(i)) m = fmaxf(m, slot(i)[ROWS * D + row]);
+#pragma unroll
+            for (int d = 16; d; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+            const float z = m == -INFINITY ? 0.f : m;
+            float acc[V] = {}, w = 0.f;
+#pragma unroll 4
+            for (int i = c0; i <= c1; ++i) {
+                if (empty(i)) continue;
+                const float* p = slot(i);
+                const float r = exp2_approx(p[ROWS * D + row] - z);
+                w = fmaf(p[ROWS * D + ROWS + row], r, w);
+                float v[V];
+                if constexpr (V == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p + row * D + lane * V);
+                else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(p + row * D + lane * V);
+#pragma unroll
+                for (int k = 0; k < V; ++k) acc[k] = fmaf(v[k], r, acc[k]);
+            }
+            const float inv = w == 0.f ? 0.f : 1.f / w;
+            const int r = rt * ROWS + row;
+            __half2 y[V / 2];
+#pragma unroll
+            for (int k = 0; k < V / 2; ++k) y[k] = __floats2half2_rn(acc[2 * k] * inv, acc[2 * k + 1] * inv);
+            uint16_t* dst = a.out + ((s.first + r / group) * a.q_heads + h * group + r % group) * D + lane * V;
+            if constexpr (V == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(y);
+            else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(y);
+        }
+    }
+}
+
+int sm_count()
+{
+    static int n[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (!n[dev] && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    return n[dev];
+}
+
+// Query rows a thread block takes: the fewest of 8, 16, 32 that hold a sequence's rows.
+int pick_nt(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+
+// Thread blocks that fit on the device at once (shared memory and registers).
+template <int D, int NT>
+cudaError_t prepare(int* ctas)
+{
+    static int cached[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!cached[dev]) {
+        e = cudaFuncSetAttribute(kv_attention_split_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D, NT>));
+        int n = 0;
+        if (e == cudaSuccess)
+            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv_attention_split_kernel<D, NT>, 32 * kWarps, sizeof(Smem<D, NT>));
+        if (e != cudaSuccess) return e;
+        cached[dev] = (n < 1 ? 1 : n) * sm_count();
+    }
+    *ctas = cached[dev];
+    return cudaSuccess;
+}
+
+template <int D, int NT>
+cudaError_t launch(cudaStream_t s, const KvAttnArgs& a, int* status)
+{
+    constexpr int ROWS = 8 * NT;
+    int ctas = 0;
+    cudaError_t e = prepare<D, NT>(&ctas);
+    if (e != cudaSuccess) return e;
+    const long long fit = (long long)(a.ws_floats / (2 * slot_floats<D, ROWS>()));
+    if (fit < 1) return cudaErrorInvalidValue;
+    ctas = (int)(fit < ctas ? fit : ctas);
+    // never more thread blocks than units there can be: every table entry used, every packed row in a tile of its own at worst
+    const int group = a.q_heads / a.c.kv_heads;
+    const long long units = ((long long)a.c.table_stride * a.c.page_size + kUnit - 1) / kUnit;
+    const long long tiles = ((long long)a.max_q * group + ROWS - 1) / ROWS;
+    const long long most = (long long)a.c.B * a.c.kv_heads * (tiles > 0 ? tiles : 1) * (units > 0 ? units : 1);
+    if (most < ctas) ctas = (int)most;
+    kv_attention_split_kernel<D, NT><<<ctas, 32 * kWarps, sizeof(Smem<D, NT>), s>>>(a, status);
+    count_launch();
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    const long long pairs = a.c.kv_heads * tiles;
+    const dim3 grid((unsigned)(pairs < 65535 ? pairs : 65535), (unsigned)a.c.B);
+    kv_attention_join_kernel<D, NT><<<grid, 128, 0, s>>>(a, ctas);
+    count_launch();
+    return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t launch_d(cudaStream_t s, const KvAttnArgs& a, int* status)
+{
+    switch (pick_nt(a.max_q * (a.q_heads / a.c.kv_heads))) {
+        case 1: return launch<D, 1>(s, a, status);
+        case 2: return launch<D, 2>(s, a, status);
+        default: return launch<D, 4>(s, a, status);
+    }
+}
+
+}  // namespace
+
+cudaError_t kv_attention_launch(cudaStream_t s, int D, const KvAttnArgs& a, int* status)
+{
+    return D == 128 ? launch_d<128>(s, a, status) : launch_d<64>(s, a, status);
+}
+
+// Workspace for the largest grid: two slots for each of at most 16 thread blocks per SM.
+size_t kv_attention_ws_floats(int D, int B, int q_heads, int kv_heads, int max_q)
+{
+    (void)B;
+    const int rows = 8 * pick_nt(max_q * (q_heads / kv_heads));
+    const int per_sm = rows == 8 ? 4 : rows == 16 ? 3 : 2;
+    return (size_t)2 * per_sm * sm_count() * rows * (D + 2);
+}
+
+}  // namespace spb

@@ -1,0 +1,87 @@
+"""Plain 64-bit models of the 4-bit operators, in numpy, for the tests."""
+import numpy as np
+
+
+def quantise(x):
+    """float64 [..., D] of fp16 values -> codes, s, m (float64) of every 32 channels: m the minimum, s the largest fp16 not
+    above (max - min) / 15, code the nearest of 0..15; a group that holds a value that is not finite: s = m = NaN."""
+    g = x.reshape(x.shape[:-1] + (x.shape[-1] // 32, 32))
+    ok = np.isfinite(g).all(-1, keepdims=True)
+    g = np.where(ok, g, 0.0)
+    lo, hi = g.min(-1, keepdims=True), g.max(-1, keepdims=True)
+    s = ((hi - lo) / 15).astype(np.float16)
+    s = np.where(s.astype(np.float64) > (hi - lo) / 15, np.nextafter(s, np.float16(0)), s).astype(np.float64)
+    with np.errstate(divide="ignore", invalid="ignore"):
+        c = np.where(s > 0, np.clip(np.rint((g - lo) / s), 0, 15), 0.0)
+    return c, np.where(ok, s, np.nan), np.where(ok, lo, np.nan)
+
+
+def entry(x):
+    """What the cache holds for x, unrounded."""
+    c, s, m = quantise(x)
+    return (m + c * s).reshape(x.shape)
+
+
+def rotate(x, pos, cos, sin, interleaved):
+    """x float64 [tokens, heads, D] of fp16 values, turned and rounded once to fp16."""
+    rot = 2 * cos.shape[1]
+    y = x.copy()
+    c, s = cos[pos].astype(np.float64)[:, None], sin[pos].astype(np.float64)[:, None]
+    if interleaved:
+        a, b = x[..., 0:rot:2], x[..., 1:rot:2]
+        y[..., 0:rot:2], y[..., 1:rot:2] = a * c - b * s, b * c + a * s
+    else:
+        a, b = x[..., :rot // 2], x[..., rot // 2:rot]
+        y[..., :rot // 2], y[..., rot // 2:rot] = a * c - b * s, b * c + a * s
+    return y.astype(np.float16).astype(np.float64)
+
+
+def attention(q, k, v, scale):
+    """q [T, Hq, D], k, v [L, Hkv, D] float64, row t sees keys 0 .. L - T + t.  Returns the output and the error that a kernel
+    with fp16 weights and values and fp32 sums may make.
+
+    Error: weights, values and the output are each rounded to fp16 (half a step, 2^-11, of sum p |v|, sum p |v| and |out|), the sum of
+    the weights is that of the unrounded ones (again 2^-11); a score is an fp32 sum of at most D/8 + 16 terms of magnitude
+    sum |q| |k| scale, so exp(score) is off by a factor of at most 2^-24 (D/8 + 16) of that, twice (numerator, denominator);
+    weights below the fp16 range lose at most 2^-32 of the largest each."""
+    T, Hq, D = q.shape
+    L, Hkv = k.shape[:2]
+    out, tol = np.zeros_like(q), np.zeros_like(q)
+    for h in range(Hq):
+        kk, vv = k[:, h // (Hq // Hkv)], v[:, h // (Hq // Hkv)]
+        for t in range(T):
+            n = L - T + t + 1
+            if n <= 0:
+                continue
+            z = (kk[:n] @ q[t, h]) * scale
+            mag = (np.abs(kk[:n]) @ np.abs(q[t, h])) * abs(scale)
+            w = np.exp(z - z.max())
+            p = w / w.sum()
+            o = p @ vv[:n]
+            a = p @ np.abs(vv[:n])
+            out[t, h] = o
+            tol[t, h] = 3 * 2.0 ** -11 * a + 2.0 ** -11 * np.abs(o) + 2 * 2.0 ** -24 * (D / 8 + 16) * mag.max() * a \
+                + n * 2.0 ** -32 * np.abs(vv[:n]).max() + 2.0 ** -24
+    return out, tol
+
+
+def linear(codes, scales, zeros, x, bias, residual, relu, fp16_weights):
+    """float64 y [N, M] and the error that fp32 sums (and, for fp16_weights, weights rounded to fp16) may make.
+
+    Error: one rounding of the result to fp16, half a step; K / 16 + 64 fp32 additions (a matrix instruction adds 16 products
+    at a time; then the groups, the warps and the thread blocks are added) of terms up to sum s (c + z) |x|; a weight
+    rounded to fp16 is off by 2^-11 of itself."""
+    M, K = codes.shape
+    G = K // scales.shape[1]
+    s, z = np.repeat(scales, G, 1), np.repeat(zeros, G, 1)
+    w = s * (codes - z)
+    y = x @ w.T
+    terms = np.abs(x) @ (np.abs(s) * (codes + z)).T
+    tol = (K / 16 + 64) * 2.0 ** -24 * terms + (2.0 ** -11 * (np.abs(x) @ np.abs(w).T) if fp16_weights else 0.0)
+    if bias is not None:
+        y = y + bias
+    if relu:
+        y = np.maximum(y, 0)
+    if residual is not None:
+        y = y + residual
+    return y, tol + 2.0 ** -11 * np.abs(y) + 2.0 ** -24
