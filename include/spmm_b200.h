@@ -323,17 +323,22 @@ int spb_linear_allreduce_finish(void* stream, uint16_t* C, const uint16_t* parts
  *   spb_int4_decode  the inverse of the layout: dense fp16 s * (c - z), rounded once;
  *   spb_linear_int4  out[N][M] = residual + act(x W^T + bias), x [N][K]; summed in fp32 and rounded to fp16 once, at the
  *                    very end (unlike spb_linear_bitmap_v3, which rounds after every step as the kernels it replaces do).
- *                    bias, residual: as there, or NULL; residual may be out itself.  No workspace; may be captured.
+ *                    bias, residual: as there, or NULL; residual may be out itself.  workspace:
+ *                    spb_int4_workspace_bytes bytes (0 for many shapes, NULL then), 16-byte aligned, need not be cleared;
+ *                    not shared by calls that may run at the same time.  With more than 8 rows of x the product takes
+ *                    the weights as spb_int4_decode returns them (rounded to fp16), with up to 8 unrounded.
  */
 size_t spb_int4_codes_bytes(int M, int K);
 size_t spb_int4_params_bytes(int M, int K, int group);
+size_t spb_int4_workspace_bytes(int M, int N, int K);
 int spb_int4_pack(void* stream, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int M, int K, int group,
                   void* packed, void* params);
 int spb_int4_encode(void* stream, const uint16_t* dense, int M, int K, int group, uint8_t* codes, uint16_t* scales,
                     uint8_t* zeros);
 int spb_int4_decode(void* stream, const void* packed, const void* params, int M, int K, int group, uint16_t* dense);
 int spb_linear_int4(void* stream, const void* packed, const void* params, int M, int K, int group, const uint16_t* x,
-                    uint16_t* out, int N, const uint16_t* bias, const uint16_t* residual, int activation);
+                    uint16_t* out, int N, const uint16_t* bias, const uint16_t* residual, int activation, void* workspace,
+                    size_t workspace_bytes);
 
 /* ------------------------------------------------------------------ 4-bit key/value cache */
 

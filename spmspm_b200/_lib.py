@@ -61,7 +61,8 @@ SIGNATURES = {
     "spb_int4_encode": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp]),
     "spb_int4_decode": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp]),
     "spb_linear_int4": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp, _vp,
-                                       ctypes.c_int]),
+                                       ctypes.c_int, _vp, ctypes.c_size_t]),
+    "spb_int4_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 3),
     "spb_kv_cache_bytes": (ctypes.c_size_t, [ctypes.c_int] * 4),
     "spb_kv_append": (ctypes.c_int, [_vp, _vp] + [ctypes.c_int] * 4 + [_vp, ctypes.c_int, _vp, _vp, ctypes.c_int, _ll]
                       + [_vp, _ll, _ll] * 3 + [ctypes.c_int, _vp, _vp, _vp] + [ctypes.c_int] * 3),

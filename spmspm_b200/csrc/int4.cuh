@@ -2,11 +2,15 @@
 //
 // Value of weight (row, k): s (c - z), with code c and zero point z in 0..15 and s fp16 per row and group of 32, 64 or 128 k.
 //
-// codes   tiles of 16 rows x 64 k, 512 bytes each, [M/16][K/64]; a tile is the left operand of four m16n8k16 matrix instructions:
-//         16 bytes a lane (lane = 4 g + t), words {row g, k 0..31}, {row g, k 32..63}, {row g + 8, ..}, {row g + 8, ..}; a
-//         word holds k = 8 t + 4 p + e of its 32, in nibble p + 4 (e & 1) + 2 (e >> 1).  Two neighbouring k are then one AND
-//         with 0x000f000f (p = 0) or 0x00f000f0 (p = 1), after a shift by 8 for e >= 2.
-// params  [M/16][K/group][16 rows] {s, z}, both fp16.
+// Rows are padded to a multiple of 128 with weights of value zero.
+//
+// codes   [M/128][K/64][8] tiles of 16 rows x 64 k, 512 bytes each, so that 128 rows of a 64-k tile are 4 KB in one piece.  A tile
+//         is the left operand of four m16n8k16 matrix instructions, 16 bytes a lane (lane = 4 g + t): words {row g, k 0..31},
+//         {row g, k 32..63}, {row g + 8, ..}, {row g + 8, ..}; a word holds k = 8 t + 4 p + e of its 32, in nibble
+//         p + 4 (e & 1) + 2 (e >> 1), so two neighbouring k are one AND with 0x000f000f (p = 0) or 0x00f000f0 (p = 1), after a
+//         shift by 8 for e >= 2.  The lane's 16 bytes are chunk 4 g + (t ^ (g >> 1)) of the tile: threads that each read one row's
+//         words of the same t then touch all shared-memory banks.
+// params  [M/128][K/group][128 rows] {s, z}, both fp16.
 #pragma once
 #include "common.cuh"
 #include <cuda_fp16.h>
@@ -22,8 +26,13 @@ struct Int4Args {
     const uint16_t* residual;   // [N][M] or null
     uint16_t* out;              // [N][M]
     int N, activation;
+    float* ws;                  // partial sums of tiles that are cut between thread blocks
+    size_t ws_floats;
 };
-cudaError_t int4_linear_launch(cudaStream_t s, const Int4Args& a, int* status);
+constexpr int kInt4SmallRows = 8;   // up to this many rows of x the mma.sync kernel runs, above it the tcgen05 one
+cudaError_t int4_wide_launch(cudaStream_t s, const Int4Args& a, int* status);
+size_t int4_wide_ws_floats(int M, int N, int K);
+__host__ __device__ __forceinline__ int int4_chunk(int g, int t) { return 4 * g + (t ^ (g >> 1)); }
 
 __host__ __device__ __forceinline__ int int4_nibble(int r)   // nibble of k = r (0..7) in the word of its lane
 {

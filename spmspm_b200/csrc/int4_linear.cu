@@ -50,8 +50,8 @@ __global__ void __launch_bounds__(32 * kWarps) int4_small_kernel(Int4Args a)
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const int rt = min(rt0 + r, rt_all - 1);   // past the end: a row tile that is there, its result is not stored
-        code[r] = reinterpret_cast<const uint4*>(a.codes) + (long long)rt * kt_all * 32 + lane;
-        par[r] = a.params + (long long)rt * groups * 16;
+        code[r] = reinterpret_cast<const uint4*>(a.codes) + ((long long)(rt / 8) * kt_all * 8 + rt % 8) * 32 + int4_chunk(g, t);
+        par[r] = a.params + (long long)(rt / 8) * groups * 128 + rt % 8 * 16;
     }
     const uint16_t* xr[NT];
     bool have[NT];
@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(32 * kWarps) int4_small_kernel(Int4Args a)
     uint4 w[kDepth][RT], xv[kDepth][NT][2];
     auto fetch = [&](int slot, int kt) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r) w[slot][r] = load_stream(code[r] + (long long)kt * 32);
+        for (int r = 0; r < RT; ++r) w[slot][r] = load_stream(code[r] + (long long)kt * 256);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(32 * kWarps) int4_small_kernel(Int4Args a)
     auto apply = [&](int grp) {   // a group is complete: scale and zero point
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            const float2 p0 = __half22float2(par[r][grp * 16 + g]), p1 = __half22float2(par[r][grp * 16 + g + 8]);
+            const float2 p0 = __half22float2(par[r][grp * 128 + g]), p1 = __half22float2(par[r][grp * 128 + g + 8]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -170,48 +170,52 @@ __global__ void __launch_bounds__(32 * kWarps) int4_small_kernel(Int4Args a)
     cluster.sync();   // nobody leaves while its sums are being read
 }
 
-// One thread per word: eight codes of one row.
-template <class F>
-__device__ __forceinline__ void for_word(int K, long long i, F&& f)   // f(word index, row, first k)
+// One thread per word, eight codes of one row: row and first k of word i.
+__device__ __forceinline__ void word_place(int K, long long i, long long& row, long long& k)
 {
-    const int q = (int)(i & 3), lane = (int)(i >> 2 & 31);
-    const long long tile = i >> 7, mt = tile / (K / 64), kt = tile % (K / 64);
-    f(mt * 16 + lane / 4 + 8 * (q >> 1), kt * 64 + 32 * (q & 1) + 8 * (lane & 3));
+    const int q = (int)(i & 3), chunk = (int)(i >> 2 & 31), g = chunk / 4, t = (chunk & 3) ^ (g >> 1);
+    const long long tile = i >> 7, rt = tile % 8, kt = tile / 8 % (K / 64), mb = tile / 8 / (K / 64);
+    row = mb * 128 + rt * 16 + g + 8 * (q >> 1);
+    k = kt * 64 + 32 * (q & 1) + 8 * t;
 }
 __global__ void int4_pack_kernel(const uint8_t* codes, uint32_t* packed, int M, int K)
 {
     const long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
-    if (i >= (long long)M * K / 8) return;
-    for_word(K, i, [&](long long row, long long k) {
+    if (i >= (long long)((M + 127) / 128 * 128) * K / 8) return;
+    long long row, k;
+    word_place(K, i, row, k);
+    uint32_t w = 0;
+    if (row < M) {
         const uint2 b = *reinterpret_cast<const uint2*>(codes + row * K + k);
-        uint32_t w = 0;
 #pragma unroll
         for (int r = 0; r < 8; ++r) w |= ((r < 4 ? b.x >> 8 * r : b.y >> 8 * (r - 4)) & 15u) << 4 * int4_nibble(r);
-        packed[i] = w;
-    });
+    }
+    packed[i] = w;
 }
 __global__ void int4_pack_params_kernel(const uint16_t* scales, const uint8_t* zeros, __half2* params, int M, int groups)
 {
     const long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
-    if (i >= (long long)M * groups) return;
-    const long long row = i / groups, grp = i % groups;
-    params[(row / 16 * groups + grp) * 16 + row % 16] =
-        __halves2half2(__ushort_as_half(scales[i]), __ushort2half_rn((unsigned short)(zeros[i] & 15)));
+    if (i >= (long long)((M + 127) / 128 * 128) * groups) return;
+    const long long row = i / 128 / groups * 128 + i % 128, grp = i / 128 % groups;
+    const bool in = row < M;
+    params[i] = __halves2half2(__ushort_as_half(in ? scales[row * groups + grp] : (unsigned short)0),
+                               __ushort2half_rn((unsigned short)(in ? zeros[row * groups + grp] & 15 : 0)));
 }
 // The value of a weight: s (c - z), rounded once to fp16.
 __global__ void int4_decode_kernel(const uint32_t* packed, const __half2* params, uint16_t* dense, int M, int K, int group)
 {
     const long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
-    if (i >= (long long)M * K / 8) return;
-    for_word(K, i, [&](long long row, long long k) {
-        const __half2 p = params[(row / 16 * (K / group) + k / group) * 16 + row % 16];
-        const uint32_t w = packed[i];
-        __half y[8];
+    if (i >= (long long)((M + 127) / 128 * 128) * K / 8) return;
+    long long row, k;
+    word_place(K, i, row, k);
+    if (row >= M) return;
+    const __half2 p = params[(row / 128 * (K / group) + k / group) * 128 + row % 128];
+    const uint32_t w = packed[i];
+    __half y[8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
-            y[r] = __hmul(__hsub(__uint2half_rn(w >> 4 * int4_nibble(r) & 15u), __high2half(p)), __low2half(p));
-        *reinterpret_cast<uint4*>(dense + row * K + k) = *reinterpret_cast<uint4*>(y);
-    });
+    for (int r = 0; r < 8; ++r)
+        y[r] = __hmul(__hsub(__uint2half_rn(w >> 4 * int4_nibble(r) & 15u), __high2half(p)), __low2half(p));
+    *reinterpret_cast<uint4*>(dense + row * K + k) = *reinterpret_cast<uint4*>(y);
 }
 // Quantises one group of one row per 8 lanes x (group / 64) values: lo = min(0, min), hi = max(0, max), s = fp16((hi - lo) / 15),
 // z = round(-lo / s), c = clamp(round(x / s) + z, 0, 15).  Zero is always a value of the group, as pruned weights need it.
@@ -283,9 +287,7 @@ template <int kGroup>
 cudaError_t launch_group(cudaStream_t s, const Int4Args& a)
 {
     const bool many = a.M / 16 >= 8 * sm_count();   // rows enough to fill the device with four row tiles a warp
-    if (a.N <= 8) return many ? launch_small<4, 1, kGroup>(s, a) : launch_small<1, 1, kGroup>(s, a);
-    if (a.N <= 16) return many ? launch_small<4, 2, kGroup>(s, a) : launch_small<2, 2, kGroup>(s, a);
-    return launch_small<2, 4, kGroup>(s, a);
+    return many ? launch_small<4, 1, kGroup>(s, a) : launch_small<1, 1, kGroup>(s, a);
 }
 
 bool check_weight(const char* who, int M, int K, int group)
@@ -304,9 +306,8 @@ unsigned blocks(long long items, int per) { return (unsigned)((items + per - 1) 
 
 }  // namespace
 
-cudaError_t int4_linear_launch(cudaStream_t s, const Int4Args& a, int* status)
+static cudaError_t int4_small_launch(cudaStream_t s, const Int4Args& a)
 {
-    (void)status;
     return a.group == 128 ? launch_group<128>(s, a) : a.group == 64 ? launch_group<64>(s, a) : launch_group<32>(s, a);
 }
 
@@ -314,8 +315,9 @@ cudaError_t int4_linear_launch(cudaStream_t s, const Int4Args& a, int* status)
 
 extern "C" {
 
-size_t spb_int4_codes_bytes(int M, int K) { return M > 0 && K > 0 ? (size_t)M * K / 2 : 0; }
-size_t spb_int4_params_bytes(int M, int K, int group) { return M > 0 && K > 0 && group > 0 ? (size_t)M * (K / group) * 4 : 0; }
+size_t spb_int4_codes_bytes(int M, int K) { return M > 0 && K > 0 ? ((size_t)M + 127) / 128 * 128 * K / 2 : 0; }
+size_t spb_int4_params_bytes(int M, int K, int group) { return M > 0 && K > 0 && group > 0 ? ((size_t)M + 127) / 128 * 128 * (K / group) * 4 : 0; }
+size_t spb_int4_workspace_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? 4 * spb::int4_wide_ws_floats(M, N, K) : 0; }
 
 int spb_int4_pack(void* stream, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int M, int K, int group,
                   void* packed, void* params)
@@ -328,8 +330,8 @@ int spb_int4_pack(void* stream, const uint8_t* codes, const uint16_t* scales, co
         return (int)cudaErrorInvalidValue;
     }
     cudaStream_t s = (cudaStream_t)stream;
-    int4_pack_kernel<<<blocks((long long)M * K / 8, 256), 256, 0, s>>>(codes, (uint32_t*)packed, M, K);
-    int4_pack_params_kernel<<<blocks((long long)M * (K / group), 256), 256, 0, s>>>(scales, zeros, (__half2*)params, M, K / group);
+    int4_pack_kernel<<<blocks((M + 127ll) / 128 * 128 * K / 8, 256), 256, 0, s>>>(codes, (uint32_t*)packed, M, K);
+    int4_pack_params_kernel<<<blocks((M + 127ll) / 128 * 128 * (K / group), 256), 256, 0, s>>>(scales, zeros, (__half2*)params, M, K / group);
     count_launch(2);
     return (int)cudaGetLastError();
 }
@@ -355,14 +357,14 @@ int spb_int4_decode(void* stream, const void* packed, const void* params, int M,
         set_error("int4_decode: null or misaligned device pointer (16 bytes)");
         return (int)cudaErrorInvalidValue;
     }
-    int4_decode_kernel<<<blocks((long long)M * K / 8, 256), 256, 0, (cudaStream_t)stream>>>((const uint32_t*)packed, (const __half2*)params,
+    int4_decode_kernel<<<blocks((M + 127ll) / 128 * 128 * K / 8, 256), 256, 0, (cudaStream_t)stream>>>((const uint32_t*)packed, (const __half2*)params,
                                                                                               dense, M, K, group);
     count_launch();
     return (int)cudaGetLastError();
 }
 
 int spb_linear_int4(void* stream, const void* packed, const void* params, int M, int K, int group, const uint16_t* x, uint16_t* out,
-                    int N, const uint16_t* bias, const uint16_t* residual, int activation)
+                    int N, const uint16_t* bias, const uint16_t* residual, int activation, void* workspace, size_t workspace_bytes)
 {
     using namespace spb;
     if (!check_weight("linear_int4", M, K, group)) return (int)cudaErrorInvalidValue;
@@ -382,6 +384,11 @@ int spb_linear_int4(void* stream, const void* packed, const void* params, int M,
         set_error("linear_int4: codes, parameters, x, out, bias and residual must be 16-byte aligned");
         return (int)cudaErrorMisalignedAddress;
     }
+    const size_t need = spb_int4_workspace_bytes(M, N, K);
+    if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need)) {
+        set_error("linear_int4: needs a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace ? workspace_bytes : (size_t)0);
+        return (int)cudaErrorInvalidValue;
+    }
     int* status = nullptr;
     cudaError_t e = device_status_ptr(&status);
     if (e != cudaSuccess) return (int)e;
@@ -391,7 +398,8 @@ int spb_linear_int4(void* stream, const void* packed, const void* params, int M,
     a.M = M, a.K = K, a.group = group;
     a.x = x, a.bias = bias, a.residual = residual, a.out = out;
     a.N = N, a.activation = activation;
-    e = int4_linear_launch((cudaStream_t)stream, a, status);
+    a.ws = (float*)workspace, a.ws_floats = workspace_bytes / 4;
+    e = N <= kInt4SmallRows ? int4_small_launch((cudaStream_t)stream, a) : int4_wide_launch((cudaStream_t)stream, a, status);
     if (e != cudaSuccess) set_error("linear_int4: %s", cudaGetErrorString(e));
     return (int)e;
 }

@@ -1,0 +1,449 @@
+// Linear layer over 4-bit weights (layout: int4.cuh) for more than a few rows of x, on tcgen05:
+//
+//   out[n][m] = residual + act(bias + sum_k w[m][k] x[n][k]),   w = s (c - z) rounded to fp16 (the value int4_decode returns)
+//
+// Rows of W are the 128-row side of the matrix instruction, rows of x its 16..256-column side.  Codes become fp16 on the way
+// into tensor memory, where the instruction takes its left operand from; x comes as 128-byte-swizzled tiles by tensor copies.
+//
+//   warp 0        copies: per stage of kKT 64-k tiles one bulk copy of codes, one of parameters, kKT tensor copies of x
+//   warp 1        issues tcgen05.mma, one elected thread
+//   warps 4-7     epilogue: accumulators -> bias, activation, residual, one rounding -> out; or fp32 partial sums -> workspace
+//   warps 8..     kGroups groups of four, thread = row of W: per 64-k tile 8 words of codes -> 32 registers of fp16 pairs (per pair
+//                 one AND/OR, one exact subtraction of offset and zero point, one multiplication by the scale) -> tcgen05.st
+//
+// Work: 128-row blocks x column tiles ("items") of K/64 k-tiles.  When the items fill the SMs evenly a thread block takes whole
+// items; otherwise all k-tiles are laid end to end and every thread block takes an equal share, partial sums of cut items go to
+// the workspace (two slots a thread block) and int4_join_kernel adds them in order of k: no atomics, the same bits every time.
+#include "int4.cuh"
+#include "sm100.cuh"
+#include <cuda.h>
+#include <mutex>
+
+namespace spb {
+namespace {
+using namespace sm100;
+
+constexpr int kGroups = 4;                          // dequantising groups of four warps
+constexpr int kThreads = 32 * (8 + 4 * kGroups);
+constexpr int kABlocks = 8;                         // left-operand blocks in tensor memory, 32 columns (64 k) each
+constexpr int kUnit = 2;                            // k-tiles that are not parted: a group of 128 k
+constexpr uint32_t kCodeBytes = 128 * 64 / 2;       // codes of one k-tile
+
+template <int NPAD> struct Cfg {
+    static constexpr int kKT = NPAD <= 64 ? 4 : 2;                       // k-tiles per stage
+    static constexpr int kAcc = NPAD <= 32 ? 4 : NPAD <= 64 ? 2 : 1;     // accumulators the k-steps take in turn (short ones are latency)
+    static constexpr uint32_t kX = NPAD * 128;                           // bytes of x per k-tile
+    static constexpr uint32_t kParamBytes = kKT * 2 * 512;               // at most two groups per k-tile
+    static constexpr uint32_t kStage = kKT * (kX + kCodeBytes) + kParamBytes;
+    static constexpr int kStages = (int)((222u * 1024) / kStage) < 8 ? (int)((222u * 1024) / kStage) : 8;
+    static constexpr uint32_t kSmem = 1024 + 1024 + kStages * kStage;    // header, alignment
+    static constexpr uint32_t kTmemCols = 512;
+};
+
+struct Params {
+    Int4Args a;
+    int kt_all, ku, ncol, items, whole;
+    int* status;
+};
+// First unit of thread block i's share of the list (items in order, ku units each).
+__host__ __device__ __forceinline__ long long share_begin(const Params& p, int ctas, int i)
+{
+    return p.whole ? (long long)p.items * i / ctas * p.ku : (long long)p.items * p.ku * i / ctas;
+}
+__device__ __forceinline__ float finish(const Int4Args& a, float y, long long m, long long n)
+{
+    if (a.bias) y += __half2float(__ushort_as_half(a.bias[m]));
+    if (a.activation) y = y < 0.f ? 0.f : y;   // NaN stays NaN
+    if (a.residual) y += __half2float(__ushort_as_half(a.residual[n * a.M + m]));
+    return y;
+}
+
+// A run of k-tiles of one item.
+struct Run {
+    int mb, n0, kt0, nkt;
+    bool first, last;   // starts / ends the item
+};
+struct Walk {
+    long long x, hi;
+    __device__ __forceinline__ Walk(const Params& p) : x(share_begin(p, gridDim.x, blockIdx.x)), hi(share_begin(p, gridDim.x, blockIdx.x + 1)) {}
+    template <int NPAD>
+    __device__ __forceinline__ bool next(const Params& p, Run& r)
+    {
+        if (x >= hi) return false;
+        const int item = (int)(x / p.ku), u0 = (int)(x - (long long)item * p.ku);
+        const int u1 = (int)min((long long)p.ku, hi - (long long)item * p.ku);
+        r.mb = item / p.ncol;
+        r.n0 = item % p.ncol * NPAD;
+        r.kt0 = u0 * kUnit;
+        r.nkt = min(u1 * kUnit, p.kt_all) - r.kt0;
+        r.first = u0 == 0;
+        r.last = u1 == p.ku;
+        x = (long long)item * p.ku + u1;
+        return true;
+    }
+};
+
+template <int NPAD>
+__global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap xmap)
+{
+    using C = Cfg<NPAD>;
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
+    uint32_t* holder = reinterpret_cast<uint32_t*>(smem + 512);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 516);
+    const uint32_t full = smem_u32(bars), empty = smem_u32(bars + 8), ready = smem_u32(bars + 16), afree = smem_u32(bars + 24),
+                   acc_full = smem_u32(bars + 32), acc_empty = smem_u32(bars + 33);
+    const uint32_t stage0 = smem_u32(smem + 1024);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
+        for (int i = 0; i < kABlocks; ++i) mbar_init(ready + 8 * i, 4), mbar_init(afree + 8 * i, 1);
+        mbar_init(acc_full, 1);
+        mbar_init(acc_empty, 4);
+        *abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == 1) tc_alloc(smem_u32(holder), C::kTmemCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *holder, tmem_a = tmem + 256;
+    grid_wait();      // x, residual, out and the workspace belong to what ran before
+    grid_release();   // the join may be set up while this kernel runs; it waits for its end
+
+    Walk walk(p);
+    Run r;
+    if (warp == 0) {
+        // ---- copies
+        const int groups_per_unit = kUnit * 64 / p.a.group;   // groups in 128 k
+        uint32_t s = 0, round = 0;
+        bool ok = true;
+        while (ok && walk.next<NPAD>(p, r)) {
+            for (int k = 0; k < r.nkt && ok; k += C::kKT) {
+                if (round) ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, (round - 1) & 1, abort_flag));
+                if (!ok) break;
+                if (elect_one()) {
+                    const int kt = r.kt0 + k, n = min(C::kKT, r.nkt - k);
+                    const uint32_t st = stage0 + s * C::kStage, bar = full + 8 * s;
+                    const long long grp0 = (long long)kt / kUnit * groups_per_unit, all = p.a.K / p.a.group;
+                    const int ng = min((long long)((n + kUnit - 1) / kUnit) * groups_per_unit, all - grp0);
+                    mbar_expect_tx(bar, n * (C::kX + kCodeBytes) + ng * 512);
+                    bulk_g2s(st + C::kKT * C::kX, reinterpret_cast<const uint8_t*>(p.a.codes) + ((long long)r.mb * p.kt_all + kt) * kCodeBytes, n * kCodeBytes, bar);
+                    bulk_g2s(st + C::kKT * (C::kX + kCodeBytes), p.a.params + (r.mb * all + grp0) * 128, ng * 512, bar);
+                    for (int i = 0; i < n; ++i) tma_load_2d(st + i * C::kX, &xmap, (kt + i) * 64, r.n0, bar);
+                }
+                __syncwarp();
+                if (++s == (uint32_t)C::kStages) s = 0, ++round;
+            }
+        }
+    } else if (warp == 1) {
+        // ---- matrix instructions
+        constexpr uint32_t idesc = f16_idesc(128, NPAD);
+        uint32_t s = 0, round = 0, t = 0, item = 0;
+        bool ok = true;
+        while (ok && walk.next<NPAD>(p, r)) {
+            if (item) ok = __all_sync(0xffffffffu, mbar_wait(acc_empty, (item - 1) & 1, abort_flag, 4));
+            tc_fence_after();
+            for (int k = 0; k < r.nkt && ok; k += C::kKT) {
+                const int n = min(C::kKT, r.nkt - k);
+                const uint32_t st = stage0 + s * C::kStage;
+                ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * s, round & 1, abort_flag, 4));
+                for (int i = 0; i < n && ok; ++i, ++t) {
+                    const uint32_t blk = t % kABlocks;
+                    ok = __all_sync(0xffffffffu, mbar_wait(ready + 8 * blk, (t / kABlocks) & 1, abort_flag, 4));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t b = kmajor_desc(st + i * C::kX);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            tc_mma_ts(tmem + (j % C::kAcc) * NPAD, tmem_a + blk * 32 + 8 * j, b + 2 * j, idesc, k > 0 || i > 0 || j >= C::kAcc);
+                        tc_commit(afree + 8 * blk);
+                        if (i == n - 1) tc_commit(empty + 8 * s);
+                    }
+                    __syncwarp();
+                }
+                if (++s == (uint32_t)C::kStages) s = 0, ++round;
+            }
+            if (ok && elect_one()) tc_commit(acc_full);
+            __syncwarp();
+            ++item;
+        }
+    } else if (warp >= 8) {
+        // ---- codes to fp16, thread = row
+        const int grp = (warp - 8) / 4, quad = warp & 3, g = lane % 8, high8 = lane / 8 & 1;
+        const uint32_t code_off = (2 * quad + lane / 16) * 512 + high8 * 8;
+        const uint32_t par_off = 4 * (32 * quad + lane);
+        const int per_tile_shift = p.a.group == 32 ? 1 : 0;
+        uint32_t s = 0, round = 0, t = 0;
+        bool ok = true;
+        while (ok && walk.next<NPAD>(p, r)) {
+            for (int k = 0; k < r.nkt && ok; k += C::kKT) {
+                const int n = min(C::kKT, r.nkt - k);
+                const uint32_t st = stage0 + s * C::kStage + C::kKT * C::kX;
+                bool waited = false;
+                for (int i = 0; i < n && ok; ++i, ++t) {
+                    if ((int)(t % kGroups) != grp) continue;
+                    const uint32_t blk = t % kABlocks;
+                    if (!waited) ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * s, round & 1, abort_flag));
+                    waited = true;
+                    if (ok && t >= kABlocks) ok = __all_sync(0xffffffffu, mbar_wait(afree + 8 * blk, (t / kABlocks - 1) & 1, abort_flag));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t par = st + C::kKT * kCodeBytes + par_off;
+                    const int gi = p.a.group == 128 ? i / 2 : i << per_tile_shift;
+                    uint32_t pw[2];
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(pw[0]) : "r"(par + gi * 512));
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(pw[1]) : "r"(par + (gi + per_tile_shift) * 512));
+                    uint32_t w[4][2];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[q][0]), "=r"(w[q][1])
+                                     : "r"(st + i * kCodeBytes + code_off + 16 * int4_chunk(g, q)));
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const __half2 sz = *reinterpret_cast<__half2*>(&pw[h]);
+                        const __half2 sc = __low2half2(sz), z = __high2half2(sz);
+                        const __half2 zl = __hadd2(z, __half2half2(__ushort_as_half((unsigned short)0x6400)));   // 1024 + z
+                        const __half2 zh = __hadd2(z, __half2half2(__ushort_as_half((unsigned short)0x5400)));   // 64 + z
+                        uint32_t o[16];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {   // k = 8 q + 2 e, + 1
+                                const uint32_t u = e & 1 ? w[q][h] >> 8 : w[q][h];
+                                const uint32_t v = e < 2 ? (u & 0x000f000fu) | 0x64006400u : (u & 0x00f000f0u) | 0x54005400u;
+                                const __half2 c = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&v), e < 2 ? zl : zh), sc);
+                                o[4 * q + e] = *reinterpret_cast<const uint32_t*>(&c);
+                            }
+                        tc_st16(tmem_a + blk * 32 + 16 * h + ((uint32_t)quad << 21), o);
+                    }
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(ready + 8 * blk);
+                }
+                if (++s == (uint32_t)C::kStages) s = 0, ++round;
+            }
+        }
+    } else if (warp >= 4) {
+        // ---- epilogue, thread = row
+        const int quad = warp & 3;
+        uint32_t item = 0;
+        bool ok = true;
+        while (ok && walk.next<NPAD>(p, r)) {
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_full, item & 1, abort_flag, 4));
+            if (!ok) break;
+            tc_fence_after();
+            const bool cut = !(r.first && r.last);
+            float* slot = p.a.ws + (2 * (size_t)blockIdx.x + r.first) * NPAD * 128 + 32 * quad + lane;
+            const long long m = (long long)r.mb * 128 + 32 * quad + lane;
+            const uint32_t base = tmem + ((uint32_t)quad << 21);
+#pragma unroll 1
+            for (int c = 0; c < NPAD && r.n0 + c < p.a.N; c += 16) {
+                uint32_t v[16];
+                float y[16];
+                tc_ld16(base + c, v);
+                tc_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) y[i] = __uint_as_float(v[i]);
+#pragma unroll
+                for (int q = 1; q < C::kAcc; ++q) {
+                    tc_ld16(base + q * NPAD + c, v);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) y[i] += __uint_as_float(v[i]);
+                }
+                if (cut) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) slot[(c + i) * 128] = y[i];
+                } else if (m < p.a.M) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const long long n = r.n0 + c + i;
+                        if (n < p.a.N) p.a.out[n * p.a.M + m] = __half_as_ushort(__float2half_rn(finish(p.a, y[i], m, n)));
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty);
+            ++item;
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (*abort_flag) {
+        if (threadIdx.x == 0) {
+            atomicOr(p.status, (int)kStatusWaitTimeout);
+            for (int i = 0; i < C::kStages; ++i)   // copies still under way get a bounded chance to land
+                for (uint32_t spin = 0; spin < 4096; ++spin)
+                    if (mbar_try(full + 8 * i, 0) || mbar_try(full + 8 * i, 1)) break;
+        }
+        __syncthreads();
+    }
+    if (warp == 1) tc_dealloc(tmem, C::kTmemCols);
+}
+
+// Adds the partial sums of the items that were cut; blockIdx.x: item, blockIdx.y: columns by 8.
+template <int NPAD>
+__global__ void __launch_bounds__(256) int4_join_kernel(const __grid_constant__ Params p, int ctas)
+{
+    grid_wait();
+    const long long x0 = (long long)blockIdx.x * p.ku, x1 = x0 + p.ku, total = (long long)p.items * p.ku;
+    auto share_of = [&](long long x) {
+        int i = (int)(((x + 1) * ctas - 1) / total);
+        while (i > 0 && share_begin(p, ctas, i) > x) --i;
+        while (i + 1 < ctas && share_begin(p, ctas, i + 1) <= x) ++i;
+        return i;
+    };
+    const int c0 = share_of(x0), c1 = share_of(x1 - 1);
+    if (c0 == c1) return;
+    const int col = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x & 31;
+    const long long n = (long long)(blockIdx.x % p.ncol) * NPAD + col, m0 = (long long)(blockIdx.x / p.ncol) * 128;
+    if (n >= p.a.N) return;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = c0; i <= c1; ++i) {
+        const long long b = share_begin(p, ctas, i);
+        if (b == share_begin(p, ctas, i + 1)) continue;
+        const float4 v = reinterpret_cast<const float4*>(p.a.ws + (2 * (size_t)i + (b <= x0)) * NPAD * 128 + col * 128)[lane];
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    const long long m = m0 + 4 * lane;
+    if (m >= p.a.M) return;   // M is a multiple of 64
+    const float y[4] = {sum.x, sum.y, sum.z, sum.w};
+    __half o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __float2half_rn(finish(p.a, y[i], m + i, n));
+    *reinterpret_cast<uint2*>(p.a.out + n * p.a.M + m) = *reinterpret_cast<uint2*>(o);
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled()
+{
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* sym = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(sym);
+    });
+    return fn;
+}
+int sm_count()
+{
+    static int n[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+        cudaGetLastError();
+        return 148;
+    }
+    if (!n[dev] && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    return n[dev];
+}
+int pad_for(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : N <= 128 ? 128 : 256; }
+
+// How a shape is dealt out: thread blocks, and whether they take whole items.
+struct Plan {
+    int npad, ncol, items, ku, ctas;
+    bool whole;
+};
+Plan plan_for(int M, int N, int K)
+{
+    Plan q;
+    q.npad = pad_for(N);
+    q.ncol = (N + q.npad - 1) / q.npad;
+    q.items = (M + 127) / 128 * q.ncol;
+    q.ku = (K / 64 + kUnit - 1) / kUnit;
+    const int sms = sm_count();
+    const long long rounds = (q.items + sms - 1) / sms;
+    q.whole = q.items >= 0.92 * rounds * sms;
+    if (q.whole) q.ctas = sms < q.items ? sms : q.items;
+    else {
+        const long long most = (long long)q.items * q.ku / 2;   // at least two units a thread block
+        q.ctas = (int)(most < 1 ? 1 : most < sms ? most : sms);
+    }
+    return q;
+}
+
+template <int NPAD>
+cudaError_t launch(cudaStream_t s, const Int4Args& a, const Plan& q, int* status)
+{
+    using C = Cfg<NPAD>;
+    static bool prepared[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!prepared[dev]) {
+        e = cudaFuncSetAttribute(int4_wide_kernel<NPAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
+        if (e != cudaSuccess) return e;
+        prepared[dev] = true;
+    }
+    EncodeTiledFn enc = encode_tiled();
+    if (!enc) return cudaErrorNotSupported;
+    CUtensorMap map;
+    const cuuint64_t dims[2] = {(cuuint64_t)a.K, (cuuint64_t)a.N};
+    const cuuint64_t strides[1] = {(cuuint64_t)a.K * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)NPAD}, estr[2] = {1, 1};
+    if (enc(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<uint16_t*>(a.x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return cudaErrorInvalidValue;
+    Params p;
+    p.a = a;
+    p.kt_all = a.K / 64;
+    p.ku = q.ku;
+    p.ncol = q.ncol;
+    p.items = q.items;
+    p.whole = q.whole;
+    p.status = status;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(q.ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, int4_wide_kernel<NPAD>, p, map);
+    count_launch();
+    if (e != cudaSuccess || q.whole) return e;
+    cfg.gridDim = dim3(q.items, (a.N < NPAD ? a.N + 7 : NPAD) / 8);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, int4_join_kernel<NPAD>, p, q.ctas);
+    count_launch();
+    return e;
+}
+
+}  // namespace
+
+size_t int4_wide_ws_floats(int M, int N, int K)
+{
+    if (N <= kInt4SmallRows) return 0;
+    const Plan q = plan_for(M, N, K);
+    return q.whole ? 0 : (size_t)2 * q.ctas * q.npad * 128;
+}
+
+cudaError_t int4_wide_launch(cudaStream_t s, const Int4Args& a, int* status)
+{
+    const Plan q = plan_for(a.M, a.N, a.K);
+    switch (q.npad) {
+        case 16: return launch<16>(s, a, q, status);
+        case 32: return launch<32>(s, a, q, status);
+        case 64: return launch<64>(s, a, q, status);
+        case 128: return launch<128>(s, a, q, status);
+        default: return launch<256>(s, a, q, status);
+    }
+}
+
+}  // namespace spb

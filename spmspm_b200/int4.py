@@ -17,8 +17,8 @@ class Int4Matrix:
     M: int
     K: int
     group: int
-    codes: torch.Tensor    # uint8 [M*K/2], tiled for the matrix instruction
-    params: torch.Tensor   # float16 [M*K/group, 2]: scale and zero point
+    codes: torch.Tensor    # uint8 [M*K/2] with M rounded up to 128, tiled for the matrix instruction
+    params: torch.Tensor   # float16 [M*K/group, 2] likewise: scale and zero point
 
     def algorithmic_bytes(self, N):
         """Bytes one linear_int4 must move: codes, scales and zero points, activations, output."""
@@ -50,8 +50,9 @@ def pack_int4(codes, scales, zeros, stream=None):
     _need(codes, "codes", torch.uint8, (M, K))
     _need(scales, "scales", torch.float16, (M, K // group), codes.device)
     _need(zeros, "zeros", torch.uint8, (M, K // group), codes.device)
-    packed = torch.empty(M * K // 2, dtype=torch.uint8, device=codes.device)
-    params = torch.empty((M * (K // group), 2), dtype=torch.float16, device=codes.device)
+    rows = -(-M // 128) * 128
+    packed = torch.empty(rows * K // 2, dtype=torch.uint8, device=codes.device)
+    params = torch.empty((rows * (K // group), 2), dtype=torch.float16, device=codes.device)
     with torch.cuda.device(codes.device):
         _check(_lib.load().spb_int4_pack(_stream_ptr(stream), _ptr(codes), _ptr(scales), _ptr(zeros), M, K, group, _ptr(packed), _ptr(params)),
                "spb_int4_pack")
@@ -74,8 +75,9 @@ def encode_int4(A, group=128, stream=None):
 
 def _check_matrix(W):
     _shape(W.M, W.K, W.group)
-    _need(W.codes, "W.codes", torch.uint8, (W.M * W.K // 2,))
-    _need(W.params, "W.params", torch.float16, (W.M * (W.K // W.group), 2), W.codes.device)
+    rows = -(-W.M // 128) * 128
+    _need(W.codes, "W.codes", torch.uint8, (rows * W.K // 2,))
+    _need(W.params, "W.params", torch.float16, (rows * (W.K // W.group), 2), W.codes.device)
 
 
 def decode_int4(W: Int4Matrix, out=None, stream=None):
@@ -89,9 +91,15 @@ def decode_int4(W: Int4Matrix, out=None, stream=None):
     return out
 
 
-def linear_int4(W: Int4Matrix, B, bias=None, residual=None, activation=ACT_NONE, out=None, stream=None):
+def int4_workspace(W, N):
+    """Bytes of the workspace `linear_int4` needs for N rows (0 for many shapes)."""
+    with torch.cuda.device(W.codes.device):
+        return _lib.load().spb_int4_workspace_bytes(W.M, N, W.K)
+
+
+def linear_int4(W: Int4Matrix, B, bias=None, residual=None, activation=ACT_NONE, out=None, workspace=None, stream=None):
     """spb_linear_int4: out[N,M] = residual + act(B W^T + bias), summed in fp32 and rounded to fp16 once.  B [N,K] as in
-    `linear`; out may be the residual itself, not B."""
+    `linear`; out may be the residual itself, not B.  workspace: int4_workspace(W, N) bytes; a new one by default."""
     _check_matrix(W)
     if not (B.is_cuda and B.dtype == torch.float16 and B.dim() == 2 and B.is_contiguous() and B.shape[1] == W.K and B.device == W.codes.device):
         raise SpmmError("B must be a contiguous CUDA float16 [N,K] tensor on the weight's device")
@@ -101,9 +109,18 @@ def linear_int4(W: Int4Matrix, B, bias=None, residual=None, activation=ACT_NONE,
         out = torch.empty((N, W.M), dtype=torch.float16, device=B.device)
     elif not (out.is_cuda and out.device == B.device and out.dtype == torch.float16 and out.is_contiguous() and tuple(out.shape) == (N, W.M)):
         raise SpmmError("out must be a contiguous CUDA float16 [N,M] tensor")
+    need = int4_workspace(W, N)
+    if need and workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=B.device)
+        if stream is not None:
+            workspace.record_stream(stream)   # its memory must not go to another tensor before that stream is done with it
+    if workspace is not None and not (workspace.is_cuda and workspace.device == B.device and workspace.is_contiguous()
+                                      and workspace.numel() * workspace.element_size() >= need):
+        raise SpmmError(f"the workspace must be a contiguous CUDA tensor of at least {need} bytes on the weight's device")
     with torch.cuda.device(B.device):
         code = _lib.load().spb_linear_int4(_stream_ptr(stream), _ptr(W.codes), _ptr(W.params), W.M, W.K, W.group, _ptr(B), _ptr(out), N,
                                            _ptr(bias) if bias is not None else ctypes.c_void_p(0),
-                                           _ptr(residual) if residual is not None else ctypes.c_void_p(0), int(activation))
+                                           _ptr(residual) if residual is not None else ctypes.c_void_p(0), int(activation), _ptr(workspace),
+                                           workspace.numel() * workspace.element_size() if workspace is not None else 0)
     _check(code, "spb_linear_int4")
     return out
