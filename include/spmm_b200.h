@@ -316,7 +316,7 @@ int spb_linear_allreduce_finish(void* stream, uint16_t* C, const uint16_t* parts
  * instead of pruned.  Weight (m, k) is s * (c - z): code c and zero point z in 0..15, scale s fp16, s and z shared by
  * `group` (32, 64 or 128) consecutive k of a row.  M and K are multiples of 64, K of the group.
  *   spb_int4_pack    brings codes [M][K] (one per byte), scales [M][K/group] and zero points [M][K/group] (one per byte), as
- *                    quantisation tools deliver them, into the library's layout (all device pointers);
+ *                    quantisation tools deliver them, into the library's layout (spb_int4_bytes bytes, 16-byte aligned; all device pointers);
  *   spb_int4_encode  makes such codes, scales and zero points from a dense fp16 matrix: per group lo = min(0, min),
  *                    hi = max(0, max), s = fp16((hi - lo) / 15), z = round(-lo / s), c = clamp(round(x / s) + z, 0, 15);
  *                    a group with a value that is not finite gets s = NaN;
@@ -328,16 +328,14 @@ int spb_linear_allreduce_finish(void* stream, uint16_t* C, const uint16_t* parts
  *                    not shared by calls that may run at the same time.  With more than 8 rows of x the product takes
  *                    the weights as spb_int4_decode returns them (rounded to fp16), with up to 8 unrounded.
  */
-size_t spb_int4_codes_bytes(int M, int K);
-size_t spb_int4_params_bytes(int M, int K, int group);
+size_t spb_int4_bytes(int M, int K, int group);
 size_t spb_int4_workspace_bytes(int M, int N, int K);
 int spb_int4_pack(void* stream, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int M, int K, int group,
-                  void* packed, void* params);
+                  void* packed);
 int spb_int4_encode(void* stream, const uint16_t* dense, int M, int K, int group, uint8_t* codes, uint16_t* scales,
                     uint8_t* zeros);
-int spb_int4_decode(void* stream, const void* packed, const void* params, int M, int K, int group, uint16_t* dense);
-int spb_linear_int4(void* stream, const void* packed, const void* params, int M, int K, int group, const uint16_t* x,
-                    uint16_t* out, int N, const uint16_t* bias, const uint16_t* residual, int activation, void* workspace,
+int spb_int4_decode(void* stream, const void* packed, int M, int K, int group, uint16_t* dense);
+int spb_linear_int4(void* stream, const void* packed, int M, int K, int group, const uint16_t* x, uint16_t* out, int N, const uint16_t* bias, const uint16_t* residual, int activation, void* workspace,
                     size_t workspace_bytes);
 
 /* ------------------------------------------------------------------ 4-bit key/value cache */

@@ -55,12 +55,11 @@ SIGNATURES = {
                                             _vp, _vp, ctypes.c_int, _vp, ctypes.c_int]),
     "spb_linear_allreduce_finish": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp,
                                                    ctypes.c_int]),
-    "spb_int4_codes_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int]),
-    "spb_int4_params_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
-    "spb_int4_pack": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp]),
+    "spb_int4_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "spb_int4_pack": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp]),
     "spb_int4_encode": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp]),
-    "spb_int4_decode": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp]),
-    "spb_linear_int4": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp, _vp,
+    "spb_int4_decode": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp]),
+    "spb_linear_int4": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp, _vp,
                                        ctypes.c_int, _vp, ctypes.c_size_t]),
     "spb_int4_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 3),
     "spb_kv_cache_bytes": (ctypes.c_size_t, [ctypes.c_int] * 4),

@@ -7,7 +7,7 @@
 // exactly, so unpacking costs 1.25 instructions per two weights; low and high nibbles are summed apart, and scale and zero
 // point are applied to the fp32 sums of a group, with sum_k x from one more matrix instruction on ones.  No weight is
 // rounded.  The warps of a thread block, and the thread blocks of a cluster, share out K; partial sums meet in shared
-// memory, in a fixed order.  Codes and x go from memory to registers with 16-byte loads, kDepth tiles ahead.
+// memory, in a fixed order.  Codes and x go from memory to registers with 16-byte loads, kDepth units ahead.
 #include "../../include/spmm_b200.h"
 #include "int4.cuh"
 #include <cooperative_groups.h>
@@ -31,27 +31,23 @@ __device__ __forceinline__ uint4 load_stream(const uint4* p)
     return v;
 }
 
-// RT row tiles of 16, NT column tiles of 8 rows of x per warp; kGT 64-k tiles per group (2: group 128), or 0: group 32.
+// RT row tiles of 16, NT column tiles of 8 rows of x per warp.
 template <int RT, int NT, int kGroup>
 __global__ void __launch_bounds__(32 * kWarps) int4_small_kernel(Int4Args a)
 {
-    constexpr int kDepth = RT == 1 ? 4 : 2;
+    constexpr int kDepth = RT == 1 ? 3 : 2;          // units whose codes and parameters are on their way
+    constexpr int kPer = 128 / kGroup;               // groups per unit
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, t = lane % 4;
-    const int kt_all = a.K / 64, rt_all = a.M / 16, groups = a.K / kGroup;
+    const int ku = (a.K + 127) / 128, rt_all = a.M / 16, kt_all = a.K / 64;
     const int parts = gridDim.y * kWarps, part = blockIdx.y * kWarps + warp;
-    // K in pieces of whole groups, as even as they come
-    constexpr int kStep = kGroup == 128 ? 2 : 1;   // 64-k tiles that stay together
-    const int steps = kt_all / kStep;
-    const int kt0 = (int)((long long)steps * part / parts) * kStep, kt1 = (int)((long long)steps * (part + 1) / parts) * kStep;
+    const int u0 = (int)((long long)ku * part / parts), u1 = (int)((long long)ku * (part + 1) / parts);
     const int rt0 = blockIdx.x * RT, n0 = blockIdx.z * 8 * NT;
 
-    const uint4* code[RT];
-    const __half2* par[RT];
+    const uint8_t* unit[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const int rt = min(rt0 + r, rt_all - 1);   // past the end: a row tile that is there, its result is not stored
-        code[r] = reinterpret_cast<const uint4*>(a.codes) + ((long long)(rt / 8) * kt_all * 8 + rt % 8) * 32 + int4_chunk(g, t);
-        par[r] = a.params + (long long)(rt / 8) * groups * 128 + rt % 8 * 16;
+        unit[r] = a.units + (long long)(rt / 8) * ku * int4_unit_bytes(kGroup) + rt % 8 * 512;
     }
     const uint16_t* xr[NT];
     bool have[NT];
@@ -62,20 +58,29 @@ __global__ void __launch_bounds__(32 * kWarps) int4_small_kernel(Int4Args a)
     }
     float out[RT][NT][4] = {};
     float low[RT][NT][4] = {}, high[RT][NT][4] = {}, xsum[NT][4] = {};
-    uint4 w[kDepth][RT], xv[kDepth][NT][2];
-    auto fetch = [&](int slot, int kt) {
+    uint4 w[kDepth][RT][2], xv[kDepth][NT][4];
+    __half2 par[kDepth][RT][kPer][2];
+    auto fetch = [&](int slot, int u) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r) w[slot][r] = load_stream(code[r] + (long long)kt * 256);
+        for (int r = 0; r < RT; ++r) {
+            const uint8_t* p = unit[r] + (long long)u * int4_unit_bytes(kGroup);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) w[slot][r][i] = load_stream(reinterpret_cast<const uint4*>(p + i * kInt4CodeBytes) + int4_chunk(g, t));
+            const __half2* q = reinterpret_cast<const __half2*>(p - (rt0 + r < rt_all ? (rt0 + r) % 8 : (rt_all - 1) % 8) * 512 + 2 * kInt4CodeBytes) +
+                               (rt0 + r < rt_all ? (rt0 + r) % 8 : (rt_all - 1) % 8) * 16 + g;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) par[slot][r][i][0] = q[i * 128], par[slot][r][i][1] = q[i * 128 + 8];
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                xv[slot][nt][h] = have[nt] ? *reinterpret_cast<const uint4*>(xr[nt] + kt * 64 + 32 * h) : make_uint4(0, 0, 0, 0);
+            for (int h = 0; h < 4; ++h)
+                xv[slot][nt][h] = have[nt] && 2 * u + h / 2 < kt_all ? *reinterpret_cast<const uint4*>(xr[nt] + u * 128 + 32 * h) : make_uint4(0, 0, 0, 0);
     };
-    auto apply = [&](int grp) {   // a group is complete: scale and zero point
+    auto apply = [&](const __half2 (&pv)[RT][kPer][2], int grp) {   // a group is complete: scale and zero point
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            const float2 p0 = __half22float2(par[r][grp * 128 + g]), p1 = __half22float2(par[r][grp * 128 + g + 8]);
+            const float2 p0 = __half22float2(pv[r][grp][0]), p1 = __half22float2(pv[r][grp][1]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -90,9 +95,9 @@ __global__ void __launch_bounds__(32 * kWarps) int4_small_kernel(Int4Args a)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) xsum[nt][0] = xsum[nt][1] = xsum[nt][2] = xsum[nt][3] = 0.f;
     };
-    auto step = [&](const uint4 (&wv)[RT], const uint4 (&xw)[NT][2], int kt) {
+    auto step = [&](const uint4 (&wv)[RT][2], const uint4 (&xw)[NT][4], const __half2 (&pv)[RT][kPer][2]) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 4; ++h) {   // 32 k each
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 mma(xsum[nt], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, xw[nt][h].x, xw[nt][h].y);
@@ -100,7 +105,8 @@ __global__ void __launch_bounds__(32 * kWarps) int4_small_kernel(Int4Args a)
             }
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                const uint32_t u = h ? wv[r].y : wv[r].x, v = h ? wv[r].w : wv[r].z;
+                const uint4 c = wv[r][h / 2];
+                const uint32_t u = h & 1 ? c.y : c.x, v = h & 1 ? c.w : c.z;
                 const uint32_t us = u >> 8, vs = v >> 8;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -108,26 +114,23 @@ __global__ void __launch_bounds__(32 * kWarps) int4_small_kernel(Int4Args a)
                     mma(high[r][nt], u & 0x00f000f0u, v & 0x00f000f0u, us & 0x00f000f0u, vs & 0x00f000f0u, xw[nt][h].z, xw[nt][h].w);
                 }
             }
-            if constexpr (kGroup == 32) apply(kt * 2 + h);
+            if ((h + 1) * 32 % kGroup == 0) apply(pv, h * 32 / kGroup);
         }
-        if constexpr (kGroup == 64) apply(kt);
-        if constexpr (kGroup == 128)
-            if (kt & 1) apply(kt / 2);
     };
 #pragma unroll
     for (int i = 0; i < kDepth; ++i)
-        if (kt0 + i < kt1) fetch(i, kt0 + i);
-    int kt = kt0;
-    for (; kt + kDepth <= kt1; kt += kDepth) {
+        if (u0 + i < u1) fetch(i, u0 + i);
+    int u = u0;
+    for (; u + kDepth <= u1; u += kDepth) {
 #pragma unroll
         for (int i = 0; i < kDepth; ++i) {
-            step(w[i], xv[i], kt + i);
-            if (kt + i + kDepth < kt1) fetch(i, kt + i + kDepth);
+            step(w[i], xv[i], par[i]);
+            if (u + i + kDepth < u1) fetch(i, u + i + kDepth);
         }
     }
 #pragma unroll
     for (int i = 0; i < kDepth; ++i)
-        if (kt + i < kt1) step(w[i], xv[i], kt + i);
+        if (u + i < u1) step(w[i], xv[i], par[i]);
 
     // sums of the warps, then of the cluster's thread blocks (blockIdx.y), in order
     __shared__ float part_sum[kWarps][RT * NT * 4][32];
@@ -170,47 +173,57 @@ __global__ void __launch_bounds__(32 * kWarps) int4_small_kernel(Int4Args a)
     cluster.sync();   // nobody leaves while its sums are being read
 }
 
-// One thread per word, eight codes of one row: row and first k of word i.
-__device__ __forceinline__ void word_place(int K, long long i, long long& row, long long& k)
+// Word i of the codes (eight codes of one row): its place in the units, its row and first k.
+__device__ __forceinline__ long long word_place(int K, int group, long long i, long long& row, long long& k)
 {
+    const int ku = (K + 127) / 128;
     const int q = (int)(i & 3), chunk = (int)(i >> 2 & 31), g = chunk / 4, t = (chunk & 3) ^ (g >> 1);
-    const long long tile = i >> 7, rt = tile % 8, kt = tile / 8 % (K / 64), mb = tile / 8 / (K / 64);
-    row = mb * 128 + rt * 16 + g + 8 * (q >> 1);
-    k = kt * 64 + 32 * (q & 1) + 8 * t;
+    const int in_unit = (int)(i & 2047), rt = in_unit / 128 % 8, kt = in_unit / 1024;
+    const long long unit = i / 2048;
+    row = unit / ku * 128 + rt * 16 + g + 8 * (q >> 1);
+    k = unit % ku * 128 + kt * 64 + 32 * (q & 1) + 8 * t;
+    return unit * (int4_unit_bytes(group) / 4) + in_unit;
 }
-__global__ void int4_pack_kernel(const uint8_t* codes, uint32_t* packed, int M, int K)
+// Parameter word of (row, group), rows and k past the end included.
+__device__ __forceinline__ long long param_place(int K, int group, long long row, long long k)
+{
+    const long long unit = row / 128 * ((K + 127) / 128) + k / 128;
+    return unit * (int4_unit_bytes(group) / 4) + 2048 + k % 128 / group * 128 + row % 128;
+}
+__global__ void int4_pack_kernel(const uint8_t* codes, uint32_t* units, int M, int K, int group)
 {
     const long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
-    if (i >= (long long)((M + 127) / 128 * 128) * K / 8) return;
+    if (i >= int4_units(M, K) * 2048) return;
     long long row, k;
-    word_place(K, i, row, k);
+    const long long at = word_place(K, group, i, row, k);
     uint32_t w = 0;
-    if (row < M) {
+    if (row < M && k < K) {
         const uint2 b = *reinterpret_cast<const uint2*>(codes + row * K + k);
 #pragma unroll
         for (int r = 0; r < 8; ++r) w |= ((r < 4 ? b.x >> 8 * r : b.y >> 8 * (r - 4)) & 15u) << 4 * int4_nibble(r);
     }
-    packed[i] = w;
+    units[at] = w;
 }
-__global__ void int4_pack_params_kernel(const uint16_t* scales, const uint8_t* zeros, __half2* params, int M, int groups)
+__global__ void int4_pack_params_kernel(const uint16_t* scales, const uint8_t* zeros, uint32_t* units, int M, int K, int group)
 {
     const long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
-    if (i >= (long long)((M + 127) / 128 * 128) * groups) return;
-    const long long row = i / 128 / groups * 128 + i % 128, grp = i / 128 % groups;
-    const bool in = row < M;
-    params[i] = __halves2half2(__ushort_as_half(in ? scales[row * groups + grp] : (unsigned short)0),
-                               __ushort2half_rn((unsigned short)(in ? zeros[row * groups + grp] & 15 : 0)));
+    const int per = (K + 127) / 128 * (128 / group), groups = K / group;
+    if (i >= (long long)(M + 127) / 128 * 128 * per) return;
+    const long long row = i / per, grp = i % per;
+    const bool in = row < M && grp < groups;
+    const __half2 v = __halves2half2(__ushort_as_half(in ? scales[row * groups + grp] : (unsigned short)0),
+                                     __ushort2half_rn((unsigned short)(in ? zeros[row * groups + grp] & 15 : 0)));
+    units[param_place(K, group, row, grp * group)] = *reinterpret_cast<const uint32_t*>(&v);
 }
 // The value of a weight: s (c - z), rounded once to fp16.
-__global__ void int4_decode_kernel(const uint32_t* packed, const __half2* params, uint16_t* dense, int M, int K, int group)
+__global__ void int4_decode_kernel(const uint32_t* units, uint16_t* dense, int M, int K, int group)
 {
     const long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
-    if (i >= (long long)((M + 127) / 128 * 128) * K / 8) return;
+    if (i >= int4_units(M, K) * 2048) return;
     long long row, k;
-    word_place(K, i, row, k);
-    if (row >= M) return;
-    const __half2 p = params[(row / 128 * (K / group) + k / group) * 128 + row % 128];
-    const uint32_t w = packed[i];
+    const uint32_t w = units[word_place(K, group, i, row, k)];
+    if (row >= M || k >= K) return;
+    const __half2 p = reinterpret_cast<const __half2*>(units)[param_place(K, group, row, k)];
     __half y[8];
 #pragma unroll
     for (int r = 0; r < 8; ++r)
@@ -315,23 +328,24 @@ static cudaError_t int4_small_launch(cudaStream_t s, const Int4Args& a)
 
 extern "C" {
 
-size_t spb_int4_codes_bytes(int M, int K) { return M > 0 && K > 0 ? ((size_t)M + 127) / 128 * 128 * K / 2 : 0; }
-size_t spb_int4_params_bytes(int M, int K, int group) { return M > 0 && K > 0 && group > 0 ? ((size_t)M + 127) / 128 * 128 * (K / group) * 4 : 0; }
+size_t spb_int4_bytes(int M, int K, int group)
+{
+    if (M <= 0 || K <= 0 || M % 64 || K % 64 || (group != 32 && group != 64 && group != 128) || K % group) return 0;
+    return (size_t)spb::int4_units(M, K) * spb::int4_unit_bytes(group);
+}
 size_t spb_int4_workspace_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? 4 * spb::int4_wide_ws_floats(M, N, K) : 0; }
 
-int spb_int4_pack(void* stream, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int M, int K, int group,
-                  void* packed, void* params)
+int spb_int4_pack(void* stream, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int M, int K, int group, void* packed)
 {
     using namespace spb;
     if (!check_weight("int4_pack", M, K, group)) return (int)cudaErrorInvalidValue;
-    if (!codes || !scales || !zeros || !packed || !params || !aligned16(codes) || !aligned16(packed) || !aligned16(params) ||
-        (reinterpret_cast<uintptr_t>(scales) & 1)) {
-        set_error("int4_pack: null or misaligned device pointer (codes, packed and params: 16 bytes)");
+    if (!codes || !scales || !zeros || !packed || !aligned16(codes) || !aligned16(packed) || (reinterpret_cast<uintptr_t>(scales) & 1)) {
+        set_error("int4_pack: null or misaligned device pointer (codes and packed: 16 bytes)");
         return (int)cudaErrorInvalidValue;
     }
     cudaStream_t s = (cudaStream_t)stream;
-    int4_pack_kernel<<<blocks((M + 127ll) / 128 * 128 * K / 8, 256), 256, 0, s>>>(codes, (uint32_t*)packed, M, K);
-    int4_pack_params_kernel<<<blocks((M + 127ll) / 128 * 128 * (K / group), 256), 256, 0, s>>>(scales, zeros, (__half2*)params, M, K / group);
+    int4_pack_kernel<<<blocks(int4_units(M, K) * 2048, 256), 256, 0, s>>>(codes, (uint32_t*)packed, M, K, group);
+    int4_pack_params_kernel<<<blocks(int4_units(M, K) * 128 * (128 / group), 256), 256, 0, s>>>(scales, zeros, (uint32_t*)packed, M, K, group);
     count_launch(2);
     return (int)cudaGetLastError();
 }
@@ -349,21 +363,20 @@ int spb_int4_encode(void* stream, const uint16_t* dense, int M, int K, int group
     return (int)cudaGetLastError();
 }
 
-int spb_int4_decode(void* stream, const void* packed, const void* params, int M, int K, int group, uint16_t* dense)
+int spb_int4_decode(void* stream, const void* packed, int M, int K, int group, uint16_t* dense)
 {
     using namespace spb;
     if (!check_weight("int4_decode", M, K, group)) return (int)cudaErrorInvalidValue;
-    if (!packed || !params || !dense || !aligned16(packed) || !aligned16(params) || !aligned16(dense)) {
+    if (!packed || !dense || !aligned16(packed) || !aligned16(dense)) {
         set_error("int4_decode: null or misaligned device pointer (16 bytes)");
         return (int)cudaErrorInvalidValue;
     }
-    int4_decode_kernel<<<blocks((M + 127ll) / 128 * 128 * K / 8, 256), 256, 0, (cudaStream_t)stream>>>((const uint32_t*)packed, (const __half2*)params,
-                                                                                              dense, M, K, group);
+    int4_decode_kernel<<<blocks(int4_units(M, K) * 2048, 256), 256, 0, (cudaStream_t)stream>>>((const uint32_t*)packed, dense, M, K, group);
     count_launch();
     return (int)cudaGetLastError();
 }
 
-int spb_linear_int4(void* stream, const void* packed, const void* params, int M, int K, int group, const uint16_t* x, uint16_t* out,
+int spb_linear_int4(void* stream, const void* packed, int M, int K, int group, const uint16_t* x, uint16_t* out,
                     int N, const uint16_t* bias, const uint16_t* residual, int activation, void* workspace, size_t workspace_bytes)
 {
     using namespace spb;
@@ -376,12 +389,12 @@ int spb_linear_int4(void* stream, const void* packed, const void* params, int M,
         set_error("linear_int4: activation must be 0 (none) or 1 (ReLU), got %d", activation);
         return (int)cudaErrorInvalidValue;
     }
-    if (!packed || !params || !x || !out) {
+    if (!packed || !x || !out) {
         set_error("linear_int4: null device pointer");
         return (int)cudaErrorInvalidValue;
     }
-    if (!aligned16(packed) || !aligned16(params) || !aligned16(x) || !aligned16(out) || !aligned16(bias) || !aligned16(residual)) {
-        set_error("linear_int4: codes, parameters, x, out, bias and residual must be 16-byte aligned");
+    if (!aligned16(packed) || !aligned16(x) || !aligned16(out) || !aligned16(bias) || !aligned16(residual)) {
+        set_error("linear_int4: the weight, x, out, bias and residual must be 16-byte aligned");
         return (int)cudaErrorMisalignedAddress;
     }
     const size_t need = spb_int4_workspace_bytes(M, N, K);
@@ -393,8 +406,7 @@ int spb_linear_int4(void* stream, const void* packed, const void* params, int M,
     cudaError_t e = device_status_ptr(&status);
     if (e != cudaSuccess) return (int)e;
     Int4Args a;
-    a.codes = (const uint32_t*)packed;
-    a.params = (const __half2*)params;
+    a.units = (const uint8_t*)packed;
     a.M = M, a.K = K, a.group = group;
     a.x = x, a.bias = bias, a.residual = residual, a.out = out;
     a.N = N, a.activation = activation;

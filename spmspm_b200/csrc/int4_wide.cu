@@ -5,7 +5,9 @@
 // Rows of W are the 128-row side of the matrix instruction, rows of x its 16..256-column side.  Codes become fp16 on the way
 // into tensor memory, where the instruction takes its left operand from; x comes as 128-byte-swizzled tiles by tensor copies.
 //
-//   warp 0        copies: per stage of kKT 64-k tiles one bulk copy of codes, one of parameters, kKT tensor copies of x
+//   warps 0, 2    copies: per stage of kKT 64-k tiles one bulk copy of codes and parameters (warp 0), one tensor copy of x
+//                 (warp 2).  Issuing a copy holds a warp up for a few hundred cycles, so there are few and two warps share them
+//                 (one warp issuing six copies a stage capped the kernel at 0.26 us a k-tile, three times what memory needs)
 //   warp 1        issues tcgen05.mma, one elected thread
 //   warps 4-7     epilogue: accumulators -> bias, activation, residual, one rounding -> out; or fp32 partial sums -> workspace
 //   warps 8..     kGroups groups of four, thread = row of W: per 64-k tile 8 words of codes -> 32 registers of fp16 pairs (per pair
@@ -26,15 +28,13 @@ using namespace sm100;
 constexpr int kGroups = 4;                          // dequantising groups of four warps
 constexpr int kThreads = 32 * (8 + 4 * kGroups);
 constexpr int kABlocks = 8;                         // left-operand blocks in tensor memory, 32 columns (64 k) each
-constexpr int kUnit = 2;                            // k-tiles that are not parted: a group of 128 k
-constexpr uint32_t kCodeBytes = 128 * 64 / 2;       // codes of one k-tile
+constexpr int kUnit = 2;                            // k-tiles of a unit
 
 template <int NPAD> struct Cfg {
     static constexpr int kKT = NPAD <= 64 ? 4 : 2;                       // k-tiles per stage
     static constexpr int kAcc = NPAD <= 32 ? 4 : NPAD <= 64 ? 2 : 1;     // accumulators the k-steps take in turn (short ones are latency)
     static constexpr uint32_t kX = NPAD * 128;                           // bytes of x per k-tile
-    static constexpr uint32_t kParamBytes = kKT * 2 * 512;               // at most two groups per k-tile
-    static constexpr uint32_t kStage = kKT * (kX + kCodeBytes) + kParamBytes;
+    static constexpr uint32_t kStage = kKT * kX + kKT / kUnit * (2 * kInt4CodeBytes + 4 * 512);   // x, units (at most four groups)
     static constexpr int kStages = (int)((222u * 1024) / kStage) < 8 ? (int)((222u * 1024) / kStage) : 8;
     static constexpr uint32_t kSmem = 1024 + 1024 + kStages * kStage;    // header, alignment
     static constexpr uint32_t kTmemCols = 512;
@@ -42,13 +42,17 @@ template <int NPAD> struct Cfg {
 
 struct Params {
     Int4Args a;
-    int kt_all, ku, ncol, items, whole;
+    int ku, ncol, items;   // units along K, column tiles, items
+    int share, extra;      // thread block i takes `share` units, one more if i < extra; whole: items instead of units
+    int whole;
     int* status;
 };
-// First unit of thread block i's share of the list (items in order, ku units each).
-__host__ __device__ __forceinline__ long long share_begin(const Params& p, int ctas, int i)
+// First unit of thread block i's share of the list (items in order, ku units each), and the thread block that has unit x.
+__device__ __forceinline__ int share_begin(const Params& p, int i) { return (i * p.share + min(i, p.extra)) * (p.whole ? p.ku : 1); }
+__device__ __forceinline__ int share_of(const Params& p, int x)   // not whole
 {
-    return p.whole ? (long long)p.items * i / ctas * p.ku : (long long)p.items * p.ku * i / ctas;
+    const int big = p.extra * (p.share + 1);
+    return x < big ? x / (p.share + 1) : p.extra + (x - big) / p.share;
 }
 __device__ __forceinline__ float finish(const Int4Args& a, float y, long long m, long long n)
 {
@@ -60,25 +64,26 @@ __device__ __forceinline__ float finish(const Int4Args& a, float y, long long m,
 
 // A run of k-tiles of one item.
 struct Run {
-    int mb, n0, kt0, nkt;
+    int mb, n0, u0, nkt;
     bool first, last;   // starts / ends the item
 };
 struct Walk {
-    long long x, hi;
-    __device__ __forceinline__ Walk(const Params& p) : x(share_begin(p, gridDim.x, blockIdx.x)), hi(share_begin(p, gridDim.x, blockIdx.x + 1)) {}
+    int x, hi, item, u;
+    __device__ __forceinline__ Walk(const Params& p) : x(share_begin(p, blockIdx.x)), hi(share_begin(p, blockIdx.x + 1)), item(x / p.ku), u(x - item * p.ku) {}
     template <int NPAD>
     __device__ __forceinline__ bool next(const Params& p, Run& r)
     {
         if (x >= hi) return false;
-        const int item = (int)(x / p.ku), u0 = (int)(x - (long long)item * p.ku);
-        const int u1 = (int)min((long long)p.ku, hi - (long long)item * p.ku);
+        const int n = min(p.ku - u, hi - x);
         r.mb = item / p.ncol;
-        r.n0 = item % p.ncol * NPAD;
-        r.kt0 = u0 * kUnit;
-        r.nkt = min(u1 * kUnit, p.kt_all) - r.kt0;
-        r.first = u0 == 0;
-        r.last = u1 == p.ku;
-        x = (long long)item * p.ku + u1;
+        r.n0 = (item - r.mb * p.ncol) * NPAD;
+        r.u0 = u;
+        r.nkt = n * kUnit;
+        r.first = u == 0;
+        r.last = u + n == p.ku;
+        x += n;
+        u = 0;
+        ++item;
         return true;
     }
 };
@@ -98,7 +103,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_con
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < C::kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
+        for (int i = 0; i < C::kStages; ++i) mbar_init(full + 8 * i, 2), mbar_init(empty + 8 * i, 1);
         for (int i = 0; i < kABlocks; ++i) mbar_init(ready + 8 * i, 4), mbar_init(afree + 8 * i, 1);
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, 4);
@@ -115,9 +120,9 @@ __global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_con
 
     Walk walk(p);
     Run r;
-    if (warp == 0) {
+    if (warp == 0 || warp == 2) {
         // ---- copies
-        const int groups_per_unit = kUnit * 64 / p.a.group;   // groups in 128 k
+        const int unit_bytes = int4_unit_bytes(p.a.group);
         uint32_t s = 0, round = 0;
         bool ok = true;
         while (ok && walk.next<NPAD>(p, r)) {
@@ -125,14 +130,15 @@ __global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_con
                 if (round) ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, (round - 1) & 1, abort_flag));
                 if (!ok) break;
                 if (elect_one()) {
-                    const int kt = r.kt0 + k, n = min(C::kKT, r.nkt - k);
+                    const int u = r.u0 + k / kUnit, n = min(C::kKT, r.nkt - k) / kUnit;
                     const uint32_t st = stage0 + s * C::kStage, bar = full + 8 * s;
-                    const long long grp0 = (long long)kt / kUnit * groups_per_unit, all = p.a.K / p.a.group;
-                    const int ng = min((long long)((n + kUnit - 1) / kUnit) * groups_per_unit, all - grp0);
-                    mbar_expect_tx(bar, n * (C::kX + kCodeBytes) + ng * 512);
-                    bulk_g2s(st + C::kKT * C::kX, reinterpret_cast<const uint8_t*>(p.a.codes) + ((long long)r.mb * p.kt_all + kt) * kCodeBytes, n * kCodeBytes, bar);
-                    bulk_g2s(st + C::kKT * (C::kX + kCodeBytes), p.a.params + (r.mb * all + grp0) * 128, ng * 512, bar);
-                    for (int i = 0; i < n; ++i) tma_load_2d(st + i * C::kX, &xmap, (kt + i) * 64, r.n0, bar);
+                    if (warp == 0) {
+                        mbar_expect_tx(bar, n * unit_bytes);
+                        bulk_g2s(st + C::kKT * C::kX, p.a.units + ((long long)r.mb * p.ku + u) * unit_bytes, n * unit_bytes, bar);
+                    } else {
+                        mbar_expect_tx(bar, C::kKT * C::kX);   // k-tiles past K come as zeros
+                        tma_load_3d(st, &xmap, 0, r.n0, u * kUnit, bar);
+                    }
                 }
                 __syncwarp();
                 if (++s == (uint32_t)C::kStages) s = 0, ++round;
@@ -175,8 +181,10 @@ __global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_con
         // ---- codes to fp16, thread = row
         const int grp = (warp - 8) / 4, quad = warp & 3, g = lane % 8, high8 = lane / 8 & 1;
         const uint32_t code_off = (2 * quad + lane / 16) * 512 + high8 * 8;
-        const uint32_t par_off = 4 * (32 * quad + lane);
-        const int per_tile_shift = p.a.group == 32 ? 1 : 0;
+        const uint32_t par_off = 2 * kInt4CodeBytes + 4 * (32 * quad + lane);
+        const uint32_t unit_bytes = int4_unit_bytes(p.a.group);
+        // parameters of the two 32-k halves of k-tile 0 and 1 of a unit: which of its groups
+        const int grp_tile = p.a.group == 128 ? 0 : p.a.group == 64 ? 1 : 2, grp_half = p.a.group == 32 ? 1 : 0;
         uint32_t s = 0, round = 0, t = 0;
         bool ok = true;
         while (ok && walk.next<NPAD>(p, r)) {
@@ -192,16 +200,16 @@ __global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_con
                     if (ok && t >= kABlocks) ok = __all_sync(0xffffffffu, mbar_wait(afree + 8 * blk, (t / kABlocks - 1) & 1, abort_flag));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t par = st + C::kKT * kCodeBytes + par_off;
-                    const int gi = p.a.group == 128 ? i / 2 : i << per_tile_shift;
+                    const uint32_t unit = st + (i / kUnit) * unit_bytes, tile = unit + (i % kUnit) * kInt4CodeBytes + code_off;
+                    const uint32_t par = unit + par_off + (i % kUnit) * grp_tile * 512;
                     uint32_t pw[2];
-                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(pw[0]) : "r"(par + gi * 512));
-                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(pw[1]) : "r"(par + (gi + per_tile_shift) * 512));
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(pw[0]) : "r"(par));
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(pw[1]) : "r"(par + grp_half * 512));
                     uint32_t w[4][2];
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
                         asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[q][0]), "=r"(w[q][1])
-                                     : "r"(st + i * kCodeBytes + code_off + 16 * int4_chunk(g, q)));
+                                     : "r"(tile + 16 * int4_chunk(g, q)));
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const __half2 sz = *reinterpret_cast<__half2*>(&pw[h]);
@@ -291,27 +299,22 @@ __global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_con
 
 // Adds the partial sums of the items that were cut; blockIdx.x: item, blockIdx.y: columns by 8.
 template <int NPAD>
-__global__ void __launch_bounds__(256) int4_join_kernel(const __grid_constant__ Params p, int ctas)
+__global__ void __launch_bounds__(256) int4_join_kernel(const __grid_constant__ Params p)
 {
+    const int x0 = blockIdx.x * p.ku, c0 = share_of(p, x0), c1 = share_of(p, x0 + p.ku - 1);
     grid_wait();
-    const long long x0 = (long long)blockIdx.x * p.ku, x1 = x0 + p.ku, total = (long long)p.items * p.ku;
-    auto share_of = [&](long long x) {
-        int i = (int)(((x + 1) * ctas - 1) / total);
-        while (i > 0 && share_begin(p, ctas, i) > x) --i;
-        while (i + 1 < ctas && share_begin(p, ctas, i + 1) <= x) ++i;
-        return i;
-    };
-    const int c0 = share_of(x0), c1 = share_of(x1 - 1);
     if (c0 == c1) return;
     const int col = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x & 31;
     const long long n = (long long)(blockIdx.x % p.ncol) * NPAD + col, m0 = (long long)(blockIdx.x / p.ncol) * 128;
     if (n >= p.a.N) return;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 sum;
+    // the first part may be either slot of its thread block, the later ones start a thread block's share
+    const float4* src = reinterpret_cast<const float4*>(p.a.ws + col * 128) + lane;
+    const float4 f = src[(2 * (size_t)c0 + 1) * (NPAD * 32)];
+    sum = f;
 #pragma unroll 4
-    for (int i = c0; i <= c1; ++i) {
-        const long long b = share_begin(p, ctas, i);
-        if (b == share_begin(p, ctas, i + 1)) continue;
-        const float4 v = reinterpret_cast<const float4*>(p.a.ws + (2 * (size_t)i + (b <= x0)) * NPAD * 128 + col * 128)[lane];
+    for (int i = c0 + 1; i <= c1; ++i) {
+        const float4 v = src[2 * (size_t)i * (NPAD * 32)];
         sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
     }
     const long long m = m0 + 4 * lane;
@@ -352,7 +355,9 @@ int pad_for(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : N <= 12
 
 // How a shape is dealt out: thread blocks, and whether they take whole items.
 struct Plan {
-    int npad, ncol, items, ku, ctas;
+    int npad, ncol;
+    long long items;
+    int ku, ctas;
     bool whole;
 };
 Plan plan_for(int M, int N, int K)
@@ -360,16 +365,12 @@ Plan plan_for(int M, int N, int K)
     Plan q;
     q.npad = pad_for(N);
     q.ncol = (N + q.npad - 1) / q.npad;
-    q.items = (M + 127) / 128 * q.ncol;
-    q.ku = (K / 64 + kUnit - 1) / kUnit;
+    q.items = (M + 127ll) / 128 * q.ncol;
+    q.ku = (K + 127) / 128;
     const int sms = sm_count();
-    const long long rounds = (q.items + sms - 1) / sms;
+    const long long rounds = (q.items + sms - 1) / sms, units = q.items * q.ku;
     q.whole = q.items >= 0.92 * rounds * sms;
-    if (q.whole) q.ctas = sms < q.items ? sms : q.items;
-    else {
-        const long long most = (long long)q.items * q.ku / 2;   // at least two units a thread block
-        q.ctas = (int)(most < 1 ? 1 : most < sms ? most : sms);
-    }
+    q.ctas = (int)(q.whole ? (sms < q.items ? (long long)sms : q.items) : units < 2 ? 1ll : units / 2 < sms ? units / 2 : (long long)sms);   // at least two units a thread block
     return q;
 }
 
@@ -390,19 +391,22 @@ cudaError_t launch(cudaStream_t s, const Int4Args& a, const Plan& q, int* status
     EncodeTiledFn enc = encode_tiled();
     if (!enc) return cudaErrorNotSupported;
     CUtensorMap map;
-    const cuuint64_t dims[2] = {(cuuint64_t)a.K, (cuuint64_t)a.N};
-    const cuuint64_t strides[1] = {(cuuint64_t)a.K * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)NPAD}, estr[2] = {1, 1};
-    if (enc(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<uint16_t*>(a.x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    // x as [K / 64][N][64]: the k-tiles of a stage are one copy
+    const cuuint64_t dims[3] = {64, (cuuint64_t)a.N, (cuuint64_t)a.K / 64};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.K * 2, 128};
+    const cuuint32_t box[3] = {64, (cuuint32_t)NPAD, (cuuint32_t)C::kKT}, estr[3] = {1, 1, 1};
+    if (enc(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<uint16_t*>(a.x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaErrorInvalidValue;
     Params p;
     p.a = a;
-    p.kt_all = a.K / 64;
     p.ku = q.ku;
     p.ncol = q.ncol;
-    p.items = q.items;
+    p.items = (int)q.items;
     p.whole = q.whole;
+    const int all = (int)(q.whole ? q.items : q.items * q.ku);
+    p.share = all / q.ctas;
+    p.extra = all % q.ctas;
     p.status = status;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -417,10 +421,10 @@ cudaError_t launch(cudaStream_t s, const Int4Args& a, const Plan& q, int* status
     e = cudaLaunchKernelEx(&cfg, int4_wide_kernel<NPAD>, p, map);
     count_launch();
     if (e != cudaSuccess || q.whole) return e;
-    cfg.gridDim = dim3(q.items, (a.N < NPAD ? a.N + 7 : NPAD) / 8);
+    cfg.gridDim = dim3((unsigned)q.items, (a.N < NPAD ? a.N + 7 : NPAD) / 8);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
-    e = cudaLaunchKernelEx(&cfg, int4_join_kernel<NPAD>, p, q.ctas);
+    e = cudaLaunchKernelEx(&cfg, int4_join_kernel<NPAD>, p);
     count_launch();
     return e;
 }
@@ -437,6 +441,7 @@ size_t int4_wide_ws_floats(int M, int N, int K)
 cudaError_t int4_wide_launch(cudaStream_t s, const Int4Args& a, int* status)
 {
     const Plan q = plan_for(a.M, a.N, a.K);
+    if (q.items * q.ku > 0x7fffffff) return cudaErrorInvalidValue;
     switch (q.npad) {
         case 16: return launch<16>(s, a, q, status);
         case 32: return launch<32>(s, a, q, status);

@@ -17,12 +17,11 @@ class Int4Matrix:
     M: int
     K: int
     group: int
-    codes: torch.Tensor    # uint8 [M*K/2] with M rounded up to 128, tiled for the matrix instruction
-    params: torch.Tensor   # float16 [M*K/group, 2] likewise: scale and zero point
+    data: torch.Tensor   # uint8: codes, scales and zero points of 128 x 128 pieces, M and K rounded up to 128
 
     def algorithmic_bytes(self, N):
         """Bytes one linear_int4 must move: codes, scales and zero points, activations, output."""
-        return self.codes.numel() + 2 * self.params.numel() + 2 * self.K * N + 2 * self.M * N
+        return self.data.numel() + 2 * self.K * N + 2 * self.M * N
 
 
 def _shape(M, K, group):
@@ -50,13 +49,11 @@ def pack_int4(codes, scales, zeros, stream=None):
     _need(codes, "codes", torch.uint8, (M, K))
     _need(scales, "scales", torch.float16, (M, K // group), codes.device)
     _need(zeros, "zeros", torch.uint8, (M, K // group), codes.device)
-    rows = -(-M // 128) * 128
-    packed = torch.empty(rows * K // 2, dtype=torch.uint8, device=codes.device)
-    params = torch.empty((rows * (K // group), 2), dtype=torch.float16, device=codes.device)
+    data = torch.empty(_lib.load().spb_int4_bytes(M, K, group), dtype=torch.uint8, device=codes.device)
     with torch.cuda.device(codes.device):
-        _check(_lib.load().spb_int4_pack(_stream_ptr(stream), _ptr(codes), _ptr(scales), _ptr(zeros), M, K, group, _ptr(packed), _ptr(params)),
+        _check(_lib.load().spb_int4_pack(_stream_ptr(stream), _ptr(codes), _ptr(scales), _ptr(zeros), M, K, group, _ptr(data)),
                "spb_int4_pack")
-    return Int4Matrix(M, K, group, packed, params)
+    return Int4Matrix(M, K, group, data)
 
 
 def encode_int4(A, group=128, stream=None):
@@ -75,25 +72,23 @@ def encode_int4(A, group=128, stream=None):
 
 def _check_matrix(W):
     _shape(W.M, W.K, W.group)
-    rows = -(-W.M // 128) * 128
-    _need(W.codes, "W.codes", torch.uint8, (rows * W.K // 2,))
-    _need(W.params, "W.params", torch.float16, (rows * (W.K // W.group), 2), W.codes.device)
+    _need(W.data, "W.data", torch.uint8, (_lib.load().spb_int4_bytes(W.M, W.K, W.group),))
 
 
 def decode_int4(W: Int4Matrix, out=None, stream=None):
     """The dense fp16 matrix [M, K] that W stands for, s (c - z) rounded once."""
     _check_matrix(W)
     if out is None:
-        out = torch.empty((W.M, W.K), dtype=torch.float16, device=W.codes.device)
-    _need(out, "out", torch.float16, (W.M, W.K), W.codes.device)
+        out = torch.empty((W.M, W.K), dtype=torch.float16, device=W.data.device)
+    _need(out, "out", torch.float16, (W.M, W.K), W.data.device)
     with torch.cuda.device(out.device):
-        _check(_lib.load().spb_int4_decode(_stream_ptr(stream), _ptr(W.codes), _ptr(W.params), W.M, W.K, W.group, _ptr(out)), "spb_int4_decode")
+        _check(_lib.load().spb_int4_decode(_stream_ptr(stream), _ptr(W.data), W.M, W.K, W.group, _ptr(out)), "spb_int4_decode")
     return out
 
 
 def int4_workspace(W, N):
     """Bytes of the workspace `linear_int4` needs for N rows (0 for many shapes)."""
-    with torch.cuda.device(W.codes.device):
+    with torch.cuda.device(W.data.device):
         return _lib.load().spb_int4_workspace_bytes(W.M, N, W.K)
 
 
@@ -101,7 +96,7 @@ def linear_int4(W: Int4Matrix, B, bias=None, residual=None, activation=ACT_NONE,
     """spb_linear_int4: out[N,M] = residual + act(B W^T + bias), summed in fp32 and rounded to fp16 once.  B [N,K] as in
     `linear`; out may be the residual itself, not B.  workspace: int4_workspace(W, N) bytes; a new one by default."""
     _check_matrix(W)
-    if not (B.is_cuda and B.dtype == torch.float16 and B.dim() == 2 and B.is_contiguous() and B.shape[1] == W.K and B.device == W.codes.device):
+    if not (B.is_cuda and B.dtype == torch.float16 and B.dim() == 2 and B.is_contiguous() and B.shape[1] == W.K and B.device == W.data.device):
         raise SpmmError("B must be a contiguous CUDA float16 [N,K] tensor on the weight's device")
     N = B.shape[0]
     _check_tail(W.M, N, bias, residual, activation, B.device)
@@ -118,7 +113,7 @@ def linear_int4(W: Int4Matrix, B, bias=None, residual=None, activation=ACT_NONE,
                                       and workspace.numel() * workspace.element_size() >= need):
         raise SpmmError(f"the workspace must be a contiguous CUDA tensor of at least {need} bytes on the weight's device")
     with torch.cuda.device(B.device):
-        code = _lib.load().spb_linear_int4(_stream_ptr(stream), _ptr(W.codes), _ptr(W.params), W.M, W.K, W.group, _ptr(B), _ptr(out), N,
+        code = _lib.load().spb_linear_int4(_stream_ptr(stream), _ptr(W.data), W.M, W.K, W.group, _ptr(B), _ptr(out), N,
                                            _ptr(bias) if bias is not None else ctypes.c_void_p(0),
                                            _ptr(residual) if residual is not None else ctypes.c_void_p(0), int(activation), _ptr(workspace),
                                            workspace.numel() * workspace.element_size() if workspace is not None else 0)
