@@ -27,8 +27,8 @@ using namespace sm100;
 
 constexpr int kGroups = 4;                          // dequantising groups of four warps
 constexpr int kThreads = 32 * (8 + 4 * kGroups);
-constexpr int kABlocks = 8;                         // left-operand blocks in tensor memory, 32 columns (64 k) each
-constexpr int kUnit = 2;                            // k-tiles of a unit
+constexpr int kUnit = 2;                            // k-tiles of a unit: what a group expands per turn and one commit covers
+constexpr int kABlocks = 4;                         // left-operand blocks in tensor memory, one unit (64 columns) each
 
 template <int NPAD> struct Cfg {
     static constexpr int kKT = NPAD <= 64 ? 4 : 2;                       // k-tiles per stage
@@ -155,19 +155,19 @@ __global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_con
             for (int k = 0; k < r.nkt && ok; k += C::kKT) {
                 const int n = min(C::kKT, r.nkt - k);
                 const uint32_t st = stage0 + s * C::kStage;
-                ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * s, round & 1, abort_flag, 4));
-                for (int i = 0; i < n && ok; ++i, ++t) {
+                // the groups only report a unit after the stage's copies have landed, x included
+                for (int i = 0; i < n && ok; i += kUnit, ++t) {
                     const uint32_t blk = t % kABlocks;
-                    ok = __all_sync(0xffffffffu, mbar_wait(ready + 8 * blk, (t / kABlocks) & 1, abort_flag, 4));
+                    ok = __all_sync(0xffffffffu, mbar_wait(ready + 8 * blk, (t / kABlocks) & 1, abort_flag));
                     if (!ok) break;
                     tc_fence_after();
                     if (elect_one()) {
                         const uint64_t b = kmajor_desc(st + i * C::kX);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            tc_mma_ts(tmem + (j % C::kAcc) * NPAD, tmem_a + blk * 32 + 8 * j, b + 2 * j, idesc, k > 0 || i > 0 || j >= C::kAcc);
+                        for (int j = 0; j < 4 * kUnit; ++j)
+                            tc_mma_ts(tmem + (j % C::kAcc) * NPAD, tmem_a + blk * 64 + 8 * j, b + (j / 4) * (C::kX >> 4) + 2 * (j % 4), idesc, k > 0 || i > 0 || j >= C::kAcc);
                         tc_commit(afree + 8 * blk);
-                        if (i == n - 1) tc_commit(empty + 8 * s);
+                        if (i + kUnit >= n) tc_commit(empty + 8 * s);
                     }
                     __syncwarp();
                 }
@@ -191,42 +191,43 @@ __global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_con
             for (int k = 0; k < r.nkt && ok; k += C::kKT) {
                 const int n = min(C::kKT, r.nkt - k);
                 const uint32_t st = stage0 + s * C::kStage + C::kKT * C::kX;
-                bool waited = false;
-                for (int i = 0; i < n && ok; ++i, ++t) {
+                // every stage's copies are waited for, also where the group has no unit: a parity only tells neighbouring phases
+                // apart, so a group that skipped a stage could take the phase before for the one it needs
+                ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * s, round & 1, abort_flag));
+                for (int i = 0; i < n && ok; i += kUnit, ++t) {
                     if ((int)(t % kGroups) != grp) continue;
                     const uint32_t blk = t % kABlocks;
-                    if (!waited) ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * s, round & 1, abort_flag));
-                    waited = true;
-                    if (ok && t >= kABlocks) ok = __all_sync(0xffffffffu, mbar_wait(afree + 8 * blk, (t / kABlocks - 1) & 1, abort_flag));
+                    if (t >= kABlocks) ok = __all_sync(0xffffffffu, mbar_wait(afree + 8 * blk, (t / kABlocks - 1) & 1, abort_flag));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t unit = st + (i / kUnit) * unit_bytes, tile = unit + (i % kUnit) * kInt4CodeBytes + code_off;
-                    const uint32_t par = unit + par_off + (i % kUnit) * grp_tile * 512;
-                    uint32_t pw[2];
-                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(pw[0]) : "r"(par));
-                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(pw[1]) : "r"(par + grp_half * 512));
-                    uint32_t w[4][2];
+                    const uint32_t unit = st + (i / kUnit) * unit_bytes;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[q][0]), "=r"(w[q][1])
-                                     : "r"(tile + 16 * int4_chunk(g, q)));
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const __half2 sz = *reinterpret_cast<__half2*>(&pw[h]);
-                        const __half2 sc = __low2half2(sz), z = __high2half2(sz);
-                        const __half2 zl = __hadd2(z, __half2half2(__ushort_as_half((unsigned short)0x6400)));   // 1024 + z
-                        const __half2 zh = __hadd2(z, __half2half2(__ushort_as_half((unsigned short)0x5400)));   // 64 + z
-                        uint32_t o[16];
+                    for (int kt = 0; kt < kUnit; ++kt) {
+                        const uint32_t tile = unit + kt * kInt4CodeBytes + code_off, par = unit + par_off + kt * grp_tile * 512;
+                        uint32_t pw[2], w[4][2];
+                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(pw[0]) : "r"(par));
+                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(pw[1]) : "r"(par + grp_half * 512));
 #pragma unroll
                         for (int q = 0; q < 4; ++q)
+                            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[q][0]), "=r"(w[q][1]) : "r"(tile + 16 * int4_chunk(g, q)));
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {   // k = 8 q + 2 e, + 1
-                                const uint32_t u = e & 1 ? w[q][h] >> 8 : w[q][h];
-                                const uint32_t v = e < 2 ? (u & 0x000f000fu) | 0x64006400u : (u & 0x00f000f0u) | 0x54005400u;
-                                const __half2 c = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&v), e < 2 ? zl : zh), sc);
-                                o[4 * q + e] = *reinterpret_cast<const uint32_t*>(&c);
-                            }
-                        tc_st16(tmem_a + blk * 32 + 16 * h + ((uint32_t)quad << 21), o);
+                        for (int h = 0; h < 2; ++h) {
+                            const __half2 sz = *reinterpret_cast<__half2*>(&pw[h]);
+                            const __half2 sc = __low2half2(sz), z = __high2half2(sz);
+                            const __half2 zl = __hadd2(z, __half2half2(__ushort_as_half((unsigned short)0x6400)));   // 1024 + z
+                            const __half2 zh = __hadd2(z, __half2half2(__ushort_as_half((unsigned short)0x5400)));   // 64 + z
+                            uint32_t o[16];
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {   // k = 8 q + 2 e, + 1
+                                    const uint32_t u = e & 1 ? w[q][h] >> 8 : w[q][h];
+                                    const uint32_t v = e < 2 ? (u & 0x000f000fu) | 0x64006400u : (u & 0x00f000f0u) | 0x54005400u;
+                                    const __half2 c = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&v), e < 2 ? zl : zh), sc);
+                                    o[4 * q + e] = *reinterpret_cast<const uint32_t*>(&c);
+                                }
+                            tc_st16(tmem_a + blk * 64 + 32 * kt + 16 * h + ((uint32_t)quad << 21), o);
+                        }
                     }
                     tc_wait_st();
                     tc_fence_before();
