@@ -34,7 +34,7 @@ size_t int4_wide_ws_floats(int M, int N, int K);
 __host__ __device__ __forceinline__ int int4_chunk(int g, int t) { return 4 * g + (t ^ (g >> 1)); }
 
 constexpr int kInt4CodeBytes = 128 * 64 / 2;   // codes of one 64-k tile of 128 rows
-__host__ __device__ __forceinline__ int int4_unit_bytes(int group) { return 2 * kInt4CodeBytes + 512 * (128 / group); }
+__host__ __device__ constexpr int int4_unit_bytes(int group) { return 2 * kInt4CodeBytes + 512 * (128 / group); }
 __host__ __device__ __forceinline__ long long int4_units(int M, int K) { return (long long)((M + 127) / 128) * ((K + 127) / 128); }
 __host__ __device__ __forceinline__ int int4_nibble(int r)   // nibble of k = r (0..7) in the word of its lane
 {

@@ -25,19 +25,22 @@ namespace spb {
 namespace {
 using namespace sm100;
 
-constexpr int kGroups = 4;                          // dequantising groups of four warps
-constexpr int kThreads = 32 * (8 + 4 * kGroups);
 constexpr int kUnit = 2;                            // k-tiles of a unit: what a group expands per turn and one commit covers
-constexpr int kABlocks = 4;                         // left-operand blocks in tensor memory, one unit (64 columns) each
 
 template <int NPAD> struct Cfg {
+    static constexpr int kGroups = 4;                                    // dequantising groups of four warps
+    static constexpr int kThreads = 32 * (8 + 4 * kGroups);
+    static constexpr int kABlocks = kGroups;                             // left-operand blocks in tensor memory, one unit (64 columns) per group
     static constexpr int kKT = NPAD <= 64 ? 4 : 2;                       // k-tiles per stage
+    static constexpr int kUS = kKT / kUnit;                              // units per stage: groups share out kTurn stages
+    static constexpr int kTurn = kGroups / kUS;
     static constexpr int kAcc = NPAD <= 32 ? 4 : NPAD <= 64 ? 2 : 1;     // accumulators the k-steps take in turn (short ones are latency)
     static constexpr uint32_t kX = NPAD * 128;                           // bytes of x per k-tile
     static constexpr uint32_t kStage = kKT * kX + kKT / kUnit * (2 * kInt4CodeBytes + 4 * 512);   // x, units (at most four groups)
     static constexpr int kStages = (int)((222u * 1024) / kStage) < 8 ? (int)((222u * 1024) / kStage) : 8;
     static constexpr uint32_t kSmem = 1024 + 1024 + kStages * kStage;    // header, alignment
-    static constexpr uint32_t kTmemCols = 512;
+    static constexpr uint32_t kTmemCols = 512, kTmemA = 512 - 64 * kABlocks;   // accumulators from 0, operand blocks at the end
+    static_assert(kAcc * NPAD <= (int)kTmemA, "accumulators and operand blocks overlap");
 };
 
 struct Params {
@@ -88,8 +91,8 @@ struct Walk {
     }
 };
 
-template <int NPAD>
-__global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap xmap)
+template <int NPAD, int kGroup>
+__global__ void __launch_bounds__(Cfg<NPAD>::kThreads, 1) int4_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap xmap)
 {
     using C = Cfg<NPAD>;
     extern __shared__ uint8_t raw[];
@@ -104,7 +107,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_con
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::kStages; ++i) mbar_init(full + 8 * i, 2), mbar_init(empty + 8 * i, 1);
-        for (int i = 0; i < kABlocks; ++i) mbar_init(ready + 8 * i, 4), mbar_init(afree + 8 * i, 1);
+        for (int i = 0; i < C::kABlocks; ++i) mbar_init(ready + 8 * i, 4), mbar_init(afree + 8 * i, 1);
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, 4);
         *abort_flag = 0;
@@ -114,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *holder, tmem_a = tmem + 256;
+    constexpr uint32_t tmem = 0, tmem_a = C::kTmemA;   // all columns: the allocation starts at 0
     grid_wait();      // x, residual, out and the workspace belong to what ran before
     grid_release();   // the join may be set up while this kernel runs; it waits for its end
 
@@ -122,12 +125,12 @@ __global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_con
     Run r;
     if (warp == 0 || warp == 2) {
         // ---- copies
-        const int unit_bytes = int4_unit_bytes(p.a.group);
+        constexpr int unit_bytes = int4_unit_bytes(kGroup);
         uint32_t s = 0, round = 0;
         bool ok = true;
         while (ok && walk.next<NPAD>(p, r)) {
             for (int k = 0; k < r.nkt && ok; k += C::kKT) {
-                if (round) ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, (round - 1) & 1, abort_flag));
+                if (round) ok = mbar_wait(empty + 8 * s, (round - 1) & 1, abort_flag);
                 if (!ok) break;
                 if (elect_one()) {
                     const int u = r.u0 + k / kUnit, n = min(C::kKT, r.nkt - k) / kUnit;
@@ -147,31 +150,37 @@ __global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_con
     } else if (warp == 1) {
         // ---- matrix instructions
         constexpr uint32_t idesc = f16_idesc(128, NPAD);
-        uint32_t s = 0, round = 0, t = 0, item = 0;
+        uint32_t s = 0, turn = 0, item = 0, phase = 0;   // phase: bit b, parity of operand block b's next use
         bool ok = true;
         while (ok && walk.next<NPAD>(p, r)) {
-            if (item) ok = __all_sync(0xffffffffu, mbar_wait(acc_empty, (item - 1) & 1, abort_flag, 4));
+            if (item) ok = mbar_wait(acc_empty, (item - 1) & 1, abort_flag, 4);
             tc_fence_after();
             for (int k = 0; k < r.nkt && ok; k += C::kKT) {
-                const int n = min(C::kKT, r.nkt - k);
-                const uint32_t st = stage0 + s * C::kStage;
                 // the groups only report a unit after the stage's copies have landed, x included
-                for (int i = 0; i < n && ok; i += kUnit, ++t) {
-                    const uint32_t blk = t % kABlocks;
-                    ok = __all_sync(0xffffffffu, mbar_wait(ready + 8 * blk, (t / kABlocks) & 1, abort_flag));
+#pragma unroll
+                for (int i = 0; i < C::kUS; ++i) {
+                    if (k + i * kUnit >= r.nkt || !ok) break;
+                    const uint32_t blk = turn * C::kUS + i;
+                    ok = mbar_wait(ready + 8 * blk, phase >> blk & 1, abort_flag);
                     if (!ok) break;
+                    phase ^= 1u << blk;
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint64_t b = kmajor_desc(st + i * C::kX);
+                        const uint32_t b = kmajor_desc_low(stage0 + s * C::kStage + i * kUnit * C::kX), more = k > 0 || i > 0;
 #pragma unroll
-                        for (int j = 0; j < 4 * kUnit; ++j)
-                            tc_mma_ts(tmem + (j % C::kAcc) * NPAD, tmem_a + blk * 64 + 8 * j, b + (j / 4) * (C::kX >> 4) + 2 * (j % 4), idesc, k > 0 || i > 0 || j >= C::kAcc);
+                        for (int c = 0; c < C::kTurn; ++c)   // the block as a constant: see tc_mma_ts
+                            if (turn == c)
+#pragma unroll
+                                for (int j = 0; j < 4 * kUnit; ++j)
+                                    tc_mma_ts(j % C::kAcc * NPAD, C::kTmemA + (c * C::kUS + i) * 64 + 8 * j, b + (j / 4) * (C::kX >> 4) + 2 * (j % 4), kKMajorDescHigh,
+                                              idesc, j >= C::kAcc ? 1u : more);
                         tc_commit(afree + 8 * blk);
-                        if (i + kUnit >= n) tc_commit(empty + 8 * s);
+                        if (i + 1 == C::kUS || k + (i + 1) * kUnit >= r.nkt) tc_commit(empty + 8 * s);
                     }
                     __syncwarp();
                 }
-                if (++s == (uint32_t)C::kStages) s = 0, ++round;
+                if (++s == (uint32_t)C::kStages) s = 0;
+                if (++turn == (uint32_t)C::kTurn) turn = 0;
             }
             if (ok && elect_one()) tc_commit(acc_full);
             __syncwarp();
@@ -179,62 +188,67 @@ __global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_con
         }
     } else if (warp >= 8) {
         // ---- codes to fp16, thread = row
+        // the units of kTurn consecutive stages go to the groups in order; group's operand block: its own
         const int grp = (warp - 8) / 4, quad = warp & 3, g = lane % 8, high8 = lane / 8 & 1;
-        const uint32_t code_off = (2 * quad + lane / 16) * 512 + high8 * 8;
-        const uint32_t par_off = 2 * kInt4CodeBytes + 4 * (32 * quad + lane);
-        const uint32_t unit_bytes = int4_unit_bytes(p.a.group);
-        // parameters of the two 32-k halves of k-tile 0 and 1 of a unit: which of its groups
-        const int grp_tile = p.a.group == 128 ? 0 : p.a.group == 64 ? 1 : 2, grp_half = p.a.group == 32 ? 1 : 0;
-        uint32_t s = 0, round = 0, t = 0;
+        const int my_turn = grp / C::kUS, my_unit = grp % C::kUS;
+        constexpr uint32_t unit_bytes = int4_unit_bytes(kGroup);
+        const uint32_t code_off = C::kKT * C::kX + my_unit * unit_bytes + (2 * quad + lane / 16) * 512 + high8 * 8;
+        const uint32_t par_off = C::kKT * C::kX + my_unit * unit_bytes + 2 * kInt4CodeBytes + 4 * (32 * quad + lane);
+        const uint32_t a_addr = tmem_a + grp * 64 + ((uint32_t)quad << 21);
+        uint32_t mask_low, mask_high, bits_low, bits_high;   // kept in registers for and_or
+        asm volatile("mov.b32 %0, 0x000f000f;\n\tmov.b32 %1, 0x00f000f0;\n\tmov.b32 %2, 0x64006400;\n\tmov.b32 %3, 0x54005400;"
+                     : "=r"(mask_low), "=r"(mask_high), "=r"(bits_low), "=r"(bits_high));
+        uint32_t s = 0, round = 0, used = 0;
+        int turn = 0;
         bool ok = true;
         while (ok && walk.next<NPAD>(p, r)) {
             for (int k = 0; k < r.nkt && ok; k += C::kKT) {
-                const int n = min(C::kKT, r.nkt - k);
-                const uint32_t st = stage0 + s * C::kStage + C::kKT * C::kX;
                 // every stage's copies are waited for, also where the group has no unit: a parity only tells neighbouring phases
                 // apart, so a group that skipped a stage could take the phase before for the one it needs
-                ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * s, round & 1, abort_flag));
-                for (int i = 0; i < n && ok; i += kUnit, ++t) {
-                    if ((int)(t % kGroups) != grp) continue;
-                    const uint32_t blk = t % kABlocks;
-                    if (t >= kABlocks) ok = __all_sync(0xffffffffu, mbar_wait(afree + 8 * blk, (t / kABlocks - 1) & 1, abort_flag));
+                ok = mbar_wait(full + 8 * s, round & 1, abort_flag);
+                if (ok && turn == my_turn && k + my_unit * kUnit < r.nkt) {
+                    if (used) ok = mbar_wait(afree + 8 * grp, (used - 1) & 1, abort_flag);
+                    ++used;
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t unit = st + (i / kUnit) * unit_bytes;
+                    const uint32_t st = stage0 + s * C::kStage;
+                    uint32_t pw = 0;
+                    __half2 sc, zl, zh;
+                    uint32_t w[4][2];
 #pragma unroll
-                    for (int kt = 0; kt < kUnit; ++kt) {
-                        const uint32_t tile = unit + kt * kInt4CodeBytes + code_off, par = unit + par_off + kt * grp_tile * 512;
-                        uint32_t pw[2], w[4][2];
-                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(pw[0]) : "r"(par));
-                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(pw[1]) : "r"(par + grp_half * 512));
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[q][0]), "=r"(w[q][1]) : "r"(tile + 16 * int4_chunk(g, q)));
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const __half2 sz = *reinterpret_cast<__half2*>(&pw[h]);
-                            const __half2 sc = __low2half2(sz), z = __high2half2(sz);
-                            const __half2 zl = __hadd2(z, __half2half2(__ushort_as_half((unsigned short)0x6400)));   // 1024 + z
-                            const __half2 zh = __hadd2(z, __half2half2(__ushort_as_half((unsigned short)0x5400)));   // 64 + z
-                            uint32_t o[16];
+                    for (int h = 0; h < 2 * kUnit; ++h) {   // 32 k each
+                        if (h * 32 % kGroup == 0) {
+                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(pw) : "r"(st + par_off + h * 32 / kGroup * 512));
+                            const __half2 sz = *reinterpret_cast<__half2*>(&pw), z = __high2half2(sz);
+                            sc = __low2half2(sz);
+                            zl = __hadd2(z, *reinterpret_cast<__half2*>(&bits_low));     // 1024 + z
+                            zh = __hadd2(z, *reinterpret_cast<__half2*>(&bits_high));    // 64 + z
+                        }
+                        if (h % 2 == 0) {
 #pragma unroll
                             for (int q = 0; q < 4; ++q)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {   // k = 8 q + 2 e, + 1
-                                    const uint32_t u = e & 1 ? w[q][h] >> 8 : w[q][h];
-                                    const uint32_t v = e < 2 ? (u & 0x000f000fu) | 0x64006400u : (u & 0x00f000f0u) | 0x54005400u;
-                                    const __half2 c = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&v), e < 2 ? zl : zh), sc);
-                                    o[4 * q + e] = *reinterpret_cast<const uint32_t*>(&c);
-                                }
-                            tc_st16(tmem_a + blk * 64 + 32 * kt + 16 * h + ((uint32_t)quad << 21), o);
+                                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[q][0]), "=r"(w[q][1])
+                                             : "r"(st + code_off + h / 2 * kInt4CodeBytes + 16 * int4_chunk(g, q)));
                         }
+                        uint32_t o[16];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {   // k = 8 q + 2 e, + 1
+                                const uint32_t u = e & 1 ? w[q][h % 2] >> 8 : w[q][h % 2];
+                                const uint32_t v = e < 2 ? and_or(u, mask_low, bits_low) : and_or(u, mask_high, bits_high);
+                                const __half2 c = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&v), e < 2 ? zl : zh), sc);
+                                o[4 * q + e] = *reinterpret_cast<const uint32_t*>(&c);
+                            }
+                        tc_st16(a_addr + 16 * h, o);
                     }
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(ready + 8 * blk);
+                    if (lane == 0) mbar_arrive(ready + 8 * grp);
                 }
                 if (++s == (uint32_t)C::kStages) s = 0, ++round;
+                if (++turn == C::kTurn) turn = 0;
             }
         }
     } else if (warp >= 4) {
@@ -243,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_con
         uint32_t item = 0;
         bool ok = true;
         while (ok && walk.next<NPAD>(p, r)) {
-            ok = __all_sync(0xffffffffu, mbar_wait(acc_full, item & 1, abort_flag, 4));
+            ok = mbar_wait(acc_full, item & 1, abort_flag, 4);
             if (!ok) break;
             tc_fence_after();
             const bool cut = !(r.first && r.last);
@@ -295,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_wide_kernel(const __grid_con
         }
         __syncthreads();
     }
-    if (warp == 1) tc_dealloc(tmem, C::kTmemCols);
+    if (warp == 1) tc_dealloc(*holder, C::kTmemCols);
 }
 
 // Adds the partial sums of the items that were cut; blockIdx.x: item, blockIdx.y: columns by 8.
@@ -375,7 +389,7 @@ Plan plan_for(int M, int N, int K)
     return q;
 }
 
-template <int NPAD>
+template <int NPAD, int kGroup>
 cudaError_t launch(cudaStream_t s, const Int4Args& a, const Plan& q, int* status)
 {
     using C = Cfg<NPAD>;
@@ -385,7 +399,7 @@ cudaError_t launch(cudaStream_t s, const Int4Args& a, const Plan& q, int* status
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!prepared[dev]) {
-        e = cudaFuncSetAttribute(int4_wide_kernel<NPAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
+        e = cudaFuncSetAttribute(int4_wide_kernel<NPAD, kGroup>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
         if (e != cudaSuccess) return e;
         prepared[dev] = true;
     }
@@ -414,12 +428,12 @@ cudaError_t launch(cudaStream_t s, const Int4Args& a, const Plan& q, int* status
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(q.ctas);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(C::kThreads);
     cfg.dynamicSmemBytes = C::kSmem;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, int4_wide_kernel<NPAD>, p, map);
+    e = cudaLaunchKernelEx(&cfg, int4_wide_kernel<NPAD, kGroup>, p, map);
     count_launch();
     if (e != cudaSuccess || q.whole) return e;
     cfg.gridDim = dim3((unsigned)q.items, (a.N < NPAD ? a.N + 7 : NPAD) / 8);
@@ -428,6 +442,18 @@ cudaError_t launch(cudaStream_t s, const Int4Args& a, const Plan& q, int* status
     e = cudaLaunchKernelEx(&cfg, int4_join_kernel<NPAD>, p);
     count_launch();
     return e;
+}
+
+template <int kGroup>
+cudaError_t launch_group(cudaStream_t s, const Int4Args& a, const Plan& q, int* status)
+{
+    switch (q.npad) {
+        case 16: return launch<16, kGroup>(s, a, q, status);
+        case 32: return launch<32, kGroup>(s, a, q, status);
+        case 64: return launch<64, kGroup>(s, a, q, status);
+        case 128: return launch<128, kGroup>(s, a, q, status);
+        default: return launch<256, kGroup>(s, a, q, status);
+    }
 }
 
 }  // namespace
@@ -443,13 +469,7 @@ cudaError_t int4_wide_launch(cudaStream_t s, const Int4Args& a, int* status)
 {
     const Plan q = plan_for(a.M, a.N, a.K);
     if (q.items * q.ku > 0x7fffffff) return cudaErrorInvalidValue;
-    switch (q.npad) {
-        case 16: return launch<16>(s, a, q, status);
-        case 32: return launch<32>(s, a, q, status);
-        case 64: return launch<64>(s, a, q, status);
-        case 128: return launch<128>(s, a, q, status);
-        default: return launch<256>(s, a, q, status);
-    }
+    return a.group == 128 ? launch_group<128>(s, a, q, status) : a.group == 64 ? launch_group<64>(s, a, q, status) : launch_group<32>(s, a, q, status);
 }
 
 }  // namespace spb

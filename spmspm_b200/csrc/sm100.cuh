@@ -6,7 +6,7 @@
 namespace spb {
 namespace sm100 {
 
-constexpr uint32_t kSpinLimit = 1u << 22;   // polls before a wait gives up
+constexpr uint32_t kSpinLimit = 1u << 21;   // polls before a wait gives up
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count)
@@ -29,14 +29,15 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity)
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-// Bounded wait; false, with *abort_flag raised, when the limit is reached or another thread has already given up.  quick: polls
-// before the thread starts to sleep between them.
+// Bounded wait of a whole warp, all lanes with the same answer; false, with *abort_flag raised, when the limit is reached or
+// another warp has already given up.  quick: polls before the warp starts to sleep between them.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t quick = 64)
 {
+    if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
     for (uint32_t i = 0; i < kSpinLimit; ++i) {
-        if (mbar_try(bar, parity)) return true;
+        if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
         if (i > quick) {
-            if (*abort_flag) return false;
+            if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
             __nanosleep(40);
         }
     }
@@ -77,17 +78,14 @@ __device__ __forceinline__ void tc_commit(uint32_t bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-// D[tensor memory] (+)= A[tensor memory] B[shared], kind::f16, one elected thread
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+// D[tensor memory] (+)= A[tensor memory] B[shared], kind::f16, one elected thread.  Issuing costs 12 cycles when the operands are
+// constants and 45 to 90 when they have to be moved to uniform registers first, which for few columns is more than the product
+// takes: d, a and idesc should be compile-time constants (an allocation of all 512 columns starts at 0), and of the descriptor only
+// the low word varies.
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b_low, uint32_t b_high, uint32_t idesc, uint32_t accumulate)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-                 "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-// D[tensor memory] (+)= A[shared] B[shared]
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
-{
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d), "r"(a), "r"(b_low), "r"(b_high), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -106,14 +104,20 @@ __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t (&r)[16])
 }
 // Descriptor of a 128-byte-swizzled shared-memory tile whose rows are 64 fp16 (128 bytes) along the contraction, 8-row groups
 // 1024 bytes apart; the tile starts on a 1024-byte boundary, a k-step of 16 is 2 further in the descriptor.
-__device__ __forceinline__ uint64_t kmajor_desc(uint32_t addr)
-{
-    return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
+__device__ __forceinline__ uint32_t kmajor_desc_low(uint32_t addr) { return (addr & 0x3ffffu) >> 4 | 1u << 16; }
+constexpr uint32_t kKMajorDescHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
 // fp16 x fp16 -> fp32, both operands K-major
 __host__ __device__ constexpr uint32_t f16_idesc(int m, int n)
 {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// (x & mask) | bits in one instruction; mask and bits in registers
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits)
+{
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+    return y;
 }
 
 }  // namespace sm100
