@@ -325,8 +325,8 @@ int spb_linear_allreduce_finish(void* stream, uint16_t* C, const uint16_t* parts
  *                    very end (unlike spb_linear_bitmap_v3, which rounds after every step as the kernels it replaces do).
  *                    bias, residual: as there, or NULL; residual may be out itself.  workspace:
  *                    spb_int4_workspace_bytes bytes (0 for many shapes, NULL then), 16-byte aligned, need not be cleared;
- *                    not shared by calls that may run at the same time.  With more than 8 rows of x the product takes
- *                    the weights as spb_int4_decode returns them (rounded to fp16), with up to 8 unrounded.
+ *                    not shared by calls that may run at the same time.  With more than 16 rows of x the product takes
+ *                    the weights as spb_int4_decode returns them (rounded to fp16), with up to 16 unrounded.
  */
 size_t spb_int4_bytes(int M, int K, int group);
 size_t spb_int4_workspace_bytes(int M, int N, int K);

@@ -28,9 +28,10 @@ struct Int4Args {
     float* ws;                  // partial sums of tiles that are cut between thread blocks
     size_t ws_floats;
 };
-constexpr int kInt4SmallRows = 8;   // up to this many rows of x the mma.sync kernel runs, above it the tcgen05 one
+constexpr int kInt4StreamRows = 16;   // up to this many rows of x the mma.sync kernel runs, above it the tcgen05 one
+cudaError_t int4_stream_launch(cudaStream_t s, const Int4Args& a, int* status);
 cudaError_t int4_wide_launch(cudaStream_t s, const Int4Args& a, int* status);
-size_t int4_wide_ws_floats(int M, int N, int K);
+size_t int4_ws_floats(int M, int N, int K);
 __host__ __device__ __forceinline__ int int4_chunk(int g, int t) { return 4 * g + (t ^ (g >> 1)); }
 
 constexpr int kInt4CodeBytes = 128 * 64 / 2;   // codes of one 64-k tile of 128 rows

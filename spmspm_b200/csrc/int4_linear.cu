@@ -1,177 +1,9 @@
-// Linear layer over 4-bit weights (layout: int4.cuh) for few rows of x, and the kernels that bring weights into the layout.
-//
-//   y[n][m] = residual + act(bias + sum over groups of s (sum_k c x - z sum_k x))      summed in fp32, rounded once
-//
-// int4_small_kernel: bound by the bytes of the codes while N is small.  The codes enter mma.sync.m16n8k16 as they are: a
-// nibble masked out of its word is an fp16 subnormal, c 2^-24 (low nibble of a byte) or c 2^-20 (high), multiplied
-// exactly, so unpacking costs 1.25 instructions per two weights; low and high nibbles are summed apart, and scale and zero
-// point are applied to the fp32 sums of a group, with sum_k x from one more matrix instruction on ones.  No weight is
-// rounded.  The warps of a thread block, and the thread blocks of a cluster, share out K; partial sums meet in shared
-// memory, in a fixed order.  Codes and x go from memory to registers with 16-byte loads, kDepth units ahead.
+// 4-bit weights (layout: int4.cuh): bringing them into the layout and back, and the entry point of the linear layer over them.
 #include "../../include/spmm_b200.h"
 #include "int4.cuh"
-#include <cooperative_groups.h>
-
-namespace cg = cooperative_groups;
 
 namespace spb {
 namespace {
-
-constexpr int kWarps = 8;
-
-__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
-{
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint4 load_stream(const uint4* p)
-{
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-
-// RT row tiles of 16, NT column tiles of 8 rows of x per warp.
-template <int RT, int NT, int kGroup>
-__global__ void __launch_bounds__(32 * kWarps) int4_small_kernel(Int4Args a)
-{
-    constexpr int kDepth = RT == 1 ? 3 : 2;          // units whose codes and parameters are on their way
-    constexpr int kPer = 128 / kGroup;               // groups per unit
-    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, t = lane % 4;
-    const int ku = (a.K + 127) / 128, rt_all = a.M / 16, kt_all = a.K / 64;
-    const int parts = gridDim.y * kWarps, part = blockIdx.y * kWarps + warp;
-    const int u0 = (int)((long long)ku * part / parts), u1 = (int)((long long)ku * (part + 1) / parts);
-    const int rt0 = blockIdx.x * RT, n0 = blockIdx.z * 8 * NT;
-
-    const uint8_t* unit[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-        const int rt = min(rt0 + r, rt_all - 1);   // past the end: a row tile that is there, its result is not stored
-        unit[r] = a.units + (long long)(rt / 8) * ku * int4_unit_bytes(kGroup) + rt % 8 * 512;
-    }
-    const uint16_t* xr[NT];
-    bool have[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        have[nt] = n0 + nt * 8 + g < a.N;
-        xr[nt] = a.x + (long long)(have[nt] ? n0 + nt * 8 + g : 0) * a.K + 8 * t;
-    }
-    float out[RT][NT][4] = {};
-    float low[RT][NT][4] = {}, high[RT][NT][4] = {}, xsum[NT][4] = {};
-    uint4 w[kDepth][RT][2], xv[kDepth][NT][4];
-    __half2 par[kDepth][RT][kPer][2];
-    auto fetch = [&](int slot, int u) {
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            const uint8_t* p = unit[r] + (long long)u * int4_unit_bytes(kGroup);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) w[slot][r][i] = load_stream(reinterpret_cast<const uint4*>(p + i * kInt4CodeBytes) + int4_chunk(g, t));
-            const __half2* q = reinterpret_cast<const __half2*>(p - (rt0 + r < rt_all ? (rt0 + r) % 8 : (rt_all - 1) % 8) * 512 + 2 * kInt4CodeBytes) +
-                               (rt0 + r < rt_all ? (rt0 + r) % 8 : (rt_all - 1) % 8) * 16 + g;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) par[slot][r][i][0] = q[i * 128], par[slot][r][i][1] = q[i * 128 + 8];
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int h = 0; h < 4; ++h)
-                xv[slot][nt][h] = have[nt] && 2 * u + h / 2 < kt_all ? *reinterpret_cast<const uint4*>(xr[nt] + u * 128 + 32 * h) : make_uint4(0, 0, 0, 0);
-    };
-    auto apply = [&](const __half2 (&pv)[RT][kPer][2], int grp) {   // a group is complete: scale and zero point
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            const float2 p0 = __half22float2(pv[r][grp][0]), p1 = __half22float2(pv[r][grp][1]);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float dot = fmaf(low[r][nt][i], 16.f, high[r][nt][i]) * 1048576.f;
-                    const float2 p = i < 2 ? p0 : p1;
-                    out[r][nt][i] = fmaf(p.x, fmaf(-p.y, xsum[nt][i & 1], dot), out[r][nt][i]);
-                    low[r][nt][i] = high[r][nt][i] = 0.f;
-                }
-            }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) xsum[nt][0] = xsum[nt][1] = xsum[nt][2] = xsum[nt][3] = 0.f;
-    };
-    auto step = [&](const uint4 (&wv)[RT][2], const uint4 (&xw)[NT][4], const __half2 (&pv)[RT][kPer][2]) {
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {   // 32 k each
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                mma(xsum[nt], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, xw[nt][h].x, xw[nt][h].y);
-                mma(xsum[nt], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, xw[nt][h].z, xw[nt][h].w);
-            }
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const uint4 c = wv[r][h / 2];
-                const uint32_t u = h & 1 ? c.y : c.x, v = h & 1 ? c.w : c.z;
-                const uint32_t us = u >> 8, vs = v >> 8;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    mma(low[r][nt], u & 0x000f000fu, v & 0x000f000fu, us & 0x000f000fu, vs & 0x000f000fu, xw[nt][h].x, xw[nt][h].y);
-                    mma(high[r][nt], u & 0x00f000f0u, v & 0x00f000f0u, us & 0x00f000f0u, vs & 0x00f000f0u, xw[nt][h].z, xw[nt][h].w);
-                }
-            }
-            if ((h + 1) * 32 % kGroup == 0) apply(pv, h * 32 / kGroup);
-        }
-    };
-#pragma unroll
-    for (int i = 0; i < kDepth; ++i)
-        if (u0 + i < u1) fetch(i, u0 + i);
-    int u = u0;
-    for (; u + kDepth <= u1; u += kDepth) {
-#pragma unroll
-        for (int i = 0; i < kDepth; ++i) {
-            step(w[i], xv[i], par[i]);
-            if (u + i + kDepth < u1) fetch(i, u + i + kDepth);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < kDepth; ++i)
-        if (u + i < u1) step(w[i], xv[i], par[i]);
-
-    // sums of the warps, then of the cluster's thread blocks (blockIdx.y), in order
-    __shared__ float part_sum[kWarps][RT * NT * 4][32];
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) part_sum[warp][(r * NT + nt) * 4 + i][lane] = out[r][nt][i];
-    __syncthreads();
-    constexpr int kVals = RT * NT * 4 * 32;
-    float* flat = &part_sum[0][0][0];
-    for (int v = threadIdx.x; v < kVals; v += 32 * kWarps) {
-        float sum = flat[v];
-#pragma unroll
-        for (int i = 1; i < kWarps; ++i) sum += flat[i * kVals + v];
-        flat[v] = sum;
-    }
-    auto store = [&](int v, float y) {
-        const int l = v & 31, i = (v >> 5) & 3, nt = (v >> 7) % NT, r = (v >> 7) / NT;
-        const int m = (rt0 + r) * 16 + l / 4 + 8 * (i >> 1), n = n0 + nt * 8 + 2 * (l & 3) + (i & 1);
-        if (rt0 + r >= rt_all || n >= a.N) return;
-        if (a.bias) y += __half2float(__ushort_as_half(a.bias[m]));
-        if (a.activation) y = y < 0.f ? 0.f : y;   // NaN stays NaN
-        if (a.residual) y += __half2float(__ushort_as_half(a.residual[(long long)n * a.M + m]));
-        a.out[(long long)n * a.M + m] = __half_as_ushort(__float2half_rn(y));
-    };
-    if (gridDim.y == 1) {
-        for (int v = threadIdx.x; v < kVals; v += 32 * kWarps) store(v, flat[v]);
-        return;
-    }
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    const int ranks = gridDim.y, rank = blockIdx.y;
-    for (int v = rank * (32 * kWarps) + threadIdx.x; v < kVals; v += ranks * 32 * kWarps) {
-        float sum = 0.f;
-        for (int i = 0; i < ranks; ++i) sum += *cluster.map_shared_rank(flat + v, i);
-        store(v, sum);
-    }
-    cluster.sync();   // nobody leaves while its sums are being read
-}
 
 // Word i of the codes (eight codes of one row): its place in the units, its row and first k.
 __device__ __forceinline__ long long word_place(int K, int group, long long i, long long& row, long long& k)
@@ -265,44 +97,6 @@ __global__ void int4_encode_kernel(const uint16_t* dense, uint8_t* codes, uint16
     }
 }
 
-int sm_count()
-{
-    static int n[64] = {};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-    if (!n[dev] && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-    return n[dev];
-}
-
-template <int RT, int NT, int kGroup>
-cudaError_t launch_small(cudaStream_t s, const Int4Args& a)
-{
-    const int gx = (a.M / 16 + RT - 1) / RT, gz = (a.N + 8 * NT - 1) / (8 * NT);
-    // thread blocks that share K: enough to put about two on every SM, at least two 128-k steps for every warp
-    int split = 1;
-    while (split < 8 && (long long)gx * gz * split < 2 * sm_count() && a.K / 128 >= 2 * kWarps * 2 * split) split *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(gx, split, gz);
-    cfg.blockDim = dim3(32 * kWarps);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1;
-    attr[0].val.clusterDim.y = split;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, int4_small_kernel<RT, NT, kGroup>, a);
-    count_launch();
-    return e;
-}
-template <int kGroup>
-cudaError_t launch_group(cudaStream_t s, const Int4Args& a)
-{
-    const bool many = a.M / 16 >= 8 * sm_count();   // rows enough to fill the device with four row tiles a warp
-    return many ? launch_small<4, 1, kGroup>(s, a) : launch_small<1, 1, kGroup>(s, a);
-}
-
 bool check_weight(const char* who, int M, int K, int group)
 {
     if (M <= 0 || K <= 0 || M % 64 || K % 64) {
@@ -319,11 +113,6 @@ unsigned blocks(long long items, int per) { return (unsigned)((items + per - 1) 
 
 }  // namespace
 
-static cudaError_t int4_small_launch(cudaStream_t s, const Int4Args& a)
-{
-    return a.group == 128 ? launch_group<128>(s, a) : a.group == 64 ? launch_group<64>(s, a) : launch_group<32>(s, a);
-}
-
 }  // namespace spb
 
 extern "C" {
@@ -333,7 +122,7 @@ size_t spb_int4_bytes(int M, int K, int group)
     if (M <= 0 || K <= 0 || M % 64 || K % 64 || (group != 32 && group != 64 && group != 128) || K % group) return 0;
     return (size_t)spb::int4_units(M, K) * spb::int4_unit_bytes(group);
 }
-size_t spb_int4_workspace_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? 4 * spb::int4_wide_ws_floats(M, N, K) : 0; }
+size_t spb_int4_workspace_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? 4 * spb::int4_ws_floats(M, N, K) : 0; }
 
 int spb_int4_pack(void* stream, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int M, int K, int group, void* packed)
 {
@@ -411,7 +200,7 @@ int spb_linear_int4(void* stream, const void* packed, int M, int K, int group, c
     a.x = x, a.bias = bias, a.residual = residual, a.out = out;
     a.N = N, a.activation = activation;
     a.ws = (float*)workspace, a.ws_floats = workspace_bytes / 4;
-    e = N <= kInt4SmallRows ? int4_small_launch((cudaStream_t)stream, a) : int4_wide_launch((cudaStream_t)stream, a, status);
+    e = N <= kInt4StreamRows ? int4_stream_launch((cudaStream_t)stream, a, status) : int4_wide_launch((cudaStream_t)stream, a, status);
     if (e != cudaSuccess) set_error("linear_int4: %s", cudaGetErrorString(e));
     return (int)e;
 }

@@ -1,8 +1,8 @@
-// Linear layer over 4-bit weights (layout: int4.cuh) for more than a few rows of x, on tcgen05:
+// Linear layer over 4-bit weights (layout: int4.cuh) for more than 16 rows of x, on tcgen05:
 //
 //   out[n][m] = residual + act(bias + sum_k w[m][k] x[n][k]),   w = s (c - z) rounded to fp16 (the value int4_decode returns)
 //
-// Rows of W are the 128-row side of the matrix instruction, rows of x its 16..256-column side.  Codes become fp16 on the way
+// Rows of W are the 128-row side of the matrix instruction, rows of x its 32..256-column side.  Codes become fp16 on the way
 // into tensor memory, where the instruction takes its left operand from; x comes as 128-byte-swizzled tiles by tensor copies.
 //
 //   warps 0, 2    copies: per stage of kKT 64-k tiles one bulk copy of codes and parameters (warp 0), one tensor copy of x
@@ -12,20 +12,12 @@
 //   warps 4-7     epilogue: accumulators -> bias, activation, residual, one rounding -> out; or fp32 partial sums -> workspace
 //   warps 8..     kGroups groups of four, thread = row of W: per 64-k tile 8 words of codes -> 32 registers of fp16 pairs (per pair
 //                 one AND/OR, one exact subtraction of offset and zero point, one multiplication by the scale) -> tcgen05.st
-//
-// Work: 128-row blocks x column tiles ("items") of K/64 k-tiles.  When the items fill the SMs evenly a thread block takes whole
-// items; otherwise all k-tiles are laid end to end and every thread block takes an equal share, partial sums of cut items go to
-// the workspace (two slots a thread block) and int4_join_kernel adds them in order of k: no atomics, the same bits every time.
-#include "int4.cuh"
-#include "sm100.cuh"
+#include "int4_work.cuh"
 #include <cuda.h>
 #include <mutex>
 
 namespace spb {
 namespace {
-using namespace sm100;
-
-constexpr int kUnit = 2;                            // k-tiles of a unit: what a group expands per turn and one commit covers
 
 template <int NPAD> struct Cfg {
     static constexpr int kGroups = 4;                                    // dequantising groups of four warps
@@ -41,54 +33,6 @@ template <int NPAD> struct Cfg {
     static constexpr uint32_t kSmem = 1024 + 1024 + kStages * kStage;    // header, alignment
     static constexpr uint32_t kTmemCols = 512, kTmemA = 512 - 64 * kABlocks;   // accumulators from 0, operand blocks at the end
     static_assert(kAcc * NPAD <= (int)kTmemA, "accumulators and operand blocks overlap");
-};
-
-struct Params {
-    Int4Args a;
-    int ku, ncol, items;   // units along K, column tiles, items
-    int share, extra;      // thread block i takes `share` units, one more if i < extra; whole: items instead of units
-    int whole;
-    int* status;
-};
-// First unit of thread block i's share of the list (items in order, ku units each), and the thread block that has unit x.
-__device__ __forceinline__ int share_begin(const Params& p, int i) { return (i * p.share + min(i, p.extra)) * (p.whole ? p.ku : 1); }
-__device__ __forceinline__ int share_of(const Params& p, int x)   // not whole
-{
-    const int big = p.extra * (p.share + 1);
-    return x < big ? x / (p.share + 1) : p.extra + (x - big) / p.share;
-}
-__device__ __forceinline__ float finish(const Int4Args& a, float y, long long m, long long n)
-{
-    if (a.bias) y += __half2float(__ushort_as_half(a.bias[m]));
-    if (a.activation) y = y < 0.f ? 0.f : y;   // NaN stays NaN
-    if (a.residual) y += __half2float(__ushort_as_half(a.residual[n * a.M + m]));
-    return y;
-}
-
-// A run of k-tiles of one item.
-struct Run {
-    int mb, n0, u0, nkt;
-    bool first, last;   // starts / ends the item
-};
-struct Walk {
-    int x, hi, item, u;
-    __device__ __forceinline__ Walk(const Params& p) : x(share_begin(p, blockIdx.x)), hi(share_begin(p, blockIdx.x + 1)), item(x / p.ku), u(x - item * p.ku) {}
-    template <int NPAD>
-    __device__ __forceinline__ bool next(const Params& p, Run& r)
-    {
-        if (x >= hi) return false;
-        const int n = min(p.ku - u, hi - x);
-        r.mb = item / p.ncol;
-        r.n0 = (item - r.mb * p.ncol) * NPAD;
-        r.u0 = u;
-        r.nkt = n * kUnit;
-        r.first = u == 0;
-        r.last = u + n == p.ku;
-        x += n;
-        u = 0;
-        ++item;
-        return true;
-    }
 };
 
 template <int NPAD, int kGroup>
@@ -312,35 +256,6 @@ __global__ void __launch_bounds__(Cfg<NPAD>::kThreads, 1) int4_wide_kernel(const
     if (warp == 1) tc_dealloc(*holder, C::kTmemCols);
 }
 
-// Adds the partial sums of the items that were cut; blockIdx.x: item, blockIdx.y: columns by 8.
-template <int NPAD>
-__global__ void __launch_bounds__(256) int4_join_kernel(const __grid_constant__ Params p)
-{
-    const int x0 = blockIdx.x * p.ku, c0 = share_of(p, x0), c1 = share_of(p, x0 + p.ku - 1);
-    grid_wait();
-    if (c0 == c1) return;
-    const int col = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x & 31;
-    const long long n = (long long)(blockIdx.x % p.ncol) * NPAD + col, m0 = (long long)(blockIdx.x / p.ncol) * 128;
-    if (n >= p.a.N) return;
-    float4 sum;
-    // the first part may be either slot of its thread block, the later ones start a thread block's share
-    const float4* src = reinterpret_cast<const float4*>(p.a.ws + col * 128) + lane;
-    const float4 f = src[(2 * (size_t)c0 + 1) * (NPAD * 32)];
-    sum = f;
-#pragma unroll 4
-    for (int i = c0 + 1; i <= c1; ++i) {
-        const float4 v = src[2 * (size_t)i * (NPAD * 32)];
-        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-    }
-    const long long m = m0 + 4 * lane;
-    if (m >= p.a.M) return;   // M is a multiple of 64
-    const float y[4] = {sum.x, sum.y, sum.z, sum.w};
-    __half o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = __float2half_rn(finish(p.a, y[i], m + i, n));
-    *reinterpret_cast<uint2*>(p.a.out + n * p.a.M + m) = *reinterpret_cast<uint2*>(o);
-}
-
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                    const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiledFn encode_tiled()
@@ -355,40 +270,6 @@ EncodeTiledFn encode_tiled()
     });
     return fn;
 }
-int sm_count()
-{
-    static int n[64] = {};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
-        cudaGetLastError();
-        return 148;
-    }
-    if (!n[dev] && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-    return n[dev];
-}
-int pad_for(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : N <= 128 ? 128 : 256; }
-
-// How a shape is dealt out: thread blocks, and whether they take whole items.
-struct Plan {
-    int npad, ncol;
-    long long items;
-    int ku, ctas;
-    bool whole;
-};
-Plan plan_for(int M, int N, int K)
-{
-    Plan q;
-    q.npad = pad_for(N);
-    q.ncol = (N + q.npad - 1) / q.npad;
-    q.items = (M + 127ll) / 128 * q.ncol;
-    q.ku = (K + 127) / 128;
-    const int sms = sm_count();
-    const long long rounds = (q.items + sms - 1) / sms, units = q.items * q.ku;
-    q.whole = q.items >= 0.92 * rounds * sms;
-    q.ctas = (int)(q.whole ? (sms < q.items ? (long long)sms : q.items) : units < 2 ? 1ll : units / 2 < sms ? units / 2 : (long long)sms);   // at least two units a thread block
-    return q;
-}
-
 template <int NPAD, int kGroup>
 cudaError_t launch(cudaStream_t s, const Int4Args& a, const Plan& q, int* status)
 {
@@ -413,42 +294,13 @@ cudaError_t launch(cudaStream_t s, const Int4Args& a, const Plan& q, int* status
     if (enc(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<uint16_t*>(a.x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaErrorInvalidValue;
-    Params p;
-    p.a = a;
-    p.ku = q.ku;
-    p.ncol = q.ncol;
-    p.items = (int)q.items;
-    p.whole = q.whole;
-    const int all = (int)(q.whole ? q.items : q.items * q.ku);
-    p.share = all / q.ctas;
-    p.extra = all % q.ctas;
-    p.status = status;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(q.ctas);
-    cfg.blockDim = dim3(C::kThreads);
-    cfg.dynamicSmemBytes = C::kSmem;
-    cfg.stream = s;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, int4_wide_kernel<NPAD, kGroup>, p, map);
-    count_launch();
-    if (e != cudaSuccess || q.whole) return e;
-    cfg.gridDim = dim3((unsigned)q.items, (a.N < NPAD ? a.N + 7 : NPAD) / 8);
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = 0;
-    e = cudaLaunchKernelEx(&cfg, int4_join_kernel<NPAD>, p);
-    count_launch();
-    return e;
+    return launch_product<NPAD>(s, int4_wide_kernel<NPAD, kGroup>, C::kThreads, C::kSmem, make_params(a, q, status), q, map);
 }
 
 template <int kGroup>
 cudaError_t launch_group(cudaStream_t s, const Int4Args& a, const Plan& q, int* status)
 {
     switch (q.npad) {
-        case 16: return launch<16, kGroup>(s, a, q, status);
         case 32: return launch<32, kGroup>(s, a, q, status);
         case 64: return launch<64, kGroup>(s, a, q, status);
         case 128: return launch<128, kGroup>(s, a, q, status);
@@ -458,9 +310,8 @@ cudaError_t launch_group(cudaStream_t s, const Int4Args& a, const Plan& q, int* 
 
 }  // namespace
 
-size_t int4_wide_ws_floats(int M, int N, int K)
+size_t int4_ws_floats(int M, int N, int K)
 {
-    if (N <= kInt4SmallRows) return 0;
     const Plan q = plan_for(M, N, K);
     return q.whole ? 0 : (size_t)2 * q.ctas * q.npad * 128;
 }

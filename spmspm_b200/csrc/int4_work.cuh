@@ -1,0 +1,166 @@
+// How the kernels of the 4-bit linear layer share out their work.
+//
+// The product is a list of items (128 rows of W x a tile of rows of x), each of ku units along K (int4.cuh).  When the items fill
+// the SMs evenly a thread block takes whole items; otherwise all units are laid end to end and every thread block takes an equal
+// share.  Partial sums of items that are cut go to the workspace (two slots a thread block: an item it starts in the middle of, and
+// one it leaves in the middle of) and int4_join_kernel adds them in order of k: no atomics, the same bits every time.
+#pragma once
+#include "int4.cuh"
+#include "sm100.cuh"
+
+namespace spb {
+namespace {
+using namespace sm100;
+
+constexpr int kUnit = 2;   // k-tiles of a unit
+
+struct Params {
+    Int4Args a;
+    int ku, ncol, items;   // units along K, column tiles, items
+    int share, extra;      // thread block i takes `share` units, one more if i < extra; whole: items instead of units
+    int whole;
+    int* status;
+};
+// First unit of thread block i's share of the list (items in order, ku units each), and the thread block that has unit x.
+__device__ __forceinline__ int share_begin(const Params& p, int i) { return (i * p.share + min(i, p.extra)) * (p.whole ? p.ku : 1); }
+__device__ __forceinline__ int share_of(const Params& p, int x)   // not whole
+{
+    const int big = p.extra * (p.share + 1);
+    return x < big ? x / (p.share + 1) : p.extra + (x - big) / p.share;
+}
+__device__ __forceinline__ float finish(const Int4Args& a, float y, long long m, long long n)
+{
+    if (a.bias) y += __half2float(__ushort_as_half(a.bias[m]));
+    if (a.activation) y = y < 0.f ? 0.f : y;   // NaN stays NaN
+    if (a.residual) y += __half2float(__ushort_as_half(a.residual[n * a.M + m]));
+    return y;
+}
+
+// A run of k-tiles of one item.
+struct Run {
+    int mb, n0, u0, nkt;
+    bool first, last;   // starts / ends the item
+};
+struct Walk {
+    int x, hi, item, u;
+    __device__ __forceinline__ Walk(const Params& p) : x(share_begin(p, blockIdx.x)), hi(share_begin(p, blockIdx.x + 1)), item(x / p.ku), u(x - item * p.ku) {}
+    template <int NPAD>
+    __device__ __forceinline__ bool next(const Params& p, Run& r)
+    {
+        if (x >= hi) return false;
+        const int n = min(p.ku - u, hi - x);
+        r.mb = item / p.ncol;
+        r.n0 = (item - r.mb * p.ncol) * NPAD;
+        r.u0 = u;
+        r.nkt = n * kUnit;
+        r.first = u == 0;
+        r.last = u + n == p.ku;
+        x += n;
+        u = 0;
+        ++item;
+        return true;
+    }
+};
+
+// Adds the partial sums of the items that were cut; blockIdx.x: item, blockIdx.y: columns by 8.
+template <int NPAD>
+__global__ void __launch_bounds__(256) int4_join_kernel(const __grid_constant__ Params p)
+{
+    const int x0 = blockIdx.x * p.ku, c0 = share_of(p, x0), c1 = share_of(p, x0 + p.ku - 1);
+    grid_wait();
+    if (c0 == c1) return;
+    const int col = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x & 31;
+    const long long n = (long long)(blockIdx.x % p.ncol) * NPAD + col, m0 = (long long)(blockIdx.x / p.ncol) * 128;
+    if (n >= p.a.N) return;
+    float4 sum;
+    // the first part may be either slot of its thread block, the later ones start a thread block's share
+    const float4* src = reinterpret_cast<const float4*>(p.a.ws + col * 128) + lane;
+    const float4 f = src[(2 * (size_t)c0 + 1) * (NPAD * 32)];
+    sum = f;
+#pragma unroll 4
+    for (int i = c0 + 1; i <= c1; ++i) {
+        const float4 v = src[2 * (size_t)i * (NPAD * 32)];
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    const long long m = m0 + 4 * lane;
+    if (m >= p.a.M) return;   // M is a multiple of 64
+    const float y[4] = {sum.x, sum.y, sum.z, sum.w};
+    __half o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __float2half_rn(finish(p.a, y[i], m + i, n));
+    *reinterpret_cast<uint2*>(p.a.out + n * p.a.M + m) = *reinterpret_cast<uint2*>(o);
+}
+
+int sm_count()
+{
+    static int n[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+        cudaGetLastError();
+        return 148;
+    }
+    if (!n[dev] && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    return n[dev];
+}
+// How a shape is dealt out: thread blocks, and whether they take whole items.
+struct Plan {
+    int npad, ncol;
+    long long items;
+    int ku, ctas;
+    bool whole;
+};
+Plan plan_for(int M, int N, int K)
+{
+    Plan q;
+    q.npad = N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : N <= 128 ? 128 : 256;
+    q.ncol = (N + q.npad - 1) / q.npad;
+    q.items = (M + 127ll) / 128 * q.ncol;
+    q.ku = (K + 127) / 128;
+    const int sms = sm_count();
+    const long long rounds = (q.items + sms - 1) / sms, units = q.items * q.ku;
+    q.whole = q.items >= 0.92 * rounds * sms;
+    q.ctas = (int)(q.whole ? (sms < q.items ? (long long)sms : q.items) : units < 2 ? 1ll : units / 2 < sms ? units / 2 : (long long)sms);   // at least two units a thread block
+    return q;
+}
+
+Params make_params(const Int4Args& a, const Plan& q, int* status)
+{
+    Params p;
+    p.a = a;
+    p.ku = q.ku;
+    p.ncol = q.ncol;
+    p.items = (int)q.items;
+    p.whole = q.whole;
+    const int all = (int)(q.whole ? q.items : q.items * q.ku);
+    p.share = all / q.ctas;
+    p.extra = all % q.ctas;
+    p.status = status;
+    return p;
+}
+// The product's launch and, when items are cut, the join's; both may be set up before what precedes them has ended.
+template <int NPAD, class Kernel, class... More>
+cudaError_t launch_product(cudaStream_t s, Kernel kernel, int threads, size_t smem, const Params& p, const Plan& q, const More&... more)
+{
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(q.ctas);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p, more...);
+    count_launch();
+    if (e != cudaSuccess || q.whole) return e;
+    cfg.gridDim = dim3((unsigned)q.items, ((p.a.N < NPAD ? p.a.N : NPAD) + 7) / 8);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, int4_join_kernel<NPAD>, p);
+    count_launch();
+    return e;
+}
+
+}  // namespace
+}  // namespace spb

@@ -36,7 +36,7 @@ def run(sp, rng, M, K, N, G, bias=False, relu=False, residual=False, x=None, W=N
     got = sp.linear_int4(W, dev(x), bias=dev(b) if bias else None, residual=dev(r) if residual else None,
                          activation=sp.ACT_RELU if relu else sp.ACT_NONE).cpu().numpy().astype(np.float64)
     f = lambda a: None if a is None else a.astype(np.float64)
-    want, tol = model.linear(f(codes), f(scales), f(zeros), f(x), f(b), f(r), relu, fp16_weights=N > 8)
+    want, tol = model.linear(f(codes), f(scales), f(zeros), f(x), f(b), f(r), relu, fp16_weights=N > 16)
     err = np.abs(got - want)
     assert np.all(err <= tol), (float((err / tol).max()), np.argwhere(err > tol)[:4])
     assert sp.device_status() == 0

@@ -59,15 +59,15 @@ def test_sizes(lib_built):
     assert lib_built.spb_kv_cache_bytes(3, 24, 2, 128) == 0 and lib_built.spb_kv_cache_bytes(3, 32, 2, 80) == 0
     assert lib_built.spb_int4_bytes(64, 128, 128) == 8704 and lib_built.spb_int4_bytes(192, 192, 32) == 4 * (8192 + 2048)
     assert lib_built.spb_int4_bytes(64, 192, 128) == 0
-    assert lib_built.spb_int4_workspace_bytes(5120, 8, 5120) == 0 and lib_built.spb_int4_workspace_bytes(5120, 16, 5120) > 0
+    assert lib_built.spb_int4_workspace_bytes(5120, 1, 5120) > 0 and lib_built.spb_int4_workspace_bytes(148 * 128, 1, 5120) == 0
 
 
 @pytest.mark.parametrize("bad", [dict(M=0), dict(M=100), dict(K=96), dict(group=16), dict(group=256), dict(K=192, group=128), dict(N=0), dict(act=2),
                                  dict(codes=None), dict(x=None), dict(out=None), dict(x=A + 2), dict(bias=A + 8),
-                                 dict(residual=A + 4), dict(codes=A + 4), dict(N=40), dict(N=40, ws=A, ws_bytes=16),
+                                 dict(residual=A + 4), dict(codes=A + 4), dict(N=40, ws=None), dict(N=40, ws=A, ws_bytes=16),
                                  dict(N=40, ws=A + 4, ws_bytes=1 << 30)])
 def test_linear_refuses(lib_built, bad):
-    a = dict(stream=None, codes=A, M=64, K=128, group=64, x=A, out=A, N=1, bias=None, residual=None, act=0, ws=None, ws_bytes=0)
+    a = dict(stream=None, codes=A, M=64, K=128, group=64, x=A, out=A, N=1, bias=None, residual=None, act=0, ws=A, ws_bytes=1 << 30)
     a.update(bad)
     assert lib_built.spb_linear_int4(*a.values()) != 0 and b"linear_int4" in lib_built.spb_last_error()
 
