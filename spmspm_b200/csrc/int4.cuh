@@ -31,6 +31,7 @@ struct Int4Args {
 constexpr int kInt4StreamRows = 16;   // up to this many rows of x the mma.sync kernel runs, above it the tcgen05 one
 cudaError_t int4_stream_launch(cudaStream_t s, const Int4Args& a, int* status);
 cudaError_t int4_wide_launch(cudaStream_t s, const Int4Args& a, int* status);
+int int4_stream_clusters(int split);   // clusters of `split` thread blocks of the streaming kernel that the device holds at once
 size_t int4_ws_floats(int M, int N, int K);
 __host__ __device__ __forceinline__ int int4_chunk(int g, int t) { return 4 * g + (t ^ (g >> 1)); }
 

@@ -29,6 +29,7 @@ template <int NT, int kGroup>
 struct StreamSmem {
     uint8_t ring[kWarps][kStages][int4_unit_bytes(kGroup)];
     float sums[kWarps][8 * 4][32];   // [warp][row tile, register][lane], one tile of 8 rows of x at a time
+    float total[8 * NT][128];        // cluster: this thread block's part of the item
     uint64_t full[kWarps][kStages];
     int abort;
 };
@@ -168,10 +169,26 @@ __global__ void __launch_bounds__(32 * kWarps, 1) int4_stream_kernel(const __gri
                 for (int w = 1; w < kWarps; ++w) y += sm.sums[w][v][l];
                 const long long m = (long long)r.mb * 128 + row, nn = nt * 8 + col;
                 if (nn >= p.a.N) continue;
+                if (p.split > 1) {
+                    sm.total[nn][row] = y;
+                    continue;
+                }
                 if (!(r.first && r.last)) p.a.ws[((2 * (size_t)blockIdx.x + r.first) * (8 * NT) + nn) * 128 + row] = y;
                 else if (m < p.a.M) p.a.out[nn * p.a.M + m] = __half_as_ushort(__float2half_rn(finish(p.a, y, m, nn)));
             }
         }
+    }
+    if (p.split > 1) {
+        // the parts of the cluster's thread blocks, in order of k; each finishes every split-th stretch of 256 values
+        cluster_sync();
+        const int rank = blockIdx.x % p.split;
+        for (int e = rank * (32 * kWarps) + threadIdx.x; e < min(p.a.N, 8 * NT) * 128; e += p.split * 32 * kWarps) {
+            float y = 0.f;
+            for (int i = 0; i < p.split; ++i) y += cluster_load(smem_u32(&sm.total[0][0] + e), i);
+            const long long m = (long long)(blockIdx.x / p.split) * 128 + (e & 127), n = e >> 7;
+            if (m < p.a.M) p.a.out[n * p.a.M + m] = __half_as_ushort(__float2half_rn(finish(p.a, y, m, n)));
+        }
+        cluster_sync();   // nobody leaves while its part is being read
     }
     if (!alive) {   // a wait ran out: report, and give the copies still under way one more bounded wait
         if (lane == 0) atomicOr(p.status, (int)kStatusWaitTimeout);
@@ -199,6 +216,37 @@ cudaError_t launch_stream(cudaStream_t s, const Int4Args& a, const Plan& q, int*
 }
 
 }  // namespace
+
+int int4_stream_clusters(int split)
+{
+    static int cached[64][9] = {};   // count + 1
+    int dev = 0;
+    if (split < 2 || split > 8 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+        cudaGetLastError();
+        return 0;
+    }
+    if (!cached[dev][split]) {
+        using Smem = StreamSmem<2, 32>;   // the variant that needs most
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = split;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(split * 64);
+        cfg.blockDim = dim3(32 * kWarps);
+        cfg.dynamicSmemBytes = sizeof(Smem);
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaFuncSetAttribute(int4_stream_kernel<2, 32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem)) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, int4_stream_kernel<2, 32>, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            return 0;
+        }
+        cached[dev][split] = n + 1;
+    }
+    return cached[dev][split] - 1;
+}
 
 cudaError_t int4_stream_launch(cudaStream_t s, const Int4Args& a, int* status)
 {

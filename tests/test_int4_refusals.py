@@ -59,7 +59,7 @@ def test_sizes(lib_built):
     assert lib_built.spb_kv_cache_bytes(3, 24, 2, 128) == 0 and lib_built.spb_kv_cache_bytes(3, 32, 2, 80) == 0
     assert lib_built.spb_int4_bytes(64, 128, 128) == 8704 and lib_built.spb_int4_bytes(192, 192, 32) == 4 * (8192 + 2048)
     assert lib_built.spb_int4_bytes(64, 192, 128) == 0
-    assert lib_built.spb_int4_workspace_bytes(5120, 1, 5120) > 0 and lib_built.spb_int4_workspace_bytes(148 * 128, 1, 5120) == 0
+    assert lib_built.spb_int4_workspace_bytes(100 * 128, 1, 5120) > 0 and lib_built.spb_int4_workspace_bytes(148 * 128, 1, 5120) == 0
 
 
 @pytest.mark.parametrize("bad", [dict(M=0), dict(M=100), dict(K=96), dict(group=16), dict(group=256), dict(K=192, group=128), dict(N=0), dict(act=2),
