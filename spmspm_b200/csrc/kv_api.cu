@@ -20,8 +20,8 @@ bool check_cache(const char* who, const void* pool, int num_pages, int page_size
                   "(num_pages=%d kv_heads=%d page_size=%d)", who, num_pages, kv_heads, page_size);
         return false;
     }
-    if (B <= 0 || B > 65535 || table_stride <= 0 || n_tokens < 0 || n_tokens * kv_heads > kMaxInt) {
-        set_error("%s: batch must be 1..65535, table_stride positive and n_tokens * kv_heads below 2^31 (batch=%d table_stride=%d "
+    if (B <= 0 || B > 65535 || table_stride <= 0 || n_tokens < 0 || n_tokens > kMaxInt / kv_heads / 2) {
+        set_error("%s: batch must be 1..65535, table_stride positive and n_tokens * kv_heads below 2^30 (batch=%d table_stride=%d "
                   "n_tokens=%lld)", who, B, table_stride, n_tokens);
         return false;
     }
@@ -60,7 +60,8 @@ KvView view(void* pool, int num_pages, int page_size, int kv_heads, const int* t
     c.table = table;
     c.lens = lens;
     c.cu = cu;
-    c.n_tokens = n_tokens;
+    c.n_tokens = (int)n_tokens;
+    c.per_seq = (int)(n_tokens / B);
     c.table_stride = table_stride;
     c.num_pages = num_pages;
     c.page_size = page_size;
@@ -110,7 +111,7 @@ int spb_kv_append(void* stream, void* pool, int num_pages, int page_size, int kv
             set_error("%s: q is only taken to be rotated: cos_table and sin_table are missing", who);
             return (int)cudaErrorInvalidValue;
         }
-        if (q_heads <= 0 || q_heads > 65536 || n_tokens * (2ll * kv_heads + q_heads) > kMaxInt) {
+        if (q_heads <= 0 || q_heads > 65536 || n_tokens > kMaxInt / (2ll * kv_heads + q_heads)) {
             set_error("%s: q_heads must be positive and n_tokens * heads below 2^31 (q_heads=%d)", who, q_heads);
             return (int)cudaErrorInvalidValue;
         }
@@ -168,7 +169,7 @@ int spb_kv_attention(void* stream, const void* pool, int num_pages, int page_siz
     if (!check_cache(who, pool, num_pages, page_size, kv_heads, head_dim, page_table, table_stride, kv_lens, cu_q, batch, n_tokens) ||
         !check_vectors(who, "q", q, q_token_stride, q_head_stride))
         return (int)cudaErrorInvalidValue;
-    if (q_heads <= 0 || q_heads % kv_heads || n_tokens * q_heads > kMaxInt) {
+    if (q_heads <= 0 || q_heads % kv_heads || n_tokens > kMaxInt / q_heads) {
         set_error("%s: q_heads must be a positive multiple of kv_heads and n_tokens * q_heads below 2^31 (q_heads=%d kv_heads=%d)", who, q_heads, kv_heads);
         return (int)cudaErrorInvalidValue;
     }
@@ -198,7 +199,7 @@ int spb_kv_attention(void* stream, const void* pool, int num_pages, int page_siz
     a.ws = static_cast<float*>(workspace);
     a.ws_floats = workspace_bytes / 4;
     e = kv_attention_launch((cudaStream_t)stream, head_dim, a, status);
-    if (e != cudaSuccess) set_error("%s: %s", who, cudaGetErrorString(e));
+    if (e != cudaSuccess && e != cudaErrorInvalidValue) set_error("%s: %s", who, cudaGetErrorString(e));
     return (int)e;
 }
 

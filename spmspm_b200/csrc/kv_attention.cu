@@ -2,18 +2,20 @@
 //
 // kv_attention_split_kernel: few query rows a key head (decoding, drafts).  Everything is transposed, keys and channels on
 // the 16-row side of mma.sync.m16n8k16 and query rows on its 8-column side, so that a single row wastes 7/8 of a cheap
-// operand and not of the cache's:
+// operand and not of the cache's.  Codes are never expanded: a nibble masked out of its word is an fp16 subnormal, c 2^-24 (low
+// nibble of a byte) or c 2^-20 (high), which the instruction multiplies exactly, so unpacking costs 1.25 instructions per pair
+// of codes.  Scales and minima are applied around the products, in fp32 for the keys and on the weights for the values:
 //
-//   scores   S^T = K Q^T per group of 32 channels: the codes enter the matrix instruction as they are.  A nibble masked out
-//            of its word is an fp16 subnormal, c 2^-24 (low nibble of a byte) or c 2^-20 (high), which the instruction
-//            multiplies exactly; the high nibbles' share of q is divided by 16 beforehand.  Scale and minimum are applied to
-//            the fp32 sum of a group: z = s (q.c) + m sum(q), so keys are never rounded, and the cost is 1.25 instructions
-//            per pair of codes instead of three.  q is first multiplied by a power of two that brings its row's largest
-//            magnitude to [2^8, 2^9): the division by 16 then loses nothing above 2^-25 of that magnitude.
+//   scores   S^T = K Q^T per group of 32 channels, z = sum over groups of s (q.c) + m sum(q); the second term is one more matrix
+//            instruction on the group sums of q, split into two fp16 values.  The high nibbles' share of q is divided by 16
+//            beforehand; q is first multiplied by a power of two that brings its row's largest magnitude to [2^8, 2^9), so that the
+//            division loses nothing above 2^-25 of that magnitude.
 //   softmax  running maximum and sum in fp32 per row, in base 2.  The accumulators are only rescaled when a maximum grows by more
 //            than 2^8; weights are kept 2^7 too large, so that in fp16 they span 2^-31 .. 1 relative to the largest.
-//   values   O^T += V^T P^T: pairs of codes become fp16 with one AND/OR, one subtraction (exact) and one fused multiply-add
-//            (one rounding, the value that kv_read returns); P^T comes from S^T with two 8 x 8 transposes in registers.
+//   values   O^T = sum over tokens of (P s) c + P m: P^T comes from S^T with two 8 x 8 transposes in registers and is multiplied
+//            by the tokens' scales, one product per group, rounded to fp16 like P itself; the minima are one more matrix
+//            instruction per 16 tokens.  Scales of 2 and more would leave the fp16 range: the whole row is then shifted down by
+//            the scale's exponent, as if its maximum had grown.
 //
 // Work: the context is cut in units of 64 tokens (four warps, one 16-token block each); all units of all (sequence, key
 // head, row tile) are laid end to end and every thread block takes an equal share, found from the lengths on the device.
@@ -22,29 +24,28 @@
 // Every warp streams its own blocks: one bulk copy per block into its own ring, nobody waits for another warp except at
 // the end of a row tile.
 #include "kv_int4.cuh"
+#include "sm100.cuh"
 #include <cstdio>
 
 namespace spb {
 namespace {
+using namespace sm100;
 
 constexpr int kWarps = 4;
-constexpr int kStages = 4;                 // 16-token blocks in flight per warp
-constexpr uint32_t kSpin = 1u << 22;       // polls before a wait gives up
+constexpr int kStages = 3;                 // 16-token blocks in flight per warp
 constexpr float kShift = 7.f, kSlack = 8.f;
 constexpr int kUnit = kKvBlock * kWarps;   // tokens a thread block advances per step
+__host__ __device__ constexpr int blocks_per_sm(int nt) { return nt == 1 ? 4 : nt == 2 ? 3 : 2; }
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity)
 {
-    for (uint32_t i = 0; i < kSpin; ++i) {
-        uint32_t ok;
-        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-        if (ok) return true;
+    for (uint32_t i = 0; i < kSpinLimit; ++i) {
+        if (mbar_try(bar, parity)) return true;
         if (i > 1024) __nanosleep(40);
     }
     return false;
 }
+
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -70,57 +71,52 @@ __device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<
 struct Seq {
     int b = 0;
     int len = 0, qlen = 0, tiles = 0;   // tokens in the cache, new tokens, row tiles
-    long long first = 0;                // first packed row
-    long long units = 0;                // 64-token units of one row tile
-    long long begin = 0, total = 0;     // its range of the list
+    int first = 0;                      // first packed row
+    int units = 0;                      // 64-token units of one row tile
+    int begin = 0, total = 0;           // its range of the list
 };
 template <int ROWS>
 __device__ __forceinline__ void load_seq(Seq& s, const KvView& c, int b, int group)
 {
-    long long first, n;
-    kv_rows(c, b, first, n);
+    kv_rows(c, b, s.first, s.qlen);
     s.b = b;
-    s.first = first;
-    s.qlen = (int)n;
     s.len = max(c.lens[b], 0);
-    s.tiles = (int)((n * group + ROWS - 1) / ROWS);
+    s.tiles = (s.qlen * group + ROWS - 1) / ROWS;
     // tokens past the table's width have no page: they are not walked over
-    const long long held = min((long long)s.len, (long long)c.table_stride * c.page_size);
-    s.units = max((held + kUnit - 1) / kUnit, 1ll);
-    s.total = (long long)c.kv_heads * s.tiles * s.units;
+    const int held = (int)min((long long)s.len, (long long)c.table_stride * c.page_size);
+    s.units = max((held - 1) / kUnit + 1, 1);
+    s.total = c.kv_heads * s.tiles * s.units;
 }
 template <int ROWS>
-__device__ __forceinline__ long long list_length(const KvView& c, int group)
+__device__ __forceinline__ int list_length(const KvView& c, int group)
 {
-    long long sum = 0;
+    int sum = 0;
     for (int b = threadIdx.x & 31; b < c.B; b += 32) {
         Seq s;
         load_seq<ROWS>(s, c, b, group);
         sum += s.total;
     }
-#pragma unroll
-    for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum;
+    return __reduce_add_sync(0xffffffffu, sum);
 }
 // The sequence that holds unit x of the list (x inside the list); every lane gets the same.
 template <int ROWS>
-__device__ __forceinline__ void find_seq(Seq& s, const KvView& c, int group, long long x)
+__device__ __forceinline__ void find_seq(Seq& s, const KvView& c, int group, int x)
 {
     const int lane = threadIdx.x & 31;
-    long long before = 0;
+    int before = 0;
     for (int b0 = 0; b0 < c.B; b0 += 32) {
         Seq t;
         if (b0 + lane < c.B) load_seq<ROWS>(t, c, b0 + lane, group);
-        long long incl = t.total;
+        int incl = t.total;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
-            const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += y;
         }
         const uint32_t past = __ballot_sync(0xffffffffu, before + incl > x);
         if (past) {
             const int l = __ffs(past) - 1;
-            const long long begin = before + __shfl_sync(0xffffffffu, incl - t.total, l);
+            const int begin = before + __shfl_sync(0xffffffffu, incl - t.total, l);
             load_seq<ROWS>(s, c, b0 + l, group);
             s.begin = begin;
             return;
@@ -132,26 +128,28 @@ template <int ROWS>
 __device__ __forceinline__ void next_seq(Seq& s, const KvView& c, int group)
 {
     do {
-        const long long end = s.begin + s.total;
+        const int end = s.begin + s.total;
         load_seq<ROWS>(s, c, s.b + 1, group);
         s.begin = end;
     } while (s.total == 0 && s.b + 1 < c.B);
 }
-__device__ __forceinline__ long long share_begin(long long total, int ctas, int i) { return total * i / ctas; }
-// Thread block whose share holds unit x.
-__device__ __forceinline__ int share_of(long long total, int ctas, long long x)
-{
-    int i = (int)(((x + 1) * ctas - 1) / total);
-    while (i > 0 && share_begin(total, ctas, i) > x) --i;
-    while (i + 1 < ctas && share_begin(total, ctas, i + 1) <= x) ++i;
-    return i;
-}
+// Thread block i of n takes total / n units, the first total % n of them one more.
+struct Shares {
+    int share, extra;
+    __device__ __forceinline__ Shares(int total, int n) : share(total / n), extra(total - total / n * n) {}
+    __device__ __forceinline__ int begin(int i) const { return i * share + min(i, extra); }
+    __device__ __forceinline__ int of(int x) const   // thread block that has unit x
+    {
+        const int big = extra * (share + 1);
+        return x < big ? x / (share + 1) : extra + (x - big) / share;
+    }
+};
 
 // ws: slot n (two per thread block): [rows][D] sums, then [rows] maxima and [rows] sums of weights
 template <int D, int ROWS>
 __host__ __device__ constexpr size_t slot_floats() { return (size_t)ROWS * (D + 2); }
 
-// Keys that row r of a row tile may see.
+// Keys that row r of a sequence's rows may see.
 __device__ __forceinline__ int visible_keys(const Seq& s, int row, int group)
 {
     return max(s.len - s.qlen + row / group + 1, 0);
@@ -161,15 +159,15 @@ template <int D, int NT>
 struct Smem {
     alignas(128) uint8_t ring[kWarps][kStages][KvLayout<D>::kBlockBytes];
     alignas(16) float merge[kWarps - 1][NT * (D / 16) * 4 * 32 + 4 * NT * 32];
-    uint2 qfrag[NT][D / 16][32];                 // q operand, [row tile of 8][k-step][lane]
-    float qsum[NT][KvLayout<D>::kGroups][8];     // sum of q over a group, in units of the score sums
-    float factor[NT][8];                         // score sums -> base-2 scores
+    uint2 qfrag[NT][D / 16][32];   // q operand, [tile of 8 rows][k-step][lane]
+    uint32_t qsum[NT][32];         // group sums of q as an operand: lane 4 g + t holds groups 2 (t & 1), + 1 of row g, high (t < 2) or low part
+    float factor[NT][8];           // score sums -> base-2 scores
     uint64_t full[kWarps][kStages];
     int ok[kWarps][kStages];
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(KvAttnArgs a, int* status)
+__global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_split_kernel(KvAttnArgs a, int* status)
 {
     using L = KvLayout<D>;
     constexpr int G = L::kGroups, KS = D / 16, MT = D / 16, ROWS = 8 * NT;
@@ -180,64 +178,63 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(KvAttnA
     const int group = a.q_heads / c.kv_heads;
 
     if (lane == 0) {
-        for (int i = 0; i < kStages; ++i)
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&sm.full[warp][i])) : "memory");
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (int i = 0; i < kStages; ++i) mbar_init(smem_u32(&sm.full[warp][i]), 1);
+        mbar_init_fence();
     }
     __syncthreads();
+    grid_wait();
+    grid_release();   // the join may be set up while this kernel runs; it waits for its end
 
-    const long long total = list_length<ROWS>(c, group);
-    const long long lo = share_begin(total, gridDim.x, blockIdx.x), hi = share_begin(total, gridDim.x, blockIdx.x + 1);
-    if (lo >= hi) return;
+    const int total = list_length<ROWS>(c, group);
+    const Shares shares(total, gridDim.x);
+    const int lo = shares.begin(blockIdx.x), count = shares.begin(blockIdx.x + 1) - lo;
+    if (count <= 0) return;
 
     // ---- this warp's copies: lane l looks after every 32nd unit of the share
-    Seq ps;   // the lane's own place in the list
-    find_seq<ROWS>(ps, c, group, lo);
-    auto block_of = [&](long long x) -> long long {   // pool offset of this warp's block of unit x; -1: nothing to fetch
+    Seq s;
+    find_seq<ROWS>(s, c, group, lo);
+    Seq ps = s;   // the lane's own place in the list
+    auto block_of = [&](int x) -> long long {   // pool offset of this warp's block of unit x; -1: nothing to fetch
         while (x >= ps.begin + ps.total) next_seq<ROWS>(ps, c, group);
-        const long long r = x - ps.begin, pair = r / ps.units;
-        const int rt = (int)(pair % ps.tiles), h = (int)(pair / ps.tiles);
-        const long long pos = ((r % ps.units) * kWarps + warp) * kKvBlock;
+        const int r = x - ps.begin, pair = r / ps.units, h = pair / ps.tiles, rt = pair - h * ps.tiles;
+        const int pos = ((r - pair * ps.units) * kWarps + warp) * kKvBlock;
         const int last_row = min((rt + 1) * ROWS, ps.qlen * group) - 1;
         if (pos >= visible_keys(ps, last_row, group)) return -1;
         const long long off = kv_block_offset<D>(c, ps.b, h, pos);
         if (off < 0) atomicOr(status, kStatusBadCache);
         return off;
     };
-    auto issue = [&](int stage, long long off) {   // one lane
-        const uint32_t bar = smem_u32(&sm.full[warp][stage]);
-        sm.ok[warp][stage] = off >= 0;
-        if (off >= 0) {
-            asm volatile("{ .reg .b64 st; mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1; }" ::"r"(bar), "r"(L::kBlockBytes) : "memory");
-            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                             smem_u32(sm.ring[warp][stage])), "l"(c.pool + off), "r"(L::kBlockBytes), "r"(bar) : "memory");
-        } else {
-            asm volatile("{ .reg .b64 st; mbarrier.arrive.shared::cta.b64 st, [%0]; }" ::"r"(bar) : "memory");
-        }
-    };
-    const int count = (int)min(hi - lo, 0x7fffffffll);
-    int issued = 0;                 // units whose copy is under way or done
+    const uint32_t ring = smem_u32(sm.ring[warp]), bars = smem_u32(sm.full[warp]);
+    int issued = 0, istage = 0;     // units whose copy is under way or done
     bool alive = true;              // no wait has run out
-    long long my_off = lane < count ? block_of(lo + lane) : -1;
-    auto refill = [&](int upto) {   // whole warp
-        for (; alive && issued < min(upto, count); ++issued) {
-            if (issued && issued % 32 == 0) my_off = issued + lane < count ? block_of(lo + issued + lane) : -1;
-            if (lane == issued % 32) issue(issued % kStages, my_off);
+    long long my_off = -1;
+    auto refill = [&]() {           // whole warp
+        if (!alive || issued >= count) return;
+        if ((issued & 31) == 0) my_off = issued + lane < count ? block_of(lo + issued + lane) : -1;
+        if (lane == (issued & 31)) {
+            const uint32_t bar = bars + 8 * istage;
+            sm.ok[warp][istage] = my_off >= 0;
+            if (my_off >= 0) {
+                mbar_expect_tx(bar, L::kBlockBytes);
+                bulk_g2s(ring + istage * L::kBlockBytes, c.pool + my_off, L::kBlockBytes, bar);
+            } else {
+                mbar_arrive(bar);
+            }
         }
+        ++issued;
+        if (++istage == kStages) istage = 0;
     };
-    refill(kStages);
+    for (int i = 0; i < kStages; ++i) refill();
 
     // ---- consumer
-    Seq s;
-    find_seq<ROWS>(s, c, group, lo);
-    long long x = lo;
-    int done = 0, waited = 0;       // units passed, units whose copy has been waited for
+    int x = lo, stage = 0, waited = 0;   // waited: units whose copy has been waited for
+    uint32_t parity = 0;
+    const int hi = lo + count;
     while (x < hi) {
         while (x >= s.begin + s.total) next_seq<ROWS>(s, c, group);
-        const long long pair = (x - s.begin) / s.units;
-        const int rt = (int)(pair % s.tiles), h = (int)(pair / s.tiles);
-        const long long pair_begin = s.begin + pair * s.units, pair_end = pair_begin + s.units;
-        const long long seg_begin = x, seg_end = min(hi, pair_end);
+        const int pair = (x - s.begin) / s.units, h = pair / s.tiles, rt = pair - h * s.tiles;
+        const int pair_begin = s.begin + pair * s.units, pair_end = pair_begin + s.units;
+        const int seg_begin = x, seg_end = min(hi, pair_end);
         if ((long long)s.len > (long long)c.table_stride * c.page_size && threadIdx.x == 0) atomicOr(status, kStatusBadCache);
         const int rows = min(ROWS, s.qlen * group - rt * ROWS);   // rows of this tile
         const int kmin = visible_keys(s, rt * ROWS, group), kmax = visible_keys(s, rt * ROWS + rows - 1, group);
@@ -247,12 +244,13 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(KvAttnA
         for (int nt = warp; nt < NT; nt += kWarps) {
             const int row = nt * 8 + g, abs_row = rt * ROWS + row;
             const bool have = row < rows;
-            const uint16_t* src = a.q + (s.first + (have ? abs_row / group : 0)) * a.q_tok + (h * group + (have ? abs_row % group : 0)) * a.q_head;
+            const uint16_t* src = a.q + (long long)(s.first + (have ? abs_row / group : 0)) * a.q_tok + (h * group + (have ? abs_row % group : 0)) * a.q_head;
             uint2 raw[KS];
             float big = 0.f;
 #pragma unroll
+            for (int j = 0; j < KS; ++j) raw[j] = have ? *reinterpret_cast<const uint2*>(src + 16 * j + 4 * t) : make_uint2(0, 0);
+#pragma unroll
             for (int j = 0; j < KS; ++j) {
-                raw[j] = have ? *reinterpret_cast<const uint2*>(src + 16 * j + 4 * t) : make_uint2(0, 0);
                 const float2 u = __half22float2(as_h2(raw[j].x)), w = __half22float2(as_h2(raw[j].y));
                 big = fmaxf(big, fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(w.x), fabsf(w.y))));
             }
@@ -269,41 +267,51 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(KvAttnA
                 sum[j / 2] += (u.x + u.y) + (w.x + w.y);
                 sm.qfrag[nt][j][lane] = make_uint2(h2_bits(__floats2half2_rn(u.x * k, u.y * k)), h2_bits(__floats2half2_rn(w.x * k, w.y * k)));
             }
+            float mine[2] = {0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < G; ++w) {
                 sum[w] += __shfl_xor_sync(0xffffffffu, sum[w], 1);
                 sum[w] += __shfl_xor_sync(0xffffffffu, sum[w], 2);
-                if (t == 0) sm.qsum[nt][w][g] = sum[w] * exp2f((float)(e - 24));
+                if (w / 2 == (t & 1)) mine[w & 1] = sum[w] * up;
             }
+            const __half2 high = __floats2half2_rn(mine[0], mine[1]);
+            const float2 back = __half22float2(high);
+            sm.qsum[nt][lane] = h2_bits(t < 2 ? high : __floats2half2_rn(mine[0] - back.x, mine[1] - back.y));
             if (t == 0) sm.factor[nt][g] = a.scale * 1.4426950408889634f * exp2f((float)(24 - e));
         }
         __syncthreads();
 
-        float o[NT][MT][4];
+        float o[NT][MT][4];      // sum of P s c, rows of the high nibbles 2^-20, of the low ones 2^-24 of it
+        float om[NT][4];         // sum of P m, row = group
         float mx[NT][2], sum[NT][2];
+        int shift = 0;           // exponent that the scales of the values have asked for; part of mx
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+            om[nt][0] = om[nt][1] = om[nt][2] = om[nt][3] = 0.f;
             mx[nt][0] = mx[nt][1] = -INFINITY;
             sum[nt][0] = sum[nt][1] = 0.f;
         }
+        auto rescale = [&](int nt, float r0, float r1) {
+            sum[nt][0] *= r0, sum[nt][1] *= r1;
+            om[nt][0] *= r0, om[nt][1] *= r1;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) o[nt][i][0] *= r0, o[nt][i][1] *= r1, o[nt][i][2] *= r0, o[nt][i][3] *= r1;
+        };
 
-        for (; x < seg_end; ++x, ++done) {
-            const int stage = done % kStages;
+        int pos = ((x - pair_begin) * kWarps + warp) * kKvBlock;
+        for (int left = seg_end - x; left > 0; --left, pos += kUnit) {
             if (alive) {
-                alive = wait_full(smem_u32(&sm.full[warp][stage]), (done / kStages) & 1);
-                alive = __all_sync(0xffffffffu, alive);
+                alive = __all_sync(0xffffffffu, wait_full(bars + 8 * stage, parity));
                 if (alive) ++waited;
                 else if (lane == 0) atomicOr(status, kStatusWaitTimeout);   // the rest counts as unseen
             }
-            const int pos = (int)(((x - pair_begin) * kWarps + warp) * kKvBlock);
             if (alive && sm.ok[warp][stage]) {
                 const uint8_t* blk = sm.ring[warp][stage];
                 const bool edge = pos + kKvBlock > kmin;   // some row does not see all of these tokens
-                // keys: one word of codes per group for tokens g and g + 8
-                uint32_t k0[G], k1[G];
-                __half2 p0[G], p1[G];
+                // ---- scores.  keys: one word of codes per group for tokens g and g + 8
+                uint32_t k0[G], k1[G], p0[G], p1[G];
                 {
                     const uint32_t* kc = reinterpret_cast<const uint32_t*>(blk + L::kKCodes);
                     const uint32_t* kp = reinterpret_cast<const uint32_t*>(blk + L::kKParams);
@@ -320,28 +328,106 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(KvAttnA
                     }
                 }
                 float z[NT][4];
+                {
+                    // minima of the lane's two groups, as an operand (lanes without a group: zero)
+                    uint32_t m0, m1;
+                    if constexpr (G == 4) {
+                        const bool odd = t & 1;
+                        m0 = __byte_perm(odd ? p0[2] : p0[0], odd ? p0[3] : p0[1], 0x7632);
+                        m1 = __byte_perm(odd ? p1[2] : p1[0], odd ? p1[3] : p1[1], 0x7632);
+                    } else {
+                        m0 = (t & 1) ? 0u : __byte_perm(p0[0], p0[1], 0x7632);
+                        m1 = (t & 1) ? 0u : __byte_perm(p1[0], p1[1], 0x7632);
+                    }
+                    const uint32_t am[4] = {m0, m1, 0u, 0u};
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) z[nt][0] = z[nt][1] = z[nt][2] = z[nt][3] = 0.f;
+                    for (int nt = 0; nt < NT; ++nt) {
+                        z[nt][0] = z[nt][1] = z[nt][2] = z[nt][3] = 0.f;
+                        mma(z[nt], am, sm.qsum[nt][lane], 0u);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) z[nt][i] *= 0x1p-24f;
+                    }
+                }
 #pragma unroll
                 for (int w = 0; w < G; ++w) {
                     const uint32_t h0 = k0[w] >> 8, h1 = k1[w] >> 8;
                     const uint32_t alow[4] = {k0[w] & 0x000f000fu, k1[w] & 0x000f000fu, h0 & 0x000f000fu, h1 & 0x000f000fu};
                     const uint32_t ahigh[4] = {k0[w] & 0x00f000f0u, k1[w] & 0x00f000f0u, h0 & 0x00f000f0u, h1 & 0x00f000f0u};
-                    const float2 f0 = __half22float2(p0[w]), f1 = __half22float2(p1[w]);
+                    const float s0 = __low2float(as_h2(p0[w])), s1 = __low2float(as_h2(p1[w]));
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float acc[4] = {0.f, 0.f, 0.f, 0.f};
                         const uint2 ql = sm.qfrag[nt][2 * w][lane], qh = sm.qfrag[nt][2 * w + 1][lane];
-                        const float2 qs = *reinterpret_cast<const float2*>(&sm.qsum[nt][w][2 * t]);
                         mma(acc, alow, ql.x, ql.y);
                         mma(acc, ahigh, qh.x, qh.y);
-                        z[nt][0] = fmaf(f0.x, acc[0], fmaf(f0.y, qs.x, z[nt][0]));
-                        z[nt][1] = fmaf(f0.x, acc[1], fmaf(f0.y, qs.y, z[nt][1]));
-                        z[nt][2] = fmaf(f1.x, acc[2], fmaf(f1.y, qs.x, z[nt][2]));
-                        z[nt][3] = fmaf(f1.x, acc[3], fmaf(f1.y, qs.y, z[nt][3]));
+                        z[nt][0] = fmaf(s0, acc[0], z[nt][0]);
+                        z[nt][1] = fmaf(s0, acc[1], z[nt][1]);
+                        z[nt][2] = fmaf(s1, acc[2], z[nt][2]);
+                        z[nt][3] = fmaf(s1, acc[3], z[nt][3]);
                     }
                 }
-                bool grow = false;
+                // ---- values of tokens 2t, 2t+1 (j = 0) and 2t+8, 2t+9 (j = 1): codes, scales of all groups, minima of group g
+                uint32_t vw[2][G], vs[2][G], vm[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint8_t* vc = blk + L::kVCodes + j * 4 * D + lane * (D / 8);
+                    const uint32_t* vp = reinterpret_cast<const uint32_t*>(blk + L::kVParams) + (t + 4 * j) * 2 * G;
+                    if constexpr (G == 4) {
+                        *reinterpret_cast<uint4*>(vw[j]) = *reinterpret_cast<const uint4*>(vc);
+                        const uint4 u = *reinterpret_cast<const uint4*>(vp), w = *reinterpret_cast<const uint4*>(vp + 4);
+                        vs[j][0] = u.x, vs[j][1] = u.z, vs[j][2] = w.x, vs[j][3] = w.z;
+                    } else {
+                        *reinterpret_cast<uint2*>(vw[j]) = *reinterpret_cast<const uint2*>(vc);
+                        const uint4 u = *reinterpret_cast<const uint4*>(vp);
+                        vs[j][0] = u.x, vs[j][1] = u.z;
+                    }
+                    vm[j] = g < G ? vp[2 * (g & (G - 1)) + 1] : 0u;
+                }
+                if (edge) {
+                    // Tokens that no row sees count as zero, whatever the page holds there.  A token that some rows see and
+                    // others do not may be NaN for the first and must not touch the others: it is taken out of the products
+                    // and put back row by row.
+                    uint32_t nan_tokens[G] = {};
+                    bool any = false;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int tok = 2 * t + 8 * j + e;
+                            const uint32_t keep = e ? 0x0000ffffu : 0xffff0000u;
+                            const bool unseen = pos + tok >= kmax;
+#pragma unroll
+                            for (int w = 0; w < G; ++w) {
+                                const bool bad = ((vs[j][w] >> 16 * e) & 0x7c00u) == 0x7c00u;
+                                if (bad && !unseen) nan_tokens[w] |= 1u << tok, any = true;
+                                if (bad || unseen) vs[j][w] &= keep;
+                            }
+                            if (unseen || ((vm[j] >> 16 * e) & 0x7c00u) == 0x7c00u) vm[j] &= keep;
+                        }
+                    if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+                        for (int w = 0; w < G; ++w) {   // the quad holds all 16 tokens
+                            nan_tokens[w] |= __shfl_xor_sync(0xffffffffu, nan_tokens[w], 1);
+                            nan_tokens[w] |= __shfl_xor_sync(0xffffffffu, nan_tokens[w], 2);
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int seen = visible_keys(s, rt * ROWS + nt * 8 + 2 * t + e, group) - pos;
+                                const uint32_t mask = seen >= 16 ? 0xffffu : seen <= 0 ? 0u : (1u << seen) - 1;
+#pragma unroll
+                                for (int i = 0; i < MT; ++i)
+                                    if (nan_tokens[i / 2] & mask) o[nt][i][e] = o[nt][i][2 + e] = __int_as_float(0x7fffffff);
+                            }
+                    }
+                }
+                // ---- softmax
+                uint32_t large = 0;   // bit 14 of an fp16 value: 2 or more
+#pragma unroll
+                for (int w = 0; w < G; ++w) large |= vs[0][w] | vs[1][w];
+                bool grow = (large & 0x40004000u) != 0;
+                const float slack = kSlack - (float)shift;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const float2 f = *reinterpret_cast<const float2*>(&sm.factor[nt][2 * t]);
@@ -355,9 +441,22 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(KvAttnA
                         if (g + 8 >= s0) z[nt][2] = -INFINITY;
                         if (g + 8 >= s1) z[nt][3] = -INFINITY;
                     }
-                    grow = grow || fmaxf(z[nt][0], z[nt][2]) > mx[nt][0] + kSlack || fmaxf(z[nt][1], z[nt][3]) > mx[nt][1] + kSlack;
+                    grow = grow || fmaxf(z[nt][0], z[nt][2]) > mx[nt][0] + slack || fmaxf(z[nt][1], z[nt][3]) > mx[nt][1] + slack;
                 }
                 if (__any_sync(0xffffffffu, grow)) {
+                    int need = 0;   // exponent of the largest finite scale of the block
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int w = 0; w < G; ++w)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int ex = (int)(vs[j][w] >> (16 * e + 10) & 31u) - 15;
+                                if (ex < 16) need = max(need, ex);
+                            }
+                    need = max((int)__reduce_max_sync(0xffffffffu, (unsigned)need), shift) - shift;
+                    shift += need;
+                    const float fs = (float)shift;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float n0 = fmaxf(z[nt][0], z[nt][2]), n1 = fmaxf(z[nt][1], z[nt][3]);
@@ -366,13 +465,11 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(KvAttnA
                             n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, d));
                             n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, d));
                         }
-                        n0 = fmaxf(n0, mx[nt][0]), n1 = fmaxf(n1, mx[nt][1]);
+                        n0 = fmaxf(n0 + fs, mx[nt][0] + (float)need), n1 = fmaxf(n1 + fs, mx[nt][1] + (float)need);
                         const float r0 = mx[nt][0] == -INFINITY ? 0.f : exp2_approx(mx[nt][0] - n0);
                         const float r1 = mx[nt][1] == -INFINITY ? 0.f : exp2_approx(mx[nt][1] - n1);
                         mx[nt][0] = n0, mx[nt][1] = n1;
-                        sum[nt][0] *= r0, sum[nt][1] *= r1;
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) o[nt][i][0] *= r0, o[nt][i][1] *= r1, o[nt][i][2] *= r0, o[nt][i][3] *= r1;
+                        rescale(nt, r0, r1);
                     }
                 }
                 uint32_t b0[NT], b1[NT];
@@ -387,84 +484,49 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(KvAttnA
                     b0[nt] = transpose8x8(h2_bits(__floats2half2_rn(w0, w1)));
                     b1[nt] = transpose8x8(h2_bits(__floats2half2_rn(w2, w3)));
                 }
-                // values: tokens 2t, 2t+1 (j = 0) and 2t+8, 2t+9 (j = 1), D/8 channels of group vg
-                const int vg = g * G / 8;
-                uint32_t vw[2][D / 32];
-                __half2 vs[2], vm[2];
+                // ---- weighted values
+                {
+                    const uint32_t am[4] = {vm[0], 0u, vm[1], 0u};
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint8_t* vc = blk + L::kVCodes + j * 4 * D + lane * (D / 8);
-                    if constexpr (G == 4) *reinterpret_cast<uint4*>(vw[j]) = *reinterpret_cast<const uint4*>(vc);
-                    else *reinterpret_cast<uint2*>(vw[j]) = *reinterpret_cast<const uint2*>(vc);
-                    const uint2 p = *reinterpret_cast<const uint2*>(blk + L::kVParams + ((t + 4 * j) * G + vg) * 8);
-                    vs[j] = as_h2(p.x);
-                    vm[j] = as_h2(p.y);
+                    for (int nt = 0; nt < NT; ++nt) mma(om[nt], am, b0[nt], b1[nt]);
                 }
-                if (edge) {
-                    // Tokens that no row sees count as zero, whatever the page holds there.  A token that some rows see and
-                    // others do not may be NaN for the first and must not touch the others: it is taken out of the product
-                    // and put back row by row.
-                    uint32_t nan_tokens = 0;
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        uint32_t sb = h2_bits(vs[j]), mb = h2_bits(vm[j]);
+                for (int w = 0; w < G; ++w) {
+                    const uint32_t x0 = vw[0][w], x1 = vw[1][w], y0 = x0 >> 8, y1 = x1 >> 8;
+                    const uint32_t even[4] = {x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u};
+                    const uint32_t odd[4] = {y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u};
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int tok = 2 * t + 8 * j + e;
-                            const uint32_t keep = e ? 0x0000ffffu : 0xffff0000u;
-                            const bool bad = ((sb >> 16 * e) & 0x7c00u) == 0x7c00u || ((mb >> 16 * e) & 0x7c00u) == 0x7c00u;
-                            const bool unseen = pos + tok >= kmax;
-                            if (bad && !unseen) nan_tokens |= 1u << tok;
-                            if (bad || unseen) sb &= keep, mb &= keep;
-                        }
-                        vs[j] = as_h2(sb), vm[j] = as_h2(mb);
-                    }
-                    if (__any_sync(0xffffffffu, nan_tokens != 0)) {
-                        nan_tokens |= __shfl_xor_sync(0xffffffffu, nan_tokens, 1);   // the quad holds one group's 16 tokens
-                        nan_tokens |= __shfl_xor_sync(0xffffffffu, nan_tokens, 2);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int seen = visible_keys(s, rt * ROWS + nt * 8 + 2 * t + e, group) - pos;
-                                const uint32_t mask = seen >= 16 ? 0xffffu : seen <= 0 ? 0u : (1u << seen) - 1;
-                                if (nan_tokens & mask)
-#pragma unroll
-                                    for (int i = 0; i < MT; ++i) o[nt][i][e] = o[nt][i][2 + e] = __int_as_float(0x7fffffff);
-                            }
-                    }
-                }
-                const __half2 off_low = __half2half2(__ushort_as_half((unsigned short)0x6400));    // 1024: nibble at bit 0
-                const __half2 off_high = __half2half2(__ushort_as_half((unsigned short)0x5400));   // 64: nibble at bit 4
-#pragma unroll
-                for (int k = 0; k < D / 32; ++k) {
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {   // m-tile 2 k + u
-                        uint32_t av[4];
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const uint32_t w = u ? vw[j][k] >> 8 : vw[j][k];
-                            const __half2 lowc = __hsub2(as_h2((w & 0x000f000fu) | 0x64006400u), off_low);
-                            const __half2 highc = __hsub2(as_h2((w & 0x00f000f0u) | 0x54005400u), off_high);
-                            av[2 * j] = h2_bits(__hfma2(lowc, vs[j], vm[j]));
-                            av[2 * j + 1] = h2_bits(__hfma2(highc, vs[j], vm[j]));
-                        }
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma(o[nt][2 * k + u], av, b0[nt], b1[nt]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint32_t c0 = h2_bits(__hmul2(as_h2(b0[nt]), as_h2(vs[0][w]))), c1 = h2_bits(__hmul2(as_h2(b1[nt]), as_h2(vs[1][w])));
+                        mma(o[nt][2 * w], even, c0, c1);
+                        mma(o[nt][2 * w + 1], odd, c0, c1);
                     }
                 }
             }
             __syncwarp();
-            refill(done + 1 + kStages);
+            if (++stage == kStages) stage = 0, parity ^= 1;
+            refill();
         }
+        x = seg_end;
 
         // ---- join the four warps
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e) {
 #pragma unroll
                 for (int d = 4; d < 32; d *= 2) sum[nt][e] += __shfl_xor_sync(0xffffffffu, sum[nt][e], d);
+#pragma unroll
+                for (int w = 0; w < G; ++w) {
+                    const float m = __shfl_sync(0xffffffffu, om[nt][e], 4 * w + t);
+#pragma unroll
+                    for (int i = 2 * w; i < 2 * w + 2; ++i) {
+                        o[nt][i][e] = fmaf(o[nt][i][e], 0x1p24f, m);
+                        o[nt][i][2 + e] = fmaf(o[nt][i][2 + e], 0x1p20f, m);
+                    }
+                }
+            }
+        }
         if (warp) {
             float* dst = sm.merge[warp - 1];
 #pragma unroll
@@ -512,18 +574,14 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(KvAttnA
                     if (whole) {
                         const float inv = total_w == 0.f ? 0.f : 1.f / total_w;   // no visible key: zeros
                         const int r = rt * ROWS + row;
-                        uint32_t y[MT];
+                        uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + ((long long)(s.first + r / group) * a.q_heads + h * group + r % group) * D) + g;
 #pragma unroll
-                        for (int i = 0; i < MT; ++i) y[i] = h2_bits(__floats2half2_rn(o[nt][i][e] * inv, o[nt][i][2 + e] * inv));
-                        uint4* dst = reinterpret_cast<uint4*>(a.out + ((s.first + r / group) * a.q_heads + h * group + r % group) * D + g * (D / 8));
-#pragma unroll
-                        for (int i = 0; i < MT / 4; ++i) dst[i] = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                        for (int i = 0; i < MT; ++i) dst[8 * i] = h2_bits(__floats2half2_rn(o[nt][i][e] * inv, o[nt][i][2 + e] * inv));
                     } else {
                         float* slot = a.ws + (2 * (size_t)blockIdx.x + (seg_begin == pair_begin)) * slot_floats<D, ROWS>();
-                        float4* dst = reinterpret_cast<float4*>(slot + row * D + g * (D / 8));
+                        float2* dst = reinterpret_cast<float2*>(slot + row * D) + g;
 #pragma unroll
-                        for (int i = 0; i < MT / 2; ++i)
-                            dst[i] = make_float4(o[nt][2 * i][e], o[nt][2 * i][2 + e], o[nt][2 * i + 1][e], o[nt][2 * i + 1][2 + e]);
+                        for (int i = 0; i < MT; ++i) dst[8 * i] = make_float2(o[nt][i][e], o[nt][i][2 + e]);
                         if (g == 0) {
                             slot[ROWS * D + row] = e ? n1 : n0;
                             slot[ROWS * D + ROWS + row] = total_w;
@@ -534,7 +592,7 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(KvAttnA
         }
     }
     // only after a wait that ran out: give the copies still under way one more bounded wait before the memory goes away
-    for (; waited < issued; ++waited) wait_full(smem_u32(&sm.full[warp][waited % kStages]), (waited / kStages) & 1);
+    for (; waited < issued; ++waited) wait_full(bars + 8 * (waited % kStages), (waited / kStages) & 1);
 }
 
 // Adds the parts of the row tiles that were cut between thread blocks; one thread block per (key head and row tile,
@@ -545,37 +603,37 @@ __global__ void __launch_bounds__(128) kv_attention_join_kernel(KvAttnArgs a, in
     constexpr int ROWS = 8 * NT, V = D / 32;
     const KvView& c = a.c;
     const int group = a.q_heads / c.kv_heads, lane = threadIdx.x & 31;
-    const long long total = list_length<ROWS>(c, group);
-    if (total == 0) return;
+    // the lengths are none of the preceding kernel's results, and what wrote them had ended before that kernel let this one start
+    const int total = list_length<ROWS>(c, group);
     Seq s;
     load_seq<ROWS>(s, c, blockIdx.y, group);
-    long long begin = 0;
+    int begin = 0;
     for (int b = lane; b < (int)blockIdx.y; b += 32) {
         Seq o;
         load_seq<ROWS>(o, c, b, group);
         begin += o.total;
     }
-#pragma unroll
-    for (int o = 16; o; o /= 2) begin += __shfl_xor_sync(0xffffffffu, begin, o);
-    for (long long pair = blockIdx.x; pair < (long long)c.kv_heads * s.tiles; pair += gridDim.x) {
-        const int rt = (int)(pair % s.tiles), h = (int)(pair / s.tiles);
-        const long long p0 = begin + pair * s.units, p1 = p0 + s.units;
-        const int c0 = share_of(total, ctas, p0), c1 = share_of(total, ctas, p1 - 1);
+    begin = __reduce_add_sync(0xffffffffu, begin);
+    grid_wait();
+    if (total == 0) return;
+    const Shares shares(total, ctas);
+    for (int pair = blockIdx.x; pair < c.kv_heads * s.tiles; pair += gridDim.x) {
+        const int h = pair / s.tiles, rt = pair - h * s.tiles;
+        const int p0 = begin + pair * s.units, p1 = p0 + s.units;
+        const int c0 = shares.of(p0), c1 = shares.of(p1 - 1);
         if (c0 == c1) continue;
         const int rows = min(ROWS, s.qlen * group - rt * ROWS);
+        // the first part is the end of its thread block's share, the later ones start theirs (slot 0)
+        auto slot = [&](int i) { return a.ws + (2 * (size_t)i + (i == c0)) * slot_floats<D, ROWS>(); };
         for (int row = threadIdx.x / 32; row < rows; row += 4) {
-            auto slot = [&](int i) { return a.ws + (2 * (size_t)i + (share_begin(total, ctas, i) <= p0)) * slot_floats<D, ROWS>(); };
-            auto empty = [&](int i) { return share_begin(total, ctas, i) >= share_begin(total, ctas, i + 1); };
             float m = -INFINITY;
-            for (int i = c0 + lane; i <= c1; i += 32)
-                if (!empty(i)) m = fmaxf(m, slot(i)[ROWS * D + row]);
+            for (int i = c0 + lane; i <= c1; i += 32) m = fmaxf(m, slot(i)[ROWS * D + row]);
 #pragma unroll
             for (int d = 16; d; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
             const float z = m == -INFINITY ? 0.f : m;
             float acc[V] = {}, w = 0.f;
 #pragma unroll 4
             for (int i = c0; i <= c1; ++i) {
-                if (empty(i)) continue;
                 const float* p = slot(i);
                 const float r = exp2_approx(p[ROWS * D + row] - z);
                 w = fmaf(p[ROWS * D + ROWS + row], r, w);
@@ -590,7 +648,7 @@ __global__ void __launch_bounds__(128) kv_attention_join_kernel(KvAttnArgs a, in
             __half2 y[V / 2];
 #pragma unroll
             for (int k = 0; k < V / 2; ++k) y[k] = __floats2half2_rn(acc[2 * k] * inv, acc[2 * k + 1] * inv);
-            uint16_t* dst = a.out + ((s.first + r / group) * a.q_heads + h * group + r % group) * D + lane * V;
+            uint16_t* dst = a.out + ((long long)(s.first + r / group) * a.q_heads + h * group + r % group) * D + lane * V;
             if constexpr (V == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(y);
             else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(y);
         }
@@ -644,17 +702,32 @@ cudaError_t launch(cudaStream_t s, const KvAttnArgs& a, int* status)
     const int group = a.q_heads / a.c.kv_heads;
     const long long units = ((long long)a.c.table_stride * a.c.page_size + kUnit - 1) / kUnit;
     const long long tiles = ((long long)a.max_q * group + ROWS - 1) / ROWS;
-    const long long most = (long long)a.c.B * a.c.kv_heads * (tiles > 0 ? tiles : 1) * (units > 0 ? units : 1);
+    const long long most = (long long)a.c.B * a.c.kv_heads * (tiles > 0 ? tiles : 1) * units;
+    if (((long long)a.c.n_tokens * group / ROWS + a.c.B) * a.c.kv_heads * units > 0x7fffffff) {
+        set_error("kv_attention: too much work for one call (rows times context)");
+        return cudaErrorInvalidValue;
+    }
     if (most < ctas) ctas = (int)most;
-    kv_attention_split_kernel<D, NT><<<ctas, 32 * kWarps, sizeof(Smem<D, NT>), s>>>(a, status);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(32 * kWarps);
+    cfg.dynamicSmemBytes = sizeof(Smem<D, NT>);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kv_attention_split_kernel<D, NT>, a, status);
     count_launch();
-    e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    const long long pairs = a.c.kv_heads * tiles;
-    const dim3 grid((unsigned)(pairs < 65535 ? pairs : 65535), (unsigned)a.c.B);
-    kv_attention_join_kernel<D, NT><<<grid, 128, 0, s>>>(a, ctas);
+    const long long pairs = a.c.kv_heads * (tiles > 0 ? tiles : 1);
+    cfg.gridDim = dim3((unsigned)(pairs < 65535 ? pairs : 65535), (unsigned)a.c.B);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<D, NT>, a, ctas);
     count_launch();
-    return cudaGetLastError();
+    return e;
 }
 
 template <int D>
@@ -674,13 +747,12 @@ cudaError_t kv_attention_launch(cudaStream_t s, int D, const KvAttnArgs& a, int*
     return D == 128 ? launch_d<128>(s, a, status) : launch_d<64>(s, a, status);
 }
 
-// Workspace for the largest grid: two slots for each of at most 16 thread blocks per SM.
+// Workspace for the largest grid: two slots for each thread block that fits.
 size_t kv_attention_ws_floats(int D, int B, int q_heads, int kv_heads, int max_q)
 {
     (void)B;
     const int rows = 8 * pick_nt(max_q * (q_heads / kv_heads));
-    const int per_sm = rows == 8 ? 4 : rows == 16 ? 3 : 2;
-    return (size_t)2 * per_sm * sm_count() * rows * (D + 2);
+    return (size_t)2 * blocks_per_sm(rows / 8) * sm_count() * rows * (D + 2);
 }
 
 }  // namespace spb

@@ -13,9 +13,10 @@
 //             reads its row with one 16-byte (D = 128) or 8-byte load; and with 0x000f000f / 0x00f000f0 masks every
 //             register of the operand is one AND (after one shift for e >= 2).
 //   K params  [token][group] {s, m}
-//   V codes   the operand is V^T (channels x tokens): lane 4 g + t takes channels g D/8 .. g D/8 + D/8 - 1 of tokens 2t, 2t+1
-//             (first half, j = 0) and 2t + 8, 2t + 9 (j = 1).  Two tokens share a word: halfword (token & 1) holds four
-//             channels 4 k .. 4 k + 3 of the lane's D/8, one per nibble.  Byte address j * 16 D/4 + lane * D/8 + 4 k + 2 (token & 1).
+//   V codes   the operand is V^T (channels x tokens) in tiles of 16 channels: lane 4 g + t takes channels 16 i + 2 g and 16 i + 2 g + 1 of
+//             every tile i, tokens 2t, 2t+1 (first half, j = 0) and 2t + 8, 2t + 9 (j = 1).  Word k of a lane is group k, tiles
+//             2 k and 2 k + 1; halfword (token & 1) of it, byte (tile & 1), nibble (channel & 1).
+//             Byte address j * 4 D + (4 g + t) * D/8 + 4 k + 2 (token & 1) + (tile & 1).
 //   V params  [token pair][group] {s of the even token, s of the odd, m of the even, m of the odd}
 #pragma once
 #include "common.cuh"
@@ -41,7 +42,8 @@ struct KvView {
     const int* table;        // [B][table_stride] page numbers
     const int* lens;         // [B] tokens of each sequence in the cache, the new ones included
     const int* cu;           // [B + 1] first row of each sequence among the new tokens, or null: n_tokens / B each
-    long long n_tokens;      // rows of the packed new tokens
+    int n_tokens;            // rows of the packed new tokens
+    int per_seq;             // n_tokens / B
     int table_stride;        // entries a row of the table has
     int num_pages, page_size, kv_heads, B;
 };
@@ -74,13 +76,13 @@ cudaError_t kv_attention_launch(cudaStream_t s, int D, const KvAttnArgs& a, int*
 size_t kv_attention_ws_floats(int D, int B, int q_heads, int kv_heads, int max_q);
 
 // New tokens of sequence b: first row and count.  cu is the caller's: clamped, so that bad offsets cannot index outside.
-__device__ __forceinline__ void kv_rows(const KvView& c, int b, long long& first, long long& count)
+__device__ __forceinline__ void kv_rows(const KvView& c, int b, int& first, int& count)
 {
     if (c.cu) {
-        first = min(max((long long)c.cu[b], 0ll), c.n_tokens);
-        count = min(max((long long)c.cu[b + 1], first), c.n_tokens) - first;
+        first = min(max(c.cu[b], 0), c.n_tokens);
+        count = min(max(c.cu[b + 1], first), c.n_tokens) - first;
     } else {
-        count = c.n_tokens / c.B;
+        count = c.per_seq;
         first = count * b;
     }
 }
@@ -88,14 +90,13 @@ __device__ __forceinline__ void kv_rows(const KvView& c, int b, long long& first
 // Byte offset in the pool of the 16-token block that holds token `pos` of sequence b, head h; -1 when the table has no
 // usable page there (past its width, negative or not below num_pages).
 template <int D>
-__device__ __forceinline__ long long kv_block_offset(const KvView& c, int b, int h, long long pos)
+__device__ __forceinline__ long long kv_block_offset(const KvView& c, int b, int h, int pos)
 {
-    const long long pi = pos / c.page_size;
-    if (pi >= c.table_stride) return -1;
+    const unsigned pi = (unsigned)pos / (unsigned)c.page_size, in_page = (unsigned)pos - pi * c.page_size;
+    if (pi >= (unsigned)c.table_stride) return -1;
     const int page = c.table[(long long)b * c.table_stride + pi];
     if (page < 0 || page >= c.num_pages) return -1;
-    const long long blocks = c.page_size / kKvBlock;
-    return (((long long)page * c.kv_heads + h) * blocks + (pos % c.page_size) / kKvBlock) * KvLayout<D>::kBlockBytes;
+    return (((long long)page * c.kv_heads + h) * (c.page_size / kKvBlock) + in_page / kKvBlock) * KvLayout<D>::kBlockBytes;
 }
 
 }  // namespace spb

@@ -36,19 +36,29 @@ def rotate(x, pos, cos, sin, interleaved):
     return y.astype(np.float16).astype(np.float64)
 
 
-def attention(q, k, v, scale):
-    """q [T, Hq, D], k, v [L, Hkv, D] float64, row t sees keys 0 .. L - T + t.  Returns the output and the error that a kernel
-    with fp16 weights and values and fp32 sums may make.
+def scaled_codes(x):
+    """s c of what the cache holds for x: the part above the group's minimum."""
+    c, s, m = quantise(x)
+    return (c * s).reshape(x.shape)
 
-    Error: weights, values and the output are each rounded to fp16 (half a step, 2^-11, of sum p |v|, sum p |v| and |out|), the sum of
-    the weights is that of the unrounded ones (again 2^-11); a score is an fp32 sum of at most D/8 + 16 terms of magnitude
-    sum |q| |k| scale, so exp(score) is off by a factor of at most 2^-24 (D/8 + 16) of that, twice (numerator, denominator);
-    weights below the fp16 range lose at most 2^-32 of the largest each."""
+
+def attention(q, k, v, sc, scale):
+    """q [T, Hq, D], k, v, sc [L, Hkv, D] float64 (sc = scaled_codes of the values, v = m + sc), row t sees keys 0 .. L - T + t.
+    Returns the output and the error that a kernel with fp16 weights and fp32 sums may make.
+
+    The kernel sums p~ m + (p~ s)~ c, where ~ rounds to fp16, off by a factor 1 + d with |d| <= 2^-11:
+        p~ m + (p~ s)~ c = p (1 + d1) (m + (1 + d2) s c) = p v + d1 p v + (1 + d1) d2 p s c
+    so the weights cost 2^-11 sum p |v| and their products with the scales 2^-11 sum p s c (a little more, for d1 d2); the sum of
+    the weights is that of the unrounded ones, which costs another 2^-11 of sum p |v| at most; the output is rounded once, 2^-11
+    |out|.  A score is an fp32 sum of at most D/8 + 16 terms of magnitude sum |q| |k| scale (its part for the minima is taken
+    with group sums of q rounded to 22 bits, 2^-22 of sum |q| |k|, within four of the 2^-24 terms), so exp(score) is off by a
+    factor of at most 2^-24 (D/8 + 20) of that, twice (numerator, denominator); weights and their products below the fp16
+    range lose at most 2^-32 of the largest weight, or 2^-25 c in absolute terms after the factor 2^7 they carry, each."""
     T, Hq, D = q.shape
     L, Hkv = k.shape[:2]
     out, tol = np.zeros_like(q), np.zeros_like(q)
     for h in range(Hq):
-        kk, vv = k[:, h // (Hq // Hkv)], v[:, h // (Hq // Hkv)]
+        kk, vv, ss = (x[:, h // (Hq // Hkv)] for x in (k, v, sc))
         for t in range(T):
             n = L - T + t + 1
             if n <= 0:
@@ -60,8 +70,8 @@ def attention(q, k, v, scale):
             o = p @ vv[:n]
             a = p @ np.abs(vv[:n])
             out[t, h] = o
-            tol[t, h] = 3 * 2.0 ** -11 * a + 2.0 ** -11 * np.abs(o) + 2 * 2.0 ** -24 * (D / 8 + 16) * mag.max() * a \
-                + n * 2.0 ** -32 * np.abs(vv[:n]).max() + 2.0 ** -24
+            tol[t, h] = 2 * 2.0 ** -11 * a + 1.001 * 2.0 ** -11 * (p @ ss[:n]) + 2.0 ** -11 * np.abs(o) \
+                + 2 * 2.0 ** -24 * (D / 8 + 20) * mag.max() * a + n / w.sum() * (2.0 ** -32 * np.abs(vv[:n]).max() + 15 * 2.0 ** -32) + 2.0 ** -24
     return out, tol
 
 

@@ -59,7 +59,8 @@ class Batch:
         return self
 
     def held(self, b):
-        return model.entry(self.k[b].astype(np.float64)), model.entry(self.v[b].astype(np.float64))
+        v = self.v[b].astype(np.float64)
+        return model.entry(self.k[b].astype(np.float64)), model.entry(v), model.scaled_codes(v)
 
 
 def check_attention(sp, rng, bt, Hq, scale=None, uniform=False, q=None, **kw):
@@ -70,8 +71,8 @@ def check_attention(sp, rng, bt, Hq, scale=None, uniform=False, q=None, **kw):
     got = got.cpu().numpy().astype(np.float64)
     at = 0
     for b, t in enumerate(bt.q_lens):
-        k, v = bt.held(b)
-        want, tol = model.attention(q[at:at + t].astype(np.float64), k, v, bt.D ** -0.5 if scale is None else scale)
+        k, v, sc = bt.held(b)
+        want, tol = model.attention(q[at:at + t].astype(np.float64), k, v, sc, bt.D ** -0.5 if scale is None else scale)
         err = np.abs(got[at:at + t] - want)
         assert np.all(err <= tol), (b, t, bt.lens[b], float((err - tol).max()), float((err / np.maximum(tol, 1e-30)).max()))
         at += t
@@ -233,9 +234,9 @@ def test_rows_without_keys_get_zeros_and_rows_of_nobody_stay(sp):
     sp.kv_attention(q, bt.cache, bt.table, bt.kv_lens, cu_q=bt.cu, max_q=5, out=out)
     assert not bool(out[:2].any()) and not bool(out[2:5].any()) and bool((out[10:] == 7).all())
     for b, (first, t, skip) in {1: (5, 5, 3), 2: (7, 3, 0)}.items():
-        k, v = bt.held(b)
+        k, v, sc = bt.held(b)
         rows = slice(first, 7) if b == 1 else slice(7, 10)
-        want, tol = model.attention(q[rows].cpu().numpy().astype(np.float64), k, v, 0.125)
+        want, tol = model.attention(q[rows].cpu().numpy().astype(np.float64), k, v, sc, 0.125)
         assert np.all(np.abs(out[rows].cpu().numpy() - want) <= tol)
     assert sp.device_status() == 0
 
@@ -254,13 +255,13 @@ def test_garbage_behind_the_context_is_not_seen(sp, D):
     bt.fill()
     q = f16(rng, 6, 4, D)
     out = sp.kv_attention(dev(q), bt.cache, bt.table, bt.kv_lens).cpu().numpy().astype(np.float64)
-    k, v = bt.held(0)
+    k, v, sc = bt.held(0)
     bad = np.zeros((6, 4, D), bool)
     bad[3:, :2, 32:64] = True
     bad[5, 2:] = True
-    v[34, 0] = np.where(np.isnan(v[34, 0]), 0, v[34, 0])
+    v[34, 0], sc[34, 0] = np.where(np.isnan(v[34, 0]), 0, v[34, 0]), np.where(np.isnan(sc[34, 0]), 0, sc[34, 0])
     k[36, 1] = np.where(np.isnan(k[36, 1]), 0, k[36, 1])
-    want, tol = model.attention(q.astype(np.float64), k, v, D ** -0.5)
+    want, tol = model.attention(q.astype(np.float64), k, v, sc, D ** -0.5)
     assert np.isnan(out[bad]).all() and np.isfinite(out[~bad]).all()
     assert np.all(np.abs(out - want)[~bad] <= tol[~bad])
 
@@ -315,8 +316,8 @@ def test_attention_in_a_graph_follows_growing_contexts(sp):
         if i % 13 == 0 or i == steps - 1:
             got = out.cpu().numpy().astype(np.float64)
             for b in range(B):
-                kk, vv = bt.held(b)
-                want, tol = model.attention(qh[b:b + 1].astype(np.float64), kk[:at[b] + 1], vv[:at[b] + 1], D ** -0.5)
+                kk, vv, sc = bt.held(b)
+                want, tol = model.attention(qh[b:b + 1].astype(np.float64), kk[:at[b] + 1], vv[:at[b] + 1], sc[:at[b] + 1], D ** -0.5)
                 assert np.all(np.abs(got[b:b + 1] - want) <= tol)
     assert sp.device_status() == 0
 
