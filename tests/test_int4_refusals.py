@@ -80,3 +80,23 @@ def test_pack_encode_decode_refuse(lib_built):
     assert lib_built.spb_int4_pack(None, None, A, A, 64, 128, 64, A) != 0
     assert lib_built.spb_int4_encode(None, A, 64, 128, 64, None, A, A) != 0
     assert lib_built.spb_int4_decode(None, A, 64, 128, 64, A + 2) != 0
+
+
+def test_python_wrappers_refuse_before_any_call(lib_built):
+    """Tensors of the wrong kind are refused by name, on the CPU, before the library is asked."""
+    torch = pytest.importorskip("torch")
+    import spmspm_b200 as sp
+    for bad in (dict(head_dim=80), dict(page_size=20), dict(num_pages=0), dict(kv_heads=-1)):
+        with pytest.raises(sp.SpmmError):
+            sp.KvCacheInt4(**{**dict(num_pages=4, page_size=16, kv_heads=2, head_dim=64, device="cpu"), **bad})
+    with pytest.raises(sp.SpmmError, match="CUDA"):
+        sp.KvCacheInt4(4, 16, 2, 64, device="cpu")
+    codes, scales = torch.zeros((64, 128), dtype=torch.uint8), torch.zeros((64, 2), dtype=torch.float16)
+    with pytest.raises(sp.SpmmError, match="codes"):
+        sp.pack_int4(codes, scales, torch.zeros((64, 2), dtype=torch.uint8))
+    with pytest.raises(sp.SpmmError, match="group"):
+        sp.pack_int4(codes, scales[:, :1].expand(64, 32), codes)
+    with pytest.raises(sp.SpmmError):
+        sp.encode_int4(torch.zeros((64, 128), dtype=torch.float16))
+    with pytest.raises(sp.SpmmError, match="W.data"):
+        sp.linear_int4(sp.Int4Matrix(64, 128, 64, torch.zeros(9216, dtype=torch.uint8)), torch.zeros((1, 128), dtype=torch.float16))
