@@ -76,37 +76,37 @@ struct Seq {
     int begin = 0, total = 0;           // its range of the list
 };
 template <int ROWS>
-__device__ __forceinline__ void load_seq(Seq& s, const KvView& c, int b, int group)
+__device__ __forceinline__ void load_seq(Seq& s, const KvView& c, int b, int group, int tall)
 {
     kv_rows(c, b, s.first, s.qlen);
     s.b = b;
     s.len = max(c.lens[b], 0);
-    s.tiles = (s.qlen * group + ROWS - 1) / ROWS;
+    s.tiles = s.qlen * group >= tall ? 0 : (s.qlen * group + ROWS - 1) / ROWS;
     // tokens past the table's width have no page: they are not walked over
     const int held = (int)min((long long)s.len, (long long)c.table_stride * c.page_size);
     s.units = max((held - 1) / kUnit + 1, 1);
     s.total = c.kv_heads * s.tiles * s.units;
 }
 template <int ROWS>
-__device__ __forceinline__ int list_length(const KvView& c, int group)
+__device__ __forceinline__ int list_length(const KvView& c, int group, int tall)
 {
     int sum = 0;
     for (int b = threadIdx.x & 31; b < c.B; b += 32) {
         Seq s;
-        load_seq<ROWS>(s, c, b, group);
+        load_seq<ROWS>(s, c, b, group, tall);
         sum += s.total;
     }
     return __reduce_add_sync(0xffffffffu, sum);
 }
 // The sequence that holds unit x of the list (x inside the list); every lane gets the same.
 template <int ROWS>
-__device__ __forceinline__ void find_seq(Seq& s, const KvView& c, int group, int x)
+__device__ __forceinline__ void find_seq(Seq& s, const KvView& c, int group, int tall, int x)
 {
     const int lane = threadIdx.x & 31;
     int before = 0;
     for (int b0 = 0; b0 < c.B; b0 += 32) {
         Seq t;
-        if (b0 + lane < c.B) load_seq<ROWS>(t, c, b0 + lane, group);
+        if (b0 + lane < c.B) load_seq<ROWS>(t, c, b0 + lane, group, tall);
         int incl = t.total;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
@@ -117,7 +117,7 @@ __device__ __forceinline__ void find_seq(Seq& s, const KvView& c, int group, int
         if (past) {
             const int l = __ffs(past) - 1;
             const int begin = before + __shfl_sync(0xffffffffu, incl - t.total, l);
-            load_seq<ROWS>(s, c, b0 + l, group);
+            load_seq<ROWS>(s, c, b0 + l, group, tall);
             s.begin = begin;
             return;
         }
@@ -125,11 +125,11 @@ __device__ __forceinline__ void find_seq(Seq& s, const KvView& c, int group, int
     }
 }
 template <int ROWS>
-__device__ __forceinline__ void next_seq(Seq& s, const KvView& c, int group)
+__device__ __forceinline__ void next_seq(Seq& s, const KvView& c, int group, int tall)
 {
     do {
         const int end = s.begin + s.total;
-        load_seq<ROWS>(s, c, s.b + 1, group);
+        load_seq<ROWS>(s, c, s.b + 1, group, tall);
         s.begin = end;
     } while (s.total == 0 && s.b + 1 < c.B);
 }
@@ -185,17 +185,17 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
     grid_wait();
     grid_release();   // the join may be set up while this kernel runs; it waits for its end
 
-    const int total = list_length<ROWS>(c, group);
+    const int total = list_length<ROWS>(c, group, a.tall);
     const Shares shares(total, gridDim.x);
     const int lo = shares.begin(blockIdx.x), count = shares.begin(blockIdx.x + 1) - lo;
     if (count <= 0) return;
 
     // ---- this warp's copies: lane l looks after every 32nd unit of the share
     Seq s;
-    find_seq<ROWS>(s, c, group, lo);
+    find_seq<ROWS>(s, c, group, a.tall, lo);
     Seq ps = s;   // the lane's own place in the list
     auto block_of = [&](int x) -> long long {   // pool offset of this warp's block of unit x; -1: nothing to fetch
-        while (x >= ps.begin + ps.total) next_seq<ROWS>(ps, c, group);
+        while (x >= ps.begin + ps.total) next_seq<ROWS>(ps, c, group, a.tall);
         const int r = x - ps.begin, pair = r / ps.units, h = pair / ps.tiles, rt = pair - h * ps.tiles;
         const int pos = ((r - pair * ps.units) * kWarps + warp) * kKvBlock;
         const int last_row = min((rt + 1) * ROWS, ps.qlen * group) - 1;
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
     uint32_t parity = 0;
     const int hi = lo + count;
     while (x < hi) {
-        while (x >= s.begin + s.total) next_seq<ROWS>(s, c, group);
+        while (x >= s.begin + s.total) next_seq<ROWS>(s, c, group, a.tall);
         const int pair = (x - s.begin) / s.units, h = pair / s.tiles, rt = pair - h * s.tiles;
         const int pair_begin = s.begin + pair * s.units, pair_end = pair_begin + s.units;
         const int seg_begin = x, seg_end = min(hi, pair_end);
@@ -604,13 +604,13 @@ __global__ void __launch_bounds__(128) kv_attention_join_kernel(KvAttnArgs a, in
     const KvView& c = a.c;
     const int group = a.q_heads / c.kv_heads, lane = threadIdx.x & 31;
     // the lengths are none of the preceding kernel's results, and what wrote them had ended before that kernel let this one start
-    const int total = list_length<ROWS>(c, group);
+    const int total = list_length<ROWS>(c, group, a.tall);
     Seq s;
-    load_seq<ROWS>(s, c, blockIdx.y, group);
+    load_seq<ROWS>(s, c, blockIdx.y, group, a.tall);
     int begin = 0;
     for (int b = lane; b < (int)blockIdx.y; b += 32) {
         Seq o;
-        load_seq<ROWS>(o, c, b, group);
+        load_seq<ROWS>(o, c, b, group, a.tall);
         begin += o.total;
     }
     begin = __reduce_add_sync(0xffffffffu, begin);
@@ -742,8 +742,22 @@ cudaError_t launch_d(cudaStream_t s, const KvAttnArgs& a, int* status)
 
 }  // namespace
 
-cudaError_t kv_attention_launch(cudaStream_t s, int D, const KvAttnArgs& a, int* status)
+// Rows a key head from which a sequence goes to the tcgen05 kernel, whose row tiles have 128 rows; and how many of its thread
+// blocks there have to be, each of which walks over a whole context by itself (the split kernel shares one out among all SMs).
+constexpr int kTallRows = 64, kTallItems = 24;
+
+cudaError_t kv_attention_launch(cudaStream_t s, int D, const KvAttnArgs& args, int* status)
 {
+    KvAttnArgs a = args;
+    const int group = a.q_heads / a.c.kv_heads;
+    if (!a.c.cu) a.max_q = a.c.per_seq;
+    a.tall = 0x7fffffff;
+    if ((long long)a.max_q * group >= kTallRows && (((long long)a.c.n_tokens * group + 255) / 256) * a.c.kv_heads >= kTallItems) {
+        a.tall = kTallRows;
+        const cudaError_t e = kv_prefill_launch(s, D, a, a.tall, status);
+        if (e != cudaSuccess) return e;
+        if (!a.c.cu) return cudaSuccess;   // all sequences are alike
+    }
     return D == 128 ? launch_d<128>(s, a, status) : launch_d<64>(s, a, status);
 }
 

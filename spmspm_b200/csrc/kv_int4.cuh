@@ -69,10 +69,12 @@ struct KvAttnArgs {
     float scale;
     float* ws;
     size_t ws_floats;
+    int tall;          // sequences with this many rows a key head (new tokens times query heads that share it) go to kv_prefill
 };
 cudaError_t kv_append_launch(cudaStream_t s, int D, const KvAppendArgs& a, int* status);
 cudaError_t kv_read_launch(cudaStream_t s, int D, const KvReadArgs& a, int* status);
 cudaError_t kv_attention_launch(cudaStream_t s, int D, const KvAttnArgs& a, int* status);
+cudaError_t kv_prefill_launch(cudaStream_t s, int D, const KvAttnArgs& a, int tall, int* status);
 size_t kv_attention_ws_floats(int D, int B, int q_heads, int kv_heads, int max_q);
 
 // New tokens of sequence b: first row and count.  cu is the caller's: clamped, so that bad offsets cannot index outside.

@@ -53,25 +53,28 @@ def attention(q, k, v, sc, scale):
     |out|.  A score is an fp32 sum of at most D/8 + 16 terms of magnitude sum |q| |k| scale (its part for the minima is taken
     with group sums of q rounded to 22 bits, 2^-22 of sum |q| |k|, within four of the 2^-24 terms), so exp(score) is off by a
     factor of at most 2^-24 (D/8 + 20) of that, twice (numerator, denominator); weights and their products below the fp16
-    range lose at most 2^-32 of the largest weight, or 2^-25 c in absolute terms after the factor 2^7 they carry, each."""
+    range lose at most 2^-32 of the largest weight, or 2^-25 c in absolute terms after the factor 2^7 they carry, each.
+
+    The kernel for many rows sums p~ v with keys and values rounded to fp16: handed those (k and v as kv_read returns them, sc zero)
+    the same bound holds for it without its second term."""
     T, Hq, D = q.shape
     L, Hkv = k.shape[:2]
     out, tol = np.zeros_like(q), np.zeros_like(q)
+    seen = np.arange(L)[None] <= np.arange(L - T, L)[:, None]          # [T, L]
+    some = seen.any(1)
     for h in range(Hq):
         kk, vv, ss = (x[:, h // (Hq // Hkv)] for x in (k, v, sc))
-        for t in range(T):
-            n = L - T + t + 1
-            if n <= 0:
-                continue
-            z = (kk[:n] @ q[t, h]) * scale
-            mag = (np.abs(kk[:n]) @ np.abs(q[t, h])) * abs(scale)
-            w = np.exp(z - z.max())
-            p = w / w.sum()
-            o = p @ vv[:n]
-            a = p @ np.abs(vv[:n])
-            out[t, h] = o
-            tol[t, h] = 2 * 2.0 ** -11 * a + 1.001 * 2.0 ** -11 * (p @ ss[:n]) + 2.0 ** -11 * np.abs(o) \
-                + 2 * 2.0 ** -24 * (D / 8 + 20) * mag.max() * a + n / w.sum() * (2.0 ** -32 * np.abs(vv[:n]).max() + 15 * 2.0 ** -32) + 2.0 ** -24
+        with np.errstate(invalid="ignore"):
+            z = np.where(seen, (q[:, h] @ kk.T) * scale, -np.inf)
+            mag = np.where(seen, (np.abs(q[:, h]) @ np.abs(kk).T) * abs(scale), 0).max(1, initial=0)[:, None]
+            w = np.where(some[:, None], np.exp(z - z.max(1, initial=-np.inf, keepdims=True)), 0)
+            total = np.where(some, w.sum(1), 1)[:, None]
+        p = w / total
+        o, a = p @ vv, p @ np.abs(vv)
+        biggest = np.where(seen[:, :, None], np.abs(vv)[None], 0).max((1, 2), initial=0)[:, None] if L * T * D < 1 << 24 else np.abs(vv).max()
+        out[:, h] = o
+        tol[:, h] = 2 * 2.0 ** -11 * a + 1.001 * 2.0 ** -11 * (p @ ss) + 2.0 ** -11 * np.abs(o) \
+            + 2 * 2.0 ** -24 * (D / 8 + 20) * mag * a + seen.sum(1)[:, None] / total * (2.0 ** -32 * biggest + 15 * 2.0 ** -32) + 2.0 ** -24
     return out, tol
 
 

@@ -63,6 +63,22 @@ class Batch:
         return model.entry(self.k[b].astype(np.float64)), model.entry(v), model.scaled_codes(v)
 
 
+def is_tall(bt, Hq, t):
+    """Whether a sequence with t new tokens goes to the kernel for many rows, which takes keys and values as kv_read returns them."""
+    group = Hq // bt.heads
+    return (max(bt.q_lens) * group >= 64 and -(-sum(bt.q_lens) * group // 256) * bt.heads >= 24 and t * group >= 64)
+
+
+def reference(bt, b, q, Hq, scale, tweak=None):
+    k, v, sc = bt.held(b)
+    if is_tall(bt, Hq, bt.q_lens[b]):
+        with np.errstate(over="ignore"):
+            k, v, sc = k.astype(np.float16).astype(np.float64), v.astype(np.float16).astype(np.float64), 0 * sc
+    if tweak is not None:
+        tweak(k, v, sc)
+    return model.attention(q.astype(np.float64), k, v, sc, scale)
+
+
 def check_attention(sp, rng, bt, Hq, scale=None, uniform=False, q=None, **kw):
     n = sum(bt.q_lens)
     q = f16(rng, n, Hq, bt.D) if q is None else q
@@ -71,8 +87,7 @@ def check_attention(sp, rng, bt, Hq, scale=None, uniform=False, q=None, **kw):
     got = got.cpu().numpy().astype(np.float64)
     at = 0
     for b, t in enumerate(bt.q_lens):
-        k, v, sc = bt.held(b)
-        want, tol = model.attention(q[at:at + t].astype(np.float64), k, v, sc, bt.D ** -0.5 if scale is None else scale)
+        want, tol = reference(bt, b, q[at:at + t], Hq, bt.D ** -0.5 if scale is None else scale)
         err = np.abs(got[at:at + t] - want)
         assert np.all(err <= tol), (b, t, bt.lens[b], float((err - tol).max()), float((err / np.maximum(tol, 1e-30)).max()))
         at += t
@@ -205,6 +220,74 @@ def test_several_new_tokens_are_causal(sp, D, Hkv, group, lens, q_lens):
     rng = np.random.default_rng(D + group + sum(lens))
     bt = Batch(sp, rng, lens, q_lens, Hkv, D, 32).fill()
     check_attention(sp, rng, bt, Hkv * group)
+
+
+@pytest.mark.parametrize("D,Hkv,group", [(128, 24, 1), (64, 24, 1), (128, 8, 8), (64, 8, 5), (128, 24, 2)])
+@pytest.mark.parametrize("lens,q_lens", [((128,), (128,)), ((300, 70, 513), (299, 64, 129)), ((257, 40, 9, 700), (256, 3, 0, 65)), ((1000, 90), (130, 90))])
+def test_many_new_tokens(sp, D, Hkv, group, lens, q_lens):
+    """Prompts and chunks, with short sequences among them: row tiles that end inside, that see nothing of a key tile, odd groups."""
+    rng = np.random.default_rng(D + group + sum(lens))
+    bt = Batch(sp, rng, lens, q_lens, Hkv, D, 16 if D == 64 else 64).fill()
+    assert any(is_tall(bt, Hkv * group, t) for t in q_lens)
+    check_attention(sp, rng, bt, Hkv * group)
+
+
+def test_many_new_tokens_uniform_and_without_a_bound(sp):
+    rng = np.random.default_rng(21)
+    bt = Batch(sp, rng, (150, 140), (140, 140), 24, 64, 32).fill()
+    check_attention(sp, rng, bt, 24, uniform=True)
+    q = dev(f16(rng, 280, 24, 64))
+    want = sp.kv_attention(q, bt.cache, bt.table, bt.kv_lens)
+    assert torch.equal(sp.kv_attention(q, bt.cache, bt.table, bt.kv_lens, cu_q=bt.cu), want)
+    assert torch.equal(sp.kv_attention(q, bt.cache, bt.table, bt.kv_lens, max_q=280), want)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_new_tokens_with_nothing_to_see_and_nan(sp, D):
+    """More new tokens than the cache holds; NaN behind the context, and in values and keys that only some rows may see."""
+    rng = np.random.default_rng(22)
+    bt = Batch(sp, rng, (150, 400, 0), (200, 300, 70), 24, D, 64)
+    bt.cache.pool.view(torch.float16).fill_(float("nan"))
+    bt.k[0], bt.v[0] = bt.k[0][:150], bt.v[0][:150]
+    bt.v[1][230, 3, 40] = np.nan       # rows 130.. of the second sequence see token 230
+    bt.k[1][399, 5, 3] = np.inf        # its last row alone sees token 399
+    bt.fill()
+    q = f16(rng, 570, 24, D)
+    out = sp.kv_attention(dev(q), bt.cache, bt.table, bt.kv_lens, cu_q=bt.cu, max_q=300).cpu().numpy().astype(np.float64)
+    assert not out[:50].any() and not out[500:].any()
+    want, tol = reference(bt, 0, q[50:200], 24, D ** -0.5)
+    assert np.all(np.abs(out[50:200] - want) <= tol)
+
+    def tweak(k, v, sc):
+        v[np.isnan(v)] = 0
+        k[np.isnan(k)] = 0
+        sc[np.isnan(sc)] = 0
+    want, tol = reference(bt, 1, q[200:500], 24, D ** -0.5, tweak)
+    got = out[200:500]
+    bad = np.zeros(got.shape, bool)
+    bad[130:, 3, 32:64] = True
+    bad[299, 5] = True
+    assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all()
+    assert np.all(np.abs(got - want)[~bad] <= tol[~bad])
+    assert sp.device_status() == 0
+
+
+def test_many_new_tokens_bad_pages(sp):
+    """A page number outside the pool: its tokens count as unseen, the rest as if they were all there is."""
+    rng = np.random.default_rng(23)
+    bt = Batch(sp, rng, (320,), (100,), 24, 64, 64).fill()
+    q = f16(rng, 100, 24, 64)
+    table = bt.table_h.copy()
+    table[0, 1] = 1000
+    sp.reset_device_status()
+    out = sp.kv_attention(dev(q), bt.cache, dev(table), bt.kv_lens, max_q=100).cpu().numpy().astype(np.float64)
+    assert sp.device_status() == 8
+    sp.reset_device_status()
+    k, v, sc = bt.held(0)
+    keep = np.r_[0:64, 128:320]
+    want, tol = model.attention(q.astype(np.float64), k[keep].astype(np.float16).astype(np.float64), v[keep].astype(np.float16).astype(np.float64),
+                                0 * sc[keep], 0.125)
+    assert np.all(np.abs(out - want) <= tol)
 
 
 def test_many_sequences_and_empty_ones(sp):
