@@ -104,5 +104,24 @@ def load():
     return _lib
 
 
+_ext = None
+
+
+def ext():
+    """The extension that calls the 4-bit operators from tensors (csrc/torch_ext.cpp), on the library that load() has loaded."""
+    global _ext
+    if _ext is None:
+        load()
+        try:
+            from . import _torch_ext
+        except ImportError as e:
+            raise RuntimeError(f"spmspm_b200/_torch_ext.so cannot be loaded ({e}): build it with "
+                               "`python -c 'import __graft_entry__ as g; g.build()'`. There is no fallback path.") from e
+        from .api import SpmmError
+        _torch_ext.init(LIB_PATH, SpmmError)
+        _ext = _torch_ext
+    return _ext
+
+
 def last_error():
     return load().spb_last_error().decode()

@@ -33,18 +33,6 @@ def _stream_ptr(stream=None):
     return ctypes.c_void_p(s.cuda_stream)
 
 
-def _call(name, dev, stream, *args):
-    """Library entry point on the tensors' device, on `stream` or torch's current one there."""
-    fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == dev:
-        code = fn(stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(dev), *args)
-    else:
-        with torch.cuda.device(dev):
-            code = fn(stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(dev), *args)
-    if code:
-        _check(code, name)
-
-
 # --------------------------------------------------------------------------- encoder (host)
 
 @dataclass

@@ -1,0 +1,281 @@
+// Python calls of the 4-bit operators, straight from tensors to the C entry points.
+//
+// A decode step makes these calls with kernels of a few microseconds, so that checking the arguments and marshalling them
+// in Python took longer than the work (attention 17 us of host time, 8 of them launches).  The checks are the wrappers' own:
+// kind, type, shape, layout and device of every tensor; sizes and alignment are checked again behind the C boundary.  The
+// library is the one spmspm_b200._lib has loaded.
+#include <torch/csrc/utils/pybind.h>
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <dlfcn.h>
+
+#include <cmath>
+#include <optional>
+#include <string>
+
+#include "../../include/spmm_b200.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+PyObject* g_error = nullptr;
+decltype(&spb_last_error) p_last_error;
+decltype(&spb_kv_append) p_kv_append;
+decltype(&spb_kv_read) p_kv_read;
+decltype(&spb_kv_attention) p_kv_attention;
+decltype(&spb_kv_attention_workspace_bytes) p_kv_attention_workspace_bytes;
+decltype(&spb_linear_int4) p_linear_int4;
+decltype(&spb_int4_workspace_bytes) p_int4_workspace_bytes;
+decltype(&spb_int4_bytes) p_int4_bytes;
+
+[[noreturn]] void fail(const std::string& what)
+{
+    PyErr_SetString(g_error, what.c_str());
+    throw py::error_already_set();
+}
+void check(int code, const char* name)
+{
+    if (code) fail(std::string(name) + " failed: cudaError " + std::to_string(code) + ": " + p_last_error());
+}
+std::string shape_text(at::IntArrayRef s)
+{
+    std::string t = "[";
+    for (size_t i = 0; i < s.size(); ++i) t += (i ? ", " : "") + std::to_string(s[i]);
+    return t + "]";
+}
+
+void init(const std::string& path, py::object error)
+{
+    void* lib = dlopen(path.c_str(), RTLD_NOW);
+    if (!lib) throw std::runtime_error(dlerror());
+    auto get = [&](auto& f, const char* name) {
+        f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(dlsym(lib, name));
+        if (!f) throw std::runtime_error(std::string(name) + " is missing in " + path);
+    };
+    get(p_last_error, "spb_last_error");
+    get(p_kv_append, "spb_kv_append");
+    get(p_kv_read, "spb_kv_read");
+    get(p_kv_attention, "spb_kv_attention");
+    get(p_kv_attention_workspace_bytes, "spb_kv_attention_workspace_bytes");
+    get(p_linear_int4, "spb_linear_int4");
+    get(p_int4_workspace_bytes, "spb_int4_workspace_bytes");
+    get(p_int4_bytes, "spb_int4_bytes");
+    g_error = error.release().ptr();
+}
+
+// Device and stream of a call: the tensors' device is made current, the stream is the given one or torch's current one there.
+struct Place {
+    c10::cuda::CUDAGuard guard;
+    c10::cuda::CUDAStream stream;
+    bool given;
+    Place(int dev, std::optional<int64_t> s)
+        : guard((c10::DeviceIndex)dev),
+          stream(s ? c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(*s), (c10::DeviceIndex)dev) : c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev)),
+          given(s.has_value())
+    {
+    }
+    void* ptr() const { return stream.stream(); }
+    // a new workspace; its memory must not go to another tensor before a stream given by hand is done with it
+    Tensor workspace(size_t bytes, const Tensor& like) const
+    {
+        Tensor w = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+        if (given) w.record_stream(stream.unwrap());
+        return w;
+    }
+};
+// Workspace of the caller, or a new one.
+Tensor pick_workspace(const Place& at_, const OptTensor& given, size_t need, const Tensor& like, const char* where, size_t& have)
+{
+    if (!given) {
+        have = need;
+        return need ? at_.workspace(need, like) : Tensor();
+    }
+    have = given->nbytes();
+    if (!given->is_cuda() || given->device() != like.device() || !given->is_contiguous() || have < need)
+        fail("the workspace must be a contiguous CUDA tensor of at least " + std::to_string(need) + " bytes on the " + where + "'s device");
+    return *given;
+}
+void dense_half(const Tensor& t, const char* name, at::IntArrayRef shape, c10::Device dev, const char* where)
+{
+    if (t.device() != dev || t.scalar_type() != at::kHalf || !t.is_contiguous() || t.sizes() != shape)
+        fail(std::string(name) + " must be a contiguous CUDA float16 " + shape_text(shape) + " tensor on the " + where + "'s device");
+}
+
+// ---------------------------------------------------------------------------------------------------- 4-bit cache
+
+struct Cache {
+    Tensor pool;
+    int num_pages, page_size, kv_heads, head_dim;
+};
+struct Batch {
+    const int *table, *lens, *cu;
+    int width, batch;
+};
+Batch check_batch(const Cache& c, const Tensor& table, const Tensor& lens, const OptTensor& cu)
+{
+    const auto dev = c.pool.device();
+    if (table.device() != dev || table.scalar_type() != at::kInt || table.dim() != 2 || !table.is_contiguous() || !table.numel())
+        fail("page_table must be a contiguous CUDA int32 [batch, pages] tensor on the cache's device");
+    const int64_t n = table.size(0);
+    if (lens.device() != dev || lens.scalar_type() != at::kInt || lens.dim() != 1 || lens.size(0) != n || !lens.is_contiguous())
+        fail("kv_lens must be a contiguous CUDA int32 [" + std::to_string(n) + "] tensor on the cache's device");
+    if (cu && (cu->device() != dev || cu->scalar_type() != at::kInt || cu->dim() != 1 || cu->size(0) != n + 1 || !cu->is_contiguous()))
+        fail("cu_q must be a contiguous CUDA int32 [" + std::to_string(n + 1) + "] tensor on the cache's device");
+    return {table.const_data_ptr<int>(), lens.const_data_ptr<int>(), cu ? cu->const_data_ptr<int>() : nullptr, (int)table.size(1), (int)n};
+}
+// [tokens, heads, head_dim] with contiguous channels and strides that hold four channels together
+const uint16_t* check_vectors(const Cache& c, const Tensor& t, const char* name, int64_t tokens, int64_t heads)
+{
+    if (t.device() != c.pool.device() || t.scalar_type() != at::kHalf || t.dim() != 3 || t.size(2) != c.head_dim || (heads >= 0 && t.size(1) != heads) ||
+        (tokens >= 0 && t.size(0) != tokens))
+        fail(std::string(name) + " must be a CUDA float16 [" + (tokens >= 0 ? std::to_string(tokens) : "tokens") + ", " +
+             (heads >= 0 ? std::to_string(heads) : "heads") + ", " + std::to_string(c.head_dim) + "] tensor on the cache's device");
+    const auto* p = static_cast<const uint16_t*>(t.const_data_ptr());
+    if (t.numel() && (t.stride(2) != 1 || t.stride(0) & 3 || t.stride(1) & 3 || reinterpret_cast<uintptr_t>(p) & 7))
+        fail(std::string(name) + " must have contiguous channels, strides that are multiples of 4 and an 8-byte aligned start");
+    return p;
+}
+void check_rows(int64_t n, const Batch& b)
+{
+    if (!b.cu && n % b.batch) fail("without cu_q the tokens must divide evenly among the sequences");
+}
+
+OptTensor kv_append(const Cache& c, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lens, const OptTensor& cu, const OptTensor& q,
+                    const OptTensor& cos, const OptTensor& sin, bool interleaved, const OptTensor& q_out, std::optional<int64_t> stream)
+{
+    const Batch b = check_batch(c, table, lens, cu);
+    const uint16_t* kp = check_vectors(c, k, "k", -1, c.kv_heads);
+    const int64_t n = k.size(0);
+    const uint16_t* vp = check_vectors(c, v, "v", n, c.kv_heads);
+    check_rows(n, b);
+    if (cos.has_value() != sin.has_value()) fail("cos and sin are given together");
+    int64_t rot = 0, max_pos = 0;
+    if (cos) {
+        for (const auto* t : {&*cos, &*sin})
+            if (t->device() != c.pool.device() || t->scalar_type() != at::kFloat || t->dim() != 2 || !t->is_contiguous() || t->sizes() != cos->sizes() || !t->size(0))
+                fail(std::string(t == &*cos ? "cos" : "sin") + " must be a contiguous CUDA float32 [positions, rot/2] tensor on the cache's device");
+        max_pos = cos->size(0), rot = 2 * cos->size(1);
+        if (rot == 0 || rot % 8 || rot > c.head_dim) fail("the rotated channels must be a multiple of 8 up to head_dim");
+    }
+    OptTensor out;
+    const uint16_t* qp = nullptr;
+    if (!q && q_out) fail("q_out without q");
+    if (q) {
+        if (!cos) fail("q is only taken to be rotated: cos and sin are missing");
+        qp = check_vectors(c, *q, "q", n, -1);
+        if (!q->size(1)) fail("q has no heads");
+        if (q_out) {
+            dense_half(*q_out, "q_out", q->sizes(), c.pool.device(), "cache");
+            out = *q_out;
+        } else {
+            out = at::empty(q->sizes(), q->options());
+        }
+    }
+    if (n) {
+        const Place at_(c.pool.get_device(), stream);
+        check(p_kv_append(at_.ptr(), c.pool.data_ptr(), c.num_pages, c.page_size, c.kv_heads, c.head_dim, b.table, b.width, b.lens, b.cu, b.batch, n, kp,
+                          k.stride(0), k.stride(1), vp, v.stride(0), v.stride(1), qp, q ? q->stride(0) : 0, q ? q->stride(1) : 0, q ? (int)q->size(1) : 0,
+                          out ? static_cast<uint16_t*>(out->data_ptr()) : nullptr, cos ? cos->const_data_ptr<float>() : nullptr,
+                          sin ? sin->const_data_ptr<float>() : nullptr, (int)max_pos, (int)rot, interleaved),
+              "spb_kv_append");
+    }
+    return out;
+}
+
+std::pair<Tensor, Tensor> kv_read(const Cache& c, const Tensor& table, const Tensor& lens, const OptTensor& cu, std::optional<int64_t> n_tokens,
+                                  const OptTensor& k_out, const OptTensor& v_out, std::optional<int64_t> stream)
+{
+    const Batch b = check_batch(c, table, lens, cu);
+    if (!n_tokens && !k_out) fail("n_tokens or k_out is needed");
+    const int64_t n = n_tokens ? *n_tokens : k_out->dim() ? k_out->size(0) : 0;
+    if (n < 0) fail("n_tokens must not be negative");
+    check_rows(n, b);
+    const int64_t shape[3] = {n, c.kv_heads, c.head_dim};
+    auto make = [&](const OptTensor& given, const char* name) {
+        if (!given) return at::empty(shape, c.pool.options().dtype(at::kHalf));
+        dense_half(*given, name, shape, c.pool.device(), "cache");
+        return *given;
+    };
+    Tensor k = make(k_out, "k_out"), v = make(v_out, "v_out");
+    if (n) {
+        const Place at_(c.pool.get_device(), stream);
+        check(p_kv_read(at_.ptr(), c.pool.data_ptr(), c.num_pages, c.page_size, c.kv_heads, c.head_dim, b.table, b.width, b.lens, b.cu, b.batch, n,
+                        static_cast<uint16_t*>(k.data_ptr()), static_cast<uint16_t*>(v.data_ptr())),
+              "spb_kv_read");
+    }
+    return {k, v};
+}
+
+size_t kv_attention_workspace(const Cache& c, int64_t q_heads, int64_t batch, int64_t max_q)
+{
+    const c10::cuda::CUDAGuard guard(c.pool.device());
+    return p_kv_attention_workspace_bytes(c.head_dim, (int)batch, (int)q_heads, c.kv_heads, (int)max_q);
+}
+
+Tensor kv_attention(const Tensor& q, const Cache& c, const Tensor& table, const Tensor& lens, const OptTensor& cu, std::optional<int64_t> max_q,
+                    std::optional<double> scale, const OptTensor& out_given, const OptTensor& ws_given, std::optional<int64_t> stream)
+{
+    const Batch b = check_batch(c, table, lens, cu);
+    const uint16_t* qp = check_vectors(c, q, "q", -1, -1);
+    const int64_t n = q.size(0), heads = q.size(1);
+    if (!heads || heads % c.kv_heads) fail("the heads of q must be a positive multiple of the cache's");
+    check_rows(n, b);
+    const int64_t most = max_q ? *max_q : b.cu ? n : n / b.batch;
+    if (most < 0 || most > n) fail("max_q must be in 0..tokens");
+    if (out_given) dense_half(*out_given, "out", q.sizes(), c.pool.device(), "cache");
+    Tensor out = out_given ? *out_given : at::empty(q.sizes(), q.options());
+    if (!n) return out;
+    const Place at_(c.pool.get_device(), stream);
+    size_t have;
+    const Tensor ws = pick_workspace(at_, ws_given, p_kv_attention_workspace_bytes(c.head_dim, b.batch, (int)heads, c.kv_heads, (int)most), q, "cache", have);
+    check(p_kv_attention(at_.ptr(), c.pool.data_ptr(), c.num_pages, c.page_size, c.kv_heads, c.head_dim, b.table, b.width, b.lens, b.cu, b.batch, n, qp,
+                         q.stride(0), q.stride(1), (int)heads, (int)most, (float)(scale ? *scale : 1 / std::sqrt((double)c.head_dim)),
+                         static_cast<uint16_t*>(out.data_ptr()), ws.data_ptr(), have),
+          "spb_kv_attention");
+    return out;
+}
+
+// -------------------------------------------------------------------------------------------------- 4-bit weights
+
+Tensor linear_int4(const Tensor& data, int64_t M, int64_t K, int64_t group, const Tensor& x, const OptTensor& bias, const OptTensor& residual,
+                   int64_t activation, const OptTensor& out_given, const OptTensor& ws_given, std::optional<int64_t> stream)
+{
+    const auto dev = data.device();
+    const size_t bytes = p_int4_bytes((int)M, (int)K, (int)group);
+    if (!bytes) fail("M and K must be positive multiples of 64 and the group 32, 64 or 128 and divide K");
+    if (!data.is_cuda() || data.scalar_type() != at::kByte || !data.is_contiguous() || data.dim() != 1 || (size_t)data.size(0) != bytes)
+        fail("W.data must be the contiguous CUDA uint8 tensor that pack_int4 made");
+    if (x.device() != dev || x.scalar_type() != at::kHalf || x.dim() != 2 || x.size(1) != K || !x.size(0) || !x.is_contiguous())
+        fail("B must be a contiguous CUDA float16 [N,K] tensor on the weight's device");
+    const int64_t N = x.size(0), shape[2] = {N, M};
+    if (activation != 0 && activation != 1) fail("activation must be ACT_NONE or ACT_RELU");
+    if (bias && (bias->device() != dev || bias->scalar_type() != at::kHalf || !bias->is_contiguous() || bias->dim() != 1 || bias->size(0) != M))
+        fail("bias must be a contiguous CUDA float16 [M] tensor");
+    if (residual) dense_half(*residual, "residual", shape, dev, "weight");
+    if (out_given) dense_half(*out_given, "out", shape, dev, "weight");
+    Tensor out = out_given ? *out_given : at::empty(shape, x.options());
+    const Place at_(data.get_device(), stream);
+    size_t have;
+    const Tensor ws = pick_workspace(at_, ws_given, p_int4_workspace_bytes((int)M, (int)N, (int)K), x, "weight", have);
+    auto half = [](const OptTensor& t) { return t ? static_cast<const uint16_t*>(t->const_data_ptr()) : nullptr; };
+    check(p_linear_int4(at_.ptr(), data.const_data_ptr(), (int)M, (int)K, (int)group, static_cast<const uint16_t*>(x.const_data_ptr()),
+                        static_cast<uint16_t*>(out.data_ptr()), (int)N, half(bias), half(residual), (int)activation, ws.defined() ? ws.data_ptr() : nullptr, have),
+          "spb_linear_int4");
+    return out;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_torch_ext, m)
+{
+    m.def("init", &init);
+    py::class_<Cache>(m, "Cache").def(py::init([](Tensor pool, int pages, int page_size, int heads, int dim) { return Cache{pool, pages, page_size, heads, dim}; }));
+    m.def("kv_append", &kv_append);
+    m.def("kv_read", &kv_read);
+    m.def("kv_attention", &kv_attention);
+    m.def("kv_attention_workspace", &kv_attention_workspace);
+    m.def("linear_int4", &linear_int4);
+}

@@ -2,13 +2,12 @@
 
 Weight (m, k) is s (c - z): code c and zero point z in 0..15, scale s fp16, both shared by 32, 64 or 128 consecutive k.
 """
-import functools
 from dataclasses import dataclass
 
 import torch
 
 from . import _lib
-from .api import ACT_NONE, SpmmError, _call, _check, _check_tail, _ptr, _stream_ptr
+from .api import ACT_NONE, SpmmError, _check, _ptr, _stream_ptr
 
 
 @dataclass
@@ -70,17 +69,9 @@ def encode_int4(A, group=128, stream=None):
     return pack_int4(codes, scales, zeros, stream)
 
 
-@functools.lru_cache(maxsize=1024)
-def _bytes(M, K, group):
-    _shape(M, K, group)
-    return _lib.load().spb_int4_bytes(M, K, group)
-
-
 def _check_matrix(W):
-    data = W.data
-    if not data.is_cuda or data.dtype is not torch.uint8 or not data.is_contiguous() or data.shape != (_bytes(W.M, W.K, W.group),):
-        raise SpmmError("W.data must be the contiguous CUDA uint8 tensor that pack_int4 made")
-    return data
+    _shape(W.M, W.K, W.group)
+    _need(W.data, "W.data", torch.uint8, (_lib.load().spb_int4_bytes(W.M, W.K, W.group),))
 
 
 def decode_int4(W: Int4Matrix, out=None, stream=None):
@@ -94,44 +85,13 @@ def decode_int4(W: Int4Matrix, out=None, stream=None):
     return out
 
 
-@functools.lru_cache(maxsize=4096)
-def _workspace_bytes(dev, M, N, K):
-    with torch.cuda.device(dev):
-        return _lib.load().spb_int4_workspace_bytes(M, N, K)
-
-
 def int4_workspace(W, N):
     """Bytes of the workspace `linear_int4` needs for N rows (0 for many shapes)."""
-    return _workspace_bytes(W.data.get_device(), W.M, N, W.K)
+    with torch.cuda.device(W.data.device):
+        return _lib.load().spb_int4_workspace_bytes(W.M, N, W.K)
 
 
 def linear_int4(W: Int4Matrix, B, bias=None, residual=None, activation=ACT_NONE, out=None, workspace=None, stream=None):
     """spb_linear_int4: out[N,M] = residual + act(B W^T + bias), summed in fp32 and rounded to fp16 once.  B [N,K] as in
     `linear`; out may be the residual itself, not B.  workspace: int4_workspace(W, N) bytes; a new one by default."""
-    data = _check_matrix(W)
-    dev = data.get_device()
-    shape = B.shape
-    if B.get_device() != dev or B.dtype is not torch.float16 or len(shape) != 2 or shape[1] != W.K or not shape[0] or not B.is_contiguous():
-        raise SpmmError("B must be a contiguous CUDA float16 [N,K] tensor on the weight's device")
-    N = shape[0]
-    if bias is not None or residual is not None or activation != ACT_NONE:
-        _check_tail(W.M, N, bias, residual, activation, B.device)
-    if out is None:
-        out = torch.empty((N, W.M), dtype=torch.float16, device=B.device)
-    elif out.get_device() != dev or out.dtype is not torch.float16 or not out.is_contiguous() or out.shape != (N, W.M):
-        raise SpmmError("out must be a contiguous CUDA float16 [N,M] tensor")
-    need = _workspace_bytes(dev, W.M, N, W.K)
-    if workspace is None:
-        have, ws = need, None
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=B.device)
-            if stream is not None:
-                workspace.record_stream(stream)   # its memory must not go to another tensor before that stream is done with it
-            ws = workspace.data_ptr()
-    else:
-        have, ws = workspace.numel() * workspace.element_size(), workspace.data_ptr()
-        if workspace.get_device() != dev or not workspace.is_contiguous() or have < need:
-            raise SpmmError(f"the workspace must be a contiguous CUDA tensor of at least {need} bytes on the weight's device")
-    _call("spb_linear_int4", dev, stream, data.data_ptr(), W.M, W.K, W.group, B.data_ptr(), out.data_ptr(), N,
-          None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(), int(activation), ws, have)
-    return out
+    return _lib.ext().linear_int4(W.data, W.M, W.K, W.group, B, bias, residual, activation, out, workspace, None if stream is None else stream.cuda_stream)
