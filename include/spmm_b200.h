@@ -369,7 +369,7 @@ int spb_linear_int4(void* stream, const void* packed, int M, int K, int group, c
  *                     workspace: spb_kv_attention_workspace_bytes bytes, 16-byte aligned, need not be cleared; not shared by
  *                     calls that may run at the same time.
  * k, v and q are fp16 with contiguous channels; token and head strides in elements, multiples of 4; pointers 8-byte aligned
- * (out and the workspace 16).  The same bits come out for the same call on the same device.
+ * (out, q_out, the angle tables and the workspace 16).  The same bits come out for the same call on the same device.
  */
 size_t spb_kv_cache_bytes(int num_pages, int page_size, int kv_heads, int head_dim);
 int spb_kv_append(void* stream, void* pool, int num_pages, int page_size, int kv_heads, int head_dim, const int* page_table,

@@ -101,11 +101,15 @@ int spb_kv_append(void* stream, void* pool, int num_pages, int page_size, int kv
         set_error("%s: rot_dim must be a multiple of 8 up to head_dim and max_pos positive (rot_dim=%d max_pos=%d)", who, rot_dim, max_pos);
         return (int)cudaErrorInvalidValue;
     }
-    if (cos_table && ((reinterpret_cast<uintptr_t>(cos_table) | reinterpret_cast<uintptr_t>(sin_table)) & 3)) {
-        set_error("%s: cos_table and sin_table must be 4-byte aligned", who);
+    if (cos_table && ((reinterpret_cast<uintptr_t>(cos_table) | reinterpret_cast<uintptr_t>(sin_table)) & 15)) {
+        set_error("%s: cos_table and sin_table must be 16-byte aligned", who);
         return (int)cudaErrorInvalidValue;
     }
     if (q) {
+        if (!aligned16(q_out)) {
+            set_error("%s: q_out must be 16-byte aligned", who);
+            return (int)cudaErrorInvalidValue;
+        }
         if (!check_vectors(who, "q", q, q_token_stride, q_head_stride) || !check_vectors(who, "q_out", q_out, 0, 0)) return (int)cudaErrorInvalidValue;
         if (!cos_table) {
             set_error("%s: q is only taken to be rotated: cos_table and sin_table are missing", who);

@@ -1,8 +1,8 @@
 // Writing and reading the paged 4-bit key/value cache (layout: kv_int4.cuh).
 //
-// kv_append: one pass over the new tokens.  A vector (one head of one token) is held by D/4 lanes, four channels each;
+// kv_append: one pass over the new tokens.  A vector (one head of one token) is held by D/8 lanes, eight channels each;
 // keys and queries are turned by their position's angles, the minimum and maximum of every 32 channels are found with
-// three shuffles among eight lanes, and the codes go straight to their places in the block.
+// two shuffles among four lanes, and the codes go straight to their places in the block.
 //
 //   rotation   y = (a cos - b sin, b cos + a sin), exact up to 2^-48 and rounded once to fp16, so that the codes that follow do
 //              not depend on how the sum was taken (in 32 bits one value in some thousands would land on the other
@@ -44,26 +44,63 @@ __device__ __forceinline__ bool locate(const KvView& c, int tok, int& b, int& po
     return true;
 }
 
-__device__ __forceinline__ void load4(const uint16_t* p, __half (&x)[4])
-{
-    const uint2 r = *reinterpret_cast<const uint2*>(p);
-    *reinterpret_cast<uint2*>(x) = r;
-}
+// Tokens of the packed input one after the other, with the place of each in the cache; searched for once per sequence.
+struct Cursor {
+    int b = 0, pos = -1, end = 0;   // end: first row behind the sequence
+    long long off = -1;             // offset of the token's block in the pool, -1: none
+    __device__ __forceinline__ bool move_to(const KvView& c, int tok)
+    {
+        if (tok < end) {
+            ++pos;
+            return true;
+        }
+        const bool found = tok < c.n_tokens && locate(c, tok, b, pos);
+        end = !found ? 0 : c.cu ? c.cu[b + 1] : (b + 1) * c.per_seq;
+        off = -1;
+        return found;
+    }
+    template <int D>
+    __device__ __forceinline__ bool find_block(const KvView& c, int head)
+    {
+        if (off < 0 || pos % kKvBlock == 0) off = kv_block_offset<D>(c, b, head, pos);
+        return off >= 0;
+    }
+};
+
+__device__ __forceinline__ void load4(const uint16_t* p, __half (&x)[4]) { *reinterpret_cast<uint2*>(x) = *reinterpret_cast<const uint2*>(p); }
+
 // a * c + b * d rounded once to fp16.  Both products are taken exactly as pairs of fp32 values, and so is the sum, up to 2^-48 of its
 // larger term; the last step to fp32 rounds to odd (an inexact result gets its last bit set), which keeps the rounding
 // to fp16 right.  Fp32 throughout: the conversions that 64-bit arithmetic needs run at an eighth of its rate.
-__device__ __forceinline__ __half turn(__half ah, float c, __half bh, float d)
+__device__ __forceinline__ __half turn_exactly(float a, float c, float b, float d)
 {
-    const float a = __half2float(ah), b = __half2float(bh);
     const float p = __fmul_rn(a, c), q = __fmul_rn(b, d);
     const float pl = __fmaf_rn(a, c, -p), ql = __fmaf_rn(b, d, -q);
     const float s = __fadd_rn(p, q), z = __fsub_rn(s, p);
     const float e = __fadd_rn(__fsub_rn(p, __fsub_rn(s, z)), __fsub_rn(q, z));   // s + e = p + q
     const float t = __fadd_rn(e, __fadd_rn(pl, ql));
     const float f = __fadd_rn(s, t), rest = __fsub_rn(t, __fsub_rn(f, s));
+    if (!(fabsf(s) <= 3e38f)) return __float2half_rn(s);   // infinities and NaN as the plain sum has them
     uint32_t bits = __float_as_uint(f);
     if (rest != 0.f && !(bits & 1u)) bits += (rest > 0.f) == (f > 0.f) ? 1u : 0xffffffffu;
     return __float2half_rn(__uint_as_float(bits));
+}
+// Four of them.  In plain fp32 a sum is off by less than 2^-23 of |b d| + |sum|: when both ends of that range round to the same fp16
+// value it is the right one, and only otherwise (one value in a thousand) is the exact form worked out.
+__device__ __forceinline__ void turn4(const float (&a)[4], const float (&c)[4], const float (&b)[4], const float (&d)[4], __half (&y)[4])
+{
+    uint32_t differ = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float p = b[i] * d[i], s = fmaf(a[i], c[i], p), e = (fabsf(p) + fabsf(s)) * 0x1p-23f;
+        const __half2 ends = __floats2half2_rn(s - e, s + e);
+        y[i] = __low2half(ends);
+        const uint32_t bits = *reinterpret_cast<const uint32_t*>(&ends);
+        differ |= (bits ^ bits >> 16) & 0xffffu;
+    }
+    if (differ)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = turn_exactly(a[i], c[i], b[i], d[i]);
 }
 
 // The vector's channels c0 .. c0 + 3, turned by the angles of position pos.
@@ -72,178 +109,185 @@ __device__ __forceinline__ void load_turned(const uint16_t* vec, int c0, const K
     load4(vec + c0, x);
     if (c0 >= a.rot) return;
     const int half_rot = a.rot / 2;
-    const float* cs = a.cosv + (long long)pos * half_rot;
-    const float* sn = a.sinv + (long long)pos * half_rot;
-    if (a.interleaved) {
+    float u[4], w[4], c[4], s[4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float c = cs[c0 / 2 + i], s = sn[c0 / 2 + i];
-            const __half u = x[2 * i], w = x[2 * i + 1];
-            x[2 * i] = turn(u, c, w, -s);
-            x[2 * i + 1] = turn(w, c, u, s);
-        }
+    for (int i = 0; i < 4; ++i) u[i] = __half2float(x[i]);
+    if (a.interleaved) {
+        const float2 cc = *reinterpret_cast<const float2*>(a.cosv + (long long)pos * half_rot + c0 / 2);
+        const float2 ss = *reinterpret_cast<const float2*>(a.sinv + (long long)pos * half_rot + c0 / 2);
+        c[0] = c[1] = cc.x, c[2] = c[3] = cc.y;
+        s[0] = -ss.x, s[1] = ss.x, s[2] = -ss.y, s[3] = ss.y;
+        w[0] = u[1], w[1] = u[0], w[2] = u[3], w[3] = u[2];
     } else {
         const bool upper = c0 >= half_rot;   // half_rot is a multiple of 4: all four channels on one side
         const int i0 = upper ? c0 - half_rot : c0;
         __half o[4];
         load4(vec + (upper ? c0 - half_rot : c0 + half_rot), o);
+        *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(a.cosv + (long long)pos * half_rot + i0);
+        *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(a.sinv + (long long)pos * half_rot + i0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = turn(x[i], cs[i0 + i], o[i], upper ? sn[i0 + i] : -sn[i0 + i]);
+        for (int i = 0; i < 4; ++i) w[i] = __half2float(o[i]), s[i] = upper ? s[i] : -s[i];
     }
+    turn4(u, c, w, s, x);
 }
 
-// One vector per D/4 lanes; the vectors of a token are its keys, its values and, when q is given, its queries.  A warp goes through
-// `rows` consecutive tokens of the packed input for its vectors: one for a few tokens, more for many, so that finding the token's
-// place is paid once.
+// One vector per D/8 lanes, eight channels each; the vectors of a token are its keys, its values and, when q is given, its queries.  A
+// warp goes through `rows` consecutive tokens of the packed input for its vectors: one for a few tokens, more for many, so
+// that finding the token's place is paid once.
 template <int D>
 __global__ void __launch_bounds__(32 * kWarps) kv_append_kernel(KvAppendArgs a, int rows, int* status)
 {
     using L = KvLayout<D>;
-    constexpr int kLanes = D / 4, kPer = 32 / kLanes;
-    const int lane = threadIdx.x & 31, sub = lane % kLanes, c0 = 4 * sub;
+    constexpr int kLanes = D / 8, kPer = 32 / kLanes;
+    const int lane = threadIdx.x & 31, sub = lane % kLanes, c0 = 8 * sub;
     const unsigned vecs = 2 * a.c.kv_heads + (a.q ? a.q_heads : 0);
     const unsigned item = (blockIdx.x * kWarps + threadIdx.x / 32) * kPer + lane / kLanes;
     const unsigned chunk = item / vecs, vec = item - chunk * vecs;
     const bool is_q = vec >= 2 * a.c.kv_heads, is_v = !is_q && vec >= a.c.kv_heads;
     const int head = is_q ? vec - 2 * a.c.kv_heads : is_v ? vec - a.c.kv_heads : vec;
-    int b = 0, pos = -1, end = 0;   // end: first row behind the sequence
+    const uint16_t* src = is_q ? a.q + head * a.q_head : is_v ? a.v + head * a.v_head : a.k + head * a.k_head;
+    const long long step = is_q ? a.q_tok : is_v ? a.v_tok : a.k_tok;
+    const bool turned = a.cosv && !is_v;
+    Cursor at;
     for (int i = 0; i < rows; ++i) {
         const int tok = (int)chunk * rows + i;
-        bool write = tok < a.c.n_tokens;
-        if (write) {
-            if (tok < end) ++pos;
-            else {
-                write = locate(a.c, tok, b, pos);
-                end = !write ? 0 : a.c.cu ? a.c.cu[b + 1] : (b + 1) * a.c.per_seq;
-            }
-        }
-        write = write && pos >= 0;
-        if (write && a.cosv && !is_v && pos >= a.max_pos) {   // no angles for this position
+        bool write = at.move_to(a.c, tok) && at.pos >= 0;
+        if (write && turned && at.pos >= a.max_pos) {   // no angles for this position
             if (sub == 0) atomicOr(status, kStatusBadCache);
             write = false;
         }
-        __half x[4] = {};
+        __half x[2][4] = {};
         if (write) {
-            if (is_v) load4(a.v + (long long)tok * a.v_tok + head * a.v_head + c0, x);
-            else {
-                const uint16_t* src = is_q ? a.q + (long long)tok * a.q_tok + head * a.q_head : a.k + (long long)tok * a.k_tok + head * a.k_head;
-                if (a.cosv) load_turned(src, c0, a, pos, x);
-                else load4(src + c0, x);
+            const uint16_t* p = src + tok * step;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                if (turned) load_turned(p, c0 + 4 * k, a, at.pos, x[k]);
+                else load4(p + c0 + 4 * k, x[k]);
             }
         }
         if (is_q) {
-            if (write) *reinterpret_cast<uint2*>(a.q_out + ((long long)tok * a.q_heads + head) * D + c0) = *reinterpret_cast<uint2*>(x);
+            if (write) *reinterpret_cast<uint4*>(a.q_out + ((long long)tok * a.q_heads + head) * D + c0) = *reinterpret_cast<uint4*>(x);
             write = false;
         }
         if (!__any_sync(0xffffffffu, write)) continue;
-        // minimum and maximum of the eight lanes that hold a group; every lane of the warp takes part
-        float f[4], lo, hi;
+        // minimum and maximum of the four lanes that hold a group, as {min, -max}; NaN spreads, every lane of the warp takes part
+        const __half2* h2 = reinterpret_cast<const __half2*>(x);
+        const __half2 lo2 = __hmin2_nan(__hmin2_nan(h2[0], h2[1]), __hmin2_nan(h2[2], h2[3]));
+        const __half2 hi2 = __hmax2_nan(__hmax2_nan(h2[0], h2[1]), __hmax2_nan(h2[2], h2[3]));
+        __half2 ends = __hmin2_nan(__lows2half2(lo2, __hneg2(hi2)), __highs2half2(lo2, __hneg2(hi2)));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) f[k] = __half2float(x[k]);
-        lo = fminf(fminf(f[0], f[1]), fminf(f[2], f[3]));
-        hi = fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
-        // a value that is not finite makes this NaN, and the sum of the group's
-        float bad = (f[0] - f[0]) + (f[1] - f[1]) + (f[2] - f[2]) + (f[3] - f[3]);
-#pragma unroll
-        for (int o = 1; o < 8; o *= 2) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            bad += __shfl_xor_sync(0xffffffffu, bad, o);
+        for (int o = 1; o < 4; o *= 2) {
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<uint32_t*>(&ends), o);
+            ends = __hmin2_nan(ends, *reinterpret_cast<const __half2*>(&other));
         }
-        const bool finite = bad == 0.f;
-        // every step rounded down: 15 times an fp16 value is an fp32 value, so nothing falls below the largest fp16 that fits
-        __half s = __float2half_rd(__fdiv_rd(__fsub_rd(hi, lo), 15.f)), m = __float2half_rn(lo);
-        const float sf = __half2float(s), inv = __frcp_rn(sf);
-        uint32_t code[4];
+        const float lo = __low2float(ends), hi = -__high2float(ends);
+        const bool finite = lo >= -65504.f && hi <= 65504.f;
+        // s: the largest fp16 value with 15 s <= hi - lo.  A factor a little above 1/15 cannot fall below it and is one value too high at
+        // most; 15 s is exact in fp32, and so is the comparison with the difference rounded down.
+        const float span = __fsub_rd(hi, lo);
+        __half s = __float2half_rd(span * 0x1.111116p-4f);
+        if (15.f * __half2float(s) > span) s = __ushort_as_half((unsigned short)(__half_as_ushort(s) - 1));
+        const float sf = __half2float(s), inv = __fdividef(1.f, sf);
+        uint32_t code[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            // The quotient by the reciprocal is off by less than 2^-19; only next to a border of two codes is it divided out.
-            const float d = __fsub_rn(f[k], lo);
+        for (int k = 0; k < 8; ++k) {
+            // The quotient by the reciprocal is off by less than 2^-18; only next to a border of two codes is it divided out.
+            const float d = __fsub_rn(__half2float(x[k / 4][k % 4]), lo);
             float q = d * inv, n = rintf(q);
             if (fabsf(fabsf(q - n) - 0.5f) < 0x1p-16f) n = rintf(__fdiv_rn(d, sf));
-            code[k] = finite && sf > 0.f ? (uint32_t)fminf(n, 15.f) : 0u;
+            code[k] = (uint32_t)fminf(n, 15.f);
         }
+        __half m = __float2half_rn(lo);
+        const bool plain = finite && sf > 0.f;   // a constant group has no codes
         if (!finite) s = m = __ushort_as_half((unsigned short)0x7fff);
-        // keys: two lanes, four apart, share a word; values: they exchange the bytes of neighbouring channel pairs
-        const uint32_t kbits = code[0] | code[1] << 16 | code[2] << 8 | code[3] << 24;
-        const uint32_t low = code[0] | code[1] << 4, high = code[2] | code[3] << 4;
-        const bool upper = sub & 4;
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, is_v ? (upper ? low : high) : kbits, 4);
+        // Keys: words t and t + 1 of the group; this lane has the nibbles of one of their two halves, the lane two away those of the
+        // other.  Values: a byte for each of four channel pairs, whose other byte of the halfword that lane has.
+        uint32_t mine[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint32_t* c = code + 4 * k;
+            mine[k] = !plain ? 0u : is_v ? c[0] | c[1] << 4 | (c[2] | c[3] << 4) << 16 : c[0] | c[1] << 16 | c[2] << 8 | c[3] << 24;
+        }
+        const bool upper = sub & 2;
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine[upper ? 0 : 1], 2), kept = mine[upper ? 1 : 0];
+        const uint32_t word = upper ? other | kept << (is_v ? 8 : 4) : kept | other << (is_v ? 8 : 4);
         if (!write) continue;
-        const long long off = kv_block_offset<D>(a.c, b, head, pos);
-        if (off < 0) {
+        if (!at.find_block<D>(a.c, head)) {
             if (sub == 0) atomicOr(status, kStatusBadCache);
             continue;
         }
-        uint8_t* blk = a.c.pool + off;
-        const int t16 = pos % kKvBlock, grp = sub / 8;
+        uint8_t* blk = a.c.pool + at.off;
+        const int t16 = at.pos % kKvBlock, grp = sub / 4, pair = 2 * (sub & 1) + upper;   // the word or the two channel pairs this lane stores
         if (!is_v) {
-            if (!upper) reinterpret_cast<uint32_t*>(blk + L::kKCodes)[t16 * (D / 8) + (sub & 3) * L::kGroups + grp] = kbits | other << 4;
-            if ((sub & 7) == 0) reinterpret_cast<__half2*>(blk + L::kKParams)[t16 * L::kGroups + grp] = __halves2half2(s, m);
+            reinterpret_cast<uint32_t*>(blk + L::kKCodes)[t16 * (D / 8) + pair * L::kGroups + grp] = word;
+            if ((sub & 3) == 0) reinterpret_cast<__half2*>(blk + L::kKParams)[t16 * L::kGroups + grp] = __halves2half2(s, m);
         } else {
-            const int j = t16 / 8, t = (t16 % 8) / 2, e = t16 & 1, g = 2 * (sub & 3) + upper;
-            *reinterpret_cast<uint16_t*>(blk + L::kVCodes + j * 4 * D + (4 * g + t) * (D / 8) + 4 * grp + 2 * e) = (uint16_t)(upper ? other | high << 8 : low | other << 8);
-            if ((sub & 7) == 0) {
-                __half* p = reinterpret_cast<__half*>(blk + L::kVParams) + ((t16 / 2) * L::kGroups + grp) * 4 + e;
-                p[0] = s;
-                p[2] = m;
+            const int j = t16 / 8, t = (t16 % 8) / 2, e = t16 & 1;
+            uint8_t* p = blk + L::kVCodes + j * 4 * D + (4 * 2 * pair + t) * (D / 8) + 4 * grp + 2 * e;
+            *reinterpret_cast<uint16_t*>(p) = (uint16_t)word;
+            *reinterpret_cast<uint16_t*>(p + 4 * (D / 8)) = (uint16_t)(word >> 16);
+            if ((sub & 3) == 0) {
+                __half* q = reinterpret_cast<__half*>(blk + L::kVParams) + ((t16 / 2) * L::kGroups + grp) * 4 + e;
+                q[0] = s;
+                q[2] = m;
             }
         }
     }
 }
 
-// The values of one vector, four channels a lane: m + code * s with one rounding.
+// The values of one vector, eight channels a lane: m + code * s with one rounding.
 template <int D>
 __global__ void __launch_bounds__(32 * kWarps) kv_read_kernel(KvReadArgs a, int rows, int* status)
 {
     using L = KvLayout<D>;
-    constexpr int kLanes = D / 4, kPer = 32 / kLanes;
-    const int lane = threadIdx.x & 31, sub = lane % kLanes, c0 = 4 * sub, grp = sub / 8;
+    constexpr int kLanes = D / 8, kPer = 32 / kLanes;
+    const int lane = threadIdx.x & 31, sub = lane % kLanes, c0 = 8 * sub, grp = sub / 4;
     const unsigned vecs = 2 * a.c.kv_heads;
     const unsigned item = (blockIdx.x * kWarps + threadIdx.x / 32) * kPer + lane / kLanes;
     const unsigned chunk = item / vecs, vec = item - chunk * vecs;
     const bool is_v = vec >= a.c.kv_heads;
     const int head = is_v ? vec - a.c.kv_heads : vec;
-    int b = 0, pos = -1, end = 0;
+    uint16_t* out = (is_v ? a.v : a.k) + head * D + c0;
+    Cursor at;
     for (int i = 0; i < rows; ++i) {
         const int tok = (int)chunk * rows + i;
-        if (tok >= a.c.n_tokens) return;
-        if (tok < end) ++pos;
-        else {
-            if (!locate(a.c, tok, b, pos)) continue;
-            end = a.c.cu ? a.c.cu[b + 1] : (b + 1) * a.c.per_seq;
-        }
-        uint16_t* dst = (is_v ? a.v : a.k) + ((long long)tok * a.c.kv_heads + head) * D + c0;
-        const long long off = pos >= 0 ? kv_block_offset<D>(a.c, b, head, pos) : -1;
-        if (off < 0) {
-            if (pos >= 0 && sub == 0) atomicOr(status, kStatusBadCache);
-            *reinterpret_cast<uint2*>(dst) = make_uint2(0, 0);
+        if (!at.move_to(a.c, tok)) continue;
+        uint16_t* dst = out + (long long)tok * a.c.kv_heads * D;
+        if (at.pos < 0 || !at.find_block<D>(a.c, head)) {
+            if (at.pos >= 0 && sub == 0) atomicOr(status, kStatusBadCache);
+            *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(dst + 4) = make_uint2(0, 0);
             continue;
         }
-        const uint8_t* blk = a.c.pool + off;
-        const int t16 = pos % kKvBlock;
-        uint32_t pair[2];   // codes as fp16: 1024 + code
+        const uint8_t* blk = a.c.pool + at.off;
+        const int t16 = at.pos % kKvBlock;
+        uint32_t pair[4];   // two codes each, in the low nibbles of the halves
         __half s, m;
         if (!is_v) {
-            const uint32_t w = reinterpret_cast<const uint32_t*>(blk + L::kKCodes)[t16 * (D / 8) + (sub & 3) * L::kGroups + grp] >> ((sub & 4) ? 4 : 0);
-            pair[0] = w & 0x000f000fu, pair[1] = w >> 8 & 0x000f000fu;
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(blk + L::kKCodes) + t16 * (D / 8) + 2 * (sub & 1) * L::kGroups + grp;
+            const int shift = (sub & 2) ? 4 : 0;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) pair[2 * k] = w[k * L::kGroups] >> shift & 0x000f000fu, pair[2 * k + 1] = w[k * L::kGroups] >> (8 + shift) & 0x000f000fu;
             const __half2 p = reinterpret_cast<const __half2*>(blk + L::kKParams)[t16 * L::kGroups + grp];
             s = __low2half(p), m = __high2half(p);
         } else {
-            const int j = t16 / 8, t = (t16 % 8) / 2, e = t16 & 1, g = 2 * (sub & 3);
-            const uint8_t* at = blk + L::kVCodes + j * 4 * D + (4 * g + t) * (D / 8) + 4 * grp + 2 * e + (sub >> 2 & 1);
-            const uint32_t low = at[0], high = at[4 * (D / 8)];
-            pair[0] = (low & 15) | (low & 240) << 12, pair[1] = (high & 15) | (high & 240) << 12;
-            const __half* p = reinterpret_cast<const __half*>(blk + L::kVParams) + ((t16 / 2) * L::kGroups + grp) * 4 + e;
-            s = p[0], m = p[2];
-        }
-        __half2 y[2];
+            const int j = t16 / 8, t = (t16 % 8) / 2, e = t16 & 1;
+            const uint8_t* p = blk + L::kVCodes + j * 4 * D + (4 * 4 * (sub & 1) + t) * (D / 8) + 4 * grp + 2 * e + (sub >> 1 & 1);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const uint32_t c = pair[k] | 0x64006400u;
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t c = p[4 * k * (D / 8)];
+                pair[k] = (c & 15) | (c & 240) << 12;
+            }
+            const __half* q = reinterpret_cast<const __half*>(blk + L::kVParams) + ((t16 / 2) * L::kGroups + grp) * 4 + e;
+            s = q[0], m = q[2];
+        }
+        __half2 y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t c = pair[k] | 0x64006400u;   // 1024 + code
             y[k] = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), __half2half2(__ushort_as_half((unsigned short)0x6400))), __half2half2(s), __half2half2(m));
         }
         *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(y);
+        *reinterpret_cast<uint2*>(dst + 4) = *reinterpret_cast<uint2*>(y + 2);
     }
 }
 
@@ -252,7 +296,7 @@ int rows_for(long long vectors) { return vectors >= 8ll * 64 * 150 ? 8 : 1; }
 template <int D>
 unsigned blocks_for(int n_tokens, int rows, int vecs)
 {
-    const long long items = (n_tokens + rows - 1ll) / rows * vecs, per = kWarps * (32 / (D / 4));
+    const long long items = (n_tokens + rows - 1ll) / rows * vecs, per = kWarps * (32 / (D / 8));
     return (unsigned)((items + per - 1) / per);
 }
 
