@@ -17,11 +17,11 @@
 //            instruction per 16 tokens.  Scales of 2 and more would leave the fp16 range: the whole row is then shifted down by
 //            the scale's exponent, as if its maximum had grown.
 //
-// Work: the context is cut in units of 64 tokens (four warps, one 16-token block each); all units of all (sequence, key
+// Work: the context is cut in units of 128 or 64 tokens (four warps, two 16-token blocks or one each); all units of all (sequence, key
 // head, row tile) are laid end to end and every thread block takes an equal share, found from the lengths on the device.
 // A share that covers a whole row tile is finished where it is; the others leave fp32 (O, max, sum) in the workspace,
 // two slots a thread block, and kv_attention_join_kernel adds them in order: no atomics, the same bits every time.
-// Every warp streams its own blocks: one bulk copy per block into its own ring, nobody waits for another warp except at
+// Every warp streams its own blocks: bulk copies into its own ring, nobody waits for another warp except at
 // the end of a row tile.
 #include "kv_int4.cuh"
 #include "sm100.cuh"
@@ -32,10 +32,13 @@ namespace {
 using namespace sm100;
 
 constexpr int kWarps = 4;
-constexpr int kStages = 3;                 // 16-token blocks in flight per warp
 constexpr float kShift = 7.f, kSlack = 8.f;
-constexpr int kUnit = kKvBlock * kWarps;   // tokens a thread block advances per step
-__host__ __device__ constexpr int blocks_per_sm(int nt) { return nt == 1 ? 4 : nt == 2 ? 3 : 2; }
+// By the tiles of 8 query rows: 16-token blocks a warp takes per step, steps in flight per warp, thread blocks per SM.  Two blocks a step
+// share the operands of q and the softmax's bookkeeping; with four row tiles there are no registers for them.
+__host__ __device__ constexpr int step_blocks(int nt) { return nt <= 2 ? 2 : 1; }
+__host__ __device__ constexpr int stages(int nt) { return nt <= 2 ? 2 : 3; }
+__host__ __device__ constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+__host__ __device__ constexpr int unit_tokens(int nt) { return kKvBlock * kWarps * step_blocks(nt); }   // that a thread block advances per step
 
 __device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity)
 {
@@ -72,7 +75,7 @@ struct Seq {
     int b = 0;
     int len = 0, qlen = 0, tiles = 0;   // tokens in the cache, new tokens, row tiles
     int first = 0;                      // first packed row
-    int units = 0;                      // 64-token units of one row tile
+    int units = 0;                      // units of one row tile
     int begin = 0, total = 0;           // its range of the list
 };
 template <int ROWS>
@@ -84,6 +87,7 @@ __device__ __forceinline__ void load_seq(Seq& s, const KvView& c, int b, int gro
     s.tiles = s.qlen * group >= tall ? 0 : (s.qlen * group + ROWS - 1) / ROWS;
     // tokens past the table's width have no page: they are not walked over
     const int held = (int)min((long long)s.len, (long long)c.table_stride * c.page_size);
+    constexpr int kUnit = unit_tokens(ROWS / 8);
     s.units = max((held - 1) / kUnit + 1, 1);
     s.total = c.kv_heads * s.tiles * s.units;
 }
@@ -157,20 +161,20 @@ __device__ __forceinline__ int visible_keys(const Seq& s, int row, int group)
 
 template <int D, int NT>
 struct Smem {
-    alignas(128) uint8_t ring[kWarps][kStages][KvLayout<D>::kBlockBytes];
+    alignas(128) uint8_t ring[kWarps][stages(NT)][step_blocks(NT) * KvLayout<D>::kBlockBytes];
     alignas(16) float merge[kWarps - 1][NT * (D / 16) * 4 * 32 + 4 * NT * 32];
     uint2 qfrag[NT][D / 16][32];   // q operand, [tile of 8 rows][k-step][lane]
     uint32_t qsum[NT][32];         // group sums of q as an operand: lane 4 g + t holds groups 2 (t & 1), + 1 of row g, high (t < 2) or low part
     float factor[NT][8];           // score sums -> base-2 scores
-    uint64_t full[kWarps][kStages];
-    int ok[kWarps][kStages];
+    uint64_t full[kWarps][stages(NT)];
+    int ok[kWarps][stages(NT)];    // blocks of the step that are there
 };
 
 template <int D, int NT>
 __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_split_kernel(KvAttnArgs a, int* status)
 {
     using L = KvLayout<D>;
-    constexpr int G = L::kGroups, KS = D / 16, MT = D / 16, ROWS = 8 * NT;
+    constexpr int G = L::kGroups, KS = D / 16, MT = D / 16, ROWS = 8 * NT, TT = step_blocks(NT), kStages = stages(NT), kUnit = unit_tokens(NT);
     extern __shared__ __align__(128) uint8_t smem_raw[];
     Smem<D, NT>& sm = *reinterpret_cast<Smem<D, NT>*>(smem_raw);
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, t = lane % 4;
@@ -194,31 +198,40 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
     Seq s;
     find_seq<ROWS>(s, c, group, a.tall, lo);
     Seq ps = s;   // the lane's own place in the list
-    auto block_of = [&](int x) -> long long {   // pool offset of this warp's block of unit x; -1: nothing to fetch
+    long long my_off[TT];           // pool offsets of this warp's blocks of the lane's unit; -1: nothing to fetch
+    auto find_blocks = [&](int x) {
         while (x >= ps.begin + ps.total) next_seq<ROWS>(ps, c, group, a.tall);
         const int r = x - ps.begin, pair = r / ps.units, h = pair / ps.tiles, rt = pair - h * ps.tiles;
-        const int pos = ((r - pair * ps.units) * kWarps + warp) * kKvBlock;
-        const int last_row = min((rt + 1) * ROWS, ps.qlen * group) - 1;
-        if (pos >= visible_keys(ps, last_row, group)) return -1;
-        const long long off = kv_block_offset<D>(c, ps.b, h, pos);
-        if (off < 0) atomicOr(status, kStatusBadCache);
-        return off;
+        const int pos = ((r - pair * ps.units) * kWarps + warp) * (kKvBlock * TT);
+        const int seen = visible_keys(ps, min((rt + 1) * ROWS, ps.qlen * group) - 1, group);
+#pragma unroll
+        for (int k = 0; k < TT; ++k) {
+            my_off[k] = -1;
+            if (pos + k * kKvBlock < seen) {
+                my_off[k] = kv_block_offset<D>(c, ps.b, h, pos + k * kKvBlock);
+                if (my_off[k] < 0) atomicOr(status, kStatusBadCache);
+            }
+        }
     };
     const uint32_t ring = smem_u32(sm.ring[warp]), bars = smem_u32(sm.full[warp]);
     int issued = 0, istage = 0;     // units whose copy is under way or done
     bool alive = true;              // no wait has run out
-    long long my_off = -1;
     auto refill = [&]() {           // whole warp
         if (!alive || issued >= count) return;
-        if ((issued & 31) == 0) my_off = issued + lane < count ? block_of(lo + issued + lane) : -1;
+        if ((issued & 31) == 0 && issued + lane < count) find_blocks(lo + issued + lane);
         if (lane == (issued & 31)) {
-            const uint32_t bar = bars + 8 * istage;
-            sm.ok[warp][istage] = my_off >= 0;
-            if (my_off >= 0) {
-                mbar_expect_tx(bar, L::kBlockBytes);
-                bulk_g2s(ring + istage * L::kBlockBytes, c.pool + my_off, L::kBlockBytes, bar);
+            const uint32_t bar = bars + 8 * istage, dst = ring + istage * (TT * L::kBlockBytes);
+            int there = 0;
+#pragma unroll
+            for (int k = 0; k < TT; ++k) there |= (my_off[k] >= 0) << k;
+            sm.ok[warp][istage] = there;
+            mbar_expect_tx(bar, __popc(there) * L::kBlockBytes);
+            if (TT == 2 && there == 3 && my_off[TT - 1] == my_off[0] + L::kBlockBytes) {
+                bulk_g2s(dst, c.pool + my_off[0], 2 * L::kBlockBytes, bar);
             } else {
-                mbar_arrive(bar);
+#pragma unroll
+                for (int k = 0; k < TT; ++k)
+                    if (my_off[k] >= 0) bulk_g2s(dst + k * L::kBlockBytes, c.pool + my_off[k], L::kBlockBytes, bar);
             }
         }
         ++issued;
@@ -300,166 +313,195 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
             for (int i = 0; i < MT; ++i) o[nt][i][0] *= r0, o[nt][i][1] *= r1, o[nt][i][2] *= r0, o[nt][i][3] *= r1;
         };
 
-        int pos = ((x - pair_begin) * kWarps + warp) * kKvBlock;
-        for (int left = seg_end - x; left > 0; --left, pos += kUnit) {
+        int pos0 = ((x - pair_begin) * kWarps + warp) * (kKvBlock * TT);
+        for (int left = seg_end - x; left > 0; --left, pos0 += kUnit) {
             if (alive) {
                 alive = __all_sync(0xffffffffu, wait_full(bars + 8 * stage, parity));
                 if (alive) ++waited;
                 else if (lane == 0) atomicOr(status, kStatusWaitTimeout);   // the rest counts as unseen
             }
-            if (alive && sm.ok[warp][stage]) {
-                const uint8_t* blk = sm.ring[warp][stage];
-                const bool edge = pos + kKvBlock > kmin;   // some row does not see all of these tokens
+            const int there = alive ? sm.ok[warp][stage] : 0;
+            if (there) {
+                const uint8_t* blk0 = sm.ring[warp][stage];
+                // some row does not see all of these tokens, or a block is not there: it counts as unseen
+                const bool edge = pos0 + TT * kKvBlock > kmin || there != (1 << TT) - 1;
+                auto seen_by = [&](int row, int k) {   // tokens of block k that a row of the tile sees
+                    return (there >> k & 1) ? visible_keys(s, rt * ROWS + row, group) - (pos0 + k * kKvBlock) : 0;
+                };
                 // ---- scores.  keys: one word of codes per group for tokens g and g + 8
-                uint32_t k0[G], k1[G], p0[G], p1[G];
-                {
-                    const uint32_t* kc = reinterpret_cast<const uint32_t*>(blk + L::kKCodes);
-                    const uint32_t* kp = reinterpret_cast<const uint32_t*>(blk + L::kKParams);
+                uint32_t k0[TT][G], k1[TT][G], p0[TT][G], p1[TT][G];
+#pragma unroll
+                for (int k = 0; k < TT; ++k) {
+                    const uint32_t* kc = reinterpret_cast<const uint32_t*>(blk0 + k * L::kBlockBytes + L::kKCodes);
+                    const uint32_t* kp = reinterpret_cast<const uint32_t*>(blk0 + k * L::kBlockBytes + L::kKParams);
                     if constexpr (G == 4) {
-                        *reinterpret_cast<uint4*>(k0) = *reinterpret_cast<const uint4*>(kc + g * 16 + t * 4);
-                        *reinterpret_cast<uint4*>(k1) = *reinterpret_cast<const uint4*>(kc + (g + 8) * 16 + t * 4);
-                        *reinterpret_cast<uint4*>(p0) = *reinterpret_cast<const uint4*>(kp + g * 4);
-                        *reinterpret_cast<uint4*>(p1) = *reinterpret_cast<const uint4*>(kp + (g + 8) * 4);
+                        *reinterpret_cast<uint4*>(k0[k]) = *reinterpret_cast<const uint4*>(kc + g * 16 + t * 4);
+                        *reinterpret_cast<uint4*>(k1[k]) = *reinterpret_cast<const uint4*>(kc + (g + 8) * 16 + t * 4);
+                        *reinterpret_cast<uint4*>(p0[k]) = *reinterpret_cast<const uint4*>(kp + g * 4);
+                        *reinterpret_cast<uint4*>(p1[k]) = *reinterpret_cast<const uint4*>(kp + (g + 8) * 4);
                     } else {
-                        *reinterpret_cast<uint2*>(k0) = *reinterpret_cast<const uint2*>(kc + g * 8 + t * 2);
-                        *reinterpret_cast<uint2*>(k1) = *reinterpret_cast<const uint2*>(kc + (g + 8) * 8 + t * 2);
-                        *reinterpret_cast<uint2*>(p0) = *reinterpret_cast<const uint2*>(kp + g * 2);
-                        *reinterpret_cast<uint2*>(p1) = *reinterpret_cast<const uint2*>(kp + (g + 8) * 2);
+                        *reinterpret_cast<uint2*>(k0[k]) = *reinterpret_cast<const uint2*>(kc + g * 8 + t * 2);
+                        *reinterpret_cast<uint2*>(k1[k]) = *reinterpret_cast<const uint2*>(kc + (g + 8) * 8 + t * 2);
+                        *reinterpret_cast<uint2*>(p0[k]) = *reinterpret_cast<const uint2*>(kp + g * 2);
+                        *reinterpret_cast<uint2*>(p1[k]) = *reinterpret_cast<const uint2*>(kp + (g + 8) * 2);
                     }
                 }
-                float z[NT][4];
+                float z[TT][NT][4];
                 {
                     // minima of the lane's two groups, as an operand (lanes without a group: zero)
-                    uint32_t m0, m1;
-                    if constexpr (G == 4) {
-                        const bool odd = t & 1;
-                        m0 = __byte_perm(odd ? p0[2] : p0[0], odd ? p0[3] : p0[1], 0x7632);
-                        m1 = __byte_perm(odd ? p1[2] : p1[0], odd ? p1[3] : p1[1], 0x7632);
-                    } else {
-                        m0 = (t & 1) ? 0u : __byte_perm(p0[0], p0[1], 0x7632);
-                        m1 = (t & 1) ? 0u : __byte_perm(p1[0], p1[1], 0x7632);
-                    }
-                    const uint32_t am[4] = {m0, m1, 0u, 0u};
+                    uint32_t qs[NT];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        z[nt][0] = z[nt][1] = z[nt][2] = z[nt][3] = 0.f;
-                        mma(z[nt], am, sm.qsum[nt][lane], 0u);
+                    for (int nt = 0; nt < NT; ++nt) qs[nt] = sm.qsum[nt][lane];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) z[nt][i] *= 0x1p-24f;
+                    for (int k = 0; k < TT; ++k) {
+                        uint32_t am[4] = {0u, 0u, 0u, 0u};
+                        if constexpr (G == 4) {
+                            const bool odd = t & 1;
+                            am[0] = __byte_perm(odd ? p0[k][2] : p0[k][0], odd ? p0[k][3] : p0[k][1], 0x7632);
+                            am[1] = __byte_perm(odd ? p1[k][2] : p1[k][0], odd ? p1[k][3] : p1[k][1], 0x7632);
+                        } else if (!(t & 1)) {
+                            am[0] = __byte_perm(p0[k][0], p0[k][1], 0x7632);
+                            am[1] = __byte_perm(p1[k][0], p1[k][1], 0x7632);
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            z[k][nt][0] = z[k][nt][1] = z[k][nt][2] = z[k][nt][3] = 0.f;
+                            mma(z[k][nt], am, qs[nt], 0u);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) z[k][nt][i] *= 0x1p-24f;
+                        }
                     }
                 }
 #pragma unroll
                 for (int w = 0; w < G; ++w) {
-                    const uint32_t h0 = k0[w] >> 8, h1 = k1[w] >> 8;
-                    const uint32_t alow[4] = {k0[w] & 0x000f000fu, k1[w] & 0x000f000fu, h0 & 0x000f000fu, h1 & 0x000f000fu};
-                    const uint32_t ahigh[4] = {k0[w] & 0x00f000f0u, k1[w] & 0x00f000f0u, h0 & 0x00f000f0u, h1 & 0x00f000f0u};
-                    const float s0 = __low2float(as_h2(p0[w])), s1 = __low2float(as_h2(p1[w]));
+                    uint2 ql[NT], qh[NT];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                        const uint2 ql = sm.qfrag[nt][2 * w][lane], qh = sm.qfrag[nt][2 * w + 1][lane];
-                        mma(acc, alow, ql.x, ql.y);
-                        mma(acc, ahigh, qh.x, qh.y);
-                        z[nt][0] = fmaf(s0, acc[0], z[nt][0]);
-                        z[nt][1] = fmaf(s0, acc[1], z[nt][1]);
-                        z[nt][2] = fmaf(s1, acc[2], z[nt][2]);
-                        z[nt][3] = fmaf(s1, acc[3], z[nt][3]);
+                    for (int nt = 0; nt < NT; ++nt) ql[nt] = sm.qfrag[nt][2 * w][lane], qh[nt] = sm.qfrag[nt][2 * w + 1][lane];
+#pragma unroll
+                    for (int k = 0; k < TT; ++k) {
+                        const uint32_t u = k0[k][w], v = k1[k][w], us = u >> 8, vs = v >> 8;
+                        const uint32_t alow[4] = {u & 0x000f000fu, v & 0x000f000fu, us & 0x000f000fu, vs & 0x000f000fu};
+                        const uint32_t ahigh[4] = {u & 0x00f000f0u, v & 0x00f000f0u, us & 0x00f000f0u, vs & 0x00f000f0u};
+                        const float s0 = __low2float(as_h2(p0[k][w])), s1 = __low2float(as_h2(p1[k][w]));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma(acc, alow, ql[nt].x, ql[nt].y);
+                            mma(acc, ahigh, qh[nt].x, qh[nt].y);
+                            z[k][nt][0] = fmaf(s0, acc[0], z[k][nt][0]);
+                            z[k][nt][1] = fmaf(s0, acc[1], z[k][nt][1]);
+                            z[k][nt][2] = fmaf(s1, acc[2], z[k][nt][2]);
+                            z[k][nt][3] = fmaf(s1, acc[3], z[k][nt][3]);
+                        }
                     }
                 }
-                // ---- values of tokens 2t, 2t+1 (j = 0) and 2t+8, 2t+9 (j = 1): codes, scales of all groups, minima of group g
-                uint32_t vw[2][G], vs[2][G], vm[2];
+                // ---- scales of the values of tokens 2t, 2t+1 (j = 0) and 2t+8, 2t+9 (j = 1), all groups; minima of group g
+                uint32_t vs[TT][2][G], vm[TT][2], large = 0;   // large: bit 14 of an fp16 value, 2 or more
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint8_t* vc = blk + L::kVCodes + j * 4 * D + lane * (D / 8);
-                    const uint32_t* vp = reinterpret_cast<const uint32_t*>(blk + L::kVParams) + (t + 4 * j) * 2 * G;
-                    if constexpr (G == 4) {
-                        *reinterpret_cast<uint4*>(vw[j]) = *reinterpret_cast<const uint4*>(vc);
-                        const uint4 u = *reinterpret_cast<const uint4*>(vp), w = *reinterpret_cast<const uint4*>(vp + 4);
-                        vs[j][0] = u.x, vs[j][1] = u.z, vs[j][2] = w.x, vs[j][3] = w.z;
-                    } else {
-                        *reinterpret_cast<uint2*>(vw[j]) = *reinterpret_cast<const uint2*>(vc);
-                        const uint4 u = *reinterpret_cast<const uint4*>(vp);
-                        vs[j][0] = u.x, vs[j][1] = u.z;
+                for (int k = 0; k < TT; ++k) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t* vp = reinterpret_cast<const uint32_t*>(blk0 + k * L::kBlockBytes + L::kVParams) + (t + 4 * j) * 2 * G;
+                        if constexpr (G == 4) {
+                            const uint4 u = *reinterpret_cast<const uint4*>(vp), w = *reinterpret_cast<const uint4*>(vp + 4);
+                            vs[k][j][0] = u.x, vs[k][j][1] = u.z, vs[k][j][2] = w.x, vs[k][j][3] = w.z;
+                        } else {
+                            const uint4 u = *reinterpret_cast<const uint4*>(vp);
+                            vs[k][j][0] = u.x, vs[k][j][1] = u.z;
+                        }
+                        vm[k][j] = g < G ? vp[2 * (g & (G - 1)) + 1] : 0u;
                     }
-                    vm[j] = g < G ? vp[2 * (g & (G - 1)) + 1] : 0u;
                 }
                 if (edge) {
                     // Tokens that no row sees count as zero, whatever the page holds there.  A token that some rows see and
                     // others do not may be NaN for the first and must not touch the others: it is taken out of the products
                     // and put back row by row.
-                    uint32_t nan_tokens[G] = {};
-                    bool any = false;
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int k = 0; k < TT; ++k) {
+                        uint32_t nan_tokens[G] = {};
+                        bool any = false;
+                        const int most = (there >> k & 1) ? kmax - (pos0 + k * kKvBlock) : 0;
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int tok = 2 * t + 8 * j + e;
-                            const uint32_t keep = e ? 0x0000ffffu : 0xffff0000u;
-                            const bool unseen = pos + tok >= kmax;
-#pragma unroll
-                            for (int w = 0; w < G; ++w) {
-                                const bool bad = ((vs[j][w] >> 16 * e) & 0x7c00u) == 0x7c00u;
-                                if (bad && !unseen) nan_tokens[w] |= 1u << tok, any = true;
-                                if (bad || unseen) vs[j][w] &= keep;
-                            }
-                            if (unseen || ((vm[j] >> 16 * e) & 0x7c00u) == 0x7c00u) vm[j] &= keep;
-                        }
-                    if (__any_sync(0xffffffffu, any)) {
-#pragma unroll
-                        for (int w = 0; w < G; ++w) {   // the quad holds all 16 tokens
-                            nan_tokens[w] |= __shfl_xor_sync(0xffffffffu, nan_tokens[w], 1);
-                            nan_tokens[w] |= __shfl_xor_sync(0xffffffffu, nan_tokens[w], 2);
-                        }
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
+                        for (int j = 0; j < 2; ++j)
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                const int seen = visible_keys(s, rt * ROWS + nt * 8 + 2 * t + e, group) - pos;
-                                const uint32_t mask = seen >= 16 ? 0xffffu : seen <= 0 ? 0u : (1u << seen) - 1;
+                                const int tok = 2 * t + 8 * j + e;
+                                const uint32_t keep = e ? 0x0000ffffu : 0xffff0000u;
+                                const bool unseen = tok >= most;
 #pragma unroll
-                                for (int i = 0; i < MT; ++i)
-                                    if (nan_tokens[i / 2] & mask) o[nt][i][e] = o[nt][i][2 + e] = __int_as_float(0x7fffffff);
+                                for (int w = 0; w < G; ++w) {
+                                    const bool bad = ((vs[k][j][w] >> 16 * e) & 0x7c00u) == 0x7c00u;
+                                    if (bad && !unseen) nan_tokens[w] |= 1u << tok, any = true;
+                                    if (bad || unseen) vs[k][j][w] &= keep;
+                                }
+                                if (unseen || ((vm[k][j] >> 16 * e) & 0x7c00u) == 0x7c00u) vm[k][j] &= keep;
                             }
+                        if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+                            for (int w = 0; w < G; ++w) {   // the quad holds all 16 tokens
+                                nan_tokens[w] |= __shfl_xor_sync(0xffffffffu, nan_tokens[w], 1);
+                                nan_tokens[w] |= __shfl_xor_sync(0xffffffffu, nan_tokens[w], 2);
+                            }
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const int seen = seen_by(nt * 8 + 2 * t + e, k);
+                                    const uint32_t mask = seen >= 16 ? 0xffffu : seen <= 0 ? 0u : (1u << seen) - 1;
+#pragma unroll
+                                    for (int i = 0; i < MT; ++i)
+                                        if (nan_tokens[i / 2] & mask) o[nt][i][e] = o[nt][i][2 + e] = __int_as_float(0x7fffffff);
+                                }
+                        }
                     }
                 }
-                // ---- softmax
-                uint32_t large = 0;   // bit 14 of an fp16 value: 2 or more
 #pragma unroll
-                for (int w = 0; w < G; ++w) large |= vs[0][w] | vs[1][w];
+                for (int k = 0; k < TT; ++k)
+#pragma unroll
+                    for (int w = 0; w < G; ++w) large |= vs[k][0][w] | vs[k][1][w];
+                // ---- softmax
                 bool grow = (large & 0x40004000u) != 0;
                 const float slack = kSlack - (float)shift;
+                float top[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const float2 f = *reinterpret_cast<const float2*>(&sm.factor[nt][2 * t]);
-                    z[nt][0] *= f.x, z[nt][2] *= f.x;
-                    z[nt][1] *= f.y, z[nt][3] *= f.y;
-                    if (edge) {
-                        const int row = rt * ROWS + nt * 8 + 2 * t;
-                        const int s0 = visible_keys(s, row, group) - pos, s1 = visible_keys(s, row + 1, group) - pos;
-                        if (g >= s0) z[nt][0] = -INFINITY;
-                        if (g >= s1) z[nt][1] = -INFINITY;
-                        if (g + 8 >= s0) z[nt][2] = -INFINITY;
-                        if (g + 8 >= s1) z[nt][3] = -INFINITY;
+#pragma unroll
+                    for (int k = 0; k < TT; ++k) {
+                        z[k][nt][0] *= f.x, z[k][nt][2] *= f.x;
+                        z[k][nt][1] *= f.y, z[k][nt][3] *= f.y;
+                        if (edge) {
+                            const int s0 = seen_by(nt * 8 + 2 * t, k), s1 = seen_by(nt * 8 + 2 * t + 1, k);
+                            if (g >= s0) z[k][nt][0] = -INFINITY;
+                            if (g >= s1) z[k][nt][1] = -INFINITY;
+                            if (g + 8 >= s0) z[k][nt][2] = -INFINITY;
+                            if (g + 8 >= s1) z[k][nt][3] = -INFINITY;
+                        }
+                        const float n0 = fmaxf(z[k][nt][0], z[k][nt][2]), n1 = fmaxf(z[k][nt][1], z[k][nt][3]);
+                        top[nt][0] = k ? fmaxf(top[nt][0], n0) : n0;
+                        top[nt][1] = k ? fmaxf(top[nt][1], n1) : n1;
                     }
-                    grow = grow || fmaxf(z[nt][0], z[nt][2]) > mx[nt][0] + slack || fmaxf(z[nt][1], z[nt][3]) > mx[nt][1] + slack;
+                    grow = grow || top[nt][0] > mx[nt][0] + slack || top[nt][1] > mx[nt][1] + slack;
                 }
                 if (__any_sync(0xffffffffu, grow)) {
-                    int need = 0;   // exponent of the largest finite scale of the block
+                    int need = 0;   // exponent of the largest finite scale of the blocks
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int k = 0; k < TT; ++k)
 #pragma unroll
-                        for (int w = 0; w < G; ++w)
+                        for (int j = 0; j < 2; ++j)
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int ex = (int)(vs[j][w] >> (16 * e + 10) & 31u) - 15;
-                                if (ex < 16) need = max(need, ex);
-                            }
+                            for (int w = 0; w < G; ++w)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const int ex = (int)(vs[k][j][w] >> (16 * e + 10) & 31u) - 15;
+                                    if (ex < 16) need = max(need, ex);
+                                }
                     need = max((int)__reduce_max_sync(0xffffffffu, (unsigned)need), shift) - shift;
                     shift += need;
                     const float fs = (float)shift;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        float n0 = fmaxf(z[nt][0], z[nt][2]), n1 = fmaxf(z[nt][1], z[nt][3]);
+                        float n0 = top[nt][0], n1 = top[nt][1];
 #pragma unroll
                         for (int d = 4; d < 32; d *= 2) {
                             n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, d));
@@ -472,34 +514,45 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
                         rescale(nt, r0, r1);
                     }
                 }
-                uint32_t b0[NT], b1[NT];
+                uint32_t b0[TT][NT], b1[TT][NT];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const float m0 = (mx[nt][0] == -INFINITY ? 0.f : mx[nt][0]) - kShift;
                     const float m1 = (mx[nt][1] == -INFINITY ? 0.f : mx[nt][1]) - kShift;
-                    const float w0 = exp2_approx(z[nt][0] - m0), w1 = exp2_approx(z[nt][1] - m1);
-                    const float w2 = exp2_approx(z[nt][2] - m0), w3 = exp2_approx(z[nt][3] - m1);
-                    sum[nt][0] += w0 + w2;
-                    sum[nt][1] += w1 + w3;
-                    b0[nt] = transpose8x8(h2_bits(__floats2half2_rn(w0, w1)));
-                    b1[nt] = transpose8x8(h2_bits(__floats2half2_rn(w2, w3)));
+#pragma unroll
+                    for (int k = 0; k < TT; ++k) {
+                        const float w0 = exp2_approx(z[k][nt][0] - m0), w1 = exp2_approx(z[k][nt][1] - m1);
+                        const float w2 = exp2_approx(z[k][nt][2] - m0), w3 = exp2_approx(z[k][nt][3] - m1);
+                        sum[nt][0] += w0 + w2;
+                        sum[nt][1] += w1 + w3;
+                        b0[k][nt] = transpose8x8(h2_bits(__floats2half2_rn(w0, w1)));
+                        b1[k][nt] = transpose8x8(h2_bits(__floats2half2_rn(w2, w3)));
+                    }
                 }
                 // ---- weighted values
-                {
-                    const uint32_t am[4] = {vm[0], 0u, vm[1], 0u};
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma(om[nt], am, b0[nt], b1[nt]);
-                }
+                for (int k = 0; k < TT; ++k) {
+                    uint32_t vw[2][G];
 #pragma unroll
-                for (int w = 0; w < G; ++w) {
-                    const uint32_t x0 = vw[0][w], x1 = vw[1][w], y0 = x0 >> 8, y1 = x1 >> 8;
-                    const uint32_t even[4] = {x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u};
-                    const uint32_t odd[4] = {y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u};
+                    for (int j = 0; j < 2; ++j) {
+                        const uint8_t* vc = blk0 + k * L::kBlockBytes + L::kVCodes + j * 4 * D + lane * (D / 8);
+                        if constexpr (G == 4) *reinterpret_cast<uint4*>(vw[j]) = *reinterpret_cast<const uint4*>(vc);
+                        else *reinterpret_cast<uint2*>(vw[j]) = *reinterpret_cast<const uint2*>(vc);
+                    }
+                    const uint32_t am[4] = {vm[k][0], 0u, vm[k][1], 0u};
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const uint32_t c0 = h2_bits(__hmul2(as_h2(b0[nt]), as_h2(vs[0][w]))), c1 = h2_bits(__hmul2(as_h2(b1[nt]), as_h2(vs[1][w])));
-                        mma(o[nt][2 * w], even, c0, c1);
-                        mma(o[nt][2 * w + 1], odd, c0, c1);
+                    for (int nt = 0; nt < NT; ++nt) mma(om[nt], am, b0[k][nt], b1[k][nt]);
+#pragma unroll
+                    for (int w = 0; w < G; ++w) {
+                        const uint32_t x0 = vw[0][w], x1 = vw[1][w], y0 = x0 >> 8, y1 = x1 >> 8;
+                        const uint32_t even[4] = {x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u};
+                        const uint32_t odd[4] = {y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u};
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const uint32_t c0 = h2_bits(__hmul2(as_h2(b0[k][nt]), as_h2(vs[k][0][w]))), c1 = h2_bits(__hmul2(as_h2(b1[k][nt]), as_h2(vs[k][1][w])));
+                            mma(o[nt][2 * w], even, c0, c1);
+                            mma(o[nt][2 * w + 1], odd, c0, c1);
+                        }
                     }
                 }
             }
@@ -700,7 +753,7 @@ cudaError_t launch(cudaStream_t s, const KvAttnArgs& a, int* status)
     ctas = (int)(fit < ctas ? fit : ctas);
     // never more thread blocks than units there can be: every table entry used, every packed row in a tile of its own at worst
     const int group = a.q_heads / a.c.kv_heads;
-    const long long units = ((long long)a.c.table_stride * a.c.page_size + kUnit - 1) / kUnit;
+    const long long units = ((long long)a.c.table_stride * a.c.page_size - 1) / unit_tokens(NT) + 1;
     const long long tiles = ((long long)a.max_q * group + ROWS - 1) / ROWS;
     const long long most = (long long)a.c.B * a.c.kv_heads * (tiles > 0 ? tiles : 1) * units;
     if (((long long)a.c.n_tokens * group / ROWS + a.c.B) * a.c.kv_heads * units > 0x7fffffff) {
