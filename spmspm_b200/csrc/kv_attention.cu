@@ -17,7 +17,7 @@
 //            instruction per 16 tokens.  Scales of 2 and more would leave the fp16 range: the whole row is then shifted down by
 //            the scale's exponent, as if its maximum had grown.
 //
-// Work: the context is cut in units of 128 or 64 tokens (four warps, two 16-token blocks or one each); all units of all (sequence, key
+// Work: the context is cut in units of 128 tokens (four warps, two 16-token blocks each); all units of all (sequence, key
 // head, row tile) are laid end to end and every thread block takes an equal share, found from the lengths on the device.
 // A share that covers a whole row tile is finished where it is; the others leave fp32 (O, max, sum) in the workspace,
 // two slots a thread block, and kv_attention_join_kernel adds them in order: no atomics, the same bits every time.
@@ -33,13 +33,14 @@ using namespace sm100;
 
 constexpr int kWarps = 4;
 constexpr float kShift = 7.f, kSlack = 8.f;
-// By the tiles of 8 query rows: 16-token blocks a warp takes per step, steps in flight per warp, thread blocks per SM.  Two blocks a step
-// share the operands of q and the softmax's bookkeeping; with four row tiles there are no registers for them.
-__host__ __device__ constexpr int step_blocks(int nt) { return nt <= 2 ? 2 : 1; }
-__host__ __device__ constexpr int stages(int nt) { return nt <= 2 ? 2 : 3; }
+// 16-token blocks a warp takes per step (they share the operands of q and the softmax's bookkeeping: two measured 105 -> 82 us at
+// 262139 tokens) and steps in flight per warp.
+constexpr int TT = 2, kStages = 2;
+constexpr int kUnit = kKvBlock * kWarps * TT;   // tokens a thread block advances per step
+// Tiles of 8 query rows a thread block takes: one, or two for more than 8 rows.  Four (32 rows) left two thread blocks of 255
+// registers per SM and took 210 us where two take 122 (16 sequences of 8000, 32 rows); one took 156, reading the cache twice as often.
+int pick_nt(int rows) { return rows <= 8 ? 1 : 2; }
 __host__ __device__ constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
-__host__ __device__ constexpr int unit_tokens(int nt) { return kKvBlock * kWarps * step_blocks(nt); }   // that a thread block advances per step
-
 __device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity)
 {
     for (uint32_t i = 0; i < kSpinLimit; ++i) {
@@ -87,7 +88,6 @@ __device__ __forceinline__ void load_seq(Seq& s, const KvView& c, int b, int gro
     s.tiles = s.qlen * group >= tall ? 0 : (s.qlen * group + ROWS - 1) / ROWS;
     // tokens past the table's width have no page: they are not walked over
     const int held = (int)min((long long)s.len, (long long)c.table_stride * c.page_size);
-    constexpr int kUnit = unit_tokens(ROWS / 8);
     s.units = max((held - 1) / kUnit + 1, 1);
     s.total = c.kv_heads * s.tiles * s.units;
 }
@@ -161,20 +161,20 @@ __device__ __forceinline__ int visible_keys(const Seq& s, int row, int group)
 
 template <int D, int NT>
 struct Smem {
-    alignas(128) uint8_t ring[kWarps][stages(NT)][step_blocks(NT) * KvLayout<D>::kBlockBytes];
+    alignas(128) uint8_t ring[kWarps][kStages][TT * KvLayout<D>::kBlockBytes];
     alignas(16) float merge[kWarps - 1][NT * (D / 16) * 4 * 32 + 4 * NT * 32];
     uint2 qfrag[NT][D / 16][32];   // q operand, [tile of 8 rows][k-step][lane]
     uint32_t qsum[NT][32];         // group sums of q as an operand: lane 4 g + t holds groups 2 (t & 1), + 1 of row g, high (t < 2) or low part
     float factor[NT][8];           // score sums -> base-2 scores
-    uint64_t full[kWarps][stages(NT)];
-    int ok[kWarps][stages(NT)];    // blocks of the step that are there
+    uint64_t full[kWarps][kStages];
+    int ok[kWarps][kStages];    // blocks of the step that are there
 };
 
 template <int D, int NT>
 __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_split_kernel(KvAttnArgs a, int* status)
 {
     using L = KvLayout<D>;
-    constexpr int G = L::kGroups, KS = D / 16, MT = D / 16, ROWS = 8 * NT, TT = step_blocks(NT), kStages = stages(NT), kUnit = unit_tokens(NT);
+    constexpr int G = L::kGroups, KS = D / 16, MT = D / 16, ROWS = 8 * NT;
     extern __shared__ __align__(128) uint8_t smem_raw[];
     Smem<D, NT>& sm = *reinterpret_cast<Smem<D, NT>*>(smem_raw);
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, t = lane % 4;
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
             for (int k = 0; k < TT; ++k) there |= (my_off[k] >= 0) << k;
             sm.ok[warp][istage] = there;
             mbar_expect_tx(bar, __popc(there) * L::kBlockBytes);
-            if (TT == 2 && there == 3 && my_off[TT - 1] == my_off[0] + L::kBlockBytes) {
+            if (there == 3 && my_off[TT - 1] == my_off[0] + L::kBlockBytes) {
                 bulk_g2s(dst, c.pool + my_off[0], 2 * L::kBlockBytes, bar);
             } else {
 #pragma unroll
@@ -648,14 +648,17 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
     for (; waited < issued; ++waited) wait_full(bars + 8 * (waited % kStages), (waited / kStages) & 1);
 }
 
-// Adds the parts of the row tiles that were cut between thread blocks; one thread block per (key head and row tile,
-// sequence), one warp per row in turn.
+// Adds the parts of the row tiles that were cut between thread blocks, in order.  blockIdx.y: sequence, blockIdx.x: key head and row
+// tile, and row if there are as many thread blocks (`spread`).  With many row tiles each has few parts: a warp takes a row.  With few, a
+// thread block takes a row and its warps share out the parts (one key head, 444 parts: 207 -> 28 us).
+constexpr int kJoinWarps = 8;
 template <int D, int NT>
-__global__ void __launch_bounds__(128) kv_attention_join_kernel(KvAttnArgs a, int ctas)
+__global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvAttnArgs a, int ctas, int spread)
 {
     constexpr int ROWS = 8 * NT, V = D / 32;
+    __shared__ float part_sum[kJoinWarps][D], part_weight[kJoinWarps];
     const KvView& c = a.c;
-    const int group = a.q_heads / c.kv_heads, lane = threadIdx.x & 31;
+    const int group = a.q_heads / c.kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     // the lengths are none of the preceding kernel's results, and what wrote them had ended before that kernel let this one start
     const int total = list_length<ROWS>(c, group, a.tall);
     Seq s;
@@ -670,7 +673,8 @@ __global__ void __launch_bounds__(128) kv_attention_join_kernel(KvAttnArgs a, in
     grid_wait();
     if (total == 0) return;
     const Shares shares(total, ctas);
-    for (int pair = blockIdx.x; pair < c.kv_heads * s.tiles; pair += gridDim.x) {
+    const int step = spread ? spread : kJoinWarps, pairs = spread ? gridDim.x / spread : gridDim.x;
+    for (int pair = spread ? blockIdx.x / spread : blockIdx.x; pair < c.kv_heads * s.tiles; pair += pairs) {
         const int h = pair / s.tiles, rt = pair - h * s.tiles;
         const int p0 = begin + pair * s.units, p1 = p0 + s.units;
         const int c0 = shares.of(p0), c1 = shares.of(p1 - 1);
@@ -678,7 +682,7 @@ __global__ void __launch_bounds__(128) kv_attention_join_kernel(KvAttnArgs a, in
         const int rows = min(ROWS, s.qlen * group - rt * ROWS);
         // the first part is the end of its thread block's share, the later ones start theirs (slot 0)
         auto slot = [&](int i) { return a.ws + (2 * (size_t)i + (i == c0)) * slot_floats<D, ROWS>(); };
-        for (int row = threadIdx.x / 32; row < rows; row += 4) {
+        for (int row = spread ? blockIdx.x % spread : warp; row < rows; row += step) {
             float m = -INFINITY;
             for (int i = c0 + lane; i <= c1; i += 32) m = fmaxf(m, slot(i)[ROWS * D + row]);
 #pragma unroll
@@ -686,7 +690,7 @@ __global__ void __launch_bounds__(128) kv_attention_join_kernel(KvAttnArgs a, in
             const float z = m == -INFINITY ? 0.f : m;
             float acc[V] = {}, w = 0.f;
 #pragma unroll 4
-            for (int i = c0; i <= c1; ++i) {
+            for (int i = c0 + (spread ? warp : 0); i <= c1; i += spread ? kJoinWarps : 1) {
                 const float* p = slot(i);
                 const float r = exp2_approx(p[ROWS * D + row] - z);
                 w = fmaf(p[ROWS * D + ROWS + row], r, w);
@@ -696,14 +700,29 @@ __global__ void __launch_bounds__(128) kv_attention_join_kernel(KvAttnArgs a, in
 #pragma unroll
                 for (int k = 0; k < V; ++k) acc[k] = fmaf(v[k], r, acc[k]);
             }
-            const float inv = w == 0.f ? 0.f : 1.f / w;
             const int r = rt * ROWS + row;
-            __half2 y[V / 2];
+            uint16_t* dst = a.out + ((long long)(s.first + r / group) * a.q_heads + h * group + r % group) * D;
+            if (!spread) {
+                const float inv = w == 0.f ? 0.f : 1.f / w;
+                __half2 y[V / 2];
 #pragma unroll
-            for (int k = 0; k < V / 2; ++k) y[k] = __floats2half2_rn(acc[2 * k] * inv, acc[2 * k + 1] * inv);
-            uint16_t* dst = a.out + ((long long)(s.first + r / group) * a.q_heads + h * group + r % group) * D + lane * V;
-            if constexpr (V == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(y);
-            else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(y);
+                for (int k = 0; k < V / 2; ++k) y[k] = __floats2half2_rn(acc[2 * k] * inv, acc[2 * k + 1] * inv);
+                if constexpr (V == 4) *reinterpret_cast<uint2*>(dst + lane * V) = *reinterpret_cast<uint2*>(y);
+                else *reinterpret_cast<uint32_t*>(dst + lane * V) = *reinterpret_cast<uint32_t*>(y);
+                continue;
+            }
+#pragma unroll
+            for (int k = 0; k < V; ++k) part_sum[warp][lane * V + k] = acc[k];
+            if (lane == 0) part_weight[warp] = w;
+            __syncthreads();
+            const int ch = threadIdx.x;
+            if (ch < D) {
+                float y = 0.f, all = 0.f;
+#pragma unroll
+                for (int i = 0; i < kJoinWarps; ++i) y += part_sum[i][ch], all += part_weight[i];
+                dst[ch] = __half_as_ushort(__float2half_rn(all == 0.f ? 0.f : y / all));
+            }
+            __syncthreads();
         }
     }
 }
@@ -717,8 +736,6 @@ int sm_count()
     return n[dev];
 }
 
-// Query rows a thread block takes: the fewest of 8, 16, 32 that hold a sequence's rows.
-int pick_nt(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 
 // Thread blocks that fit on the device at once (shared memory and registers).
 template <int D, int NT>
@@ -753,7 +770,7 @@ cudaError_t launch(cudaStream_t s, const KvAttnArgs& a, int* status)
     ctas = (int)(fit < ctas ? fit : ctas);
     // never more thread blocks than units there can be: every table entry used, every packed row in a tile of its own at worst
     const int group = a.q_heads / a.c.kv_heads;
-    const long long units = ((long long)a.c.table_stride * a.c.page_size - 1) / unit_tokens(NT) + 1;
+    const long long units = ((long long)a.c.table_stride * a.c.page_size - 1) / kUnit + 1;
     const long long tiles = ((long long)a.max_q * group + ROWS - 1) / ROWS;
     const long long most = (long long)a.c.B * a.c.kv_heads * (tiles > 0 ? tiles : 1) * units;
     if (((long long)a.c.n_tokens * group / ROWS + a.c.B) * a.c.kv_heads * units > 0x7fffffff) {
@@ -774,11 +791,13 @@ cudaError_t launch(cudaStream_t s, const KvAttnArgs& a, int* status)
     e = cudaLaunchKernelEx(&cfg, kv_attention_split_kernel<D, NT>, a, status);
     count_launch();
     if (e != cudaSuccess) return e;
-    const long long pairs = a.c.kv_heads * (tiles > 0 ? tiles : 1);
-    cfg.gridDim = dim3((unsigned)(pairs < 65535 ? pairs : 65535), (unsigned)a.c.B);
-    cfg.blockDim = dim3(128);
+    const long long rows = (long long)a.max_q * group, pairs = a.c.kv_heads * (tiles > 0 ? tiles : 1);
+    const long long spread = pairs * a.c.B * 4 > ctas ? 0 : rows < 1 ? 1 : rows < ROWS ? rows : ROWS;   // five parts and more
+    const long long x = pairs * (spread ? spread : 1), most_x = 0x7fffffff / ROWS * ROWS;
+    cfg.gridDim = dim3((unsigned)(x < most_x ? x : most_x / (spread ? spread : 1) * (spread ? spread : 1)), (unsigned)a.c.B);
+    cfg.blockDim = dim3(32 * kJoinWarps);
     cfg.dynamicSmemBytes = 0;
-    e = cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<D, NT>, a, ctas);
+    e = cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<D, NT>, a, ctas, (int)spread);
     count_launch();
     return e;
 }
@@ -788,8 +807,7 @@ cudaError_t launch_d(cudaStream_t s, const KvAttnArgs& a, int* status)
 {
     switch (pick_nt(a.max_q * (a.q_heads / a.c.kv_heads))) {
         case 1: return launch<D, 1>(s, a, status);
-        case 2: return launch<D, 2>(s, a, status);
-        default: return launch<D, 4>(s, a, status);
+        default: return launch<D, 2>(s, a, status);
     }
 }
 
