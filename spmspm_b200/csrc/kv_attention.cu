@@ -91,43 +91,50 @@ __device__ __forceinline__ void load_seq(Seq& s, const KvView& c, int b, int gro
     s.units = max((held - 1) / kUnit + 1, 1);
     s.total = c.kv_heads * s.tiles * s.units;
 }
+// The list as a warp sees it: its length, and of up to 32 sequences lane b's, so that finding one needs no second look at memory.
 template <int ROWS>
-__device__ __forceinline__ int list_length(const KvView& c, int group, int tall)
-{
-    int sum = 0;
-    for (int b = threadIdx.x & 31; b < c.B; b += 32) {
-        Seq s;
-        load_seq<ROWS>(s, c, b, group, tall);
-        sum += s.total;
+struct List {
+    Seq mine;
+    int total;   // units of the list
+    __device__ __forceinline__ List(const KvView& c, int group, int tall)
+    {
+        const int lane = threadIdx.x & 31;
+        int sum = 0;
+        for (int b = lane; b < c.B; b += 32) {
+            load_seq<ROWS>(mine, c, b, group, tall);
+            sum += mine.total;
+        }
+        total = __reduce_add_sync(0xffffffffu, sum);
     }
-    return __reduce_add_sync(0xffffffffu, sum);
-}
-// The sequence that holds unit x of the list (x inside the list); every lane gets the same.
-template <int ROWS>
-__device__ __forceinline__ void find_seq(Seq& s, const KvView& c, int group, int tall, int x)
-{
-    const int lane = threadIdx.x & 31;
-    int before = 0;
-    for (int b0 = 0; b0 < c.B; b0 += 32) {
-        Seq t;
-        if (b0 + lane < c.B) load_seq<ROWS>(t, c, b0 + lane, group, tall);
-        int incl = t.total;
+    // The sequence that holds unit x of the list (x inside the list); every lane gets the same.
+    __device__ __forceinline__ void find(Seq& s, const KvView& c, int group, int tall, int x)
+    {
+        const int lane = threadIdx.x & 31;
+        int before = 0;
+        for (int b0 = 0; b0 < c.B; b0 += 32) {
+            Seq t;
+            if (c.B <= 32) t = mine;
+            else if (b0 + lane < c.B) load_seq<ROWS>(t, c, b0 + lane, group, tall);
+            int incl = t.total;
 #pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const int y = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += y;
+            for (int o = 1; o < 32; o *= 2) {
+                const int y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += y;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, before + incl > x);
+            if (past) {
+                const int l = __ffs(past) - 1;
+                s.b = b0 + l;
+                s.len = __shfl_sync(0xffffffffu, t.len, l), s.qlen = __shfl_sync(0xffffffffu, t.qlen, l);
+                s.tiles = __shfl_sync(0xffffffffu, t.tiles, l), s.first = __shfl_sync(0xffffffffu, t.first, l);
+                s.units = __shfl_sync(0xffffffffu, t.units, l), s.total = __shfl_sync(0xffffffffu, t.total, l);
+                s.begin = before + __shfl_sync(0xffffffffu, incl - t.total, l);
+                return;
+            }
+            before += __shfl_sync(0xffffffffu, incl, 31);
         }
-        const uint32_t past = __ballot_sync(0xffffffffu, before + incl > x);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            const int begin = before + __shfl_sync(0xffffffffu, incl - t.total, l);
-            load_seq<ROWS>(s, c, b0 + l, group, tall);
-            s.begin = begin;
-            return;
-        }
-        before += __shfl_sync(0xffffffffu, incl, 31);
     }
-}
+};
 template <int ROWS>
 __device__ __forceinline__ void next_seq(Seq& s, const KvView& c, int group, int tall)
 {
@@ -171,7 +178,7 @@ struct Smem {
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_split_kernel(KvAttnArgs a, int* status)
+__global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_split_kernel(KvAttnArgs a, int whole_tiles, int* status)
 {
     using L = KvLayout<D>;
     constexpr int G = L::kGroups, KS = D / 16, MT = D / 16, ROWS = 8 * NT;
@@ -189,14 +196,52 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
     grid_wait();
     grid_release();   // the join may be set up while this kernel runs; it waits for its end
 
-    const int total = list_length<ROWS>(c, group, a.tall);
-    const Shares shares(total, gridDim.x);
-    const int lo = shares.begin(blockIdx.x), count = shares.begin(blockIdx.x + 1) - lo;
+    List<ROWS> list(c, group, a.tall);
+    const Shares shares(list.total, gridDim.x);
+    int lo = shares.begin(blockIdx.x), hi = shares.begin(blockIdx.x + 1);
+    Seq s;
+    if (whole_tiles) {   // short contexts: the ends of a share move up to the next row tile, nothing is cut
+        auto next_tile = [&](int x) {
+            if (x >= list.total) return list.total;
+            list.find(s, c, group, a.tall, x);
+            return s.begin + (x - s.begin + s.units - 1) / s.units * s.units;
+        };
+        lo = next_tile(lo), hi = next_tile(hi);
+    }
+    const int count = hi - lo;
     if (count <= 0) return;
+    list.find(s, c, group, a.tall, lo);
+
+    // ---- segments: runs of units of one row tile
+    struct Segment {
+        int h, rt, rows, kmin, kmax, tile_begin, begin, end;
+        bool whole;
+    } seg;
+    auto set_segment = [&](int x) {
+        while (x >= s.begin + s.total) next_seq<ROWS>(s, c, group, a.tall);
+        const int pair = (x - s.begin) / s.units;
+        seg.h = pair / s.tiles;
+        seg.rt = pair - seg.h * s.tiles;
+        seg.tile_begin = s.begin + pair * s.units;
+        seg.begin = x;
+        seg.end = min(hi, seg.tile_begin + s.units);
+        seg.whole = x == seg.tile_begin && seg.end == seg.tile_begin + s.units;
+        seg.rows = min(ROWS, s.qlen * group - seg.rt * ROWS);   // rows of this tile
+        seg.kmin = visible_keys(s, seg.rt * ROWS, group), seg.kmax = visible_keys(s, seg.rt * ROWS + seg.rows - 1, group);
+    };
+    uint2 raw[KS];   // q of the next segment's rows, warps below NT: 8 rows each
+    auto load_q = [&]() {
+        const int row = warp * 8 + g, abs_row = seg.rt * ROWS + row;
+        const bool have = row < seg.rows;
+        const uint16_t* src = a.q + (long long)(s.first + (have ? abs_row / group : 0)) * a.q_tok + (seg.h * group + (have ? abs_row % group : 0)) * a.q_head;
+        if (warp < NT)
+#pragma unroll
+            for (int j = 0; j < KS; ++j) raw[j] = have ? *reinterpret_cast<const uint2*>(src + 16 * j + 4 * t) : make_uint2(0, 0);
+    };
+    set_segment(lo);
+    load_q();
 
     // ---- this warp's copies: lane l looks after every 32nd unit of the share
-    Seq s;
-    find_seq<ROWS>(s, c, group, a.tall, lo);
     Seq ps = s;   // the lane's own place in the list
     long long my_off[TT];           // pool offsets of this warp's blocks of the lane's unit; -1: nothing to fetch
     auto find_blocks = [&](int x) {
@@ -240,28 +285,15 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
     for (int i = 0; i < kStages; ++i) refill();
 
     // ---- consumer
-    int x = lo, stage = 0, waited = 0;   // waited: units whose copy has been waited for
+    int stage = 0, waited = 0;   // waited: units whose copy has been waited for
     uint32_t parity = 0;
-    const int hi = lo + count;
-    while (x < hi) {
-        while (x >= s.begin + s.total) next_seq<ROWS>(s, c, group, a.tall);
-        const int pair = (x - s.begin) / s.units, h = pair / s.tiles, rt = pair - h * s.tiles;
-        const int pair_begin = s.begin + pair * s.units, pair_end = pair_begin + s.units;
-        const int seg_begin = x, seg_end = min(hi, pair_end);
+    for (bool more = true; more;) {
         if ((long long)s.len > (long long)c.table_stride * c.page_size && threadIdx.x == 0) atomicOr(status, kStatusBadCache);
-        const int rows = min(ROWS, s.qlen * group - rt * ROWS);   // rows of this tile
-        const int kmin = visible_keys(s, rt * ROWS, group), kmax = visible_keys(s, rt * ROWS + rows - 1, group);
-
-        // q of the tile: warps take the 8-row subtiles in turn
+        // q of the tile
         __syncthreads();
-        for (int nt = warp; nt < NT; nt += kWarps) {
-            const int row = nt * 8 + g, abs_row = rt * ROWS + row;
-            const bool have = row < rows;
-            const uint16_t* src = a.q + (long long)(s.first + (have ? abs_row / group : 0)) * a.q_tok + (h * group + (have ? abs_row % group : 0)) * a.q_head;
-            uint2 raw[KS];
+        if (warp < NT) {
+            const int nt = warp;
             float big = 0.f;
-#pragma unroll
-            for (int j = 0; j < KS; ++j) raw[j] = have ? *reinterpret_cast<const uint2*>(src + 16 * j + 4 * t) : make_uint2(0, 0);
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
                 const float2 u = __half22float2(as_h2(raw[j].x)), w = __half22float2(as_h2(raw[j].y));
@@ -313,8 +345,8 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
             for (int i = 0; i < MT; ++i) o[nt][i][0] *= r0, o[nt][i][1] *= r1, o[nt][i][2] *= r0, o[nt][i][3] *= r1;
         };
 
-        int pos0 = ((x - pair_begin) * kWarps + warp) * (kKvBlock * TT);
-        for (int left = seg_end - x; left > 0; --left, pos0 += kUnit) {
+        int pos0 = ((seg.begin - seg.tile_begin) * kWarps + warp) * (kKvBlock * TT);
+        for (int left = seg.end - seg.begin; left > 0; --left, pos0 += kUnit) {
             if (alive) {
                 alive = __all_sync(0xffffffffu, wait_full(bars + 8 * stage, parity));
                 if (alive) ++waited;
@@ -324,9 +356,9 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
             if (there) {
                 const uint8_t* blk0 = sm.ring[warp][stage];
                 // some row does not see all of these tokens, or a block is not there: it counts as unseen
-                const bool edge = pos0 + TT * kKvBlock > kmin || there != (1 << TT) - 1;
+                const bool edge = pos0 + TT * kKvBlock > seg.kmin || there != (1 << TT) - 1;
                 auto seen_by = [&](int row, int k) {   // tokens of block k that a row of the tile sees
-                    return (there >> k & 1) ? visible_keys(s, rt * ROWS + row, group) - (pos0 + k * kKvBlock) : 0;
+                    return (there >> k & 1) ? visible_keys(s, seg.rt * ROWS + row, group) - (pos0 + k * kKvBlock) : 0;
                 };
                 // ---- scores.  keys: one word of codes per group for tokens g and g + 8
                 uint32_t k0[TT][G], k1[TT][G], p0[TT][G], p1[TT][G];
@@ -420,7 +452,7 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
                     for (int k = 0; k < TT; ++k) {
                         uint32_t nan_tokens[G] = {};
                         bool any = false;
-                        const int most = (there >> k & 1) ? kmax - (pos0 + k * kKvBlock) : 0;
+                        const int most = (there >> k & 1) ? seg.kmax - (pos0 + k * kKvBlock) : 0;
 #pragma unroll
                         for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -560,7 +592,13 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
             if (++stage == kStages) stage = 0, parity ^= 1;
             refill();
         }
-        x = seg_end;
+        const Segment done = seg;
+        const int first = s.first;
+        more = seg.end < hi;
+        if (more) {   // q of the next segment is on its way while this one is finished
+            set_segment(seg.end);
+            load_q();
+        }
 
         // ---- join the four warps
 #pragma unroll
@@ -618,20 +656,19 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
                         o[nt][i][2] = fmaf(v.z, r0, o[nt][i][2]), o[nt][i][3] = fmaf(v.w, r1, o[nt][i][3]);
                     }
                 }
-                const bool whole = seg_begin == pair_begin && seg_end == pair_end;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int row = nt * 8 + 2 * t + e;
-                    if (row >= rows) continue;
+                    if (row >= done.rows) continue;
                     const float total_w = e ? t1 : t0;
-                    if (whole) {
+                    if (done.whole) {
                         const float inv = total_w == 0.f ? 0.f : 1.f / total_w;   // no visible key: zeros
-                        const int r = rt * ROWS + row;
-                        uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + ((long long)(s.first + r / group) * a.q_heads + h * group + r % group) * D) + g;
+                        const int r = done.rt * ROWS + row;
+                        uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + ((long long)(first + r / group) * a.q_heads + done.h * group + r % group) * D) + g;
 #pragma unroll
                         for (int i = 0; i < MT; ++i) dst[8 * i] = h2_bits(__floats2half2_rn(o[nt][i][e] * inv, o[nt][i][2 + e] * inv));
                     } else {
-                        float* slot = a.ws + (2 * (size_t)blockIdx.x + (seg_begin == pair_begin)) * slot_floats<D, ROWS>();
+                        float* slot = a.ws + (2 * (size_t)blockIdx.x + (done.begin == done.tile_begin)) * slot_floats<D, ROWS>();
                         float2* dst = reinterpret_cast<float2*>(slot + row * D) + g;
 #pragma unroll
                         for (int i = 0; i < MT; ++i) dst[8 * i] = make_float2(o[nt][i][e], o[nt][i][2 + e]);
@@ -656,20 +693,21 @@ template <int D, int NT>
 __global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvAttnArgs a, int ctas, int spread)
 {
     constexpr int ROWS = 8 * NT, V = D / 32;
-    __shared__ float part_sum[kJoinWarps][D], part_weight[kJoinWarps];
+    __shared__ float part_sum[kJoinWarps][D], part_weight[kJoinWarps], part_max[kJoinWarps];
     const KvView& c = a.c;
     const int group = a.q_heads / c.kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     // the lengths are none of the preceding kernel's results, and what wrote them had ended before that kernel let this one start
-    const int total = list_length<ROWS>(c, group, a.tall);
     Seq s;
-    load_seq<ROWS>(s, c, blockIdx.y, group, a.tall);
-    int begin = 0;
-    for (int b = lane; b < (int)blockIdx.y; b += 32) {
+    int begin = 0, total = 0;
+    for (int b = lane; b < c.B; b += 32) {
         Seq o;
         load_seq<ROWS>(o, c, b, group, a.tall);
-        begin += o.total;
+        total += o.total;
+        if (b < (int)blockIdx.y) begin += o.total;
     }
+    load_seq<ROWS>(s, c, blockIdx.y, group, a.tall);
     begin = __reduce_add_sync(0xffffffffu, begin);
+    total = __reduce_add_sync(0xffffffffu, total);
     grid_wait();
     if (total == 0) return;
     const Shares shares(total, ctas);
@@ -683,22 +721,34 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvAt
         // the first part is the end of its thread block's share, the later ones start theirs (slot 0)
         auto slot = [&](int i) { return a.ws + (2 * (size_t)i + (i == c0)) * slot_floats<D, ROWS>(); };
         for (int row = spread ? blockIdx.x % spread : warp; row < rows; row += step) {
-            float m = -INFINITY;
-            for (int i = c0 + lane; i <= c1; i += 32) m = fmaxf(m, slot(i)[ROWS * D + row]);
+            // four parts at a time, all their loads under way together
+            float m = -INFINITY, acc[V] = {}, w = 0.f;
+            const int stride = spread ? kJoinWarps : 1;
+            for (int i0 = c0 + (spread ? warp : 0); i0 <= c1; i0 += 4 * stride) {
+                float pm[4], pw[4], v[4][V];
 #pragma unroll
-            for (int d = 16; d; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-            const float z = m == -INFINITY ? 0.f : m;
-            float acc[V] = {}, w = 0.f;
-#pragma unroll 4
-            for (int i = c0 + (spread ? warp : 0); i <= c1; i += spread ? kJoinWarps : 1) {
-                const float* p = slot(i);
-                const float r = exp2_approx(p[ROWS * D + row] - z);
-                w = fmaf(p[ROWS * D + ROWS + row], r, w);
-                float v[V];
-                if constexpr (V == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p + row * D + lane * V);
-                else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(p + row * D + lane * V);
+                for (int j = 0; j < 4; ++j) {
+                    const int i = min(i0 + j * stride, c1);
+                    const float* p = slot(i);
+                    const bool in = i0 + j * stride <= c1;
+                    pm[j] = in ? p[ROWS * D + row] : -INFINITY;
+                    pw[j] = in ? p[ROWS * D + ROWS + row] : 0.f;
+                    if constexpr (V == 4) *reinterpret_cast<float4*>(v[j]) = *reinterpret_cast<const float4*>(p + row * D + lane * V);
+                    else *reinterpret_cast<float2*>(v[j]) = *reinterpret_cast<const float2*>(p + row * D + lane * V);
+                }
+                const float n = fmaxf(m, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]))), z = n == -INFINITY ? 0.f : n, r = exp2_approx(m - z);
+                m = n;
+                w *= r;
 #pragma unroll
-                for (int k = 0; k < V; ++k) acc[k] = fmaf(v[k], r, acc[k]);
+                for (int k = 0; k < V; ++k) acc[k] *= r;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (i0 + j * stride <= c1) {
+                        const float q = exp2_approx(pm[j] - z);
+                        w = fmaf(pw[j], q, w);
+#pragma unroll
+                        for (int k = 0; k < V; ++k) acc[k] = fmaf(v[j][k], q, acc[k]);
+                    }
             }
             const int r = rt * ROWS + row;
             uint16_t* dst = a.out + ((long long)(s.first + r / group) * a.q_heads + h * group + r % group) * D;
@@ -713,13 +763,19 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvAt
             }
 #pragma unroll
             for (int k = 0; k < V; ++k) part_sum[warp][lane * V + k] = acc[k];
-            if (lane == 0) part_weight[warp] = w;
+            if (lane == 0) part_weight[warp] = w, part_max[warp] = m;
             __syncthreads();
             const int ch = threadIdx.x;
             if (ch < D) {
-                float y = 0.f, all = 0.f;
+                float y = 0.f, all = 0.f, n = part_max[0];
 #pragma unroll
-                for (int i = 0; i < kJoinWarps; ++i) y += part_sum[i][ch], all += part_weight[i];
+                for (int i = 1; i < kJoinWarps; ++i) n = fmaxf(n, part_max[i]);
+                const float z = n == -INFINITY ? 0.f : n;
+#pragma unroll
+                for (int i = 0; i < kJoinWarps; ++i) {
+                    const float q = exp2_approx(part_max[i] - z);
+                    y = fmaf(part_sum[i][ch], q, y), all = fmaf(part_weight[i], q, all);
+                }
                 dst[ch] = __half_as_ushort(__float2half_rn(all == 0.f ? 0.f : y / all));
             }
             __syncthreads();
@@ -777,7 +833,9 @@ cudaError_t launch(cudaStream_t s, const KvAttnArgs& a, int* status)
         set_error("kv_attention: too much work for one call (rows times context)");
         return cudaErrorInvalidValue;
     }
-    if (most < ctas) ctas = (int)most;
+    // A tile of up to four units is done whole: cutting it saves a unit's time or two (1.5 us each), the join costs 3.5 us.
+    const int whole = units <= 4;
+    if (whole ? most / units < ctas : most < ctas) ctas = (int)(whole ? most / units : most);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -788,9 +846,9 @@ cudaError_t launch(cudaStream_t s, const KvAttnArgs& a, int* status)
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kv_attention_split_kernel<D, NT>, a, status);
+    e = cudaLaunchKernelEx(&cfg, kv_attention_split_kernel<D, NT>, a, whole, status);
     count_launch();
-    if (e != cudaSuccess) return e;
+    if (e != cudaSuccess || whole) return e;
     const long long rows = (long long)a.max_q * group, pairs = a.c.kv_heads * (tiles > 0 ? tiles : 1);
     const long long spread = pairs * a.c.B * 4 > ctas ? 0 : rows < 1 ? 1 : rows < ROWS ? rows : ROWS;   // five parts and more
     const long long x = pairs * (spread ? spread : 1), most_x = 0x7fffffff / ROWS * ROWS;
