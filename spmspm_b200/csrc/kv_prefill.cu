@@ -1,17 +1,18 @@
 // Attention over the paged 4-bit cache for many query rows a key head (prompts and chunks of prompts), on tcgen05.
 //
-// A thread block takes up to 256 rows (two tiles of 128) of one sequence and key head and walks over the keys in tiles of 128:
+// A thread block takes up to 256 rows (two tiles of 128) of one sequence and key head and walks over the keys in tiles of 64:
 //
-//   warp 0        copies the 8 blocks of a key tile (4-bit keys and values) into a two-stage ring
+//   warp 0        copies the 4 blocks of a key tile (4-bit keys and values) into a four-stage ring
 //   warp 1        issues tcgen05.mma, one elected thread
 //   warps 4-7, 8-11   softmax of row tile 0 and 1, thread = row: scores from tensor memory, running maximum and sum in fp32 and
 //                 base 2, weights back to tensor memory as fp16 where the next product takes its left operand from
-//   warps 12-19   expand one block each: keys [key][channel] and values transposed, [channel][key], as 128-byte-swizzled tiles
-//                 (m + s c with one rounding, the values that kv_read returns)
+//   warps 12-19   expand one block each, four warps the even key tiles and four the odd: keys [key][channel] and values transposed,
+//                 [channel][key], as 128-byte-swizzled tiles (m + s c with one rounding, the values that kv_read returns)
 //
-// S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory over S, V^T in shared memory) of the two row tiles
-// alternate, so that the tensor core works on one while the other's softmax runs; S(i + 1) of a tile is issued behind
-// P V (i) of the same tile, which therefore has ended when S(i + 1) has.  The accumulators are rescaled, by the softmax
+// S = Q K^T (both operands in shared memory) has two buffers per row tile in tensor memory, P lies over S, and O += P V (V^T in shared
+// memory) is followed by the scores of the key tile after the next in the buffer it has read: the softmax warps always
+// find their next scores done.  (Key tiles of 128 leave room for one buffer; softmax and products then wait for each
+// other, 6700 cycles per 256 x 128 scores whatever the softmax took.)  The accumulators are rescaled, by the softmax
 // warps, only when a row's maximum has grown by more than 2^8; weights are kept 2^7 too large so that fp16 holds 2^-31 .. 1.
 //
 // Bound: 4 D flops a row and key on the tensor core, 16 exponentials a cycle (as many cycles at D = 128), and the
@@ -23,22 +24,22 @@ namespace spb {
 namespace {
 using namespace sm100;
 
-constexpr int kRows = 256, kKeys = 128, kBlocks = kKeys / kKvBlock, kRaw = 2, kInfo = 4;
-constexpr int kEdge = 4;   // 256 rows see at most 255 keys apart: three tiles
-constexpr int kThreads = 32 * 20;
+constexpr int kRows = 256, kKeys = 64, kBlocks = kKeys / kKvBlock, kRaw = 4, kInfo = 16;
+constexpr int kEdge = 6;   // 256 rows see at most 255 keys apart: five tiles
+constexpr int kThreads = 32 * 20, kExpand = 12;   // first expanding warp
 constexpr float kShift = 7.f, kSlack = 8.f;
 
 template <int D>
 struct Smem {
     uint8_t q[2][D / 64][128 * 128];          // [row tile][64 channels][row][128 bytes], swizzled
-    uint8_t k[D / 64][kKeys * 128];           // [64 channels][key][128 bytes]
-    uint8_t v[kKeys / 64][D * 128];           // [64 keys][channel][128 bytes]
+    uint8_t k[2][D / 64][kKeys * 128];        // [key tile & 1][64 channels][key][128 bytes]
+    uint8_t v[2][D * 128];                    // [key tile & 1][channel][64 keys]
     uint8_t raw[kRaw][kBlocks][KvLayout<D>::kBlockBytes];
-    uint64_t raw_full[kRaw], raw_empty[kRaw], k_ready, k_free, v_ready, v_free, s_full[2], p_ready[2], o_full[2];
+    uint64_t raw_full[kRaw], raw_empty[kRaw], k_ready[2], k_free[2], v_ready[2], v_free[2], s_full[2][2], p_ready[2][2], pv_done[2], o_full[2];
     uint32_t holder;
     int abort;
     int blocks[kInfo];                        // blocks of the key tile that are there
-    uint16_t nan[kEdge][D / kKvGroup][kBlocks];   // tokens whose values are NaN, taken out of the products (tiles at the causal edge)
+    alignas(8) uint16_t nan[kEdge][D / kKvGroup][kBlocks];   // tokens whose values are NaN, taken out of the products (tiles at the causal edge)
 };
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
@@ -51,12 +52,113 @@ __device__ __forceinline__ float exp2_approx(float x)
 }
 __device__ __forceinline__ uint32_t swizzled(uint32_t base, int row, int chunk) { return base + row * 128 + ((chunk ^ (row & 7)) << 4); }
 
+// Two fp32 values an instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// What a stretch of 16 scores needs: nothing (all rows of the warp see all of it), a look at each, or nobody sees it.
+enum class Care { kNone, kEach, kUnseen };
+// Keys of the tile that the rows of a warp see, and blocks that are there.
+struct Sight {
+    int mine, least, most;   // of this row, the least and most of the warp's
+    uint32_t there;
+    __device__ __forceinline__ Care of(int q) const   // stretch 16 q ..
+    {
+        if (!(there >> q & 1) || 16 * q >= most) return Care::kUnseen;
+        return 16 * q + 16 <= least ? Care::kNone : Care::kEach;
+    }
+};
+// The largest of 64 scores, in base 2.
+__device__ __forceinline__ float row_top(const uint32_t (&v)[kKeys], float f, const Sight& s)
+{
+    float top = -INFINITY;
+    if (s.there == (1u << kBlocks) - 1 && s.least >= kKeys && f >= 0.f) {
+        float m[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m[k] = __uint_as_float(v[16 * k + 15]);
+#pragma unroll
+        for (int e = 0; e < 14; e += 2)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m[k] = max3(m[k], __uint_as_float(v[16 * k + e]), __uint_as_float(v[16 * k + e + 1]));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m[k] = fmaxf(m[k], __uint_as_float(v[16 * k + 14]));
+        return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * f;
+    }
+#pragma unroll
+    for (int q = 0; q < kBlocks; ++q)
+        if (s.of(q) != Care::kUnseen)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, 16 * q + e < s.mine ? __uint_as_float(v[16 * q + e]) * f : -INFINITY);
+    return top;
+}
+// The scores' weights 2^(f s - base), to tensor memory as fp16; their sum.
+__device__ __forceinline__ float row_weights(uint32_t addr, uint32_t (&v)[kKeys], float f, float base, const Sight& s)
+{
+    const uint64_t ff = pack2(f, f), bb = pack2(-base, -base);
+    uint64_t sum = 0;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        uint32_t p[16];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int q = 2 * half + h;
+            const Care care = s.of(q);
+            if (care == Care::kUnseen) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[8 * h + e] = 0;
+            } else {
+                float x[16];
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) unpack2(fma2(pack2(__uint_as_float(v[16 * q + e]), __uint_as_float(v[16 * q + e + 1])), ff, bb), x[e], x[e + 1]);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = exp2_approx(x[e]);
+                if (care == Care::kEach)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = 16 * q + e < s.mine ? x[e] : 0.f;
+                uint64_t a = pack2(x[0], x[1]), b = pack2(x[2], x[3]);
+#pragma unroll
+                for (int e = 4; e < 16; e += 4) a = add2(a, pack2(x[e], x[e + 1])), b = add2(b, pack2(x[e + 2], x[e + 3]));
+                sum = add2(sum, add2(a, b));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[8 * h + e] = h2_bits(__floats2half2_rn(x[2 * e], x[2 * e + 1]));
+            }
+        }
+        tc_st16(addr + 16 * half, p);
+    }
+    float x, y;
+    unpack2(sum, x, y);
+    return x + y;
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) kv_prefill_kernel(KvAttnArgs a, int tall, int* status)
 {
     using L = KvLayout<D>;
     constexpr int G = L::kGroups, KSteps = D / 16;
-    constexpr uint32_t kS = 0, kO = 256;   // tensor memory columns: scores of tile t at 128 t, outputs at 256 + D t
+    constexpr uint32_t kS = 0, kO = 256;   // tensor memory columns: scores of row tile t and key tile i at 128 t + 64 (i & 1), outputs at 256 + D t
     extern __shared__ uint8_t smem_raw[];
     Smem<D>& sm = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
@@ -103,18 +205,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefill_kernel(KvAttnArgs a, i
     const int n0 = ntile == 1 ? n1 : (min(visible(row0 + 127), held) + kKeys - 1) / kKeys;   // of row tile 0
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kRaw; ++i) mbar_init(smem_u32(&sm.raw_full[i]), 1), mbar_init(smem_u32(&sm.raw_empty[i]), 8);
-        mbar_init(smem_u32(&sm.k_ready), 8);
-        mbar_init(smem_u32(&sm.v_ready), 8);
-        mbar_init(smem_u32(&sm.k_free), 1);
-        mbar_init(smem_u32(&sm.v_free), 1);
-        for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&sm.s_full[i]), 1), mbar_init(smem_u32(&sm.p_ready[i]), 4), mbar_init(smem_u32(&sm.o_full[i]), 1);
+        for (int i = 0; i < kRaw; ++i) mbar_init(smem_u32(&sm.raw_full[i]), 1), mbar_init(smem_u32(&sm.raw_empty[i]), 4);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&sm.k_ready[i]), 4), mbar_init(smem_u32(&sm.k_free[i]), 1);
+            mbar_init(smem_u32(&sm.v_ready[i]), 4), mbar_init(smem_u32(&sm.v_free[i]), 1);
+            mbar_init(smem_u32(&sm.s_full[i][0]), 1), mbar_init(smem_u32(&sm.s_full[i][1]), 1);
+            mbar_init(smem_u32(&sm.p_ready[i][0]), 4), mbar_init(smem_u32(&sm.p_ready[i][1]), 4), mbar_init(smem_u32(&sm.pv_done[i]), 1), mbar_init(smem_u32(&sm.o_full[i]), 1);
+        }
         sm.abort = 0;
         mbar_init_fence();
     }
     if (warp == 1) tc_alloc(smem_u32(&sm.holder), 512);   // all columns: the allocation starts at 0
     // q of both tiles, rows past the end as zeros
-    if (warp >= 4 && warp < 12) {
+    if (warp >= 4 && warp < 12) {   // one thread a row
         const int tile = (warp - 4) / 4, r = (warp & 3) * 32 + lane, row = tile * 128 + r;
         const bool have = row < rows;
         const int abs_row = row0 + (have ? row : 0);
@@ -161,79 +264,78 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefill_kernel(KvAttnArgs a, i
     } else if (warp == 1) {
         // ---- matrix instructions
         const uint32_t q0 = kmajor_desc_low(smem_u32(sm.q)), k0 = kmajor_desc_low(smem_u32(sm.k)), v0 = kmajor_desc_low(smem_u32(sm.v));
-        auto scores = [&](int t) {
+        auto scores = [&](int i, int t) {   // of key tile i, row tile t
             if (elect_one()) {
+                const uint32_t kd = k0 + (i & 1) * (uint32_t)(sizeof(sm.k[0]) >> 4), qd = q0 + t * (uint32_t)(sizeof(sm.q[0]) >> 4), d = kS + t * 128 + (i & 1) * 64;
 #pragma unroll
-                for (int tt = 0; tt < 2; ++tt)
-                    if (t == tt)
-#pragma unroll
-                        for (int j = 0; j < KSteps; ++j)
-                            tc_mma_ss(kS + tt * 128, q0 + (tt * (D / 64) + j / 4) * 1024 + 2 * (j % 4), k0 + j / 4 * 1024 + 2 * (j % 4), kKMajorDescHigh, f16_idesc(128, kKeys), j > 0);
-                tc_commit(smem_u32(&sm.s_full[t]));
+                for (int j = 0; j < KSteps; ++j)
+                    tc_mma_ss(d, qd + j / 4 * 1024 + 2 * (j % 4), kd + j / 4 * (kKeys * 8) + 2 * (j % 4), kKMajorDescHigh, f16_idesc(128, kKeys), j > 0);
+                tc_commit(smem_u32(&sm.s_full[t][i & 1]));
+                if (t == ntile - 1) tc_commit(smem_u32(&sm.k_free[i & 1]));   // the last row tile sees most: it is never the first to end
             }
             __syncwarp();
         };
-        if (n1 > 0) {
-            ok = mbar_wait(smem_u32(&sm.k_ready), 0, abort_flag);
+        for (int i = 0; i < 2 && i < n1 && ok; ++i) {
+            ok = mbar_wait(smem_u32(&sm.k_ready[i]), 0, abort_flag);
+            if (!ok) break;
             tc_fence_after();
-            if (ok) {
-                if (n0 > 0) scores(0);
-                if (ntile == 2) scores(1);
-                if (elect_one()) tc_commit(smem_u32(&sm.k_free));
-                __syncwarp();
-            }
+            if (i < n0) scores(i, 0);
+            if (ntile == 2) scores(i, 1);
         }
         for (int i = 0; i < n1 && ok; ++i) {
             bool have_v = false, have_k = false;
             for (int t = 0; t < ntile && ok; ++t) {
                 const int n = t == 0 ? n0 : n1;
                 if (i >= n) continue;
-                ok = mbar_wait(smem_u32(&sm.p_ready[t]), i & 1, abort_flag);
-                if (ok && !have_v) ok = have_v = mbar_wait(smem_u32(&sm.v_ready), i & 1, abort_flag);
+                ok = mbar_wait(smem_u32(&sm.p_ready[t][i & 1]), i / 2 & 1, abort_flag);   // per buffer: the softmax may be two tiles ahead
+                if (ok && !have_v) ok = have_v = mbar_wait(smem_u32(&sm.v_ready[i & 1]), i / 2 & 1, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
+                    const uint32_t vd = v0 + (i & 1) * (uint32_t)(sizeof(sm.v[0]) >> 4), pa = kS + t * 128 + (i & 1) * 64, d = kO + t * D;
 #pragma unroll
-                    for (int tt = 0; tt < 2; ++tt)
-                        if (t == tt)
-#pragma unroll
-                            for (int j = 0; j < kKeys / 16; ++j)
-                                tc_mma_ts(kO + tt * D, kS + tt * 128 + 8 * j, v0 + j / 4 * (D * 8) + 2 * (j % 4), kKMajorDescHigh, f16_idesc(128, D), i > 0 || j > 0);
+                    for (int j = 0; j < kKeys / 16; ++j) tc_mma_ts(d, pa + 8 * j, vd + 2 * j, kKMajorDescHigh, f16_idesc(128, D), i > 0 || j > 0);
+                    tc_commit(smem_u32(&sm.pv_done[t]));
                     if (i == n - 1) tc_commit(smem_u32(&sm.o_full[t]));
-                    if (t == ntile - 1) tc_commit(smem_u32(&sm.v_free));   // the last tile is never the first to end
+                    if (t == ntile - 1) tc_commit(smem_u32(&sm.v_free[i & 1]));
                 }
                 __syncwarp();
-                if (i + 1 < n) {
-                    if (!have_k) ok = have_k = mbar_wait(smem_u32(&sm.k_ready), (i + 1) & 1, abort_flag);
+                if (i + 2 < n) {
+                    if (!have_k) ok = have_k = mbar_wait(smem_u32(&sm.k_ready[i & 1]), (i / 2 + 1) & 1, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
-                    scores(t);
-                    if (t == ntile - 1) {
-                        if (elect_one()) tc_commit(smem_u32(&sm.k_free));
-                        __syncwarp();
-                    }
+                    scores(i + 2, t);
                 }
             }
         }
-    } else if (warp >= 12) {
+    } else if (warp >= kExpand) {
         // ---- expansion: warp = block of the tile, lane 4 g + t as in the layout
-        const int blk = warp - 12, g = lane / 4, t = lane % 4;
+        const int blk = (warp - kExpand) % 4, odd = (warp - kExpand) / 4, g = lane / 4, t = lane % 4;
         uint32_t mask_low, mask_high, bits_low, bits_high;   // kept in registers for and_or
         asm volatile("mov.b32 %0, 0x000f000f;\n\tmov.b32 %1, 0x00f000f0;\n\tmov.b32 %2, 0x64006400;\n\tmov.b32 %3, 0x54005400;"
                      : "=r"(mask_low), "=r"(mask_high), "=r"(bits_low), "=r"(bits_high));
         auto low = [&](uint32_t w, __half2 s, __half2 m) { return h2_bits(__hfma2(__hsub2(as_h2(and_or(w, mask_low, bits_low)), as_h2(bits_low)), s, m)); };
         auto high = [&](uint32_t w, __half2 s, __half2 m) { return h2_bits(__hfma2(__hsub2(as_h2(and_or(w, mask_high, bits_high)), as_h2(bits_high)), s, m)); };
-        for (int i = 0; i < n1 && ok; ++i) {
+        // where the lane's values go, up to constants: keys by 16-byte chunk (2 u of each half of a 64-channel row), values by channel & 1
+        // and half of the block
+        uint32_t k_at[4], v_at[2][2];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) k_at[u] = swizzled(smem_u32(sm.k[odd]), blk * kKvBlock + g, 2 * u + (t >> 1)) + (t & 1) * 8;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) v_at[r][j] = swizzled(smem_u32(sm.v[odd]), 2 * g + r, blk * 2 + j) + 4 * t;
+        // a group of four warps has every other tile, and with it every other stage and one of each two buffers: it waits for every phase
+        for (int i = odd; i < n1 && ok; i += 2) {
             const int s = i % kRaw, pos = i * kKeys + blk * kKvBlock;
             ok = mbar_wait(smem_u32(&sm.raw_full[s]), (i / kRaw) & 1, abort_flag);
             if (!ok) break;
             const bool there = sm.blocks[i % kInfo] >> blk & 1;
             const uint8_t* src = sm.raw[s][blk];
-            if (i) ok = mbar_wait(smem_u32(&sm.k_free), (i - 1) & 1, abort_flag);
+            if (i >= 2) ok = mbar_wait(smem_u32(&sm.k_free[odd]), (i / 2 - 1) & 1, abort_flag);
             if (!ok) break;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int r = blk * kKvBlock + g + 8 * e;
 #pragma unroll
                 for (int w = 0; w < G; ++w) {
                     const uint32_t x = reinterpret_cast<const uint32_t*>(src + L::kKCodes)[(g + 8 * e) * (D / 8) + t * G + w], y = x >> 8;
@@ -242,14 +344,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefill_kernel(KvAttnArgs a, i
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const uint32_t v0 = u ? high(x, sc, mn) : low(x, sc, mn), v1 = u ? high(y, sc, mn) : low(y, sc, mn);
-                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(swizzled(smem_u32(sm.k[w / 2]), r, 4 * (w & 1) + 2 * u + (t >> 1)) + (t & 1) * 8), "r"(v0), "r"(v1) : "memory");
+                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(k_at[2 * (w & 1) + u] + w / 2 * (kKeys * 128) + e * 1024), "r"(v0), "r"(v1) : "memory");
                     }
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sm.k_ready));
-            if (i) ok = mbar_wait(smem_u32(&sm.v_free), (i - 1) & 1, abort_flag);
+            if (lane == 0) mbar_arrive(smem_u32(&sm.k_ready[odd]));
+            if (i >= 2) ok = mbar_wait(smem_u32(&sm.v_free[odd]), (i / 2 - 1) & 1, abort_flag);
             if (!ok) break;
             const bool edge = i >= edge0;
 #pragma unroll
@@ -275,14 +377,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefill_kernel(KvAttnArgs a, i
                         }
                     }
                     const __half2 sc = as_h2(p.x), mn = as_h2(p.y);
-                    const uint32_t dst = smem_u32(sm.v[blk / 4]) + 4 * t;
-                    const int chunk = (blk & 3) * 2 + j;
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const int ch = 32 * w + 16 * u + 2 * g;
-                        const uint32_t z = u ? y : x;
-                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(swizzled(dst, ch, chunk)), "r"(low(z, sc, mn)) : "memory");
-                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(swizzled(dst, ch + 1, chunk)), "r"(high(z, sc, mn)) : "memory");
+                        const uint32_t z = u ? y : x, rows = (32 * w + 16 * u) * 128;
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(v_at[0][j] + rows), "r"(low(z, sc, mn)) : "memory");
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(v_at[1][j] + rows), "r"(high(z, sc, mn)) : "memory");
                     }
                 }
                 if (edge) {
@@ -294,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefill_kernel(KvAttnArgs a, i
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(smem_u32(&sm.v_ready));
+                mbar_arrive(smem_u32(&sm.v_ready[odd]));
                 mbar_arrive(smem_u32(&sm.raw_empty[s]));
             }
         }
@@ -303,72 +402,47 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefill_kernel(KvAttnArgs a, i
         const int tile = (warp - 4) / 4, row = tile * 128 + (warp & 3) * 32 + lane, abs_row = row0 + row;
         const bool have = row < rows;
         const int mine = have ? min(visible(abs_row), held) : 0, n = tile == 0 ? n0 : ntile == 2 ? n1 : 0;
-        const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_addr = kS + tile * 128 + lanes, o_addr = kO + tile * D + lanes;
+        const int least = __reduce_min_sync(0xffffffffu, mine), most = __reduce_max_sync(0xffffffffu, mine);
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21, o_addr = kO + tile * D + lanes;
         const float f = a.scale * 1.4426950408889634f;
         float mx = -INFINITY, sum = 0.f;
-        const int tile_min = visible(row0 + tile * 128);   // keys that every row of the tile sees
         for (int i = 0; i < n && ok; ++i) {
-            ok = mbar_wait(smem_u32(&sm.s_full[tile]), i & 1, abort_flag);
+            ok = mbar_wait(smem_u32(&sm.s_full[tile][i & 1]), i / 2 & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t there = sm.blocks[i % kInfo];
-            const bool edge = (i + 1) * kKeys > tile_min || there != 0xffu || row0 + tile * 128 + 127 >= rows_all;
-            const int limit = mine - i * kKeys;   // first key of the tile that the row does not see
-            float top = -INFINITY;
-#pragma unroll 1
-            for (int q = 0; q < kKeys; q += 16) {
-                uint32_t v[16];
-                tc_ld16(s_addr + q, v);
-                tc_wait_ld();
-                if (edge) {
-                    const int seen = there >> (q / kKvBlock) & 1 ? limit - q : 0;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) top = fmaxf(top, e < seen ? __uint_as_float(v[e]) * f : -INFINITY);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) top = fmaxf(top, __uint_as_float(v[e]) * f);
-                }
-            }
+            const uint32_t s_addr = kS + tile * 128 + (i & 1) * 64 + lanes;
+            const Sight sight{mine - i * kKeys, least - i * kKeys, most - i * kKeys, (uint32_t)sm.blocks[i % kInfo]};
+            uint32_t v[kKeys];
+            tc_ld32(s_addr, v);
+            tc_ld32(s_addr + 32, v + 32);
+            tc_wait_ld();
+            const float top = row_top(v, f, sight);
             if (__any_sync(0xffffffffu, top > mx + kSlack)) {
-                const float now = fmaxf(top, mx), r = mx == -INFINITY ? 0.f : exp2_approx(mx - now);
+                const float now = fmaxf(top, mx), c = mx == -INFINITY ? 0.f : exp2_approx(mx - now);
                 mx = now;
-                sum *= r;
-                if (i > 0) {   // P V of the tile before has ended: S of this one was issued behind it
+                sum *= c;
+                if (i > 0) {
+                    // The accumulators rest when P V of the tile before has ended.  S of this one was issued behind P V (i - 2): at most
+                    // that one is still to come, and the phase's parity tells.
+                    ok = mbar_wait(smem_u32(&sm.pv_done[tile]), (i - 1) & 1, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
 #pragma unroll 1
                     for (int q = 0; q < D; q += 16) {
-                        uint32_t v[16];
-                        tc_ld16(o_addr + q, v);
+                        uint32_t x[16];
+                        tc_ld16(o_addr + q, x);
                         tc_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * r);
-                        tc_st16(o_addr + q, v);
+                        for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * c);
+                        tc_st16(o_addr + q, x);
                     }
                 }
             }
-            const float base = (mx == -INFINITY ? 0.f : mx) - kShift;
-#pragma unroll 1
-            for (int q = 0; q < kKeys; q += 32) {
-                uint32_t p[16];
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t v[16];
-                    tc_ld16(s_addr + q + 16 * half, v);
-                    tc_wait_ld();
-                    const int at = q + 16 * half, seen = edge ? (there >> (at / kKvBlock) & 1 ? limit - at : 0) : 16;
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        float x = exp2_approx(fmaf(__uint_as_float(v[e]), f, -base)), y = exp2_approx(fmaf(__uint_as_float(v[e + 1]), f, -base));
-                        if (edge) x = e < seen ? x : 0.f, y = e + 1 < seen ? y : 0.f;
-                        sum += x + y;
-                        p[8 * half + e / 2] = h2_bits(__floats2half2_rn(x, y));
-                    }
-                }
-                tc_st16(s_addr + q / 2, p);   // over scores that have been read
-            }
+            sum += row_weights(s_addr, v, f, (mx == -INFINITY ? 0.f : mx) - kShift, sight);
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sm.p_ready[tile]));
+            if (lane == 0) mbar_arrive(smem_u32(&sm.p_ready[tile][i & 1]));
         }
         if (tile < ntile && ok) {
             if (n > 0) ok = mbar_wait(smem_u32(&sm.o_full[tile]), 0, abort_flag);
@@ -376,29 +450,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefill_kernel(KvAttnArgs a, i
                 tc_fence_after();
                 uint32_t poison = 0;   // groups of channels that are NaN for this row
                 for (int i = edge0; i < n; ++i)
-                    for (int w = 0; w < G; ++w)
-                        for (int k = 0; k < kBlocks; ++k) {
-                            const int seen = mine - i * kKeys - k * kKvBlock;
-                            const uint32_t mask = seen >= 16 ? 0xffffu : seen <= 0 ? 0u : (1u << seen) - 1;
-                            if (sm.nan[i - edge0][w][k] & mask) poison |= 1u << w;
-                        }
+                    for (int w = 0; w < G; ++w) {
+                        const uint64_t bits = *reinterpret_cast<const uint64_t*>(sm.nan[i - edge0][w]);
+                        const int seen = mine - i * kKeys;
+                        const uint64_t mask = seen >= 64 ? ~0ull : seen <= 0 ? 0ull : (1ull << seen) - 1;
+                        if (bits & mask) poison |= 1u << w;
+                    }
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;   // no visible key: zeros
                 uint16_t* dst = a.out + ((long long)(first + abs_row / group) * a.q_heads + h * group + abs_row % group) * D;
 #pragma unroll 1
                 for (int q = 0; q < D; q += 16) {
-                    uint32_t v[16];
+                    uint32_t x[16];
                     if (n > 0) {
-                        tc_ld16(o_addr + q, v);
+                        tc_ld16(o_addr + q, x);
                         tc_wait_ld();
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) v[e] = 0;
+                        for (int e = 0; e < 16; ++e) x[e] = 0;
                     }
                     uint32_t y[8];
                     const bool bad = poison >> (q / kKvGroup) & 1;
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        y[e] = bad ? 0x7fff7fffu : h2_bits(__floats2half2_rn(__uint_as_float(v[2 * e]) * inv, __uint_as_float(v[2 * e + 1]) * inv));
+                        y[e] = bad ? 0x7fff7fffu : h2_bits(__floats2half2_rn(__uint_as_float(x[2 * e]) * inv, __uint_as_float(x[2 * e + 1]) * inv));
                     if (have) {
                         reinterpret_cast<uint4*>(dst + q)[0] = make_uint4(y[0], y[1], y[2], y[3]);
                         reinterpret_cast<uint4*>(dst + q)[1] = make_uint4(y[4], y[5], y[6], y[7]);
