@@ -29,7 +29,7 @@ template <int NT, int kGroup>
 struct StreamSmem {
     uint8_t ring[kWarps][kStages][int4_unit_bytes(kGroup)];
     float sums[kWarps][8 * 4][32];   // [warp][row tile, register][lane], one tile of 8 rows of x at a time
-    float total[8 * NT][128];        // cluster: this thread block's part of the item
+    alignas(16) float total[8 * NT][128];   // cluster: this thread block's part of the item
     uint64_t full[kWarps][kStages];
     int abort;
 };
@@ -178,18 +178,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) int4_stream_kernel(const __gri
             }
         }
     }
-    if (p.split > 1) {
-        // the parts of the cluster's thread blocks, in order of k; each finishes every split-th stretch of 256 values
-        cluster_sync();
-        const int rank = blockIdx.x % p.split;
-        for (int e = rank * (32 * kWarps) + threadIdx.x; e < min(p.a.N, 8 * NT) * 128; e += p.split * 32 * kWarps) {
-            float y = 0.f;
-            for (int i = 0; i < p.split; ++i) y += cluster_load(smem_u32(&sm.total[0][0] + e), i);
-            const long long m = (long long)(blockIdx.x / p.split) * 128 + (e & 127), n = e >> 7;
-            if (m < p.a.M) p.a.out[n * p.a.M + m] = __half_as_ushort(__float2half_rn(finish(p.a, y, m, n)));
-        }
-        cluster_sync();   // nobody leaves while its part is being read
-    }
+    if (p.split > 1) cluster_finish<8 * NT>(p, smem_u32(&sm.total[0][0]));
     if (!alive) {   // a wait ran out: report, and give the copies still under way one more bounded wait
         if (lane == 0) atomicOr(p.status, (int)kStatusWaitTimeout);
         for (int i = 0; i < kStages; ++i)

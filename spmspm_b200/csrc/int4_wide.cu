@@ -207,6 +207,8 @@ __global__ void __launch_bounds__(Cfg<NPAD>::kThreads, 1) int4_wide_kernel(const
             const bool cut = !(r.first && r.last);
             float* slot = p.a.ws + (2 * (size_t)blockIdx.x + r.first) * NPAD * 128 + 32 * quad + lane;
             const long long m = (long long)r.mb * 128 + 32 * quad + lane;
+            const float bias = p.a.bias && m < p.a.M ? __half2float(__ushort_as_half(p.a.bias[m])) : 0.f;
+            float* part = reinterpret_cast<float*>(smem + 1024);
             const uint32_t base = tmem + ((uint32_t)quad << 21);
 #pragma unroll 1
             for (int c = 0; c < NPAD && r.n0 + c < p.a.N; c += 16) {
@@ -223,15 +225,22 @@ __global__ void __launch_bounds__(Cfg<NPAD>::kThreads, 1) int4_wide_kernel(const
 #pragma unroll
                     for (int i = 0; i < 16; ++i) y[i] += __uint_as_float(v[i]);
                 }
-                if (cut) {
+                if (p.split > 1) {   // the stages are idle: this run is the thread block's only one
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) part[(c + i) * 128 + 32 * quad + lane] = y[i];
+                } else if (cut) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) slot[(c + i) * 128] = y[i];
                 } else if (m < p.a.M) {
+                    // all residuals first: they may be the output itself, and loads do not pass stores (one after the other they
+                    // cost 9216 x 36864 with 509 rows 90 us)
+                    const long long at = (r.n0 + c) * (long long)p.a.M + m;
+                    uint16_t res[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const long long n = r.n0 + c + i;
-                        if (n < p.a.N) p.a.out[n * p.a.M + m] = __half_as_ushort(__float2half_rn(finish(p.a, y[i], m, n)));
-                    }
+                    for (int i = 0; i < 16; ++i) res[i] = p.a.residual && r.n0 + c + i < p.a.N ? p.a.residual[at + (long long)i * p.a.M] : (unsigned short)0;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (r.n0 + c + i < p.a.N) p.a.out[at + (long long)i * p.a.M] = __half_as_ushort(__float2half_rn(finish(p.a, y[i], bias, res[i])));
                 }
             }
             tc_fence_before();
@@ -244,6 +253,7 @@ __global__ void __launch_bounds__(Cfg<NPAD>::kThreads, 1) int4_wide_kernel(const
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (p.split > 1) cluster_finish<NPAD>(p, stage0);
     if (*abort_flag) {
         if (threadIdx.x == 0) {
             atomicOr(p.status, (int)kStatusWaitTimeout);

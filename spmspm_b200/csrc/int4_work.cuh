@@ -29,12 +29,15 @@ __device__ __forceinline__ int share_of(const Params& p, int x)   // not whole
     const int big = p.extra * (p.share + 1);
     return x < big ? x / (p.share + 1) : p.extra + (x - big) / p.share;
 }
+__device__ __forceinline__ float finish(const Int4Args& a, float y, float bias, uint16_t residual)
+{
+    y += bias;
+    if (a.activation) y = y < 0.f ? 0.f : y;   // NaN stays NaN
+    return y + __half2float(__ushort_as_half(residual));
+}
 __device__ __forceinline__ float finish(const Int4Args& a, float y, long long m, long long n)
 {
-    if (a.bias) y += __half2float(__ushort_as_half(a.bias[m]));
-    if (a.activation) y = y < 0.f ? 0.f : y;   // NaN stays NaN
-    if (a.residual) y += __half2float(__ushort_as_half(a.residual[n * a.M + m]));
-    return y;
+    return finish(a, y, a.bias ? __half2float(__ushort_as_half(a.bias[m])) : 0.f, a.residual ? a.residual[n * a.M + m] : (unsigned short)0);
 }
 
 // A run of k-tiles of one item.
@@ -77,33 +80,71 @@ struct Walk {
     }
 };
 
-// Adds the partial sums of the items that were cut; blockIdx.x: item, blockIdx.y: columns by 8.
+// Four rows of one column, finished and stored.
+__device__ __forceinline__ void store4(const Int4Args& a, float4 sum, long long m, long long n)
+{
+    if (m >= a.M) return;   // M is a multiple of 64
+    const float y[4] = {sum.x, sum.y, sum.z, sum.w};
+    uint2 res = make_uint2(0, 0), bias = res;
+    if (a.residual) res = *reinterpret_cast<const uint2*>(a.residual + n * a.M + m);
+    if (a.bias) bias = *reinterpret_cast<const uint2*>(a.bias + m);
+    const uint16_t *rh = reinterpret_cast<const uint16_t*>(&res), *bh = reinterpret_cast<const uint16_t*>(&bias);
+    __half o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __float2half_rn(finish(a, y[i], __half2float(__ushort_as_half(bh[i])), rh[i]));
+    *reinterpret_cast<uint2*>(a.out + n * a.M + m) = *reinterpret_cast<uint2*>(o);
+}
+// The parts [column][128 rows] that a cluster's thread blocks have at `addr`, added in order of k: a warp takes a column, every
+// split-th stretch of columns a thread block.
 template <int NPAD>
-__global__ void __launch_bounds__(256) int4_join_kernel(const __grid_constant__ Params p)
+__device__ __forceinline__ void cluster_finish(const Params& p, uint32_t addr)
+{
+    cluster_sync();
+    const int rank = blockIdx.x % p.split, item = blockIdx.x / p.split, n0 = item % p.ncol * NPAD, warps = blockDim.x / 32, lane = threadIdx.x & 31;
+    for (int col = rank + p.split * (int)(threadIdx.x / 32); col < NPAD && n0 + col < p.a.N; col += p.split * warps) {
+        float4 v[8], sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = cluster_load4(addr + (col * 128 + 4 * lane) * 4, i < p.split ? i : rank);   // all under way together
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < p.split) sum.x += v[i].x, sum.y += v[i].y, sum.z += v[i].z, sum.w += v[i].w;
+        store4(p.a, sum, (long long)(item / p.ncol) * 128 + 4 * lane, n0 + col);
+    }
+    cluster_sync();   // nobody leaves while its part is being read
+}
+
+// Adds the partial sums of the items that were cut, in order; blockIdx.x: item, blockIdx.y: column, or columns by 8.  A warp takes a
+// column; with many parts (`spread`) a thread block does, its warps share out the parts.
+template <int NPAD>
+__global__ void __launch_bounds__(256) int4_join_kernel(const __grid_constant__ Params p, int spread)
 {
     const int x0 = blockIdx.x * p.ku, c0 = share_of(p, x0), c1 = share_of(p, x0 + p.ku - 1);
     grid_wait();
     if (c0 == c1) return;
-    const int col = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x & 31;
-    const long long n = (long long)(blockIdx.x % p.ncol) * NPAD + col, m0 = (long long)(blockIdx.x / p.ncol) * 128;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, col = spread ? blockIdx.y : blockIdx.y * 8 + warp;
+    const long long n = (long long)(blockIdx.x % p.ncol) * NPAD + col, m = (long long)(blockIdx.x / p.ncol) * 128 + 4 * lane;
     if (n >= p.a.N) return;
-    float4 sum;
     // the first part may be either slot of its thread block, the later ones start a thread block's share
     const float4* src = reinterpret_cast<const float4*>(p.a.ws + col * 128) + lane;
-    const float4 f = src[(2 * (size_t)c0 + 1) * (NPAD * 32)];
-    sum = f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int step = spread ? 8 : 1;
 #pragma unroll 4
-    for (int i = c0 + 1; i <= c1; ++i) {
-        const float4 v = src[2 * (size_t)i * (NPAD * 32)];
+    for (int i = c0 + (spread ? warp : 0); i <= c1; i += step) {
+        const float4 v = src[(2 * (size_t)i + (i == c0)) * (NPAD * 32)];
         sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
     }
-    const long long m = m0 + 4 * lane;
-    if (m >= p.a.M) return;   // M is a multiple of 64
-    const float y[4] = {sum.x, sum.y, sum.z, sum.w};
-    __half o[4];
+    if (spread) {
+        __shared__ float4 part[8][32];
+        part[warp][lane] = sum;
+        __syncthreads();
+        if (warp) return;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = __float2half_rn(finish(p.a, y[i], m + i, n));
-    *reinterpret_cast<uint2*>(p.a.out + n * p.a.M + m) = *reinterpret_cast<uint2*>(o);
+        for (int i = 1; i < 8; ++i) {
+            const float4 v = part[i][lane];
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+    }
+    store4(p.a, sum, m, n);
 }
 
 int sm_count()
@@ -135,17 +176,21 @@ Plan plan_for(int M, int N, int K)
     const int sms = sm_count();
     const long long rounds = (q.items + sms - 1) / sms, units = q.items * q.ku;
     q.whole = q.items >= 0.92 * rounds * sms;
-    if (N <= kInt4StreamRows && 2 * q.items <= sms) {
-        // Few items and few rows of x: the thread blocks of a cluster share an item and add up through shared memory, without a
-        // second launch (5120 x 5120, one row of x: 7.4 us against 9.9; 1024 x 1024: 3.6 against 4.8).  Eight units, one
-        // per warp, are worth a thread block.  All clusters have to fit at once: sixteen of eight did not, and 2048 x 8192 took
-        // 10.2 us in two rounds.
-        const long long most = sms / q.items, worth = (q.ku + 7) / 8;
+    if (2 * q.items <= sms) {
+        // Few items: the thread blocks of a cluster share one and add up through shared memory, without a second launch (5120 x 5120,
+        // one row of x: 7.4 us against 9.9; 1024 x 1024: 3.6 against 4.8).  The streaming kernel does eight units at a time,
+        // one per warp; the other one a unit after the other, so that with few clusters (they have eight thread blocks at most)
+        // an equal share for every SM and a join is faster again: the join costs what eight units do.  All clusters have to fit at
+        // once: sixteen of eight did not, and 2048 x 8192 took 10.2 us in two rounds.
+        const bool stream = N <= kInt4StreamRows;
+        const long long most = sms / q.items, worth = stream ? (q.ku + 7) / 8 : (q.ku + 1) / 2;
         int c = (int)(most < worth ? most : worth);
         if (c > 8) c = 8;
         while (c > 1 && int4_stream_clusters(c) < q.items) --c;
-        q.split = c;
-        q.whole = c > 1 || worth == 1;
+        if (stream || (q.ku + c - 1) / c <= units / sms + 8) {
+            q.split = c;
+            q.whole = c > 1 || worth == 1;
+        }
     }
     q.ctas = (int)(q.split > 1 ? q.items * q.split : q.whole ? (sms < q.items ? (long long)sms : q.items) : units < 2 ? 1ll : units / 2 < sms ? units / 2 : (long long)sms);   // at least two units a thread block
     return q;
@@ -185,10 +230,11 @@ cudaError_t launch_product(cudaStream_t s, Kernel kernel, int threads, size_t sm
     cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p, more...);
     count_launch();
     if (e != cudaSuccess || q.whole) return e;
-    cfg.gridDim = dim3((unsigned)q.items, ((p.a.N < NPAD ? p.a.N : NPAD) + 7) / 8);
+    const int cols = p.a.N < NPAD ? p.a.N : NPAD, spread = q.ctas > 8 * q.items;
+    cfg.gridDim = dim3((unsigned)q.items, spread ? cols : (cols + 7) / 8);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
-    e = cudaLaunchKernelEx(&cfg, int4_join_kernel<NPAD>, p);
+    e = cudaLaunchKernelEx(&cfg, int4_join_kernel<NPAD>, p, spread);
     count_launch();
     return e;
 }
