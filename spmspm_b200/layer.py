@@ -14,7 +14,9 @@ huggingface_opt_convert_Phase2.py:284-285):
 
 This module is the harness for that call sequence: layer norms, attention (torch's scaled_dot_product_attention on a
 static key/value cache) and residuals are stock PyTorch; the linear layers are spmspm_b200.spmm, and the two
-all-reduces are either the one-shot exchange over peer stores (spmspm_b200.dist.PeerReduce) or NCCL.
+all-reduces are either the one-shot exchange over peer stores (spmspm_b200.dist.PeerReduce) or NCCL.  With
+kv_cache="int4" the cache is the paged 4-bit one and attention runs over it (spmspm_b200.kv_append, kv_attention); with
+weights="int4" the matrices are quantised instead of pruned (spmspm_b200.linear_int4).
 """
 import torch
 import torch.distributed as dist
@@ -22,6 +24,8 @@ import torch.nn.functional as F
 
 from . import api
 from . import dist as spd
+from .int4 import decode_int4, encode_int4, linear_int4
+from .kv_cache import KvCacheInt4, kv_append, kv_attention
 
 
 def _gen(shape, seed, device, scale):
@@ -44,10 +48,13 @@ class SparseOptDecoderLayer:
     hidden % (64 * world) == 0 and heads % world == 0.  `reduce`: "peer" (one-shot all-reduce over peer stores),
     "nccl", or "none" for a single rank.  The key/value cache is static ([batch, heads/P, max_len, head_dim]) and the
     position is a device counter, so that a decode step has fixed shapes and can be captured into a CUDA graph.
+
+    weights: "bitmap" (pruned to `sparsity`) or "int4" (4-bit codes, groups of 128 or 64; `reduce` "nccl" or "none").
+    kv_cache: "dense" (fp16, attention by torch) or "int4" (paged, page_size tokens a page, head_dim 64 or 128).
     """
 
     def __init__(self, hidden, heads, ffn, sparsity, device, batch, max_len, group=None, reduce="peer", seed=0x5EED0005,
-                 keep_dense=False, fused=True):
+                 keep_dense=False, fused=True, weights="bitmap", kv_cache="dense", page_size=64):
         self.fused = fused   # bias / ReLU / residual inside the SpMM's launches (spb_linear_bitmap_v3) or as torch ops
         self.group = group
         self.world = dist.get_world_size(group) if dist.is_initialized() else 1
@@ -55,6 +62,11 @@ class SparseOptDecoderLayer:
         P, r = self.world, self.rank
         if hidden % (64 * P) or heads % P or ffn % (64 * P) or hidden % heads:
             raise ValueError("hidden, ffn must be multiples of 64 * world and heads a multiple of world")
+        if weights not in ("bitmap", "int4") or kv_cache not in ("dense", "int4"):
+            raise ValueError('weights must be "bitmap" or "int4" and kv_cache "dense" or "int4"')
+        if weights == "int4" and P > 1 and reduce == "peer":
+            raise ValueError('the one-shot exchange multiplies bitmap weights: weights="int4" needs reduce="nccl"')
+        self.weights, self.kv_cache = weights, kv_cache
         self.h, self.heads, self.ffn, self.d = hidden, heads, ffn, hidden // heads
         self.hp, self.fp_, self.heads_p = hidden // P, ffn // P, heads // P
         self.batch, self.max_len, self.device = batch, max_len, device
@@ -68,8 +80,13 @@ class SparseOptDecoderLayer:
         W1 = gen_pruned((ffn, hidden), seed + 4, dev, sparsity)[r * self.fp_:(r + 1) * self.fp_].contiguous()
         W2 = gen_pruned((hidden, ffn), seed + 5, dev, sparsity)[:, r * self.fp_:(r + 1) * self.fp_].contiguous()
         del Wq, Wk, Wv
-        self.dense = {"qkv": qkv, "out": Wo, "fc1": W1, "fc2": W2} if keep_dense else None
-        self.W = {k: api.encode_device(v) for k, v in (("qkv", qkv), ("out", Wo), ("fc1", W1), ("fc2", W2))}
+        dense = {"qkv": qkv, "out": Wo, "fc1": W1, "fc2": W2}
+        if weights == "int4":
+            self.W = {k: encode_int4(v, 128 if v.shape[1] % 128 == 0 else 64) for k, v in dense.items()}
+            dense = {k: decode_int4(v) for k, v in self.W.items()} if keep_dense else None
+        else:
+            self.W = {k: api.encode_device(v) for k, v in dense.items()}
+        self.dense = dense if keep_dense else None
         bq = _gen((3, hidden), seed + 6, dev, 0.02)
         self.b_qkv = bq[:, lo:hi].reshape(-1).contiguous()
         self.b_out = _gen((hidden,), seed + 7, dev, 0.02)
@@ -77,8 +94,14 @@ class SparseOptDecoderLayer:
         self.b_fc2 = _gen((hidden,), seed + 9, dev, 0.02)
         self.ln1_w, self.ln1_b = torch.ones(hidden, dtype=torch.float16, device=dev), torch.zeros(hidden, dtype=torch.float16, device=dev)
         self.ln2_w, self.ln2_b = self.ln1_w.clone(), self.ln1_b.clone()
-        self.k_cache = torch.zeros((batch, self.heads_p, max_len, self.d), dtype=torch.float16, device=dev)
-        self.v_cache = torch.zeros_like(self.k_cache)
+        if kv_cache == "int4":
+            pages = -(-max_len // page_size)
+            self.cache = KvCacheInt4(batch * pages, page_size, self.heads_p, self.d, device=dev)
+            self.page_table = torch.arange(batch * pages, dtype=torch.int32, device=dev).reshape(batch, pages)
+            self.kv_lens = torch.zeros(batch, dtype=torch.int32, device=dev)
+        else:
+            self.k_cache = torch.zeros((batch, self.heads_p, max_len, self.d), dtype=torch.float16, device=dev)
+            self.v_cache = torch.zeros_like(self.k_cache)
         self.pos = torch.zeros(1, dtype=torch.int64, device=dev)            # tokens in the cache
         self.arange = torch.arange(max_len, device=dev)
         self.split = {}
@@ -99,6 +122,8 @@ class SparseOptDecoderLayer:
 
     def _linear(self, name, x, bias=None, residual=None, relu=False):
         """x [N, K_local] -> residual + act(x W^T + bias) [N, M_local]; with `fused` in the SpMM's own launches."""
+        if self.weights == "int4":
+            return linear_int4(self.W[name], x, bias=bias, residual=residual, activation=api.ACT_RELU if relu else api.ACT_NONE)
         sk = self._split_k(name, x.shape[0])
         if self.fused:
             return api.linear(self.W[name], x, bias=bias, residual=residual, activation=api.ACT_RELU if relu else api.ACT_NONE,
@@ -148,13 +173,17 @@ class SparseOptDecoderLayer:
     # ---- forward -------------------------------------------------------------------------------------------
     def reset(self):
         self.pos.zero_()
+        if self.kv_cache == "int4":
+            self.kv_lens.zero_()
 
-    def forward(self, x, T):
-        """x [batch * T, h] (token-major within a sequence: row b * T + t), T new tokens per sequence appended at the
-        cache position.  Returns [batch * T, h]."""
+    def _attend(self, qkv, T):
+        """qkv [batch * T, 3 hp] -> attention output [batch * T, hp]; the new keys and values go into the cache."""
         Bn, hp, d = self.batch, self.hp, self.d
-        h1 = F.layer_norm(x, (self.h,), self.ln1_w, self.ln1_b)
-        qkv = self._linear("qkv", h1, self.b_qkv)                                    # [N, 3h/P]
+        if self.kv_cache == "int4":
+            q, k, v = (t.unflatten(1, (self.heads_p, d)) for t in qkv.split(hp, dim=1))                  # [B T, H/P, d]
+            self.kv_lens += T
+            kv_append(self.cache, k, v, self.page_table, self.kv_lens)
+            return kv_attention(q, self.cache, self.page_table, self.kv_lens).flatten(1)
         q, k, v = (t.reshape(Bn, T, self.heads_p, d).transpose(1, 2) for t in qkv.split(hp, dim=1))   # [B, H/P, T, d]
         idx = self.pos + self.arange[:T]                                             # device-side positions
         self.k_cache.index_copy_(2, idx, k.contiguous())
@@ -162,7 +191,14 @@ class SparseOptDecoderLayer:
         # key j is visible to query t when j <= pos + t
         mask = self.arange[None, :] <= (self.pos + self.arange[:T])[:, None]         # [T, max_len]
         attn = F.scaled_dot_product_attention(q, self.k_cache, self.v_cache, attn_mask=mask[None, None])
-        attn = attn.transpose(1, 2).reshape(Bn * T, hp).contiguous()
+        return attn.transpose(1, 2).reshape(Bn * T, hp).contiguous()
+
+    def forward(self, x, T):
+        """x [batch * T, h] (token-major within a sequence: row b * T + t), T new tokens per sequence appended at the
+        cache position.  Returns [batch * T, h]."""
+        h1 = F.layer_norm(x, (self.h,), self.ln1_w, self.ln1_b)
+        qkv = self._linear("qkv", h1, self.b_qkv)                                    # [N, 3h/P]
+        attn = self._attend(qkv, T)
         x = self._linear_reduced("out", attn, self.b_out, x)
         h2 = F.layer_norm(x, (self.h,), self.ln2_w, self.ln2_b)
         f1 = self._linear("fc1", h2, self.b_fc1, relu=True)
