@@ -34,7 +34,7 @@ __device__ __forceinline__ bool locate(const KvView& c, int tok, int& b, int& po
             else hi = mid;
         }
         b = lo;
-        const int end = c.cu[b + 1];
+        const int end = min(c.cu[b + 1], c.n_tokens);   // as kv_rows takes it
         if (tok >= end) return false;   // offsets that are not ascending
         pos = c.lens[b] - (end - tok);
     } else {
@@ -55,7 +55,7 @@ struct Cursor {
             return true;
         }
         const bool found = tok < c.n_tokens && locate(c, tok, b, pos);
-        end = !found ? 0 : c.cu ? c.cu[b + 1] : (b + 1) * c.per_seq;
+        end = !found ? 0 : c.cu ? min(c.cu[b + 1], c.n_tokens) : (b + 1) * c.per_seq;
         off = -1;
         return found;
     }

@@ -444,3 +444,20 @@ def test_shared_pages(sp):
     sp.kv_append(bt.cache, dev(bt.k[0]), dev(bt.v[0]), bt.table[:1].contiguous(), bt.kv_lens[:1].contiguous())
     sp.kv_append(bt.cache, dev(bt.k[1][16:]), dev(bt.v[1][16:]), bt.table[1:].contiguous(), bt.kv_lens[1:].contiguous())
     check_attention(sp, rng, bt, 4)
+
+
+def test_offsets_past_the_rows_touch_nothing_behind_them(sp):
+    """cu_q says more rows than there are, with enough of them for a warp to take eight: the rows there are count, as the last of the
+    sequence, and nothing behind them is written."""
+    rng = np.random.default_rng(21)
+    heads, D, n, more = 32, 64, 1203, 5
+    assert n * 2 * heads >= 8 * 64 * 150 and n % 8
+    bt = Batch(sp, rng, [n], [n], heads, D, 64)
+    cu = i32([0, n + more])
+    sp.kv_append(bt.cache, dev(bt.k[0]), dev(bt.v[0]), bt.table, bt.kv_lens, cu_q=cu)
+    whole = [torch.full((n + more, heads, D), 7.0, dtype=torch.float16, device="cuda") for _ in range(2)]
+    sp.kv_read(bt.cache, bt.table, bt.kv_lens, cu_q=cu, k_out=whole[0][:n], v_out=whole[1][:n])
+    for got, want in zip(whole, (bt.k[0], bt.v[0])):
+        assert np.array_equal(got[:n].cpu().numpy(), model.entry(want.astype(np.float64)).astype(np.float16))
+        assert bool((got[n:] == 7).all())
+    assert sp.device_status() == 0
