@@ -326,7 +326,8 @@ int spb_linear_allreduce_finish(void* stream, uint16_t* C, const uint16_t* parts
  *                    bias, residual: as there, or NULL; residual may be out itself.  workspace:
  *                    spb_int4_workspace_bytes bytes (0 for many shapes, NULL then), 16-byte aligned, need not be cleared;
  *                    not shared by calls that may run at the same time.  With more than 16 rows of x the product takes
- *                    the weights as spb_int4_decode returns them (rounded to fp16), with up to 16 unrounded.
+ *                    the weights as spb_int4_decode returns them (rounded to fp16), with up to 16 unrounded.  A row of x that
+ *                    holds an infinity may come out as NaN where the sum would be infinite.
  */
 size_t spb_int4_bytes(int M, int K, int group);
 size_t spb_int4_workspace_bytes(int M, int N, int K);
@@ -351,7 +352,7 @@ int spb_linear_int4(void* stream, const void* packed, int M, int K, int group, c
  *   page_table  [batch][table_stride] int32: page that holds tokens i * page_size .. of a sequence
  *   kv_lens     [batch] int32: tokens of the sequence in the cache, those of this call included
  *   cu_q        [batch + 1] int32: rows cu_q[b] .. cu_q[b + 1] - 1 of the packed inputs are the last tokens of sequence b; NULL:
- *               every sequence has n_tokens / batch of them.  Rows outside cu_q[0] .. cu_q[batch] - 1 are neither read nor written.
+ *               every sequence has n_tokens / batch of them.  Ascending; offsets past n_tokens count as n_tokens.  Rows outside cu_q[0] .. cu_q[batch] - 1 are neither read nor written.
  * all on the device, so that a captured step keeps working while the contexts grow.  A page number outside
  * 0 .. num_pages - 1, or a token past the table's width, sets bit 8 of the device status word; the token is then not written,
  * reads as zeros, and counts as unseen by attention.
@@ -361,11 +362,13 @@ int spb_linear_int4(void* stream, const void* packed, int M, int K, int group, c
  *                     are first turned by the angles of the token's position in the cache: pairs (i, i + rot_dim / 2), or
  *                     (2 i, 2 i + 1) if interleaved; computed in 64 bits, rounded once to fp16.  rot_dim: a multiple of 8.
  *                     A position that is negative (more new tokens than kv_lens) is skipped; one past max_pos is skipped
- *                     and sets bit 8.  Two rows of one call must not name the same slot of a page.
+ *                     and sets bit 8.  Two rows of one call must not name the same slot of a page.  q_out may be q itself.
  *   spb_kv_read       k, v [n_tokens][kv_heads][head_dim] fp16: what the cache holds for these tokens.
  *   spb_kv_attention  out[i] = softmax(scale q[i] K^T) V over the keys of its sequence up to its own position
  *                     (row cu_q[b + 1] - 1 sees all kv_lens[b]); a row that sees no key gets zeros.  q_heads is a multiple of
- *                     kv_heads.  max_q: an upper bound of the rows of one sequence; it only chooses the kernel's tiling.
+ *                     kv_heads.  max_q: an upper bound of the rows of one sequence; it only chooses the kernel.  Where there are
+                     many rows (a sequence with 64 and more of them a key head), keys and values are taken as spb_kv_read returns
+                     them, rounded to fp16; elsewhere unrounded.  A row of q that is not finite has no defined result.  out may be q itself.
  *                     workspace: spb_kv_attention_workspace_bytes bytes, 16-byte aligned, need not be cleared; not shared by
  *                     calls that may run at the same time.
  * k, v and q are fp16 with contiguous channels; token and head strides in elements, multiples of 4; pointers 8-byte aligned

@@ -96,6 +96,12 @@ void set_error(const char* fmt, ...);
 // how many kernels a piece of work takes, e.g. by reading the counter around the capture of a CUDA graph.
 void count_launch(int n = 1);
 bool aligned16(const void* p);
+// Whether [a, a + a_bytes) and [b, b + b_bytes) have a byte in common.
+inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
+}
 // Argument checks of the SpMM entry points (api.cu): cudaSuccess, or an error code with the message set.
 cudaError_t check_spmm_args(const char* who, const void* vals, const void* gtile, const void* mtile, const void* bitmap,
                             const void* max_nnz, const void* B, int M, int N, int K, const void* ws, int split_k);

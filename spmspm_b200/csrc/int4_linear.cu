@@ -186,6 +186,12 @@ int spb_linear_int4(void* stream, const void* packed, int M, int K, int group, c
         set_error("linear_int4: the weight, x, out, bias and residual must be 16-byte aligned");
         return (int)cudaErrorMisalignedAddress;
     }
+    const size_t out_bytes = 2 * (size_t)N * M;
+    if (overlap(out, out_bytes, x, 2 * (size_t)N * K) || overlap(out, out_bytes, bias, 2 * (size_t)M) ||
+        (residual != out && overlap(out, out_bytes, residual, out_bytes))) {
+        set_error("linear_int4: out overlaps x, the bias or, without being the same, the residual");
+        return (int)cudaErrorInvalidValue;
+    }
     const size_t need = spb_int4_workspace_bytes(M, N, K);
     if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need)) {
         set_error("linear_int4: needs a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace ? workspace_bytes : (size_t)0);

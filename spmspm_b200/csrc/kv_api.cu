@@ -52,6 +52,19 @@ bool check_vectors(const char* who, const char* name, const void* p, long long t
     }
     return true;
 }
+// Bytes from the first to the last element of [n][heads][dim] fp16.
+size_t span_bytes(long long n, long long tok, int heads, long long head, int dim)
+{
+    return n > 0 ? 2 * ((size_t)(n - 1) * tok + (size_t)(heads - 1) * head + dim) : 0;
+}
+// An output [n][heads][dim] may lie on the input `in` row by row (in place), but not otherwise on it.
+bool check_in_place(const char* who, const char* names, const void* out, const void* in, long long n, long long tok, int heads, long long head, int dim)
+{
+    const bool same = out == in && head == dim && (n < 2 || tok == (long long)heads * dim);
+    if (same || !overlap(out, span_bytes(n, (long long)heads * dim, heads, dim, dim), in, span_bytes(n, tok, heads, head, dim))) return true;
+    set_error("%s: %s overlap without being the same rows", who, names);
+    return false;
+}
 KvView view(void* pool, int num_pages, int page_size, int kv_heads, const int* table, int table_stride, const int* lens, const int* cu,
             int B, long long n_tokens)
 {
@@ -119,6 +132,13 @@ int spb_kv_append(void* stream, void* pool, int num_pages, int page_size, int kv
             set_error("%s: q_heads must be positive and n_tokens * heads below 2^31 (q_heads=%d)", who, q_heads);
             return (int)cudaErrorInvalidValue;
         }
+        if (!check_in_place(who, "q and q_out", q_out, q, n_tokens, q_token_stride, q_heads, q_head_stride, head_dim)) return (int)cudaErrorInvalidValue;
+        const size_t bytes = span_bytes(n_tokens, (long long)q_heads * head_dim, q_heads, head_dim, head_dim);
+        if (overlap(q_out, bytes, k, span_bytes(n_tokens, k_token_stride, kv_heads, k_head_stride, head_dim)) ||
+            overlap(q_out, bytes, v, span_bytes(n_tokens, v_token_stride, kv_heads, v_head_stride, head_dim))) {
+            set_error("%s: q_out overlaps the keys or values", who);
+            return (int)cudaErrorInvalidValue;
+        }
     }
     if (n_tokens == 0) return 0;
     int* status = nullptr;
@@ -146,6 +166,11 @@ int spb_kv_read(void* stream, const void* pool, int num_pages, int page_size, in
         !check_vectors(who, "k", k, 0, 0) || !check_vectors(who, "v", v, 0, 0))
         return (int)cudaErrorInvalidValue;
     if (n_tokens == 0) return 0;
+    const size_t bytes = 2 * (size_t)n_tokens * kv_heads * head_dim;
+    if (overlap(k, bytes, v, bytes)) {
+        set_error("%s: k and v overlap", who);
+        return (int)cudaErrorInvalidValue;
+    }
     int* status = nullptr;
     cudaError_t e = device_status_ptr(&status);
     if (e != cudaSuccess) return (int)e;
@@ -185,6 +210,7 @@ int spb_kv_attention(void* stream, const void* pool, int num_pages, int page_siz
         set_error("%s: out and the workspace must be given and 16-byte aligned", who);
         return (int)cudaErrorInvalidValue;
     }
+    if (!check_in_place(who, "q and out", out, q, n_tokens, q_token_stride, q_heads, q_head_stride, head_dim)) return (int)cudaErrorInvalidValue;
     if (workspace_bytes < spb_kv_attention_workspace_bytes(head_dim, batch, q_heads, kv_heads, max_q)) {
         set_error("%s: the workspace has %zu bytes, spb_kv_attention_workspace_bytes asks for %zu", who, workspace_bytes,
                   spb_kv_attention_workspace_bytes(head_dim, batch, q_heads, kv_heads, max_q));

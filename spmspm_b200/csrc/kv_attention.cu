@@ -25,7 +25,6 @@
 // the end of a row tile.
 #include "kv_int4.cuh"
 #include "sm100.cuh"
-#include <cstdio>
 
 namespace spb {
 namespace {
@@ -71,6 +70,8 @@ __device__ __forceinline__ float exp2_approx(float x)
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
 
+constexpr long long kMostUnits = (1ll << 31) - (1ll << 25);   // of a list
+
 // Sequence b of the work list.
 struct Seq {
     int b = 0;
@@ -95,16 +96,21 @@ __device__ __forceinline__ void load_seq(Seq& s, const KvView& c, int b, int gro
 template <int ROWS>
 struct List {
     Seq mine;
-    int total;   // units of the list
-    __device__ __forceinline__ List(const KvView& c, int group, int tall)
+    int total;       // units of the list
+    int before = 0;  // of them, those of sequences below `upto`
+    bool too_long;   // more than kMostUnits, which only sequences that share rows can bring about: refused
+    __device__ __forceinline__ List(const KvView& c, int group, int tall, int upto = 0)
     {
         const int lane = threadIdx.x & 31;
-        int sum = 0;
+        long long sum = 0;
         for (int b = lane; b < c.B; b += 32) {
             load_seq<ROWS>(mine, c, b, group, tall);
             sum += mine.total;
+            if (b < upto) before += mine.total;
         }
-        total = __reduce_add_sync(0xffffffffu, sum);
+        if (upto) before = __reduce_add_sync(0xffffffffu, before);
+        total = (int)__reduce_add_sync(0xffffffffu, (unsigned)sum);
+        too_long = __reduce_add_sync(0xffffffffu, (unsigned)min((sum + (1 << 20) - 1) >> 20, 1ll << 20)) >= 1u << 11;   // rounded up in each lane
     }
     // The sequence that holds unit x of the list (x inside the list); every lane gets the same.
     __device__ __forceinline__ void find(Seq& s, const KvView& c, int group, int tall, int x)
@@ -197,6 +203,10 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
     grid_release();   // the join may be set up while this kernel runs; it waits for its end
 
     List<ROWS> list(c, group, a.tall);
+    if (list.too_long) {
+        if (threadIdx.x == 0) atomicOr(status, kStatusBadCache);
+        return;
+    }
     const Shares shares(list.total, gridDim.x);
     int lo = shares.begin(blockIdx.x), hi = shares.begin(blockIdx.x + 1);
     Seq s;
@@ -698,18 +708,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvAt
     const int group = a.q_heads / c.kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     // the lengths are none of the preceding kernel's results, and what wrote them had ended before that kernel let this one start
     Seq s;
-    int begin = 0, total = 0;
-    for (int b = lane; b < c.B; b += 32) {
-        Seq o;
-        load_seq<ROWS>(o, c, b, group, a.tall);
-        total += o.total;
-        if (b < (int)blockIdx.y) begin += o.total;
-    }
+    const List<ROWS> list(c, group, a.tall, blockIdx.y);
+    const int total = list.total, begin = list.before;
     load_seq<ROWS>(s, c, blockIdx.y, group, a.tall);
-    begin = __reduce_add_sync(0xffffffffu, begin);
-    total = __reduce_add_sync(0xffffffffu, total);
     grid_wait();
-    if (total == 0) return;
+    if (total == 0 || list.too_long) return;
     const Shares shares(total, ctas);
     const int step = spread ? spread : kJoinWarps, pairs = spread ? gridDim.x / spread : gridDim.x;
     for (int pair = spread ? blockIdx.x / spread : blockIdx.x; pair < c.kv_heads * s.tiles; pair += pairs) {
@@ -829,7 +832,7 @@ cudaError_t launch(cudaStream_t s, const KvAttnArgs& a, int* status)
     const long long units = ((long long)a.c.table_stride * a.c.page_size - 1) / kUnit + 1;
     const long long tiles = ((long long)a.max_q * group + ROWS - 1) / ROWS;
     const long long most = (long long)a.c.B * a.c.kv_heads * (tiles > 0 ? tiles : 1) * units;
-    if (((long long)a.c.n_tokens * group / ROWS + a.c.B) * a.c.kv_heads * units > 0x7fffffff) {
+    if (((long long)a.c.n_tokens * group / ROWS + a.c.B) * a.c.kv_heads * units > kMostUnits) {
         set_error("kv_attention: too much work for one call (rows times context)");
         return cudaErrorInvalidValue;
     }

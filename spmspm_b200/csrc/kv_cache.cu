@@ -165,6 +165,7 @@ __global__ void __launch_bounds__(32 * kWarps) kv_append_kernel(KvAppendArgs a, 
                 else load4(p + c0 + 4 * k, x[k]);
             }
         }
+        __syncwarp();   // q_out may be q: all lanes of a vector have read it
         if (is_q) {
             if (write) *reinterpret_cast<uint4*>(a.q_out + ((long long)tok * a.q_heads + head) * D + c0) = *reinterpret_cast<uint4*>(x);
             write = false;

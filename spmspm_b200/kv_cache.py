@@ -25,10 +25,25 @@ class KvCacheInt4:
         if num_pages <= 0 or kv_heads <= 0 or page_size <= 0 or page_size % 16 or page_size > 65536:
             raise SpmmError("num_pages and kv_heads must be positive, page_size a multiple of 16 up to 65536")
         self.num_pages, self.page_size, self.kv_heads, self.head_dim = int(num_pages), int(page_size), int(kv_heads), int(head_dim)
-        self.pool = torch.zeros(_lib.load().spb_kv_cache_bytes(num_pages, page_size, kv_heads, head_dim), dtype=torch.uint8, device=device)
-        if not self.pool.is_cuda:
+        self._pool = torch.zeros(_lib.load().spb_kv_cache_bytes(num_pages, page_size, kv_heads, head_dim), dtype=torch.uint8, device=device)
+        if not self._pool.is_cuda:
             raise SpmmError("the cache lives on a CUDA device")
-        self._handle = _lib.ext().Cache(self.pool, self.num_pages, self.page_size, self.kv_heads, self.head_dim)
+        self._open()
+
+    def _open(self):
+        self._handle = _lib.ext().Cache(self._pool, self.num_pages, self.page_size, self.kv_heads, self.head_dim)
+
+    @property
+    def pool(self):
+        """The pages, uint8."""
+        return self._pool
+
+    def __getstate__(self):   # copies and saved caches have a handle of their own
+        return {k: v for k, v in self.__dict__.items() if k != "_handle"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._open()
 
     def token_bytes(self):
         """Bytes a token takes in one layer: codes, scales and minima of keys and values of all heads."""
@@ -43,7 +58,8 @@ def kv_append(cache, k, v, page_table, kv_lens, cu_q=None, q=None, cos=None, sin
     """spb_kv_append: write the keys and values [tokens, kv_heads, head_dim] of the new tokens.
 
     With cos and sin (float32 [positions, rot/2]) the first rot channels of the keys are first turned by the angles of the
-    token's position in the cache, and so are those of q [tokens, heads, head_dim], which is returned (q_out, or a new tensor).
+    token's position in the cache, and so are those of q [tokens, heads, head_dim], which is returned (q_out, which may be q itself,
+    or a new tensor).
     Rows that belong to no sequence leave q_out as it was."""
     return _lib.ext().kv_append(cache._handle, k, v, page_table, kv_lens, cu_q, q, cos, sin, interleaved, q_out, _raw(stream))
 
@@ -63,6 +79,6 @@ def kv_attention(q, cache, page_table, kv_lens, cu_q=None, max_q=None, scale=Non
     """spb_kv_attention: out [tokens, heads, head_dim] = softmax(scale q K^T) V over the keys of the row's sequence up to its own position.
 
     max_q: an upper bound of the new tokens of one sequence (default: tokens / batch without cu_q, all of them with it); it
-    chooses the kernel only.  scale: 1 / sqrt(head_dim) by default.  workspace: kv_attention_workspace() bytes; a new one
+    chooses the kernel only.  scale: 1 / sqrt(head_dim) by default.  out may be q itself.  workspace: kv_attention_workspace() bytes; a new one
     by default.  Rows that see no key get zeros, rows that belong to no sequence are left as they were."""
     return _lib.ext().kv_attention(q, cache._handle, page_table, kv_lens, cu_q, max_q, scale, out, workspace, _raw(stream))

@@ -461,3 +461,53 @@ def test_offsets_past_the_rows_touch_nothing_behind_them(sp):
         assert np.array_equal(got[:n].cpu().numpy(), model.entry(want.astype(np.float64)).astype(np.float16))
         assert bool((got[n:] == 7).all())
     assert sp.device_status() == 0
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_queries_may_be_turned_and_answered_in_place(sp, interleaved):
+    rng = np.random.default_rng(22)
+    lens, q_lens, heads, Hq, D = (300, 5, 90), (40, 5, 70), 24, 24, 128
+    bt = Batch(sp, rng, lens, q_lens, heads, D, 32).fill()
+    n = sum(q_lens)
+    cos, sin = (dev(f(np.arange(300)[:, None] * 10000.0 ** (-np.arange(0, 128, 2) / 128)).astype(np.float32)) for f in (np.cos, np.sin))
+    k, v, q = (dev(f16(rng, n, h, D)) for h in (heads, heads, Hq))
+    args = dict(cu_q=bt.cu, cos=cos, sin=sin, interleaved=interleaved)
+    want = sp.kv_append(bt.cache, k, v, bt.table, bt.kv_lens, q=q, **args)
+    assert sp.kv_append(bt.cache, k, v, bt.table, bt.kv_lens, q=q, q_out=q, **args) is q or torch.equal(q, want)
+    assert torch.equal(q, want)
+    for max_q in (70, 1):   # with the kernel for many rows and without
+        q = want.clone()
+        out = sp.kv_attention(q.clone(), bt.cache, bt.table, bt.kv_lens, cu_q=bt.cu, max_q=max_q)
+        sp.kv_attention(q, bt.cache, bt.table, bt.kv_lens, cu_q=bt.cu, max_q=max_q, out=q)
+        assert torch.equal(q, out)
+    with pytest.raises(sp.SpmmError, match="overlap"):
+        buf = torch.zeros(n * Hq * D + 8, dtype=torch.float16, device="cuda")
+        sp.kv_attention(buf[:-8].view(n, Hq, D), bt.cache, bt.table, bt.kv_lens, cu_q=bt.cu, out=buf[8:].view(n, Hq, D))
+    assert sp.device_status() == 0
+
+
+def test_sequences_that_share_rows_beyond_counting_are_refused(sp):
+    """cu_q that gives every other sequence all the rows: more units than the list can number."""
+    B, n, heads, D = 4000, 64, 64, 64
+    cache = sp.KvCacheInt4(1, 16, heads, D)
+    table = torch.zeros((B, 60000), dtype=torch.int32, device="cuda")
+    lens = torch.full((B,), 60000 * 16, dtype=torch.int32, device="cuda")
+    cu = i32([0] + [n if b % 2 == 0 else 0 for b in range(B)])
+    q = torch.zeros((n, heads, D), dtype=torch.float16, device="cuda")
+    assert heads * (n // 8 + B) * 7500 < 2 ** 31 - 2 ** 25 < 2 ** 31 < B // 2 * heads * (n // 8) * 7500
+    out = torch.full_like(q, 7.0)
+    sp.kv_attention(q, cache, table, lens, cu_q=cu, max_q=1, out=out)
+    assert sp.device_status() & 8
+    sp.reset_device_status()
+    assert bool((out == 7).all())
+
+
+def test_cache_is_copied_with_a_handle_of_its_own(sp):
+    import copy
+    rng = np.random.default_rng(23)
+    bt = Batch(sp, rng, (40,), (40,), 2, 64, 16).fill()
+    other = copy.deepcopy(bt.cache)
+    want = [x.clone() for x in sp.kv_read(bt.cache, bt.table, bt.kv_lens, n_tokens=40)]
+    bt.cache.pool.zero_()
+    for a, b in zip(sp.kv_read(other, bt.table, bt.kv_lens, n_tokens=40), want):
+        assert torch.equal(a, b)

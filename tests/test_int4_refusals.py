@@ -100,3 +100,29 @@ def test_python_wrappers_refuse_before_any_call(lib_built):
         sp.encode_int4(torch.zeros((64, 128), dtype=torch.float16))
     with pytest.raises(sp.SpmmError, match="W.data"):
         sp.linear_int4(sp.Int4Matrix(64, 128, 64, torch.zeros(9216, dtype=torch.uint8)), torch.zeros((1, 128), dtype=torch.float16))
+
+
+HALF = 2             # bytes of an fp16 element
+
+
+@pytest.mark.parametrize("bad", [dict(out=A + 16), dict(out=A, qt=512), dict(out=A + HALF * 4 * 256 - 16), dict(q=A + 16, out=A), dict(out=A, qh=128, qt=512)])
+def test_attention_refuses_an_output_across_the_queries(lib_built, bad):
+    assert attention(lib_built, **{**dict(qt=256, q_heads=4), **bad}) != 0 and b"overlap" in lib_built.spb_last_error()
+
+
+@pytest.mark.parametrize("bad", [dict(q_out=A + 16), dict(q_out=A, qt=512), dict(q_out=2 * A), dict(q_out=3 * A + 512), dict(q_out=2 * A - 16)])
+def test_append_refuses_turned_queries_across_its_inputs(lib_built, bad):
+    kw = dict(k=2 * A, v=3 * A, q=A, qt=256, qh=64, q_heads=4, cos=A, sin=A, max_pos=9, rot=64)
+    assert append(lib_built, **{**kw, **bad}) != 0 and b"overlap" in lib_built.spb_last_error()
+
+
+def test_read_refuses_keys_across_values(lib_built):
+    for k, v in ((A, A), (A, A + 16), (A + HALF * 4 * 128 - 16, A)):
+        assert lib_built.spb_kv_read(None, A, 4, 16, 2, 64, A, 2, A, None, 2, 4, k, v) != 0 and b"overlap" in lib_built.spb_last_error()
+
+
+@pytest.mark.parametrize("bad", [dict(out=2 * A), dict(out=2 * A + HALF * 3 * 128 - 16), dict(residual=A + 16), dict(bias=A + HALF * 3 * 64 - 16)])
+def test_linear_refuses_an_output_across_its_inputs(lib_built, bad):
+    a = dict(stream=None, codes=3 * A, M=64, K=128, group=64, x=2 * A, out=A, N=3, bias=None, residual=None, act=0, ws=5 * A, ws_bytes=1 << 30)
+    a.update(bad)
+    assert lib_built.spb_linear_int4(*a.values()) != 0 and b"overlap" in lib_built.spb_last_error()
