@@ -15,7 +15,9 @@
 //   values   O^T = sum over tokens of (P s) c + P m: P^T comes from S^T with two 8 x 8 transposes in registers and is multiplied
 //            by the tokens' scales, one product per group, rounded to fp16 like P itself; the minima are one more matrix
 //            instruction per 16 tokens.  Scales of 2 and more would leave the fp16 range: the whole row is then shifted down by
-//            the scale's exponent, as if its maximum had grown.
+//            the scale's exponent, as if its maximum had grown.  The roundings of P and of P s average out over many keys; over
+//            few they would make outputs half again as far from the exact ones (five keys: 3.0e-4, the rounding of the output alone
+//            2.0e-4).  Where no context can have more than 128 tokens, a second product is taken with what the roundings took away.
 //
 // Work: the context is cut in units of 128 tokens (four warps, two 16-token blocks each); all units of all (sequence, key
 // head, row tile) are laid end to end and every thread block takes an equal share, found from the lengths on the device.
@@ -183,7 +185,9 @@ struct Smem {
     int ok[kWarps][kStages];    // blocks of the step that are there
 };
 
-template <int D, int NT>
+// FINE: no context has more than one unit, and the second product is taken (9.0 us against 8.7: 25 sequences of 5 tokens, 12 heads).  A
+// kernel of its own: one that could do either took 10 % longer over long contexts.
+template <int D, int NT, bool FINE>
 __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_split_kernel(KvAttnArgs a, int whole_tiles, int* status)
 {
     using L = KvLayout<D>;
@@ -556,7 +560,7 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
                         rescale(nt, r0, r1);
                     }
                 }
-                uint32_t b0[TT][NT], b1[TT][NT];
+                uint32_t b0[TT][NT], b1[TT][NT], r0[TT][NT], r1[TT][NT];   // r: what rounding to fp16 took away, for short contexts
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const float m0 = (mx[nt][0] == -INFINITY ? 0.f : mx[nt][0]) - kShift;
@@ -569,6 +573,10 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
                         sum[nt][1] += w1 + w3;
                         b0[k][nt] = transpose8x8(h2_bits(__floats2half2_rn(w0, w1)));
                         b1[k][nt] = transpose8x8(h2_bits(__floats2half2_rn(w2, w3)));
+                        if (FINE) {
+                            r0[k][nt] = transpose8x8(h2_bits(__floats2half2_rn(w0 - __half2float(__float2half_rn(w0)), w1 - __half2float(__float2half_rn(w1)))));
+                            r1[k][nt] = transpose8x8(h2_bits(__floats2half2_rn(w2 - __half2float(__float2half_rn(w2)), w3 - __half2float(__float2half_rn(w3)))));
+                        }
                     }
                 }
                 // ---- weighted values
@@ -583,7 +591,10 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
                     }
                     const uint32_t am[4] = {vm[k][0], 0u, vm[k][1], 0u};
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma(om[nt], am, b0[k][nt], b1[k][nt]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma(om[nt], am, b0[k][nt], b1[k][nt]);
+                        if (FINE) mma(om[nt], am, r0[k][nt], r1[k][nt]);
+                    }
 #pragma unroll
                     for (int w = 0; w < G; ++w) {
                         const uint32_t x0 = vw[0][w], x1 = vw[1][w], y0 = x0 >> 8, y1 = x1 >> 8;
@@ -594,6 +605,13 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
                             const uint32_t c0 = h2_bits(__hmul2(as_h2(b0[k][nt]), as_h2(vs[k][0][w]))), c1 = h2_bits(__hmul2(as_h2(b1[k][nt]), as_h2(vs[k][1][w])));
                             mma(o[nt][2 * w], even, c0, c1);
                             mma(o[nt][2 * w + 1], odd, c0, c1);
+                            if (FINE) {   // P s less its rounded product
+                                const __half2 v0 = as_h2(vs[k][0][w]), v1 = as_h2(vs[k][1][w]);
+                                const uint32_t d0 = h2_bits(__hfma2(as_h2(r0[k][nt]), v0, __hfma2(as_h2(b0[k][nt]), v0, __hneg2(as_h2(c0)))));
+                                const uint32_t d1 = h2_bits(__hfma2(as_h2(r1[k][nt]), v1, __hfma2(as_h2(b1[k][nt]), v1, __hneg2(as_h2(c1)))));
+                                mma(o[nt][2 * w], even, d0, d1);
+                                mma(o[nt][2 * w + 1], odd, d0, d1);
+                            }
                         }
                     }
                 }
@@ -797,7 +815,7 @@ int sm_count()
 
 
 // Thread blocks that fit on the device at once (shared memory and registers).
-template <int D, int NT>
+template <int D, int NT, bool FINE>
 cudaError_t prepare(int* ctas)
 {
     static int cached[64] = {};
@@ -806,10 +824,10 @@ cudaError_t prepare(int* ctas)
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!cached[dev]) {
-        e = cudaFuncSetAttribute(kv_attention_split_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D, NT>));
+        e = cudaFuncSetAttribute(kv_attention_split_kernel<D, NT, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D, NT>));
         int n = 0;
         if (e == cudaSuccess)
-            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv_attention_split_kernel<D, NT>, 32 * kWarps, sizeof(Smem<D, NT>));
+            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv_attention_split_kernel<D, NT, FINE>, 32 * kWarps, sizeof(Smem<D, NT>));
         if (e != cudaSuccess) return e;
         cached[dev] = (n < 1 ? 1 : n) * sm_count();
     }
@@ -821,23 +839,23 @@ template <int D, int NT>
 cudaError_t launch(cudaStream_t s, const KvAttnArgs& a, int* status)
 {
     constexpr int ROWS = 8 * NT;
+    const int group = a.q_heads / a.c.kv_heads;
+    const long long units = ((long long)a.c.table_stride * a.c.page_size - 1) / kUnit + 1;
+    // A tile of up to four units is done whole: cutting it saves a unit's time or two (1.5 us each), the join costs 3.5 us.
+    const bool whole = units <= 4;
     int ctas = 0;
-    cudaError_t e = prepare<D, NT>(&ctas);
+    cudaError_t e = units == 1 ? prepare<D, NT, true>(&ctas) : prepare<D, NT, false>(&ctas);
     if (e != cudaSuccess) return e;
     const long long fit = (long long)(a.ws_floats / (2 * slot_floats<D, ROWS>()));
     if (fit < 1) return cudaErrorInvalidValue;
-    ctas = (int)(fit < ctas ? fit : ctas);
+    if (fit < ctas) ctas = (int)fit;
     // never more thread blocks than units there can be: every table entry used, every packed row in a tile of its own at worst
-    const int group = a.q_heads / a.c.kv_heads;
-    const long long units = ((long long)a.c.table_stride * a.c.page_size - 1) / kUnit + 1;
     const long long tiles = ((long long)a.max_q * group + ROWS - 1) / ROWS;
     const long long most = (long long)a.c.B * a.c.kv_heads * (tiles > 0 ? tiles : 1) * units;
     if (((long long)a.c.n_tokens * group / ROWS + a.c.B) * a.c.kv_heads * units > kMostUnits) {
         set_error("kv_attention: too much work for one call (rows times context)");
         return cudaErrorInvalidValue;
     }
-    // A tile of up to four units is done whole: cutting it saves a unit's time or two (1.5 us each), the join costs 3.5 us.
-    const int whole = units <= 4;
     if (whole ? most / units < ctas : most < ctas) ctas = (int)(whole ? most / units : most);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -849,7 +867,8 @@ cudaError_t launch(cudaStream_t s, const KvAttnArgs& a, int* status)
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kv_attention_split_kernel<D, NT>, a, whole, status);
+    e = units == 1 ? cudaLaunchKernelEx(&cfg, kv_attention_split_kernel<D, NT, true>, a, (int)whole, status)
+                   : cudaLaunchKernelEx(&cfg, kv_attention_split_kernel<D, NT, false>, a, (int)whole, status);
     count_launch();
     if (e != cudaSuccess || whole) return e;
     const long long rows = (long long)a.max_q * group, pairs = a.c.kv_heads * (tiles > 0 ? tiles : 1);
