@@ -12,12 +12,16 @@
 //              that costs is less than s / 64 at the top of the range.  A group with a value that is not finite reads
 //              back as NaN as a whole (s = m = NaN).
 //
-// Bound by memory: 4 D bytes in and 1.25 D out per token and head; there is no reuse, so the kernel is one load, the
-// arithmetic in registers and the stores.
+// Bound by latency and by the instructions of exact rounding, not by its bytes (4 D in and 1.25 D out per token and head): a warp takes up
+// to eight turns of vectors of one kind of one token, whose place and angles it then finds once, and loads a turn ahead.  Prompts of
+// 7300 tokens, 8 key heads and 32 query heads, half of each turned, with kv_read of them: 67 us (82 when a warp went through the
+// tokens of one head; 74 without the loads ahead), 31 at copy rate.  64 single tokens, 8 and 64 heads: 7.7 us, launch latency.
 #include "kv_int4.cuh"
+#include "sm100.cuh"
 
 namespace spb {
 namespace {
+using namespace sm100;
 
 constexpr int kWarps = 8;
 
@@ -85,92 +89,130 @@ __device__ __forceinline__ __half turn_exactly(float a, float c, float b, float 
     if (rest != 0.f && !(bits & 1u)) bits += (rest > 0.f) == (f > 0.f) ? 1u : 0xffffffffu;
     return __float2half_rn(__uint_as_float(bits));
 }
-// Four of them.  In plain fp32 a sum is off by less than 2^-23 of |b d| + |sum|: when both ends of that range round to the same fp16
-// value it is the right one, and only otherwise (one value in a thousand) is the exact form worked out.
-__device__ __forceinline__ void turn4(const float (&a)[4], const float (&c)[4], const float (&b)[4], const float (&d)[4], __half (&y)[4])
+// Eight of them, in place of a.  In plain fp32 a sum is off by less than 2^-23 of |b d| + |sum|: when both ends of that range round to the
+// same fp16 value it is the right one, and only otherwise (one value in a thousand) is the exact form worked out.
+__device__ __forceinline__ void turn8(__half (&a)[2][4], const float (&c)[8], const __half (&b)[2][4], const float (&d)[8])
 {
+    __half2 low[4], high[4];
     uint32_t differ = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float p = b[i] * d[i], s = fmaf(a[i], c[i], p), e = (fabsf(p) + fabsf(s)) * 0x1p-23f;
-        const __half2 ends = __floats2half2_rn(s - e, s + e);
-        y[i] = __low2half(ends);
-        const uint32_t bits = *reinterpret_cast<const uint32_t*>(&ends);
-        differ |= (bits ^ bits >> 16) & 0xffffu;
-    }
-    if (differ)
+    for (int i = 0; i < 8; i += 2) {
+        float lo[2], hi[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = turn_exactly(a[i], c[i], b[i], d[i]);
+        for (int e = 0; e < 2; ++e) {
+            const int j = i + e;
+            const float p = __half2float(b[j / 4][j % 4]) * d[j], s = fmaf(__half2float(a[j / 4][j % 4]), c[j], p), m = fabsf(p) + fabsf(s);
+            lo[e] = fmaf(m, -0x1p-23f, s), hi[e] = fmaf(m, 0x1p-23f, s);
+        }
+        low[i / 2] = __floats2half2_rn(lo[0], lo[1]), high[i / 2] = __floats2half2_rn(hi[0], hi[1]);
+        differ |= *reinterpret_cast<const uint32_t*>(&low[i / 2]) ^ *reinterpret_cast<const uint32_t*>(&high[i / 2]);
+    }
+    if (differ) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const __half2 l = low[j / 2], h = high[j / 2];
+            const __half lj = j & 1 ? __high2half(l) : __low2half(l), hj = j & 1 ? __high2half(h) : __low2half(h);
+            __half y = lj;
+            if (__half_as_ushort(lj) != __half_as_ushort(hj)) y = turn_exactly(__half2float(a[j / 4][j % 4]), c[j], __half2float(b[j / 4][j % 4]), d[j]);
+            low[j / 2] = j & 1 ? __halves2half2(__low2half(l), y) : __halves2half2(y, __high2half(l));
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) *reinterpret_cast<uint2*>(a[k]) = *reinterpret_cast<const uint2*>(low + 2 * k);
 }
 
-// The vector's channels c0 .. c0 + 3, turned by the angles of position pos.
-__device__ __forceinline__ void load_turned(const uint16_t* vec, int c0, const KvAppendArgs& a, int pos, __half (&x)[4])
+// Cosines and signed sines of position pos for the eight channels from c0 on: y = x c + partner s.
+__device__ __forceinline__ void load_angles(const KvAppendArgs& a, int pos, int c0, float (&c)[8], float (&s)[8])
 {
-    load4(vec + c0, x);
-    if (c0 >= a.rot) return;
     const int half_rot = a.rot / 2;
-    float u[4], w[4], c[4], s[4];
+    const float *cp = a.cosv + (long long)pos * half_rot, *sp = a.sinv + (long long)pos * half_rot;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = __half2float(x[i]);
-    if (a.interleaved) {
-        const float2 cc = *reinterpret_cast<const float2*>(a.cosv + (long long)pos * half_rot + c0 / 2);
-        const float2 ss = *reinterpret_cast<const float2*>(a.sinv + (long long)pos * half_rot + c0 / 2);
-        c[0] = c[1] = cc.x, c[2] = c[3] = cc.y;
-        s[0] = -ss.x, s[1] = ss.x, s[2] = -ss.y, s[3] = ss.y;
-        w[0] = u[1], w[1] = u[0], w[2] = u[3], w[3] = u[2];
-    } else {
-        const bool upper = c0 >= half_rot;   // half_rot is a multiple of 4: all four channels on one side
-        const int i0 = upper ? c0 - half_rot : c0;
-        __half o[4];
-        load4(vec + (upper ? c0 - half_rot : c0 + half_rot), o);
-        *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(a.cosv + (long long)pos * half_rot + i0);
-        *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(a.sinv + (long long)pos * half_rot + i0);
+    for (int k = 0; k < 8; k += 4) {
+        if (a.interleaved) {
+            const float2 cc = *reinterpret_cast<const float2*>(cp + (c0 + k) / 2), ss = *reinterpret_cast<const float2*>(sp + (c0 + k) / 2);
+            c[k] = c[k + 1] = cc.x, c[k + 2] = c[k + 3] = cc.y;
+            s[k] = -ss.x, s[k + 1] = ss.x, s[k + 2] = -ss.y, s[k + 3] = ss.y;
+        } else {
+            const bool upper = c0 + k >= half_rot;   // half_rot is a multiple of 4: all four channels on one side
+            const int i0 = c0 + k - (upper ? half_rot : 0);
+            *reinterpret_cast<float4*>(c + k) = *reinterpret_cast<const float4*>(cp + i0);
+            *reinterpret_cast<float4*>(s + k) = *reinterpret_cast<const float4*>(sp + i0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = __half2float(o[i]), s[i] = upper ? s[i] : -s[i];
+            for (int i = 0; i < 4; ++i) s[k + i] = upper ? s[k + i] : -s[k + i];
+        }
     }
-    turn4(u, c, w, s, x);
 }
 
-// One vector per D/8 lanes, eight channels each; the vectors of a token are its keys, its values and, when q is given, its queries.  A
-// warp goes through `rows` consecutive tokens of the packed input for its vectors: one for a few tokens, more for many, so
-// that finding the token's place is paid once.
-template <int D>
-__global__ void __launch_bounds__(32 * kWarps) kv_append_kernel(KvAppendArgs a, int rows, int* status)
+enum Kind { kKeys, kValues, kQueries };
+
+// Sum of c[i] 2^shift(i) of the codes in the low bits of the floats 1.5 2^23 + c: the floats' other bits are a constant, taken off.
+template <int S0, int S1, int S2, int S3>
+__device__ __forceinline__ uint32_t pack_codes(const float* t)
+{
+    constexpr uint32_t kBits = 0x4b400000u, kOff = kBits * ((1u << S0) + (1u << S1) + (1u << S2) + (1u << S3));
+    const uint32_t x = __float_as_uint(t[0]) * (1u << S0) + __float_as_uint(t[1]) * (1u << S1);
+    return x + __float_as_uint(t[2]) * (1u << S2) + __float_as_uint(t[3]) * (1u << S3) - kOff;
+}
+
+// Heads head0, head0 + 32 / (D / 8), .. of one token: `turns` of them for every D/8 lanes, which hold a head's vector.
+template <int D, Kind KIND>
+__device__ __forceinline__ void append_vectors(const KvAppendArgs& a, int tok, int b, int pos, int head, int turns, int* status)
 {
     using L = KvLayout<D>;
     constexpr int kLanes = D / 8, kPer = 32 / kLanes;
     const int lane = threadIdx.x & 31, sub = lane % kLanes, c0 = 8 * sub;
-    const unsigned vecs = 2 * a.c.kv_heads + (a.q ? a.q_heads : 0);
-    const unsigned item = (blockIdx.x * kWarps + threadIdx.x / 32) * kPer + lane / kLanes;
-    const unsigned chunk = item / vecs, vec = item - chunk * vecs;
-    const bool is_q = vec >= 2 * a.c.kv_heads, is_v = !is_q && vec >= a.c.kv_heads;
-    const int head = is_q ? vec - 2 * a.c.kv_heads : is_v ? vec - a.c.kv_heads : vec;
-    const uint16_t* src = is_q ? a.q + head * a.q_head : is_v ? a.v + head * a.v_head : a.k + head * a.k_head;
-    const long long step = is_q ? a.q_tok : is_v ? a.v_tok : a.k_tok;
-    const bool turned = a.cosv && !is_v;
-    Cursor at;
-    for (int i = 0; i < rows; ++i) {
-        const int tok = (int)chunk * rows + i;
-        bool write = at.move_to(a.c, tok) && at.pos >= 0;
-        if (write && turned && at.pos >= a.max_pos) {   // no angles for this position
-            if (sub == 0) atomicOr(status, kStatusBadCache);
-            write = false;
+    const int heads = KIND == kQueries ? a.q_heads : a.c.kv_heads;
+    bool turning = false;
+    float cs[8], sn[8];
+    if (KIND != kValues && a.cosv) {
+        if (pos >= a.max_pos) {   // no angles for this position
+            if (lane == 0) atomicOr(status, kStatusBadCache);
+            return;
         }
-        __half x[2][4] = {};
-        if (write) {
-            const uint16_t* p = src + tok * step;
+        turning = c0 < a.rot;
+        if (turning) load_angles(a, pos, c0, cs, sn);
+    }
+    uint8_t* blk = nullptr;
+    const long long head_bytes = (long long)(a.c.page_size / kKvBlock) * L::kBlockBytes;
+    if (KIND != kQueries) {
+        const long long off = kv_block_offset<D>(a.c, b, 0, pos);
+        if (off < 0) {
+            if (lane == 0) atomicOr(status, kStatusBadCache);
+            return;
+        }
+        blk = a.c.pool + off + head * head_bytes;
+    }
+    const long long head_step = KIND == kQueries ? a.q_head : KIND == kValues ? a.v_head : a.k_head;
+    const uint16_t* src = KIND == kQueries ? a.q + tok * a.q_tok : KIND == kValues ? a.v + tok * a.v_tok : a.k + tok * a.k_tok;
+    src += head * head_step + c0;
+    uint16_t* dst = KIND == kQueries ? a.q_out + ((long long)tok * a.q_heads + head) * D + c0 : nullptr;
+    const int half_rot = a.rot / 2, t16 = pos % kKvBlock;
+    uint2 next[2] = {make_uint2(0, 0), make_uint2(0, 0)};   // the next turn's channels
+    if (head < heads) next[0] = reinterpret_cast<const uint2*>(src)[0], next[1] = reinterpret_cast<const uint2*>(src)[1];
+    for (int i = 0; i < turns; ++i, head += kPer, src += kPer * head_step, blk += kPer * head_bytes, dst += kPer * D) {
+        const bool there = head < heads;
+        __half x[2][4];
+        *reinterpret_cast<uint2*>(x[0]) = next[0], *reinterpret_cast<uint2*>(x[1]) = next[1];
+        if (i + 1 < turns && head + kPer < heads) {
+            const uint2* p = reinterpret_cast<const uint2*>(src + kPer * head_step);
+            next[0] = p[0], next[1] = p[1];
+        }
+        if (there) {
+            if (KIND != kValues && turning) {
+                __half w[2][4];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                if (turned) load_turned(p, c0 + 4 * k, a, at.pos, x[k]);
-                else load4(p + c0 + 4 * k, x[k]);
+                for (int k = 0; k < 2; ++k) {
+                    if (a.interleaved) w[k][0] = x[k][1], w[k][1] = x[k][0], w[k][2] = x[k][3], w[k][3] = x[k][2];
+                    else load4(src + 4 * k + (c0 + 4 * k >= half_rot ? -half_rot : half_rot), w[k]);
+                }
+                turn8(x, cs, w, sn);
             }
         }
-        __syncwarp();   // q_out may be q: all lanes of a vector have read it
-        if (is_q) {
-            if (write) *reinterpret_cast<uint4*>(a.q_out + ((long long)tok * a.q_heads + head) * D + c0) = *reinterpret_cast<uint4*>(x);
-            write = false;
+        if (KIND == kQueries) {
+            __syncwarp();   // q_out may be q: all lanes of a vector have read it
+            if (there) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(x);
+            continue;
         }
-        if (!__any_sync(0xffffffffu, write)) continue;
         // minimum and maximum of the four lanes that hold a group, as {min, -max}; NaN spreads, every lane of the warp takes part
         const __half2* h2 = reinterpret_cast<const __half2*>(x);
         const __half2 lo2 = __hmin2_nan(__hmin2_nan(h2[0], h2[1]), __hmin2_nan(h2[2], h2[3]));
@@ -189,15 +231,20 @@ __global__ void __launch_bounds__(32 * kWarps) kv_append_kernel(KvAppendArgs a, 
         __half s = __float2half_rd(span * 0x1.111116p-4f);
         if (15.f * __half2float(s) > span) s = __ushort_as_half((unsigned short)(__half_as_ushort(s) - 1));
         const float sf = __half2float(s), inv = __fdividef(1.f, sf);
-        uint32_t code[8];
+        // The code is the quotient rounded to even: added to 1.5 2^23 it is the sum's last bits.  The quotient by the reciprocal is off by
+        // less than 2^-18; only next to a border of two codes is it divided out.
+        constexpr float kRound = 12582912.f;
+        float t[8];
+        bool near = false;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            // The quotient by the reciprocal is off by less than 2^-18; only next to a border of two codes is it divided out.
-            const float d = __fsub_rn(__half2float(x[k / 4][k % 4]), lo);
-            float q = d * inv, n = rintf(q);
-            if (fabsf(fabsf(q - n) - 0.5f) < 0x1p-16f) n = rintf(__fdiv_rn(d, sf));
-            code[k] = (uint32_t)fminf(n, 15.f);
+            const float d = __fsub_rn(__half2float(x[k / 4][k % 4]), lo), y = __fmaf_rn(d, inv, kRound);
+            near = near || fabsf(__fmaf_rn(d, inv, kRound - y)) > 0.5f - 0x1p-16f;
+            t[k] = fminf(y, kRound + 15.f);
         }
+        if (near)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] = fminf(__fdiv_rn(__fsub_rn(__half2float(x[k / 4][k % 4]), lo), sf), 15.f) + kRound;
         __half m = __float2half_rn(lo);
         const bool plain = finite && sf > 0.f;   // a constant group has no codes
         if (!finite) s = m = __ushort_as_half((unsigned short)0x7fff);
@@ -205,26 +252,19 @@ __global__ void __launch_bounds__(32 * kWarps) kv_append_kernel(KvAppendArgs a, 
         // other.  Values: a byte for each of four channel pairs, whose other byte of the halfword that lane has.
         uint32_t mine[2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const uint32_t* c = code + 4 * k;
-            mine[k] = !plain ? 0u : is_v ? c[0] | c[1] << 4 | (c[2] | c[3] << 4) << 16 : c[0] | c[1] << 16 | c[2] << 8 | c[3] << 24;
-        }
+        for (int k = 0; k < 2; ++k) mine[k] = !plain ? 0u : KIND == kValues ? pack_codes<0, 4, 16, 20>(t + 4 * k) : pack_codes<0, 16, 8, 24>(t + 4 * k);
         const bool upper = sub & 2;
         const uint32_t other = __shfl_xor_sync(0xffffffffu, mine[upper ? 0 : 1], 2), kept = mine[upper ? 1 : 0];
-        const uint32_t word = upper ? other | kept << (is_v ? 8 : 4) : kept | other << (is_v ? 8 : 4);
-        if (!write) continue;
-        if (!at.find_block<D>(a.c, head)) {
-            if (sub == 0) atomicOr(status, kStatusBadCache);
-            continue;
-        }
-        uint8_t* blk = a.c.pool + at.off;
-        const int t16 = at.pos % kKvBlock, grp = sub / 4, pair = 2 * (sub & 1) + upper;   // the word or the two channel pairs this lane stores
-        if (!is_v) {
+        constexpr int kShift = KIND == kValues ? 8 : 4;
+        const uint32_t word = upper ? other | kept << kShift : kept | other << kShift;
+        if (!there) continue;
+        const int grp = sub / 4, pair = 2 * (sub & 1) + upper;   // the word or the two channel pairs this lane stores
+        if (KIND == kKeys) {
             reinterpret_cast<uint32_t*>(blk + L::kKCodes)[t16 * (D / 8) + pair * L::kGroups + grp] = word;
             if ((sub & 3) == 0) reinterpret_cast<__half2*>(blk + L::kKParams)[t16 * L::kGroups + grp] = __halves2half2(s, m);
         } else {
-            const int j = t16 / 8, t = (t16 % 8) / 2, e = t16 & 1;
-            uint8_t* p = blk + L::kVCodes + j * 4 * D + (4 * 2 * pair + t) * (D / 8) + 4 * grp + 2 * e;
+            const int j = t16 / 8, t2 = (t16 % 8) / 2, e = t16 & 1;
+            uint8_t* p = blk + L::kVCodes + j * 4 * D + (4 * 2 * pair + t2) * (D / 8) + 4 * grp + 2 * e;
             *reinterpret_cast<uint16_t*>(p) = (uint16_t)word;
             *reinterpret_cast<uint16_t*>(p + 4 * (D / 8)) = (uint16_t)(word >> 16);
             if ((sub & 3) == 0) {
@@ -236,12 +276,35 @@ __global__ void __launch_bounds__(32 * kWarps) kv_append_kernel(KvAppendArgs a, 
     }
 }
 
+// A warp takes some vectors of one kind of one token, so that the token's place and its angles are found once: kv_turns (q_turns) times as
+// many keys or values (queries) as it holds at once, kv_warps (q_warps) warps for all of them.
+struct AppendPlan {
+    int kv_turns, kv_warps, q_turns, q_warps;
+};
+template <int D>
+__global__ void __launch_bounds__(32 * kWarps, 4) kv_append_kernel(KvAppendArgs a, AppendPlan plan, int* status)
+{
+    constexpr int kPer = 32 / (D / 8);
+    grid_wait();
+    grid_release();
+    const int per = 2 * plan.kv_warps + plan.q_warps, sub_head = (threadIdx.x & 31) / (D / 8);
+    const unsigned item = blockIdx.x * kWarps + threadIdx.x / 32, tok = item / per;
+    const int part = item - tok * per;
+    int b, pos;
+    if (tok >= (unsigned)a.c.n_tokens || !locate(a.c, (int)tok, b, pos) || pos < 0) return;
+    if (part < plan.kv_warps) append_vectors<D, kKeys>(a, tok, b, pos, part * plan.kv_turns * kPer + sub_head, plan.kv_turns, status);
+    else if (part < 2 * plan.kv_warps) append_vectors<D, kValues>(a, tok, b, pos, (part - plan.kv_warps) * plan.kv_turns * kPer + sub_head, plan.kv_turns, status);
+    else append_vectors<D, kQueries>(a, tok, b, pos, (part - 2 * plan.kv_warps) * plan.q_turns * kPer + sub_head, plan.q_turns, status);
+}
+
 // The values of one vector, eight channels a lane: m + code * s with one rounding.
 template <int D>
 __global__ void __launch_bounds__(32 * kWarps) kv_read_kernel(KvReadArgs a, int rows, int* status)
 {
     using L = KvLayout<D>;
     constexpr int kLanes = D / 8, kPer = 32 / kLanes;
+    grid_wait();
+    grid_release();
     const int lane = threadIdx.x & 31, sub = lane % kLanes, c0 = 8 * sub, grp = sub / 4;
     const unsigned vecs = 2 * a.c.kv_heads;
     const unsigned item = (blockIdx.x * kWarps + threadIdx.x / 32) * kPer + lane / kLanes;
@@ -292,33 +355,45 @@ __global__ void __launch_bounds__(32 * kWarps) kv_read_kernel(KvReadArgs a, int 
     }
 }
 
-// Tokens a warp goes through: eight when that still leaves the device full (64 warps on each of some 150 SMs), else one.
-int rows_for(long long vectors) { return vectors >= 8ll * 64 * 150 ? 8 : 1; }
-template <int D>
-unsigned blocks_for(int n_tokens, int rows, int vecs)
+// Vectors of a token, or tokens, that a warp goes through: up to eight when that still leaves the device full (64 warps on each of some 150
+// SMs), else one.
+bool many(long long vectors) { return vectors >= 8ll * 64 * 150; }
+// Both kernels may be set up before what precedes them has ended.
+template <class Args, class... More>
+cudaError_t start(cudaStream_t s, void (*kernel)(Args, More...), long long warps, const Args& a, More... more)
 {
-    const long long items = (n_tokens + rows - 1ll) / rows * vecs, per = kWarps * (32 / (D / 8));
-    return (unsigned)((items + per - 1) / per);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((warps + kWarps - 1) / kWarps));
+    cfg.blockDim = dim3(32 * kWarps);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, more...);
+    count_launch();
+    return e;
 }
 
 }  // namespace
 
 cudaError_t kv_append_launch(cudaStream_t s, int D, const KvAppendArgs& a, int* status)
 {
-    const int vecs = 2 * a.c.kv_heads + (a.q ? a.q_heads : 0), rows = rows_for((long long)a.c.n_tokens * vecs);
-    if (D == 128) kv_append_kernel<128><<<blocks_for<128>(a.c.n_tokens, rows, vecs), 32 * kWarps, 0, s>>>(a, rows, status);
-    else kv_append_kernel<64><<<blocks_for<64>(a.c.n_tokens, rows, vecs), 32 * kWarps, 0, s>>>(a, rows, status);
-    count_launch();
-    return cudaGetLastError();
+    const int at_once = 256 / D, kv = (a.c.kv_heads + at_once - 1) / at_once, q = a.q ? (a.q_heads + at_once - 1) / at_once : 0;
+    const int most = many((long long)a.c.n_tokens * (2 * a.c.kv_heads + (a.q ? a.q_heads : 0))) ? 8 : 1;
+    AppendPlan plan;
+    plan.kv_warps = (kv + most - 1) / most, plan.kv_turns = (kv + plan.kv_warps - 1) / plan.kv_warps;
+    plan.q_warps = (q + most - 1) / most, plan.q_turns = q ? (q + plan.q_warps - 1) / plan.q_warps : 0;
+    const long long warps = (long long)a.c.n_tokens * (2 * plan.kv_warps + plan.q_warps);
+    return D == 128 ? start(s, kv_append_kernel<128>, warps, a, plan, status) : start(s, kv_append_kernel<64>, warps, a, plan, status);
 }
 
 cudaError_t kv_read_launch(cudaStream_t s, int D, const KvReadArgs& a, int* status)
 {
-    const int vecs = 2 * a.c.kv_heads, rows = rows_for((long long)a.c.n_tokens * vecs);
-    if (D == 128) kv_read_kernel<128><<<blocks_for<128>(a.c.n_tokens, rows, vecs), 32 * kWarps, 0, s>>>(a, rows, status);
-    else kv_read_kernel<64><<<blocks_for<64>(a.c.n_tokens, rows, vecs), 32 * kWarps, 0, s>>>(a, rows, status);
-    count_launch();
-    return cudaGetLastError();
+    const int vecs = 2 * a.c.kv_heads, rows = many((long long)a.c.n_tokens * vecs) ? 8 : 1;
+    const long long warps = ((a.c.n_tokens + rows - 1ll) / rows * vecs + 256 / D - 1) / (256 / D);
+    return D == 128 ? start(s, kv_read_kernel<128>, warps, a, rows, status) : start(s, kv_read_kernel<64>, warps, a, rows, status);
 }
 
 }  // namespace spb
