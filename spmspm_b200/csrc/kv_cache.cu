@@ -15,7 +15,7 @@
 // Bound by latency and by the instructions of exact rounding, not by its bytes (4 D in and 1.25 D out per token and head): a warp takes up
 // to eight turns of vectors of one kind of one token, whose place and angles it then finds once, and loads a turn ahead.  Prompts of
 // 7300 tokens, 8 key heads and 32 query heads, half of each turned, with kv_read of them: 67 us (82 when a warp went through the
-// tokens of one head; 74 without the loads ahead), 31 at copy rate.  64 single tokens, 8 and 64 heads: 7.7 us, launch latency.
+// tokens of one head; 74 without the loads ahead), 31 at copy rate.  64 single tokens, 8 and 64 heads: 7.7 us, launches.
 #include "kv_int4.cuh"
 #include "sm100.cuh"
 

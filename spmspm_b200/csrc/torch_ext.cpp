@@ -1,11 +1,12 @@
 // Python calls of the 4-bit operators, straight from tensors to the C entry points.
 //
 // A decode step makes these calls with kernels of a few microseconds, so that checking the arguments and marshalling them
-// in Python took longer than the work (attention 17 us of host time, 8 of them launches).  The checks are the wrappers' own:
+// in Python took longer than the work (attention 17 us of host time, 7 from here; an append 3.3).  The checks are the wrappers' own:
 // kind, type, shape, layout and device of every tensor; sizes and alignment are checked again behind the C boundary.  The
 // library is the one spmspm_b200._lib has loaded.
 #include <torch/csrc/utils/pybind.h>
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
@@ -66,6 +67,9 @@ void init(const std::string& path, py::object error)
     g_error = error.release().ptr();
 }
 
+// at::empty without the dispatcher's detour (0.6 us instead of 1.1; a call with one launch takes 3).
+Tensor make(at::IntArrayRef shape, at::ScalarType type, c10::Device dev) { return Tensor(at::detail::empty_cuda(shape, type, dev, std::nullopt)); }
+
 // Device and stream of a call: the tensors' device is made current, the stream is the given one or torch's current one there.
 struct Place {
     c10::cuda::CUDAGuard guard;
@@ -81,7 +85,7 @@ struct Place {
     // a new workspace; its memory must not go to another tensor before a stream given by hand is done with it
     Tensor workspace(size_t bytes, const Tensor& like) const
     {
-        Tensor w = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+        Tensor w = make({(int64_t)bytes}, at::kByte, like.device());
         if (given) w.record_stream(stream.unwrap());
         return w;
     }
@@ -171,7 +175,7 @@ OptTensor kv_append(const Cache& c, const Tensor& k, const Tensor& v, const Tens
             dense_half(*q_out, "q_out", q->sizes(), c.pool.device(), "cache");
             out = *q_out;
         } else {
-            out = at::empty(q->sizes(), q->options());
+            out = make(q->sizes(), at::kHalf, q->device());
         }
     }
     if (n) {
@@ -194,12 +198,12 @@ std::pair<Tensor, Tensor> kv_read(const Cache& c, const Tensor& table, const Ten
     if (n < 0) fail("n_tokens must not be negative");
     check_rows(n, b);
     const int64_t shape[3] = {n, c.kv_heads, c.head_dim};
-    auto make = [&](const OptTensor& given, const char* name) {
-        if (!given) return at::empty(shape, c.pool.options().dtype(at::kHalf));
+    auto output = [&](const OptTensor& given, const char* name) {
+        if (!given) return make(shape, at::kHalf, c.pool.device());
         dense_half(*given, name, shape, c.pool.device(), "cache");
         return *given;
     };
-    Tensor k = make(k_out, "k_out"), v = make(v_out, "v_out");
+    Tensor k = output(k_out, "k_out"), v = output(v_out, "v_out");
     if (n) {
         const Place at_(c.pool.get_device(), stream);
         check(p_kv_read(at_.ptr(), c.pool.data_ptr(), c.num_pages, c.page_size, c.kv_heads, c.head_dim, b.table, b.width, b.lens, b.cu, b.batch, n,
@@ -226,7 +230,7 @@ Tensor kv_attention(const Tensor& q, const Cache& c, const Tensor& table, const 
     const int64_t most = max_q ? *max_q : b.cu ? n : n / b.batch;
     if (most < 0 || most > n) fail("max_q must be in 0..tokens");
     if (out_given) dense_half(*out_given, "out", q.sizes(), c.pool.device(), "cache");
-    Tensor out = out_given ? *out_given : at::empty(q.sizes(), q.options());
+    Tensor out = out_given ? *out_given : make(q.sizes(), at::kHalf, q.device());
     if (!n) return out;
     const Place at_(c.pool.get_device(), stream);
     size_t have;
@@ -256,7 +260,7 @@ Tensor linear_int4(const Tensor& data, int64_t M, int64_t K, int64_t group, cons
         fail("bias must be a contiguous CUDA float16 [M] tensor");
     if (residual) dense_half(*residual, "residual", shape, dev, "weight");
     if (out_given) dense_half(*out_given, "out", shape, dev, "weight");
-    Tensor out = out_given ? *out_given : at::empty(shape, x.options());
+    Tensor out = out_given ? *out_given : make(shape, at::kHalf, dev);
     const Place at_(data.get_device(), stream);
     size_t have;
     const Tensor ws = pick_workspace(at_, ws_given, p_int4_workspace_bytes((int)M, (int)N, (int)K), x, "weight", have);
