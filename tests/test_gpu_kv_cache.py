@@ -511,3 +511,19 @@ def test_cache_is_copied_with_a_handle_of_its_own(sp):
     bt.cache.pool.zero_()
     for a, b in zip(sp.kv_read(other, bt.table, bt.kv_lens, n_tokens=40), want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("D,Hkv,group", [(128, 12, 1), (64, 7, 1), (128, 2, 8), (64, 1, 16)])
+def test_short_contexts_are_as_exact_as_their_rounding(sp, D, Hkv, group):
+    """Over few keys the roundings of the weights do not average out.  What is left in fp32 is below 2^-17 of the output in the root mean
+    square (scores of some tens of terms, exponentials to 2^-22), an eightieth of the 2^-11 / sqrt(3) / 1.4 that the rounding to fp16
+    makes, which is measured on the exact result: a tenth more is allowed."""
+    rng = np.random.default_rng(24)
+    lens = [1 + i % 9 for i in range(40)]
+    bt = Batch(sp, rng, lens, [1] * 40, Hkv, D, 16).fill()
+    q = f16(rng, 40, Hkv * group, D)
+    got = sp.kv_attention(dev(q), bt.cache, bt.table, bt.kv_lens).cpu().numpy().astype(np.float64)
+    want = np.stack([model.attention(q[b:b + 1].astype(np.float64), *bt.held(b), D ** -0.5)[0][0] for b in range(40)])
+    rounding = np.linalg.norm(want.astype(np.float16).astype(np.float64) - want)
+    assert np.linalg.norm(got - want) <= 1.1 * rounding
+    assert sp.device_status() == 0

@@ -132,3 +132,87 @@ def test_layer_refuses(lib_built):
     for bad in (dict(weights="int8"), dict(kv_cache="fp8")):
         with pytest.raises(ValueError):
             SparseOptDecoderLayer(256, 4, 1024, 0.0, torch.device("cuda", 0), batch=1, max_len=8, **bad)
+
+
+FIRST_CALLS_CAPTURED = """
+import torch, spmspm_b200 as sp
+torch.manual_seed(0)
+x = torch.randn(4, 256, device="cuda").half()
+codes = torch.randint(0, 16, (768, 256), device="cuda", dtype=torch.uint8)
+scales, zeros = torch.full((768, 2), 0.01, device="cuda").half(), torch.full((768, 2), 8, device="cuda", dtype=torch.uint8)
+W = sp.pack_int4(codes, scales, zeros)
+cache = sp.KvCacheInt4(8, 16, 2, 128)
+table, lens = torch.arange(8, device="cuda", dtype=torch.int32).view(4, 2), torch.full((4,), 1, device="cuda", dtype=torch.int32)
+
+def step():
+    q, k, v = (t.unflatten(1, (2, 128)) for t in sp.linear_int4(W, x).split(256, dim=1))
+    sp.kv_append(cache, k, v, table, lens)
+    return sp.kv_attention(q, cache, table, lens)
+
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = step()
+g.replay()
+torch.cuda.synchronize()
+first = y.clone()
+assert torch.equal(step(), first) and bool(first.any()) and sp.device_status() == 0
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured(lib_built):
+    import subprocess
+    import sys
+    got = subprocess.run([sys.executable, "-c", FIRST_CALLS_CAPTURED], capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and got.stdout.strip() == "same", got.stderr[-2000:]
+
+
+def test_broadcast_keys_and_queries(sp):
+    """Strides of zero: one key and value for all heads, one query for all tokens."""
+    torch.manual_seed(1)
+    B, H, D = 3, 4, 64
+    table, lens = torch.arange(6, device="cuda", dtype=torch.int32).view(B, 2), torch.full((B,), 1, device="cuda", dtype=torch.int32)
+    k, v, q = (torch.randn(*s, device="cuda").half() for s in ((B, 1, D), (B, 1, D), (1, H, D)))
+    outs = []
+    for dense in (False, True):
+        kk, vv, qq = k.expand(B, H, D), v.expand(B, H, D), q.expand(B, H, D)
+        if dense:
+            kk, vv, qq = kk.contiguous(), vv.contiguous(), qq.contiguous()
+        cache = sp.KvCacheInt4(6, 16, H, D)
+        sp.kv_append(cache, kk, vv, table, lens)
+        outs.append((cache.pool.clone(), sp.kv_attention(qq, cache, table, lens)))
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+    assert sp.device_status() == 0
+
+
+def test_steps_on_two_streams_at_once(sp):
+    """Two users with caches, tensors and streams of their own, steps interleaved: the bits of one after the other."""
+    torch.manual_seed(2)
+    B, H, D, steps = 5, 8, 128, 6
+    W = sp.encode_int4((torch.randn(3 * H * D, H * D, device="cuda") * 0.02).half())
+
+    def user(seed, stream):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        x = [torch.randn(B, H * D, device="cuda", generator=g).half() for _ in range(steps)]
+        cache = sp.KvCacheInt4(B * 4, 16, H, D)
+        table, lens = torch.arange(B * 4, device="cuda", dtype=torch.int32).view(B, 4), torch.zeros(B, device="cuda", dtype=torch.int32)
+        torch.cuda.synchronize()
+
+        def step(i):
+            with torch.cuda.stream(stream):
+                q, k, v = (t.unflatten(1, (H, D)) for t in sp.linear_int4(W, x[i]).split(H * D, dim=1))
+                lens.add_(1)
+                sp.kv_append(cache, k, v, table, lens)
+                return sp.kv_attention(q, cache, table, lens)
+        return step
+    alone = []
+    for seed in (1, 2):
+        step = user(seed, torch.cuda.current_stream())
+        alone.append([step(i) for i in range(steps)])
+    a, b = user(1, torch.cuda.Stream()), user(2, torch.cuda.Stream())
+    both = [(a(i), b(i)) for i in range(steps)]
+    torch.cuda.synchronize()
+    for i, (x, y) in enumerate(both):
+        assert torch.equal(x, alone[0][i]) and torch.equal(y, alone[1][i])
+    assert sp.device_status() == 0
