@@ -23,27 +23,32 @@ namespace spb {
 namespace {
 using namespace sm100;
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 
-// Sequence of packed row `tok`, its position in the cache (negative: before the start) -> false when the row belongs to
-// no sequence (behind the last one).
-__device__ __forceinline__ bool locate(const KvView& c, int tok, int& b, int& pos)
+// Sequence of packed row `tok`, its position in the cache (negative: before the start) and the first row behind the sequence -> false when
+// the row belongs to no sequence (behind the last one).  The whole warp asks for the same row: 32 offsets are looked at together, since
+// a search that halves the range is one load's latency after the other.
+__device__ __forceinline__ bool locate(const KvView& c, int tok, int& b, int& pos, int& end)
 {
     if (c.cu) {
-        if (tok < c.cu[0] || tok >= c.cu[c.B]) return false;
-        int lo = 0, hi = c.B;   // last b with cu[b] <= tok
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (c.cu[mid] <= tok) lo = mid;
-            else hi = mid;
-        }
+        const int lane = threadIdx.x & 31;
+        int lo = 0, n = c.B;   // the last b with cu[b] <= tok is one of n from lo on
+        do {
+            const int step = (n + 31) / 32, i = lane * step;
+            const uint32_t below = __ballot_sync(0xffffffffu, i < n && c.cu[lo + min(i, n - 1)] <= tok);
+            if (!below) return false;   // before the first sequence
+            const int k = 31 - __clz(below);
+            lo += k * step;
+            n = min(step, n - k * step);
+        } while (n > 1);
         b = lo;
-        const int end = min(c.cu[b + 1], c.n_tokens);   // as kv_rows takes it
-        if (tok >= end) return false;   // offsets that are not ascending
+        end = min(c.cu[b + 1], c.n_tokens);   // as kv_rows takes it
+        if (tok >= end) return false;
         pos = c.lens[b] - (end - tok);
     } else {
         b = (unsigned)tok / (unsigned)c.per_seq;
-        pos = c.lens[b] - c.per_seq + (tok - b * c.per_seq);
+        end = (b + 1) * c.per_seq;
+        pos = c.lens[b] - (end - tok);
     }
     return true;
 }
@@ -58,8 +63,8 @@ struct Cursor {
             ++pos;
             return true;
         }
-        const bool found = tok < c.n_tokens && locate(c, tok, b, pos);
-        end = !found ? 0 : c.cu ? min(c.cu[b + 1], c.n_tokens) : (b + 1) * c.per_seq;
+        const bool found = tok < c.n_tokens && locate(c, tok, b, pos, end);
+        if (!found) end = 0;
         off = -1;
         return found;
     }
@@ -282,7 +287,7 @@ struct AppendPlan {
     int kv_turns, kv_warps, q_turns, q_warps;
 };
 template <int D>
-__global__ void __launch_bounds__(32 * kWarps, 4) kv_append_kernel(KvAppendArgs a, AppendPlan plan, int* status)
+__global__ void __launch_bounds__(32 * kWarps, 8) kv_append_kernel(KvAppendArgs a, AppendPlan plan, int* status)
 {
     constexpr int kPer = 32 / (D / 8);
     grid_wait();
@@ -290,8 +295,8 @@ __global__ void __launch_bounds__(32 * kWarps, 4) kv_append_kernel(KvAppendArgs 
     const int per = 2 * plan.kv_warps + plan.q_warps, sub_head = (threadIdx.x & 31) / (D / 8);
     const unsigned item = blockIdx.x * kWarps + threadIdx.x / 32, tok = item / per;
     const int part = item - tok * per;
-    int b, pos;
-    if (tok >= (unsigned)a.c.n_tokens || !locate(a.c, (int)tok, b, pos) || pos < 0) return;
+    int b, pos, end;
+    if (tok >= (unsigned)a.c.n_tokens || !locate(a.c, (int)tok, b, pos, end) || pos < 0) return;
     if (part < plan.kv_warps) append_vectors<D, kKeys>(a, tok, b, pos, part * plan.kv_turns * kPer + sub_head, plan.kv_turns, status);
     else if (part < 2 * plan.kv_warps) append_vectors<D, kValues>(a, tok, b, pos, (part - plan.kv_warps) * plan.kv_turns * kPer + sub_head, plan.kv_turns, status);
     else append_vectors<D, kQueries>(a, tok, b, pos, (part - 2 * plan.kv_warps) * plan.q_turns * kPer + sub_head, plan.q_turns, status);
@@ -306,16 +311,15 @@ __global__ void __launch_bounds__(32 * kWarps) kv_read_kernel(KvReadArgs a, int 
     grid_wait();
     grid_release();
     const int lane = threadIdx.x & 31, sub = lane % kLanes, c0 = 8 * sub, grp = sub / 4;
-    const unsigned vecs = 2 * a.c.kv_heads;
-    const unsigned item = (blockIdx.x * kWarps + threadIdx.x / 32) * kPer + lane / kLanes;
-    const unsigned chunk = item / vecs, vec = item - chunk * vecs;
+    const unsigned vecs = 2 * a.c.kv_heads, warps = (vecs + kPer - 1) / kPer;   // of a token
+    const unsigned item = blockIdx.x * kWarps + threadIdx.x / 32, chunk = item / warps, vec = (item - chunk * warps) * kPer + lane / kLanes;
     const bool is_v = vec >= a.c.kv_heads;
     const int head = is_v ? vec - a.c.kv_heads : vec;
     uint16_t* out = (is_v ? a.v : a.k) + head * D + c0;
     Cursor at;
     for (int i = 0; i < rows; ++i) {
         const int tok = (int)chunk * rows + i;
-        if (!at.move_to(a.c, tok)) continue;
+        if (!at.move_to(a.c, tok) || vec >= vecs) continue;
         uint16_t* dst = out + (long long)tok * a.c.kv_heads * D;
         if (at.pos < 0 || !at.find_block<D>(a.c, head)) {
             if (at.pos >= 0 && sub == 0) atomicOr(status, kStatusBadCache);
@@ -392,7 +396,7 @@ cudaError_t kv_append_launch(cudaStream_t s, int D, const KvAppendArgs& a, int* 
 cudaError_t kv_read_launch(cudaStream_t s, int D, const KvReadArgs& a, int* status)
 {
     const int vecs = 2 * a.c.kv_heads, rows = many((long long)a.c.n_tokens * vecs) ? 8 : 1;
-    const long long warps = ((a.c.n_tokens + rows - 1ll) / rows * vecs + 256 / D - 1) / (256 / D);
+    const long long warps = (a.c.n_tokens + rows - 1ll) / rows * ((vecs + 256 / D - 1) / (256 / D));
     return D == 128 ? start(s, kv_read_kernel<128>, warps, a, rows, status) : start(s, kv_read_kernel<64>, warps, a, rows, status);
 }
 
