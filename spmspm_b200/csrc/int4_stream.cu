@@ -49,6 +49,11 @@ __global__ void __launch_bounds__(32 * kWarps, 1) int4_stream_kernel(const __gri
         mbar_init_fence();
     }
     __syncthreads();
+    if (threadIdx.x == 0) {   // the first units on their way to L2 while what ran before ends
+        Walk first(p);
+        Run f;
+        if (first.next<8 * NT>(p, f)) bulk_prefetch(p.a.units + ((long long)f.mb * p.ku + f.u0) * kBytes, min(kWarps * kStages, f.nkt / kUnit) * kBytes);
+    }
     grid_wait();
     grid_release();   // the join may be set up while this kernel runs; it waits for its end
 

@@ -5,9 +5,9 @@
 // Rows of W are the 128-row side of the matrix instruction, rows of x its 32..256-column side.  Codes become fp16 on the way
 // into tensor memory, where the instruction takes its left operand from; x comes as 128-byte-swizzled tiles by tensor copies.
 //
-// Bound: 9216 x 36864, 509 rows: 281 us, 1230 TFLOP/s, 74 % of the library's dense rate, tensor pipe 69 % busy; every 128 rows of W read
+// Bound: 9216 x 36864, 509 rows: 264 us, 1310 TFLOP/s, 79 % of the library's dense rate, tensor pipe 69 % busy; every 128 rows of W read
 // all of x from L2, 2.8 GB or 10 TB/s, which is near what L2 gives.  With 32 to 64 rows the product is bound by the 8 instructions of a
-// unit, which cost the same 80 cycles for 32 columns as for 128 (16384 x 16384, 40 rows: 54 us, 22 at copy rate).  Scaling a group's sums in
+// unit, which cost the same 80 cycles for 32 columns as for 128 (16384 x 16384, 40 rows: 52 us, 22 at copy rate).  Scaling a group's sums in
 // fp32 instead of the weights, so that these need no rounding, was built and measured: 405 us and 64 us for these two with groups of
 // 128, and two and a half times as long with groups of 32, whose accumulators change hands four times a unit.
 //
@@ -33,6 +33,8 @@ template <int NPAD> struct Cfg {
     static constexpr int kUS = kKT / kUnit;                              // units per stage: groups share out kTurn stages
     static constexpr int kTurn = kGroups / kUS;
     static constexpr int kAcc = NPAD <= 32 ? 4 : NPAD <= 64 ? 2 : 1;     // accumulators the k-steps take in turn (short ones are latency)
+    static constexpr int kAhead = 2;                                     // stages between a prefetch into L2 and the copy from there (277 -> 264 us for
+                                                                         // 9216 x 36864 with 509 rows, 46 -> 43 for 28672 x 7168 with 32; 4 and 8: 1 to 3 % slower)
     static constexpr uint32_t kX = NPAD * 128;                           // bytes of x per k-tile
     static constexpr uint32_t kStage = kKT * kX + kKT / kUnit * (2 * kInt4CodeBytes + 4 * 512);   // x, units (at most four groups)
     static constexpr int kStages = (int)((222u * 1024) / kStage) < 8 ? (int)((222u * 1024) / kStage) : 8;
@@ -68,6 +70,12 @@ __global__ void __launch_bounds__(Cfg<NPAD>::kThreads, 1) int4_wide_kernel(const
     __syncthreads();
     tc_fence_after();
     constexpr uint32_t tmem = 0, tmem_a = C::kTmemA;   // all columns: the allocation starts at 0
+    if (warp == 0) {   // the first codes on their way to L2 while what ran before ends
+        Walk first(p);
+        Run f;
+        if (first.next<NPAD>(p, f) && elect_one())
+            bulk_prefetch(p.a.units + ((long long)f.mb * p.ku + f.u0) * int4_unit_bytes(kGroup), min(C::kAhead * C::kUS, f.nkt / kUnit) * int4_unit_bytes(kGroup));
+    }
     grid_wait();      // x, residual, out and the workspace belong to what ran before
     grid_release();   // the join may be set up while this kernel runs; it waits for its end
 
@@ -76,6 +84,7 @@ __global__ void __launch_bounds__(Cfg<NPAD>::kThreads, 1) int4_wide_kernel(const
     if (warp == 0 || warp == 2) {
         // ---- copies
         constexpr int unit_bytes = int4_unit_bytes(kGroup);
+        const int rows = p.items / p.ncol;
         uint32_t s = 0, round = 0;
         bool ok = true;
         while (ok && walk.next<NPAD>(p, r)) {
@@ -87,10 +96,16 @@ __global__ void __launch_bounds__(Cfg<NPAD>::kThreads, 1) int4_wide_kernel(const
                     const uint32_t st = stage0 + s * C::kStage, bar = full + 8 * s;
                     if (warp == 0) {
                         mbar_expect_tx(bar, n * unit_bytes);
-                        bulk_g2s(st + C::kKT * C::kX, p.a.units + ((long long)r.mb * p.ku + u) * unit_bytes, n * unit_bytes, bar);
+                        const uint8_t* src = p.a.units + ((long long)r.mb * p.ku + u) * unit_bytes;
+                        bulk_g2s(st + C::kKT * C::kX, src, n * unit_bytes, bar);
+                        const int more = r.nkt - k - C::kAhead * C::kKT;
+                        if (more > 0) bulk_prefetch(src + C::kAhead * C::kUS * unit_bytes, min(C::kKT, more) / kUnit * unit_bytes);
                     } else {
                         mbar_expect_tx(bar, C::kKT * C::kX);   // k-tiles past K come as zeros
                         tma_load_3d(st, &xmap, 0, r.n0, u * kUnit, bar);
+                        // of the thread blocks that read the same x, one fetches it for all
+                        const int next = u + C::kAhead * C::kUS;
+                        if (k + C::kAhead * C::kKT < r.nkt && next / C::kUS % rows == r.mb) tma_prefetch_3d(&xmap, 0, r.n0, next * kUnit);
                     }
                 }
                 __syncwarp();
