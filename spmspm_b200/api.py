@@ -33,6 +33,27 @@ def _stream_ptr(stream=None):
     return ctypes.c_void_p(s.cuda_stream)
 
 
+def _on(device, stream):
+    """Makes `stream` (default: the device's current one) the current stream: a call on a stream given by hand allocates
+    there too.  Memory from another stream's pool may still be in use on that stream, and goes back to it while the
+    given one is at work."""
+    if stream is None:
+        return torch.cuda.device(device)
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(stream.cuda_stream, device=device)
+    if stream.device != torch.device(device):
+        raise SpmmError(f"the stream is {stream.device}'s, the tensors are {device}'s")
+    return torch.cuda.stream(stream)
+
+
+def _hand_over(t, stream):
+    """A new tensor that a call on a given stream returns: its memory is not used anew before the caller's current stream,
+    too, is done with it."""
+    if stream is not None:
+        t.record_stream(torch.cuda.current_stream(t.device))
+    return t
+
+
 # --------------------------------------------------------------------------- encoder (host)
 
 @dataclass

@@ -7,7 +7,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .api import ACT_NONE, SpmmError, _check, _ptr, _stream_ptr
+from .api import ACT_NONE, SpmmError, _check, _hand_over, _on, _ptr, _stream_ptr
 
 
 @dataclass
@@ -48,11 +48,11 @@ def pack_int4(codes, scales, zeros, stream=None):
     _need(codes, "codes", torch.uint8, (M, K))
     _need(scales, "scales", torch.float16, (M, K // group), codes.device)
     _need(zeros, "zeros", torch.uint8, (M, K // group), codes.device)
-    data = torch.empty(_lib.load().spb_int4_bytes(M, K, group), dtype=torch.uint8, device=codes.device)
-    with torch.cuda.device(codes.device):
+    with _on(codes.device, stream):
+        data = torch.empty(_lib.load().spb_int4_bytes(M, K, group), dtype=torch.uint8, device=codes.device)
         _check(_lib.load().spb_int4_pack(_stream_ptr(stream), _ptr(codes), _ptr(scales), _ptr(zeros), M, K, group, _ptr(data)),
                "spb_int4_pack")
-    return Int4Matrix(M, K, group, data)
+    return Int4Matrix(M, K, group, _hand_over(data, stream))
 
 
 def encode_int4(A, group=128, stream=None):
@@ -61,10 +61,10 @@ def encode_int4(A, group=128, stream=None):
         raise SpmmError("A must be a contiguous CUDA float16 matrix")
     M, K = A.shape
     _shape(M, K, group)
-    codes = torch.empty((M, K), dtype=torch.uint8, device=A.device)
-    scales = torch.empty((M, K // group), dtype=torch.float16, device=A.device)
-    zeros = torch.empty((M, K // group), dtype=torch.uint8, device=A.device)
-    with torch.cuda.device(A.device):
+    with _on(A.device, stream):
+        codes = torch.empty((M, K), dtype=torch.uint8, device=A.device)
+        scales = torch.empty((M, K // group), dtype=torch.float16, device=A.device)
+        zeros = torch.empty((M, K // group), dtype=torch.uint8, device=A.device)
         _check(_lib.load().spb_int4_encode(_stream_ptr(stream), _ptr(A), M, K, group, _ptr(codes), _ptr(scales), _ptr(zeros)), "spb_int4_encode")
     return pack_int4(codes, scales, zeros, stream)
 
@@ -77,12 +77,12 @@ def _check_matrix(W):
 def decode_int4(W: Int4Matrix, out=None, stream=None):
     """The dense fp16 matrix [M, K] that W stands for, s (c - z) rounded once."""
     _check_matrix(W)
-    if out is None:
-        out = torch.empty((W.M, W.K), dtype=torch.float16, device=W.data.device)
-    _need(out, "out", torch.float16, (W.M, W.K), W.data.device)
-    with torch.cuda.device(out.device):
-        _check(_lib.load().spb_int4_decode(_stream_ptr(stream), _ptr(W.data), W.M, W.K, W.group, _ptr(out)), "spb_int4_decode")
-    return out
+    if out is not None:
+        _need(out, "out", torch.float16, (W.M, W.K), W.data.device)
+    with _on(W.data.device, stream):
+        y = out if out is not None else torch.empty((W.M, W.K), dtype=torch.float16, device=W.data.device)
+        _check(_lib.load().spb_int4_decode(_stream_ptr(stream), _ptr(W.data), W.M, W.K, W.group, _ptr(y)), "spb_int4_decode")
+    return out if out is not None else _hand_over(y, stream)
 
 
 def int4_workspace(W, N):

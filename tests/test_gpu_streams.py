@@ -1,0 +1,76 @@
+"""Calls on a stream given by hand (stream=): what they allocate must neither be memory that the current stream is still using nor go
+back to the current stream while the given one is at work."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def sp(lib_built):
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    import spmspm_b200
+    spmspm_b200.reset_device_status()
+    return spmspm_b200
+
+
+def hold(stream=None, ms=30):
+    """Keeps a stream busy for some milliseconds."""
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(ms * 2_000_000)
+
+
+def half(seed, *shape):
+    return torch.from_numpy(np.random.default_rng(seed).standard_normal(shape).astype(np.float16)).cuda()
+
+
+def tensors(x):
+    """The tensors a call has made."""
+    if isinstance(x, torch.Tensor):
+        return [x]
+    return list(x) if isinstance(x, (tuple, list)) else [v for v in vars(x).values() if isinstance(v, torch.Tensor)]
+
+
+def check(call):
+    """call(stream) returns new tensors: the same bits with the given stream held up and the freed memory taken and filled at once, and
+    with memory that the current stream still reads freed just before."""
+    want = [t.clone() for t in tensors(call(None))]
+    s = torch.cuda.Stream()
+    sizes = sorted({t.numel() * t.element_size() for t in want} | {1 << k for k in range(9, 23)})
+    for side in ("given", "current"):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        if side == "given":     # the call's own temporaries come back while it has not even begun
+            hold(s)
+            got = call(s)
+            others = [torch.full((n,), 0xA5, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(3)]
+        else:                   # the current stream has freed memory that it has yet to read
+            mine = [torch.full((n,), 0xA5, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(3)]
+            s.wait_stream(torch.cuda.current_stream())
+            hold()
+            others = [t.clone() for t in mine]
+            del mine
+            got = call(s)
+        s.synchronize()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(tensors(got), want, strict=True))
+        assert all(bool((t == 0xA5).all()) for t in others)
+
+
+def test_preparing_four_bit_weights(sp):
+    A = half(1, 512, 1024)
+    check(lambda s: sp.encode_int4(A, 64, stream=s))
+    rng = np.random.default_rng(2)
+    codes, zeros = (torch.from_numpy(rng.integers(0, 16, (512, k)).astype(np.uint8)).cuda() for k in (1024, 16))
+    scales = half(3, 512, 16).abs()
+    check(lambda s: sp.pack_int4(codes, scales, zeros, stream=s))
+    W = sp.encode_int4(A, 64)
+    check(lambda s: sp.decode_int4(W, stream=s))
+
+
+def test_a_stream_of_another_device_is_refused(sp):
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one device")
+    with pytest.raises(sp.SpmmError, match="stream"):
+        sp.encode_int4(half(1, 64, 128), 64, stream=torch.cuda.Stream(device=1))
