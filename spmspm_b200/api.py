@@ -248,24 +248,28 @@ def encode_device(A, stream=None):
     dev = A.device
     G = (M // 64) * (K // 64)
     nt = M * K // 64
-    tile_nnz = torch.empty(nt, dtype=torch.int32, device=dev)
-    mtile = torch.empty(4 * G, dtype=torch.int32, device=dev)
-    gtile = torch.empty(G + 1, dtype=torch.int32, device=dev)
-    bitmap = torch.empty(nt, dtype=torch.int64, device=dev)
-    max_nnz = torch.zeros(1, dtype=torch.int32, device=dev)
-    status = torch.zeros(1, dtype=torch.int32, device=dev)
-    scratch = torch.empty(lib.spb_encode_scratch_bytes(M, K), dtype=torch.uint8, device=dev)
-    cap = M * K + 8 * G
-    vals = torch.empty(cap, dtype=torch.float16, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev, stream):
+        tile_nnz = torch.empty(nt, dtype=torch.int32, device=dev)
+        mtile = torch.empty(4 * G, dtype=torch.int32, device=dev)
+        gtile = torch.empty(G + 1, dtype=torch.int32, device=dev)
+        bitmap = torch.empty(nt, dtype=torch.int64, device=dev)
+        max_nnz = torch.zeros(1, dtype=torch.int32, device=dev)
+        status = torch.zeros(1, dtype=torch.int32, device=dev)
+        scratch = torch.empty(lib.spb_encode_scratch_bytes(M, K), dtype=torch.uint8, device=dev)
+        cap = M * K + 8 * G
+        vals = torch.empty(cap, dtype=torch.float16, device=dev)
         _check(lib.spb_encode_device(_stream_ptr(stream), _ptr(A), M, K, _ptr(vals), cap, _ptr(tile_nnz), _ptr(mtile),
                                      _ptr(gtile), _ptr(bitmap), _ptr(max_nnz), _ptr(scratch), _ptr(status)),
                "spb_encode_device")
-    n = int(gtile[G].item())
-    if int(status.item()) != 0:
-        raise SpmmError("encoder overflowed its value buffer")
-    # release the worst-case buffer (an all-zero matrix keeps 16 bytes so the pointer is never null)
-    vals = vals[:n].clone() if n else torch.zeros(8, dtype=torch.float16, device=dev)
+        n = int(gtile[G].item())
+        if int(status.item()) != 0:
+            raise SpmmError("encoder overflowed its value buffer")
+        # release the worst-case buffer (an all-zero matrix keeps 16 bytes so the pointer is never null)
+        vals = vals[:n].clone() if n else torch.zeros(8, dtype=torch.float16, device=dev)
+        if stream is not None:
+            torch.cuda.current_stream().synchronize()   # ready for every stream, as its length is already
+    for t in (vals, gtile, mtile, bitmap, max_nnz, tile_nnz):
+        _hand_over(t, stream)
     return BitmapMatrix(M, K, vals, gtile, mtile, bitmap, max_nnz, tile_nnz, n)
 
 
@@ -359,15 +363,16 @@ def spmm(W: BitmapMatrix, B, split_k=None, out=None, workspace=None, stream=None
     N = B.shape[0]
     if split_k is None:
         split_k = suggest_split_k(W.M, N, W.K)
-    if out is None:
-        out = torch.empty((N, W.M), dtype=torch.float16, device=B.device)
-    if split_k > 1 and workspace is None:
-        workspace = torch.empty(split_k * N * W.M, dtype=torch.float16, device=B.device)
-    with torch.cuda.device(B.device):
+    new = out is None
+    with _on(B.device, stream):
+        if new:
+            out = torch.empty((N, W.M), dtype=torch.float16, device=B.device)
+        if split_k > 1 and workspace is None:
+            workspace = torch.empty(split_k * N * W.M, dtype=torch.float16, device=B.device)
         _init_if_possible(stream)
         spmm_splitk_api_bitmap_v3(stream, None, W.vals, W.gtile, W.mtile, W.bitmap, W.max_nnz, B, out, W.M, N, W.K,
                                   workspace, split_k)
-    return out
+    return _hand_over(out, stream) if new else out
 
 
 ACT_NONE, ACT_RELU = 0, 1
@@ -394,15 +399,16 @@ def linear(W: BitmapMatrix, B, bias=None, residual=None, activation=ACT_NONE, sp
     _check_tail(W.M, N, bias, residual, activation, B.device)
     if split_k is None:
         split_k = suggest_split_k(W.M, N, W.K)
-    if out is None:
-        out = torch.empty((N, W.M), dtype=torch.float16, device=B.device)
-    elif not (out.is_cuda and out.dtype == torch.float16 and out.is_contiguous() and tuple(out.shape) == (N, W.M)):
+    new = out is None
+    if not new and not (out.is_cuda and out.dtype == torch.float16 and out.is_contiguous() and tuple(out.shape) == (N, W.M)):
         raise SpmmError("out must be a contiguous CUDA float16 [N,M] tensor")
-    if split_k > 1 and workspace is None:
-        workspace = torch.empty(split_k * N * W.M, dtype=torch.float16, device=B.device)
-    if split_k > 1 and workspace.numel() < split_k * N * W.M:
+    if split_k > 1 and workspace is not None and workspace.numel() < split_k * N * W.M:
         raise SpmmError("workspace too small for split_k * N * M halves")
-    with torch.cuda.device(B.device):
+    with _on(B.device, stream):
+        if new:
+            out = torch.empty((N, W.M), dtype=torch.float16, device=B.device)
+        if split_k > 1 and workspace is None:
+            workspace = torch.empty(split_k * N * W.M, dtype=torch.float16, device=B.device)
         _init_if_possible(stream)
         code = _lib.load().spb_linear_bitmap_v3(_stream_ptr(stream), _ptr(W.vals), _ptr(W.gtile), _ptr(W.mtile),
                                                 _ptr(W.bitmap), _ptr(W.max_nnz), _ptr(B), _ptr(out), W.M, N, W.K,
@@ -410,19 +416,20 @@ def linear(W: BitmapMatrix, B, bias=None, residual=None, activation=ACT_NONE, sp
                                                 _ptr(residual) if residual is not None else None, int(activation),
                                                 _ptr(workspace) if workspace is not None else None, split_k)
     _check(code, "spb_linear_bitmap_v3")
-    return out
+    return _hand_over(out, stream) if new else out
 
 
 def decode_operand_b(Bc: BitmapMatrix, out=None, stream=None):
     """spb_decode_operand_b: a matrix in the second-operand layout (to_device of init_sparse_matrix_a_bitmap_v6_b)
     expanded to dense fp16 [rows, cols]."""
-    if out is None:
-        out = torch.empty((Bc.M, Bc.K), dtype=torch.float16, device=Bc.vals.device)
-    with torch.cuda.device(out.device):
+    new = out is None
+    with _on(Bc.vals.device if new else out.device, stream):
+        if new:
+            out = torch.empty((Bc.M, Bc.K), dtype=torch.float16, device=Bc.vals.device)
         code = _lib.load().spb_decode_operand_b(_stream_ptr(stream), _ptr(Bc.vals), _ptr(Bc.gtile), _ptr(Bc.bitmap), Bc.M, Bc.K,
                                                 _ptr(out))
     _check(code, "spb_decode_operand_b")
-    return out
+    return _hand_over(out, stream) if new else out
 
 
 def spmspm(W: BitmapMatrix, Bc: BitmapMatrix, split_k=None, out=None, workspace=None, stream=None):
@@ -433,17 +440,18 @@ def spmspm(W: BitmapMatrix, Bc: BitmapMatrix, split_k=None, out=None, workspace=
     N = Bc.M
     if split_k is None:
         split_k = suggest_split_k(W.M, N, W.K)
-    if out is None:
-        out = torch.empty((N, W.M), dtype=torch.float16, device=W.vals.device)
-    if split_k > 1 and workspace is None:
-        workspace = torch.empty(split_k * N * W.M, dtype=torch.float16, device=W.vals.device)
-    with torch.cuda.device(W.vals.device):
+    new = out is None
+    with _on(W.vals.device, stream):
+        if new:
+            out = torch.empty((N, W.M), dtype=torch.float16, device=W.vals.device)
+        if split_k > 1 and workspace is None:
+            workspace = torch.empty(split_k * N * W.M, dtype=torch.float16, device=W.vals.device)
         _init_if_possible(stream)
         code = _lib.load().spb_spmspm_bitmap_v3(_stream_ptr(stream), _ptr(W.vals), _ptr(W.gtile), _ptr(W.mtile), _ptr(W.bitmap),
                                                 _ptr(W.max_nnz), _ptr(Bc.vals), _ptr(Bc.gtile), _ptr(Bc.bitmap), _ptr(out),
                                                 W.M, N, W.K, _ptr(workspace) if workspace is not None else None, split_k)
     _check(code, "spb_spmspm_bitmap_v3")
-    return out
+    return _hand_over(out, stream) if new else out
 
 
 def spmm_noalloc(W: BitmapMatrix, B, split_k, out, stream=None):
@@ -473,9 +481,9 @@ def spmm_allgather(W: BitmapMatrix, B, C_peers, flag_peers, n_peers, rank, M_ful
     the local flag tensor of the exchange that produced B, if B is a gathered buffer not yet waited for."""
     if not (B.is_cuda and B.dtype == torch.float16 and B.dim() == 2 and B.is_contiguous() and B.shape[1] == W.K):
         raise SpmmError("B must be a contiguous CUDA float16 [N,K] tensor")
-    if split_k > 1 and workspace is None:
-        workspace = torch.empty(split_k * B.shape[0] * W.M, dtype=torch.float16, device=B.device)
-    with torch.cuda.device(B.device):
+    with _on(B.device, stream):
+        if split_k > 1 and workspace is None:
+            workspace = torch.empty(split_k * B.shape[0] * W.M, dtype=torch.float16, device=B.device)
         _init_if_possible(stream)
         code = _lib.load().spb_spmm_bitmap_v3_allgather(_stream_ptr(stream), _ptr(W.vals), _ptr(W.gtile), _ptr(W.mtile),
                                                         _ptr(W.bitmap), _ptr(W.max_nnz), _ptr(B), C_peers, flag_peers,
@@ -490,9 +498,9 @@ def spmm_allreduce(W: BitmapMatrix, B, part_peers, flag_peers, n_peers, rank, B_
     buffer (see spmspm_b200.dist.PeerReduce)."""
     if not (B.is_cuda and B.dtype == torch.float16 and B.dim() == 2 and B.is_contiguous() and B.shape[1] == W.K):
         raise SpmmError("B must be a contiguous CUDA float16 [N,K_shard] tensor")
-    if split_k > 1 and workspace is None:
-        workspace = torch.empty(split_k * B.shape[0] * W.M, dtype=torch.float16, device=B.device)
-    with torch.cuda.device(B.device):
+    with _on(B.device, stream):
+        if split_k > 1 and workspace is None:
+            workspace = torch.empty(split_k * B.shape[0] * W.M, dtype=torch.float16, device=B.device)
         _init_if_possible(stream)
         code = _lib.load().spb_spmm_bitmap_v3_allreduce(_stream_ptr(stream), _ptr(W.vals), _ptr(W.gtile), _ptr(W.mtile),
                                                         _ptr(W.bitmap), _ptr(W.max_nnz), _ptr(B), part_peers, flag_peers,

@@ -5,6 +5,7 @@ import pytest
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
+from spmspm_b200 import api  # noqa: E402
 
 
 @pytest.fixture(scope="module")
@@ -37,6 +38,7 @@ def check(call):
     with memory that the current stream still reads freed just before."""
     want = [t.clone() for t in tensors(call(None))]
     s = torch.cuda.Stream()
+    call(s)                     # what a stream's first call prepares
     sizes = sorted({t.numel() * t.element_size() for t in want} | {1 << k for k in range(9, 23)})
     for side in ("given", "current"):
         torch.cuda.synchronize()
@@ -56,6 +58,8 @@ def check(call):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(tensors(got), want, strict=True))
         assert all(bool((t == 0xA5).all()) for t in others)
+    if (0, s.cuda_stream) in api._initialised:
+        api.release(s)
 
 
 def test_preparing_four_bit_weights(sp):
@@ -67,6 +71,18 @@ def test_preparing_four_bit_weights(sp):
     check(lambda s: sp.pack_int4(codes, scales, zeros, stream=s))
     W = sp.encode_int4(A, 64)
     check(lambda s: sp.decode_int4(W, stream=s))
+
+
+def test_bitmap_weights(sp):
+    A, x, bias = half(4, 512, 1024) * (half(5, 512, 1024) > 0.4), half(6, 24, 1024), half(7, 512)
+    check(lambda s: sp.encode_device(A, stream=s))
+    W = sp.encode_device(A)
+    for split_k in (1, 3):
+        check(lambda s: sp.spmm(W, x, split_k=split_k, stream=s))
+        check(lambda s: sp.linear(W, x, bias=bias, split_k=split_k, stream=s))
+    Bc = sp.to_device(sp.init_sparse_matrix_a_bitmap_v6_b((half(8, 64, 1024) * (half(9, 64, 1024) > 0)).cpu().numpy()))
+    check(lambda s: sp.decode_operand_b(Bc, stream=s))
+    check(lambda s: sp.spmspm(W, Bc, split_k=2, stream=s))
 
 
 def test_a_stream_of_another_device_is_refused(sp):
