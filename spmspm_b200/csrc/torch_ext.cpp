@@ -70,32 +70,34 @@ void init(const std::string& path, py::object error)
 // at::empty without the dispatcher's detour (0.6 us instead of 1.1; a call with one launch takes 3).
 Tensor make(at::IntArrayRef shape, at::ScalarType type, c10::Device dev) { return Tensor(at::detail::empty_cuda(shape, type, dev, std::nullopt)); }
 
-// Device and stream of a call: the tensors' device is made current, the stream is the given one or torch's current one there.
+// Device and stream of a call: the tensors' device is made current, and with it the stream, the given one or torch's current one there.
+// Outputs and workspaces are then of that stream's pool: memory of another one may still be in use there, and goes back to it while this
+// stream is at work.
 struct Place {
     c10::cuda::CUDAGuard guard;
-    c10::cuda::CUDAStream stream;
-    bool given;
+    c10::cuda::CUDAStream caller, stream;
+    std::optional<c10::cuda::CUDAStreamGuard> given;
     Place(int dev, std::optional<int64_t> s)
         : guard((c10::DeviceIndex)dev),
-          stream(s ? c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(*s), (c10::DeviceIndex)dev) : c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev)),
-          given(s.has_value())
+          caller(c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev)),
+          stream(s ? c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(*s), (c10::DeviceIndex)dev) : caller)
     {
+        if (s) given.emplace(stream.unwrap());
     }
     void* ptr() const { return stream.stream(); }
-    // a new workspace; its memory must not go to another tensor before a stream given by hand is done with it
-    Tensor workspace(size_t bytes, const Tensor& like) const
+    Tensor output(at::IntArrayRef shape, c10::Device dev) const
     {
-        Tensor w = make({(int64_t)bytes}, at::kByte, like.device());
-        if (given) w.record_stream(stream.unwrap());
-        return w;
+        Tensor t = make(shape, at::kHalf, dev);
+        if (given && t.numel()) t.record_stream(caller.unwrap());   // not used anew before the caller's stream, too, is done with it
+        return t;
     }
 };
 // Workspace of the caller, or a new one.
-Tensor pick_workspace(const Place& at_, const OptTensor& given, size_t need, const Tensor& like, const char* where, size_t& have)
+Tensor pick_workspace(const OptTensor& given, size_t need, const Tensor& like, const char* where, size_t& have)
 {
     if (!given) {
         have = need;
-        return need ? at_.workspace(need, like) : Tensor();
+        return need ? make({(int64_t)need}, at::kByte, like.device()) : Tensor();
     }
     have = given->nbytes();
     if (!given->is_cuda() || given->device() != like.device() || !given->is_contiguous() || have < need)
@@ -164,28 +166,23 @@ OptTensor kv_append(const Cache& c, const Tensor& k, const Tensor& v, const Tens
         max_pos = cos->size(0), rot = 2 * cos->size(1);
         if (rot == 0 || rot % 8 || rot > c.head_dim) fail("the rotated channels must be a multiple of 8 up to head_dim");
     }
-    OptTensor out;
     const uint16_t* qp = nullptr;
     if (!q && q_out) fail("q_out without q");
     if (q) {
         if (!cos) fail("q is only taken to be rotated: cos and sin are missing");
         qp = check_vectors(c, *q, "q", n, -1);
         if (!q->size(1)) fail("q has no heads");
-        if (q_out) {
-            dense_half(*q_out, "q_out", q->sizes(), c.pool.device(), "cache");
-            out = *q_out;
-        } else {
-            out = make(q->sizes(), at::kHalf, q->device());
-        }
+        if (q_out) dense_half(*q_out, "q_out", q->sizes(), c.pool.device(), "cache");
     }
-    if (n) {
-        const Place at_(c.pool.get_device(), stream);
+    const Place at_(c.pool.get_device(), stream);
+    OptTensor out = q_out;
+    if (q && !q_out) out = at_.output(q->sizes(), q->device());
+    if (n)
         check(p_kv_append(at_.ptr(), c.pool.data_ptr(), c.num_pages, c.page_size, c.kv_heads, c.head_dim, b.table, b.width, b.lens, b.cu, b.batch, n, kp,
                           k.stride(0), k.stride(1), vp, v.stride(0), v.stride(1), qp, q ? q->stride(0) : 0, q ? q->stride(1) : 0, q ? (int)q->size(1) : 0,
                           out ? static_cast<uint16_t*>(out->data_ptr()) : nullptr, cos ? cos->const_data_ptr<float>() : nullptr,
                           sin ? sin->const_data_ptr<float>() : nullptr, (int)max_pos, (int)rot, interleaved),
               "spb_kv_append");
-    }
     return out;
 }
 
@@ -198,18 +195,14 @@ std::pair<Tensor, Tensor> kv_read(const Cache& c, const Tensor& table, const Ten
     if (n < 0) fail("n_tokens must not be negative");
     check_rows(n, b);
     const int64_t shape[3] = {n, c.kv_heads, c.head_dim};
-    auto output = [&](const OptTensor& given, const char* name) {
-        if (!given) return make(shape, at::kHalf, c.pool.device());
-        dense_half(*given, name, shape, c.pool.device(), "cache");
-        return *given;
-    };
-    Tensor k = output(k_out, "k_out"), v = output(v_out, "v_out");
-    if (n) {
-        const Place at_(c.pool.get_device(), stream);
+    if (k_out) dense_half(*k_out, "k_out", shape, c.pool.device(), "cache");
+    if (v_out) dense_half(*v_out, "v_out", shape, c.pool.device(), "cache");
+    const Place at_(c.pool.get_device(), stream);
+    Tensor k = k_out ? *k_out : at_.output(shape, c.pool.device()), v = v_out ? *v_out : at_.output(shape, c.pool.device());
+    if (n)
         check(p_kv_read(at_.ptr(), c.pool.data_ptr(), c.num_pages, c.page_size, c.kv_heads, c.head_dim, b.table, b.width, b.lens, b.cu, b.batch, n,
                         static_cast<uint16_t*>(k.data_ptr()), static_cast<uint16_t*>(v.data_ptr())),
               "spb_kv_read");
-    }
     return {k, v};
 }
 
@@ -230,11 +223,11 @@ Tensor kv_attention(const Tensor& q, const Cache& c, const Tensor& table, const 
     const int64_t most = max_q ? *max_q : b.cu ? n : n / b.batch;
     if (most < 0 || most > n) fail("max_q must be in 0..tokens");
     if (out_given) dense_half(*out_given, "out", q.sizes(), c.pool.device(), "cache");
-    Tensor out = out_given ? *out_given : make(q.sizes(), at::kHalf, q.device());
-    if (!n) return out;
     const Place at_(c.pool.get_device(), stream);
+    Tensor out = out_given ? *out_given : at_.output(q.sizes(), q.device());
+    if (!n) return out;
     size_t have;
-    const Tensor ws = pick_workspace(at_, ws_given, p_kv_attention_workspace_bytes(c.head_dim, b.batch, (int)heads, c.kv_heads, (int)most), q, "cache", have);
+    const Tensor ws = pick_workspace(ws_given, p_kv_attention_workspace_bytes(c.head_dim, b.batch, (int)heads, c.kv_heads, (int)most), q, "cache", have);
     check(p_kv_attention(at_.ptr(), c.pool.data_ptr(), c.num_pages, c.page_size, c.kv_heads, c.head_dim, b.table, b.width, b.lens, b.cu, b.batch, n, qp,
                          q.stride(0), q.stride(1), (int)heads, (int)most, (float)(scale ? *scale : 1 / std::sqrt((double)c.head_dim)),
                          static_cast<uint16_t*>(out.data_ptr()), ws.data_ptr(), have),
@@ -260,10 +253,10 @@ Tensor linear_int4(const Tensor& data, int64_t M, int64_t K, int64_t group, cons
         fail("bias must be a contiguous CUDA float16 [M] tensor");
     if (residual) dense_half(*residual, "residual", shape, dev, "weight");
     if (out_given) dense_half(*out_given, "out", shape, dev, "weight");
-    Tensor out = out_given ? *out_given : make(shape, at::kHalf, dev);
     const Place at_(data.get_device(), stream);
+    Tensor out = out_given ? *out_given : at_.output(shape, dev);
     size_t have;
-    const Tensor ws = pick_workspace(at_, ws_given, p_int4_workspace_bytes((int)M, (int)N, (int)K), x, "weight", have);
+    const Tensor ws = pick_workspace(ws_given, p_int4_workspace_bytes((int)M, (int)N, (int)K), x, "weight", have);
     auto half = [](const OptTensor& t) { return t ? static_cast<const uint16_t*>(t->const_data_ptr()) : nullptr; };
     check(p_linear_int4(at_.ptr(), data.const_data_ptr(), (int)M, (int)K, (int)group, static_cast<const uint16_t*>(x.const_data_ptr()),
                         static_cast<uint16_t*>(out.data_ptr()), (int)N, half(bias), half(residual), (int)activation, ws.defined() ? ws.data_ptr() : nullptr, have),

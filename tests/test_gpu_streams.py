@@ -85,6 +85,30 @@ def test_bitmap_weights(sp):
     check(lambda s: sp.spmspm(W, Bc, split_k=2, stream=s))
 
 
+@pytest.mark.parametrize("N", [3, 200])
+@pytest.mark.parametrize("M,K", [(1024, 2048), (20480, 256)])
+def test_linear(sp, M, K, N):
+    W, x, bias = sp.encode_int4(half(10, M, K), 128), half(11, N, K), half(12, M)
+    check(lambda s: sp.linear_int4(W, x, bias=bias, stream=s))
+
+
+@pytest.mark.parametrize("T", [1, 96])
+def test_cache(sp, T):
+    """Appending with turned queries, reading and attention; T = 96 with the kernel for many rows."""
+    B, L, heads, D = 3, 1000, 24, 64
+    cache = sp.KvCacheInt4(B * 63, 16, heads, D)
+    table = torch.arange(B * 63, dtype=torch.int32, device="cuda").view(B, 63)
+    lens = torch.full((B,), L, dtype=torch.int32, device="cuda")
+    sp.kv_append(cache, half(13, B * L, heads, D), half(14, B * L, heads, D), table, lens)
+    k, v, q = (half(i, B * T, heads, D) for i in (15, 16, 17))
+    cos = torch.cos(torch.arange(L * 32, device="cuda").view(L, 32).float())
+    sin = torch.sin(torch.arange(L * 32, device="cuda").view(L, 32).float())
+    check(lambda s: sp.kv_append(cache, k, v, table, lens, q=q, cos=cos, sin=sin, stream=s))
+    check(lambda s: sp.kv_read(cache, table, lens, n_tokens=B * T, stream=s))
+    check(lambda s: sp.kv_attention(q, cache, table, lens, stream=s))
+    assert sp.device_status() == 0
+
+
 def test_a_stream_of_another_device_is_refused(sp):
     if torch.cuda.device_count() < 2:
         pytest.skip("one device")
