@@ -24,6 +24,7 @@ using OptTensor = std::optional<Tensor>;
 
 PyObject* g_error = nullptr;
 decltype(&spb_last_error) p_last_error;
+decltype(&spb_kv_cache_bytes) p_kv_cache_bytes;
 decltype(&spb_kv_append) p_kv_append;
 decltype(&spb_kv_read) p_kv_read;
 decltype(&spb_kv_attention) p_kv_attention;
@@ -57,6 +58,7 @@ void init(const std::string& path, py::object error)
         if (!f) throw std::runtime_error(std::string(name) + " is missing in " + path);
     };
     get(p_last_error, "spb_last_error");
+    get(p_kv_cache_bytes, "spb_kv_cache_bytes");
     get(p_kv_append, "spb_kv_append");
     get(p_kv_read, "spb_kv_read");
     get(p_kv_attention, "spb_kv_attention");
@@ -116,12 +118,21 @@ struct Cache {
     Tensor pool;
     int num_pages, page_size, kv_heads, head_dim;
 };
+// The pool as the kernels take it.  A saved cache may be loaded without a device, but is used on one.
+void check_pool(const Cache& c)
+{
+    if (!c.pool.is_cuda()) fail("the cache lives on a CUDA device, its pool is on " + c.pool.device().str());
+    if (c.pool.scalar_type() != at::kByte || !c.pool.is_contiguous() ||
+        c.pool.nbytes() < p_kv_cache_bytes(c.num_pages, c.page_size, c.kv_heads, c.head_dim))
+        fail("the cache's pool must be a contiguous uint8 tensor of spb_kv_cache_bytes bytes");
+}
 struct Batch {
     const int *table, *lens, *cu;
     int width, batch;
 };
 Batch check_batch(const Cache& c, const Tensor& table, const Tensor& lens, const OptTensor& cu)
 {
+    check_pool(c);
     const auto dev = c.pool.device();
     if (table.device() != dev || table.scalar_type() != at::kInt || table.dim() != 2 || !table.is_contiguous() || !table.numel())
         fail("page_table must be a contiguous CUDA int32 [batch, pages] tensor on the cache's device");
@@ -208,6 +219,7 @@ std::pair<Tensor, Tensor> kv_read(const Cache& c, const Tensor& table, const Ten
 
 size_t kv_attention_workspace(const Cache& c, int64_t q_heads, int64_t batch, int64_t max_q)
 {
+    check_pool(c);
     const c10::cuda::CUDAGuard guard(c.pool.device());
     return p_kv_attention_workspace_bytes(c.head_dim, (int)batch, (int)q_heads, c.kv_heads, (int)max_q);
 }
