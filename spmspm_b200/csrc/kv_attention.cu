@@ -44,7 +44,7 @@ constexpr int TT = 2, kStages = 2;
 constexpr int kUnit = kKvBlock * kWarps * TT;   // tokens a thread block advances per step
 // Tiles of 8 query rows a thread block takes: one, or two for more than 8 rows.  Four (32 rows) left two thread blocks of 255
 // registers per SM and took 210 us where two take 122 (16 sequences of 8000, 32 rows); one took 156, reading the cache twice as often.
-int pick_nt(int rows) { return rows <= 8 ? 1 : 2; }
+int pick_nt(long long rows) { return rows <= 8 ? 1 : 2; }
 __host__ __device__ constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 __device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity)
 {
@@ -889,7 +889,7 @@ cudaError_t launch(cudaStream_t s, const KvAttnArgs& a, int* status)
 template <int D>
 cudaError_t launch_d(cudaStream_t s, const KvAttnArgs& a, int* status)
 {
-    switch (pick_nt(a.max_q * (a.q_heads / a.c.kv_heads))) {
+    switch (pick_nt((long long)a.max_q * (a.q_heads / a.c.kv_heads))) {
         case 1: return launch<D, 1>(s, a, status);
         default: return launch<D, 2>(s, a, status);
     }
@@ -920,7 +920,7 @@ cudaError_t kv_attention_launch(cudaStream_t s, int D, const KvAttnArgs& args, i
 size_t kv_attention_ws_floats(int D, int B, int q_heads, int kv_heads, int max_q)
 {
     (void)B;
-    const int rows = 8 * pick_nt(max_q * (q_heads / kv_heads));
+    const int rows = 8 * pick_nt((long long)max_q * (q_heads / kv_heads));
     return (size_t)2 * blocks_per_sm(rows / 8) * sm_count() * rows * (D + 2);
 }
 

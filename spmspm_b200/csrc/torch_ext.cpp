@@ -12,6 +12,7 @@
 #include <dlfcn.h>
 
 #include <cmath>
+#include <cstdint>
 #include <optional>
 #include <string>
 
@@ -47,6 +48,13 @@ std::string shape_text(at::IntArrayRef s)
     std::string t = "[";
     for (size_t i = 0; i < s.size(); ++i) t += (i ? ", " : "") + std::to_string(s[i]);
     return t + "]";
+}
+
+// A size as the C entry points take it: what does not fit is refused, not cut.
+int as_int(int64_t x, const char* name)
+{
+    if (x < INT32_MIN || x > INT32_MAX) fail(std::string(name) + " is out of range: " + std::to_string(x));
+    return (int)x;
 }
 
 void init(const std::string& path, py::object error)
@@ -137,11 +145,13 @@ Batch check_batch(const Cache& c, const Tensor& table, const Tensor& lens, const
     if (table.device() != dev || table.scalar_type() != at::kInt || table.dim() != 2 || !table.is_contiguous() || !table.numel())
         fail("page_table must be a contiguous CUDA int32 [batch, pages] tensor on the cache's device");
     const int64_t n = table.size(0);
+    if (n > 65535) fail("page_table has " + std::to_string(n) + " sequences, at most 65535 are taken");
+    const int width = as_int(table.size(1), "the width of page_table");
     if (lens.device() != dev || lens.scalar_type() != at::kInt || lens.dim() != 1 || lens.size(0) != n || !lens.is_contiguous())
         fail("kv_lens must be a contiguous CUDA int32 [" + std::to_string(n) + "] tensor on the cache's device");
     if (cu && (cu->device() != dev || cu->scalar_type() != at::kInt || cu->dim() != 1 || cu->size(0) != n + 1 || !cu->is_contiguous()))
         fail("cu_q must be a contiguous CUDA int32 [" + std::to_string(n + 1) + "] tensor on the cache's device");
-    return {table.const_data_ptr<int>(), lens.const_data_ptr<int>(), cu ? cu->const_data_ptr<int>() : nullptr, (int)table.size(1), (int)n};
+    return {table.const_data_ptr<int>(), lens.const_data_ptr<int>(), cu ? cu->const_data_ptr<int>() : nullptr, width, (int)n};
 }
 // [tokens, heads, head_dim] with contiguous channels and strides that hold four channels together
 const uint16_t* check_vectors(const Cache& c, const Tensor& t, const char* name, int64_t tokens, int64_t heads)
@@ -174,7 +184,7 @@ OptTensor kv_append(const Cache& c, const Tensor& k, const Tensor& v, const Tens
         for (const auto* t : {&*cos, &*sin})
             if (t->device() != c.pool.device() || t->scalar_type() != at::kFloat || t->dim() != 2 || !t->is_contiguous() || t->sizes() != cos->sizes() || !t->size(0))
                 fail(std::string(t == &*cos ? "cos" : "sin") + " must be a contiguous CUDA float32 [positions, rot/2] tensor on the cache's device");
-        max_pos = cos->size(0), rot = 2 * cos->size(1);
+        max_pos = as_int(cos->size(0), "the number of positions"), rot = 2 * cos->size(1);
         if (rot == 0 || rot % 8 || rot > c.head_dim) fail("the rotated channels must be a multiple of 8 up to head_dim");
     }
     const uint16_t* qp = nullptr;
@@ -182,7 +192,7 @@ OptTensor kv_append(const Cache& c, const Tensor& k, const Tensor& v, const Tens
     if (q) {
         if (!cos) fail("q is only taken to be rotated: cos and sin are missing");
         qp = check_vectors(c, *q, "q", n, -1);
-        if (!q->size(1)) fail("q has no heads");
+        if (!as_int(q->size(1), "the number of heads")) fail("q has no heads");
         if (q_out) dense_half(*q_out, "q_out", q->sizes(), c.pool.device(), "cache");
     }
     const Place at_(c.pool.get_device(), stream);
@@ -220,8 +230,11 @@ std::pair<Tensor, Tensor> kv_read(const Cache& c, const Tensor& table, const Ten
 size_t kv_attention_workspace(const Cache& c, int64_t q_heads, int64_t batch, int64_t max_q)
 {
     check_pool(c);
+    for (const auto& [x, name] : {std::pair{q_heads, "q_heads"}, {batch, "batch"}, {max_q, "max_q"}}) as_int(x, name);
     const c10::cuda::CUDAGuard guard(c.pool.device());
-    return p_kv_attention_workspace_bytes(c.head_dim, (int)batch, (int)q_heads, c.kv_heads, (int)max_q);
+    const size_t bytes = p_kv_attention_workspace_bytes(c.head_dim, (int)batch, (int)q_heads, c.kv_heads, (int)max_q);
+    if (!bytes) fail("batch must be positive, q_heads a positive multiple of the cache's heads and max_q not negative");
+    return bytes;
 }
 
 Tensor kv_attention(const Tensor& q, const Cache& c, const Tensor& table, const Tensor& lens, const OptTensor& cu, std::optional<int64_t> max_q,
@@ -229,19 +242,21 @@ Tensor kv_attention(const Tensor& q, const Cache& c, const Tensor& table, const 
 {
     const Batch b = check_batch(c, table, lens, cu);
     const uint16_t* qp = check_vectors(c, q, "q", -1, -1);
-    const int64_t n = q.size(0), heads = q.size(1);
+    const int64_t n = q.size(0);
+    const int heads = as_int(q.size(1), "the number of heads");
     if (!heads || heads % c.kv_heads) fail("the heads of q must be a positive multiple of the cache's");
     check_rows(n, b);
-    const int64_t most = max_q ? *max_q : b.cu ? n : n / b.batch;
-    if (most < 0 || most > n) fail("max_q must be in 0..tokens");
+    const int64_t bound = max_q ? *max_q : b.cu ? n : n / b.batch;
+    if (bound < 0 || bound > n) fail("max_q must be in 0..tokens");
+    const int most = as_int(bound, "max_q");
     if (out_given) dense_half(*out_given, "out", q.sizes(), c.pool.device(), "cache");
     const Place at_(c.pool.get_device(), stream);
     Tensor out = out_given ? *out_given : at_.output(q.sizes(), q.device());
     if (!n) return out;
     size_t have;
-    const Tensor ws = pick_workspace(ws_given, p_kv_attention_workspace_bytes(c.head_dim, b.batch, (int)heads, c.kv_heads, (int)most), q, "cache", have);
+    const Tensor ws = pick_workspace(ws_given, p_kv_attention_workspace_bytes(c.head_dim, b.batch, heads, c.kv_heads, most), q, "cache", have);
     check(p_kv_attention(at_.ptr(), c.pool.data_ptr(), c.num_pages, c.page_size, c.kv_heads, c.head_dim, b.table, b.width, b.lens, b.cu, b.batch, n, qp,
-                         q.stride(0), q.stride(1), (int)heads, (int)most, (float)(scale ? *scale : 1 / std::sqrt((double)c.head_dim)),
+                         q.stride(0), q.stride(1), heads, most, (float)(scale ? *scale : 1 / std::sqrt((double)c.head_dim)),
                          static_cast<uint16_t*>(out.data_ptr()), ws.data_ptr(), have),
           "spb_kv_attention");
     return out;
@@ -249,17 +264,19 @@ Tensor kv_attention(const Tensor& q, const Cache& c, const Tensor& table, const 
 
 // -------------------------------------------------------------------------------------------------- 4-bit weights
 
-Tensor linear_int4(const Tensor& data, int64_t M, int64_t K, int64_t group, const Tensor& x, const OptTensor& bias, const OptTensor& residual,
+Tensor linear_int4(const Tensor& data, int64_t rows, int64_t columns, int64_t group, const Tensor& x, const OptTensor& bias, const OptTensor& residual,
                    int64_t activation, const OptTensor& out_given, const OptTensor& ws_given, std::optional<int64_t> stream)
 {
     const auto dev = data.device();
-    const size_t bytes = p_int4_bytes((int)M, (int)K, (int)group);
+    const int M = as_int(rows, "M"), K = as_int(columns, "K");
+    const size_t bytes = p_int4_bytes(M, K, as_int(group, "the group"));
     if (!bytes) fail("M and K must be positive multiples of 64 and the group 32, 64 or 128 and divide K");
     if (!data.is_cuda() || data.scalar_type() != at::kByte || !data.is_contiguous() || data.dim() != 1 || (size_t)data.size(0) != bytes)
         fail("W.data must be the contiguous CUDA uint8 tensor that pack_int4 made");
     if (x.device() != dev || x.scalar_type() != at::kHalf || x.dim() != 2 || x.size(1) != K || !x.size(0) || !x.is_contiguous())
         fail("B must be a contiguous CUDA float16 [N,K] tensor on the weight's device");
-    const int64_t N = x.size(0), shape[2] = {N, M};
+    const int N = as_int(x.size(0), "N");
+    const int64_t shape[2] = {N, M};
     if (activation != 0 && activation != 1) fail("activation must be ACT_NONE or ACT_RELU");
     if (bias && (bias->device() != dev || bias->scalar_type() != at::kHalf || !bias->is_contiguous() || bias->dim() != 1 || bias->size(0) != M))
         fail("bias must be a contiguous CUDA float16 [M] tensor");
@@ -268,10 +285,10 @@ Tensor linear_int4(const Tensor& data, int64_t M, int64_t K, int64_t group, cons
     const Place at_(data.get_device(), stream);
     Tensor out = out_given ? *out_given : at_.output(shape, dev);
     size_t have;
-    const Tensor ws = pick_workspace(ws_given, p_int4_workspace_bytes((int)M, (int)N, (int)K), x, "weight", have);
+    const Tensor ws = pick_workspace(ws_given, p_int4_workspace_bytes(M, N, K), x, "weight", have);
     auto half = [](const OptTensor& t) { return t ? static_cast<const uint16_t*>(t->const_data_ptr()) : nullptr; };
-    check(p_linear_int4(at_.ptr(), data.const_data_ptr(), (int)M, (int)K, (int)group, static_cast<const uint16_t*>(x.const_data_ptr()),
-                        static_cast<uint16_t*>(out.data_ptr()), (int)N, half(bias), half(residual), (int)activation, ws.defined() ? ws.data_ptr() : nullptr, have),
+    check(p_linear_int4(at_.ptr(), data.const_data_ptr(), M, K, (int)group, static_cast<const uint16_t*>(x.const_data_ptr()),
+                        static_cast<uint16_t*>(out.data_ptr()), N, half(bias), half(residual), (int)activation, ws.defined() ? ws.data_ptr() : nullptr, have),
           "spb_linear_int4");
     return out;
 }

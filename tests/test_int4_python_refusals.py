@@ -32,3 +32,19 @@ def test_a_cache_loaded_without_a_device_is_not_used(sp):
     for call in calls(sp, cache, table, lens, x):
         with pytest.raises(sp.SpmmError, match="CUDA device"):
             call()
+
+
+BIG = 1 << 32
+
+
+@pytest.mark.parametrize("M,K,group", [(BIG + 64, 128, 64), (64, BIG + 128, 64), (64, 128, BIG + 64), (-BIG + 64, 128, 64)])
+def test_sizes_are_not_cut_to_32_bits(sp, M, K, group):
+    """A size whose low 32 bits fit the data."""
+    with pytest.raises(sp.SpmmError, match="out of range"):
+        sp.linear_int4(sp.Int4Matrix(M, K, group, torch.zeros(9216, dtype=torch.uint8)), torch.zeros((1, 128), dtype=torch.float16))
+
+
+def test_workspace_of_sizes_without_one(lib_built):
+    """Rows a key head are counted in 64 bits, sizes that no call takes have no workspace."""
+    small, large = (lib_built.spb_kv_attention_workspace_bytes(128, 1, 1 << 16, 1, q) for q in (0, 1 << 15))
+    assert large == lib_built.spb_kv_attention_workspace_bytes(128, 1, 1 << 16, 1, 1 << 10) != small
