@@ -360,9 +360,10 @@ int spb_linear_int4(void* stream, const void* packed, int M, int K, int group, c
  *   spb_kv_append     writes the keys and values of the new tokens.  With cos_table / sin_table ([max_pos][rot_dim / 2] fp32)
  *                     the first rot_dim channels of the keys, and of q if given (result in q_out, [n_tokens][q_heads][head_dim]),
  *                     are first turned by the angles of the token's position in the cache: pairs (i, i + rot_dim / 2), or
- *                     (2 i, 2 i + 1) if interleaved; computed in 64 bits, rounded once to fp16.  rot_dim: a multiple of 8.
- *                     A position that is negative (more new tokens than kv_lens) is skipped; one past max_pos is skipped
- *                     and sets bit 8.  Two rows of one call must not name the same slot of a page.  q_out may be q itself.
+ *                     (2 i, 2 i + 1) if interleaved; both products and their sum exact up to 2^-48 (pairs of fp32 values), rounded
+ *                     once to fp16.  rot_dim: a multiple of 8.
+ *                     A token at a negative position (more new tokens than kv_lens) is skipped: key, value and query stay as they
+ *                     were; so is one at max_pos or behind, which sets bit 8.  Two rows of one call must not name the same slot of a page.  q_out may be q itself.
  *   spb_kv_read       k, v [n_tokens][kv_heads][head_dim] fp16: what the cache holds for these tokens.
  *   spb_kv_attention  out[i] = softmax(scale q[i] K^T) V over the keys of its sequence up to its own position
  *                     (row cu_q[b + 1] - 1 sees all kv_lens[b]); a row that sees no key gets zeros.  q_heads is a multiple of

@@ -170,12 +170,12 @@ __device__ __forceinline__ void append_vectors(const KvAppendArgs& a, int tok, i
     const int heads = KIND == kQueries ? a.q_heads : a.c.kv_heads;
     bool turning = false;
     float cs[8], sn[8];
-    if (KIND != kValues && a.cosv) {
-        if (pos >= a.max_pos) {   // no angles for this position
+    if (a.cosv) {
+        if (pos >= a.max_pos) {   // no angles for this position: the whole token is skipped, its values too
             if (lane == 0) atomicOr(status, kStatusBadCache);
             return;
         }
-        turning = c0 < a.rot;
+        turning = KIND != kValues && c0 < a.rot;
         if (turning) load_angles(a, pos, c0, cs, sn);
     }
     uint8_t* blk = nullptr;

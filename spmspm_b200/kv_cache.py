@@ -60,7 +60,8 @@ def kv_append(cache, k, v, page_table, kv_lens, cu_q=None, q=None, cos=None, sin
     With cos and sin (float32 [positions, rot/2]) the first rot channels of the keys are first turned by the angles of the
     token's position in the cache, and so are those of q [tokens, heads, head_dim], which is returned (q_out, which may be q itself,
     or a new tensor).
-    Rows that belong to no sequence leave q_out as it was."""
+    Tokens before the start of the context or past the angles are skipped as a whole; their rows, and those of no sequence, leave q_out as
+    it was (a new tensor has no defined value there)."""
     return _lib.ext().kv_append(cache._handle, k, v, page_table, kv_lens, cu_q, q, cos, sin, interleaved, q_out, _raw(stream))
 
 
