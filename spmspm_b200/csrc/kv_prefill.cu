@@ -169,7 +169,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefill_kernel(KvAttnArgs a, i
     volatile int* abort_flag = &sm.abort;
 
     grid_wait();
-    grid_release();
     // ---- the item: key head blockIdx.x % heads, row tile number blockIdx.x / heads of the sequences with `tall` rows and more;
     // in a sequence the last rows, which see most, come first
     const int h = blockIdx.x % c.kv_heads, want = blockIdx.x / c.kv_heads;
@@ -236,6 +235,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prefill_kernel(KvAttnArgs a, i
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // Only now that this block has its tensor memory: a kernel that follows may take some before it waits for this one, and would have it
+    // while a block here waited for all of it.
+    grid_release();
 
     bool ok = true;
     if (warp == 0) {

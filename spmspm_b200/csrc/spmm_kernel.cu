@@ -684,10 +684,11 @@ spmm_bitmap_tcgen05_kernel(const KernelParams p, const __grid_constant__ CUtenso
     // overlaps the tail of the preceding kernel of the stream.  From here on the roles differ in what they may
     // do before that kernel has completed (griddepcontrol.wait):
     //   - the warps that stream the weight (packed values, bitmaps, offsets, max_nnz_intile) do not wait at all.
-    //     The weight arrays are never written by this library's SpMM kernels, the only kernels that let a
-    //     dependent start before they have finished; any other kernel ahead in the stream has completed all
-    //     its thread blocks before this one starts.  So the ring of stages fills with weights while the
-    //     slowest CTAs of the preceding SpMM are still in their epilogue;
+    //     The weight arrays are never written by the kernels of this library that let a dependent start before
+    //     they have finished (the SpMM itself and the 4-bit operators, which do so only after all that precedes
+    //     them has finished); any other kernel ahead in the stream has completed all its thread blocks before
+    //     this one starts.  So the ring of stages fills with weights while the slowest CTAs of the preceding
+    //     kernel are still in their epilogue;
     //   - the warp that loads the activation tiles, the epilogue warps (stores to C, to the partial sums, to
     //     the peers; the scratch of the schedules) and everything that reads the exchange flags wait first.
     // Kernels queued behind this one may be set up as soon as every CTA has passed this point.

@@ -60,3 +60,33 @@ def test_a_token_without_a_place_or_angles_is_skipped_whole(sp, kv_heads, q_head
     assert np.array_equal(got[there], turned) and np.all(got[~there] == 7)
     assert sp.device_status() == (8 if (pos >= angles).any() else 0)
     sp.reset_device_status()
+
+
+@pytest.mark.parametrize("D,heads", [(128, 24), (64, 40)])
+def test_prompt_attention_before_products_that_take_tensor_memory(sp, D, heads):
+    """Attention of a prompt, and right behind it kernels that take tensor memory before they wait for it: the same bits as one by one."""
+    rng = np.random.default_rng(D)
+    n, hidden = 600, heads * D
+    cache = sp.KvCacheInt4(2 * 16, 64, heads, D)
+    table = torch.arange(32, dtype=torch.int32, device="cuda").view(2, 16)
+    q, k, v = (dev(randn(rng, 2 * n, heads, D)) for _ in range(3))
+    sp.kv_append(cache, k, v, table, i32(n, n))
+    dense = dev(randn(rng, 640, hidden) * np.float16(0.02))
+    Q, W = sp.encode_int4(dense, 64), sp.encode_device(dense)
+    few = dev(randn(rng, 8, hidden))
+
+    def step(wait):
+        out = []
+        for follow in (lambda x: sp.linear_int4(Q, x[:300].contiguous()), lambda x: sp.spmm(W, few, split_k=1), lambda x: sp.linear_int4(Q, few)):
+            x = sp.kv_attention(q, cache, table, i32(n, n)).flatten(1)
+            if wait:
+                torch.cuda.synchronize()
+            out += [x, follow(x)]
+            if wait:
+                torch.cuda.synchronize()
+        return out
+
+    want = step(True)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(step(False), want))
+    assert sp.device_status() == 0
