@@ -14,8 +14,9 @@
 //            than 2^8; weights are kept 2^7 too large, so that in fp16 they span 2^-31 .. 1 relative to the largest.
 //   values   O^T = sum over tokens of (P s) c + P m: P^T comes from S^T with two 8 x 8 transposes in registers and is multiplied
 //            by the tokens' scales, one product per group, rounded to fp16 like P itself; the minima are one more matrix
-//            instruction per 16 tokens.  Scales of 2 and more would leave the fp16 range: the whole row is then shifted down by
-//            the scale's exponent, as if its maximum had grown.  The roundings of P and of P s average out over many keys; over
+//            instruction per 16 tokens.  The scales of a group are first brought to 1 .. 2 by the power of two of the largest one so far,
+//            so that the products, too, span 2^-31 .. 1 relative to the largest (down to scales of 2^-15, whose values are next to the
+//            smallest of fp16); when a larger one comes, the group's accumulators are scaled down.  The roundings of P and of P s average out over many keys; over
 //            few they would make outputs half again as far from the exact ones (five keys: 3.0e-4, the rounding of the output alone
 //            2.0e-4).  Where no context can have more than 128 tokens, a second product is taken with what the roundings took away.
 //
@@ -75,6 +76,9 @@ __device__ __forceinline__ float exp2_approx(float x)
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
+
+__device__ __forceinline__ float power(int exponent) { return __int_as_float((127 + exponent) << 23); }
+__device__ __forceinline__ int exponent_of(__half2 power_of_two) { return (int)(h2_bits(power_of_two) >> 26) - 15; }
 
 constexpr long long kMostUnits = (1ll << 31) - (1ll << 25);   // of a list
 
@@ -347,7 +351,9 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
         float o[NT][MT][4];      // sum of P s c, rows of the high nibbles 2^-20, of the low ones 2^-24 of it
         float om[NT][4];         // sum of P m, row = group
         float mx[NT][2], sum[NT][2];
-        int shift = 0;           // exponent that the scales of the values have asked for; part of mx
+        __half2 unit[G];         // 2^-e of a group, e the exponent of its largest scale so far, -15 at least
+#pragma unroll
+        for (int w = 0; w < G; ++w) unit[w] = __half2half2(__ushort_as_half((unsigned short)(30 << 10)));
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -356,11 +362,14 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
             mx[nt][0] = mx[nt][1] = -INFINITY;
             sum[nt][0] = sum[nt][1] = 0.f;
         }
-        auto rescale = [&](int nt, float r0, float r1) {
+        auto rescale = [&](int nt, float r0, float r1, const float (&down)[G]) {   // rows by r0, r1, groups by down
             sum[nt][0] *= r0, sum[nt][1] *= r1;
             om[nt][0] *= r0, om[nt][1] *= r1;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) o[nt][i][0] *= r0, o[nt][i][1] *= r1, o[nt][i][2] *= r0, o[nt][i][3] *= r1;
+            for (int i = 0; i < MT; ++i) {
+                const float d0 = r0 * down[i / 2], d1 = r1 * down[i / 2];
+                o[nt][i][0] *= d0, o[nt][i][1] *= d1, o[nt][i][2] *= d0, o[nt][i][3] *= d1;
+            }
         };
 
         int pos0 = ((seg.begin - seg.tile_begin) * kWarps + warp) * (kKvBlock * TT);
@@ -447,6 +456,7 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
                 }
                 // ---- scales of the values of tokens 2t, 2t+1 (j = 0) and 2t+8, 2t+9 (j = 1), all groups; minima of group g
                 uint32_t vs[TT][2][G], vm[TT][2], large = 0;   // large: bit 14 of an fp16 value, 2 or more
+                __half2 most[G];   // of a group's scales here
 #pragma unroll
                 for (int k = 0; k < TT; ++k) {
 #pragma unroll
@@ -470,14 +480,14 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
                     for (int k = 0; k < TT; ++k) {
                         uint32_t nan_tokens[G] = {};
                         bool any = false;
-                        const int most = (there >> k & 1) ? seg.kmax - (pos0 + k * kKvBlock) : 0;
+                        const int in_sight = (there >> k & 1) ? seg.kmax - (pos0 + k * kKvBlock) : 0;
 #pragma unroll
                         for (int j = 0; j < 2; ++j)
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
                                 const int tok = 2 * t + 8 * j + e;
                                 const uint32_t keep = e ? 0x0000ffffu : 0xffff0000u;
-                                const bool unseen = tok >= most;
+                                const bool unseen = tok >= in_sight;
 #pragma unroll
                                 for (int w = 0; w < G; ++w) {
                                     const bool bad = ((vs[k][j][w] >> 16 * e) & 0x7c00u) == 0x7c00u;
@@ -506,12 +516,14 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < TT; ++k)
+                for (int w = 0; w < G; ++w) {
+                    most[w] = __hmax2(as_h2(vs[0][0][w]), as_h2(vs[0][1][w]));
 #pragma unroll
-                    for (int w = 0; w < G; ++w) large |= vs[k][0][w] | vs[k][1][w];
+                    for (int k = 1; k < TT; ++k) most[w] = __hmax2(most[w], __hmax2(as_h2(vs[k][0][w]), as_h2(vs[k][1][w])));
+                    large |= h2_bits(__hmul2(most[w], unit[w]));
+                }
                 // ---- softmax
                 bool grow = (large & 0x40004000u) != 0;
-                const float slack = kSlack - (float)shift;
                 float top[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -531,24 +543,18 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
                         top[nt][0] = k ? fmaxf(top[nt][0], n0) : n0;
                         top[nt][1] = k ? fmaxf(top[nt][1], n1) : n1;
                     }
-                    grow = grow || top[nt][0] > mx[nt][0] + slack || top[nt][1] > mx[nt][1] + slack;
+                    grow = grow || top[nt][0] > mx[nt][0] + kSlack || top[nt][1] > mx[nt][1] + kSlack;
                 }
                 if (__any_sync(0xffffffffu, grow)) {
-                    int need = 0;   // exponent of the largest finite scale of the blocks
+                    float down[G];
 #pragma unroll
-                    for (int k = 0; k < TT; ++k)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int w = 0; w < G; ++w)
-#pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    const int ex = (int)(vs[k][j][w] >> (16 * e + 10) & 31u) - 15;
-                                    if (ex < 16) need = max(need, ex);
-                                }
-                    need = max((int)__reduce_max_sync(0xffffffffu, (unsigned)need), shift) - shift;
-                    shift += need;
-                    const float fs = (float)shift;
+                    for (int w = 0; w < G; ++w) {
+                        // the largest scale by its bits; an infinity or NaN, and what no fp16 range of values has, asks for nothing
+                        const uint32_t x = h2_bits(most[w]), hi = max(x & 0x7fffu, x >> 16 & 0x7fffu), e = __reduce_max_sync(0xffffffffu, hi) >> 10;
+                        const __half2 was = unit[w];
+                        if (e < 30) unit[w] = __hmin2(was, __half2half2(__ushort_as_half((unsigned short)((30 - e) << 10))));
+                        down[w] = power(exponent_of(unit[w]) - exponent_of(was));
+                    }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float n0 = top[nt][0], n1 = top[nt][1];
@@ -557,11 +563,11 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
                             n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, d));
                             n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, d));
                         }
-                        n0 = fmaxf(n0 + fs, mx[nt][0] + (float)need), n1 = fmaxf(n1 + fs, mx[nt][1] + (float)need);
+                        n0 = fmaxf(n0, mx[nt][0]), n1 = fmaxf(n1, mx[nt][1]);
                         const float r0 = mx[nt][0] == -INFINITY ? 0.f : exp2_approx(mx[nt][0] - n0);
                         const float r1 = mx[nt][1] == -INFINITY ? 0.f : exp2_approx(mx[nt][1] - n1);
                         mx[nt][0] = n0, mx[nt][1] = n1;
-                        rescale(nt, r0, r1);
+                        rescale(nt, r0, r1, down);
                     }
                 }
                 uint32_t b0[TT][NT], b1[TT][NT], r0[TT][NT], r1[TT][NT];   // r: what rounding to fp16 took away, for short contexts
@@ -604,13 +610,13 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
                         const uint32_t x0 = vw[0][w], x1 = vw[1][w], y0 = x0 >> 8, y1 = x1 >> 8;
                         const uint32_t even[4] = {x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u};
                         const uint32_t odd[4] = {y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u};
+                        const __half2 v0 = __hmul2(as_h2(vs[k][0][w]), unit[w]), v1 = __hmul2(as_h2(vs[k][1][w]), unit[w]);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            const uint32_t c0 = h2_bits(__hmul2(as_h2(b0[k][nt]), as_h2(vs[k][0][w]))), c1 = h2_bits(__hmul2(as_h2(b1[k][nt]), as_h2(vs[k][1][w])));
+                            const uint32_t c0 = h2_bits(__hmul2(as_h2(b0[k][nt]), v0)), c1 = h2_bits(__hmul2(as_h2(b1[k][nt]), v1));
                             mma(o[nt][2 * w], even, c0, c1);
                             mma(o[nt][2 * w + 1], odd, c0, c1);
                             if (FINE) {   // P s less its rounded product
-                                const __half2 v0 = as_h2(vs[k][0][w]), v1 = as_h2(vs[k][1][w]);
                                 const uint32_t d0 = h2_bits(__hfma2(as_h2(r0[k][nt]), v0, __hfma2(as_h2(b0[k][nt]), v0, __hneg2(as_h2(c0)))));
                                 const uint32_t d1 = h2_bits(__hfma2(as_h2(r1[k][nt]), v1, __hfma2(as_h2(b1[k][nt]), v1, __hneg2(as_h2(c1)))));
                                 mma(o[nt][2 * w], even, d0, d1);
@@ -641,11 +647,11 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
                 for (int d = 4; d < 32; d *= 2) sum[nt][e] += __shfl_xor_sync(0xffffffffu, sum[nt][e], d);
 #pragma unroll
                 for (int w = 0; w < G; ++w) {
-                    const float m = __shfl_sync(0xffffffffu, om[nt][e], 4 * w + t);
+                    const float m = __shfl_sync(0xffffffffu, om[nt][e], 4 * w + t), back = power(20 - exponent_of(unit[w]));
 #pragma unroll
                     for (int i = 2 * w; i < 2 * w + 2; ++i) {
-                        o[nt][i][e] = fmaf(o[nt][i][e], 0x1p24f, m);
-                        o[nt][i][2 + e] = fmaf(o[nt][i][2 + e], 0x1p20f, m);
+                        o[nt][i][e] = fmaf(o[nt][i][e], 16.f * back, m);
+                        o[nt][i][2 + e] = fmaf(o[nt][i][2 + e], back, m);
                     }
                 }
             }

@@ -90,3 +90,79 @@ def test_prompt_attention_before_products_that_take_tensor_memory(sp, D, heads):
     for _ in range(5):
         assert all(torch.equal(a, b) for a, b in zip(step(False), want))
     assert sp.device_status() == 0
+
+
+def cached(sp, k, v, page=64, capacity=0):
+    """One sequence with keys and values [L, heads, D] in a cache; the page table holds `capacity` tokens at least."""
+    L, heads, D = k.shape
+    pages = -(-L // page)
+    cache = sp.KvCacheInt4(pages, page, heads, D)
+    table = np.full((1, max(pages, -(-capacity // page))), -1, np.int32)
+    table[0, :pages] = np.arange(pages)
+    sp.kv_append(cache, dev(k), dev(v), dev(table), i32(L))
+    return cache, dev(table), i32(L)
+
+
+def held(k, v):
+    return [f(x.astype(np.float64)) for f, x in ((model.entry, k), (model.entry, v), (model.scaled_codes, v))]
+
+
+def one_key_apart(D, heads, spread, length, gap):
+    """q, k, v and a scale: one key's weight is 2^gap times that of each other, about."""
+    rng = np.random.default_rng(int(gap + D + length))
+    k = (rng.standard_normal((length, heads, D)) * 0.05).astype(np.float16)
+    v = (rng.standard_normal((length, heads, D)) * spread).astype(np.float16)
+    q = (rng.standard_normal((1, heads, D)) * 0.1).astype(np.float16)
+    q[0, :, 0], k[:, :, 0] = 1, 1
+    k[length // 3, :, 0] = 16
+    return q, k, v, gap * np.log(2) / 15
+
+
+def relative_attention(q, k, v, scale):
+    """model.attention, with what lies below the fp16 range counted relative to the values: products of weights and scales are taken in
+    units of 1 to 2 times the group's largest scale s (2^-15 if that is more), 2^-32 of the largest weight times 15 of those a key; the
+    output loses 2^-25 below the smallest normal fp16 value."""
+    kk, vv, sc = held(k, v)
+    q = q.astype(np.float64)
+    want, tol = model.attention(q, kk, vv, sc, scale)
+    group = q.shape[1] // kk.shape[1]
+    for h in range(q.shape[1]):
+        z = kk[:, h // group] @ q[:, h].T * scale
+        total = np.exp(z - z.max(0)).sum(0)[:, None]
+        s = np.maximum(sc[:, h // group].max() / 15, 2.0 ** -15)
+        tol[:, h] += len(kk) / total * 15 * 2.0 ** -32 * (2 * s - 1) + 2.0 ** -25 - 2.0 ** -24
+    return want, tol
+
+
+@pytest.mark.parametrize("D,heads", [(64, 2), (128, 1)])
+@pytest.mark.parametrize("spread,length,gap", [(1e-3, 60000, 18), (1e-3, 200000, 19), (1e-4, 60000, 16), (1.0, 60000, 17), (30.0, 60000, 14),
+                                               (1e-3, 300, 9), (3000.0, 9000, 10)])
+def test_small_values_keep_their_bits(sp, D, heads, spread, length, gap):
+    """One key takes the most weight, all others 2^-gap of it, together about as much: what they add to their groups' minima has to
+    survive whatever the values' magnitude."""
+    q, k, v, scale = one_key_apart(D, heads, spread, length, gap)
+    cache, table, lens = cached(sp, k, v)
+    got = sp.kv_attention(dev(q), cache, table, lens, scale=scale).cpu().numpy().astype(np.float64)
+    want, tol = relative_attention(q, k, v, scale)
+    assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
+    assert sp.device_status() == 0
+
+
+def test_groups_of_very_different_magnitude(sp):
+    """Groups of one head 2^12 apart, and scales of one group that grow along the context."""
+    q, k, v, scale = one_key_apart(128, 1, 1.0, 30000, 15)
+    v = (v.astype(np.float64) * np.repeat([1e-3, 4.0, 30.0, 3e-4], 32)).astype(np.float16)
+    cache, table, lens = cached(sp, k, v)
+    got = sp.kv_attention(dev(q), cache, table, lens, scale=scale).cpu().numpy().astype(np.float64)
+    for g in range(4):
+        cut = slice(32 * g, 32 * g + 32)
+        one = np.zeros_like(v)
+        one[:, :, cut] = v[:, :, cut]
+        want, tol = relative_attention(q, k, one, scale)
+        assert np.all(np.abs(got - want)[:, :, cut] <= tol[:, :, cut]), g
+    v = (v.astype(np.float64) * (2.0 ** (12 * np.arange(30000) / 30000 - 8))[:, None, None]).astype(np.float16)
+    cache, table, lens = cached(sp, k, v)
+    got = sp.kv_attention(dev(q), cache, table, lens, scale=scale).cpu().numpy().astype(np.float64)
+    want, tol = relative_attention(q, k, v, scale)
+    assert np.all(np.abs(got - want) <= tol)
+    assert sp.device_status() == 0
