@@ -18,7 +18,7 @@
 //            so that the products, too, span 2^-31 .. 1 relative to the largest (down to scales of 2^-15, whose values are next to the
 //            smallest of fp16); when a larger one comes, the group's accumulators are scaled down.  The roundings of P and of P s average out over many keys; over
 //            few they would make outputs half again as far from the exact ones (five keys: 3.0e-4, the rounding of the output alone
-//            2.0e-4).  Where no context can have more than 128 tokens, a second product is taken with what the roundings took away.
+//            2.0e-4).  Row tiles whose first row sees at most 128 keys take a second product with what the roundings took away.
 //
 // Work: the context is cut in units of 128 tokens (four warps, two 16-token blocks each); all units of all (sequence, key
 // head, row tile) are laid end to end and every thread block takes an equal share, found from the lengths on the device.
@@ -193,9 +193,297 @@ struct Smem {
     int ok[kWarps][kStages];    // blocks of the step that are there
 };
 
-// FINE: no context has more than one unit, and the second product is taken (9.0 us against 8.7: 25 sequences of 5 tokens, 12 heads).  A
-// kernel of its own: one that could do either took 10 % longer over long contexts.
+// What a warp has of a row tile.
+template <int D, int NT>
+struct Sums {
+    float o[NT][D / 16][4];    // sum of P s c in units of the group, rows of the high nibbles 2^-20, of the low ones 2^-24 of it
+    float om[NT][4];           // sum of P m, row = group
+    float mx[NT][2], sum[NT][2];
+    __half2 unit[D / kKvGroup];   // 2^-e of a group, e the exponent of its largest scale so far, -15 at least
+};
+// A warp's two blocks of a unit and how the tile's rows see them.
+struct Unit {
+    const uint8_t* blocks;
+    int there, pos;            // bits of the blocks that are there, first token
+    int kmin, kmax;            // keys that the first and the last row see
+    int before, row0, group;   // row r of the tile sees before + (row0 + r) / group keys, if that is positive
+};
+// FINE: the second product is taken.
 template <int D, int NT, bool FINE>
+__device__ __forceinline__ void attend(Sums<D, NT>& x, const Smem<D, NT>& sm, const Unit& u)
+{
+    using L = KvLayout<D>;
+    constexpr int G = L::kGroups, MT = D / 16;
+    const int lane = threadIdx.x & 31, g = lane / 4, t = lane % 4, there = u.there, pos0 = u.pos;
+    const uint8_t* blk0 = u.blocks;
+    auto &o = x.o;
+    auto &om = x.om;
+    auto &mx = x.mx, &sum = x.sum;
+    auto &unit = x.unit;
+    auto rescale = [&](int nt, float r0, float r1, const float (&down)[G]) {   // rows by r0, r1, groups by down
+        sum[nt][0] *= r0, sum[nt][1] *= r1;
+        om[nt][0] *= r0, om[nt][1] *= r1;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const float d0 = r0 * down[i / 2], d1 = r1 * down[i / 2];
+            o[nt][i][0] *= d0, o[nt][i][1] *= d1, o[nt][i][2] *= d0, o[nt][i][3] *= d1;
+        }
+    };
+        // some row does not see all of these tokens, or a block is not there: it counts as unseen
+        const bool edge = pos0 + TT * kKvBlock > u.kmin || there != (1 << TT) - 1;
+        auto seen_by = [&](int row, int k) {   // tokens of block k that a row of the tile sees
+            return (there >> k & 1) ? max(u.before + (u.row0 + row) / u.group, 0) - (pos0 + k * kKvBlock) : 0;
+        };
+        // ---- scores.  keys: one word of codes per group for tokens g and g + 8
+        uint32_t k0[TT][G], k1[TT][G], p0[TT][G], p1[TT][G];
+#pragma unroll
+        for (int k = 0; k < TT; ++k) {
+            const uint32_t* kc = reinterpret_cast<const uint32_t*>(blk0 + k * L::kBlockBytes + L::kKCodes);
+            const uint32_t* kp = reinterpret_cast<const uint32_t*>(blk0 + k * L::kBlockBytes + L::kKParams);
+            if constexpr (G == 4) {
+                *reinterpret_cast<uint4*>(k0[k]) = *reinterpret_cast<const uint4*>(kc + g * 16 + t * 4);
+                *reinterpret_cast<uint4*>(k1[k]) = *reinterpret_cast<const uint4*>(kc + (g + 8) * 16 + t * 4);
+                *reinterpret_cast<uint4*>(p0[k]) = *reinterpret_cast<const uint4*>(kp + g * 4);
+                *reinterpret_cast<uint4*>(p1[k]) = *reinterpret_cast<const uint4*>(kp + (g + 8) * 4);
+            } else {
+                *reinterpret_cast<uint2*>(k0[k]) = *reinterpret_cast<const uint2*>(kc + g * 8 + t * 2);
+                *reinterpret_cast<uint2*>(k1[k]) = *reinterpret_cast<const uint2*>(kc + (g + 8) * 8 + t * 2);
+                *reinterpret_cast<uint2*>(p0[k]) = *reinterpret_cast<const uint2*>(kp + g * 2);
+                *reinterpret_cast<uint2*>(p1[k]) = *reinterpret_cast<const uint2*>(kp + (g + 8) * 2);
+            }
+        }
+        float z[TT][NT][4];
+        {
+            // minima of the lane's two groups, as an operand (lanes without a group: zero)
+            uint32_t qs[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) qs[nt] = sm.qsum[nt][lane];
+#pragma unroll
+            for (int k = 0; k < TT; ++k) {
+                uint32_t am[4] = {0u, 0u, 0u, 0u};
+                if constexpr (G == 4) {
+                    const bool odd = t & 1;
+                    am[0] = __byte_perm(odd ? p0[k][2] : p0[k][0], odd ? p0[k][3] : p0[k][1], 0x7632);
+                    am[1] = __byte_perm(odd ? p1[k][2] : p1[k][0], odd ? p1[k][3] : p1[k][1], 0x7632);
+                } else if (!(t & 1)) {
+                    am[0] = __byte_perm(p0[k][0], p0[k][1], 0x7632);
+                    am[1] = __byte_perm(p1[k][0], p1[k][1], 0x7632);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    z[k][nt][0] = z[k][nt][1] = z[k][nt][2] = z[k][nt][3] = 0.f;
+                    mma(z[k][nt], am, qs[nt], 0u);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) z[k][nt][i] *= 0x1p-24f;
+                }
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < G; ++w) {
+            uint2 ql[NT], qh[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) ql[nt] = sm.qfrag[nt][2 * w][lane], qh[nt] = sm.qfrag[nt][2 * w + 1][lane];
+#pragma unroll
+            for (int k = 0; k < TT; ++k) {
+                const uint32_t u = k0[k][w], v = k1[k][w], us = u >> 8, vs = v >> 8;
+                const uint32_t alow[4] = {u & 0x000f000fu, v & 0x000f000fu, us & 0x000f000fu, vs & 0x000f000fu};
+                const uint32_t ahigh[4] = {u & 0x00f000f0u, v & 0x00f000f0u, us & 0x00f000f0u, vs & 0x00f000f0u};
+                const float s0 = __low2float(as_h2(p0[k][w])), s1 = __low2float(as_h2(p1[k][w]));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma(acc, alow, ql[nt].x, ql[nt].y);
+                    mma(acc, ahigh, qh[nt].x, qh[nt].y);
+                    z[k][nt][0] = fmaf(s0, acc[0], z[k][nt][0]);
+                    z[k][nt][1] = fmaf(s0, acc[1], z[k][nt][1]);
+                    z[k][nt][2] = fmaf(s1, acc[2], z[k][nt][2]);
+                    z[k][nt][3] = fmaf(s1, acc[3], z[k][nt][3]);
+                }
+            }
+        }
+        // ---- scales of the values of tokens 2t, 2t+1 (j = 0) and 2t+8, 2t+9 (j = 1), all groups; minima of group g
+        uint32_t vs[TT][2][G], vm[TT][2], large = 0;   // large: bit 14 of an fp16 value, 2 or more
+        __half2 most[G];   // of a group's scales here
+#pragma unroll
+        for (int k = 0; k < TT; ++k) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t* vp = reinterpret_cast<const uint32_t*>(blk0 + k * L::kBlockBytes + L::kVParams) + (t + 4 * j) * 2 * G;
+                if constexpr (G == 4) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(vp), w = *reinterpret_cast<const uint4*>(vp + 4);
+                    vs[k][j][0] = u.x, vs[k][j][1] = u.z, vs[k][j][2] = w.x, vs[k][j][3] = w.z;
+                } else {
+                    const uint4 u = *reinterpret_cast<const uint4*>(vp);
+                    vs[k][j][0] = u.x, vs[k][j][1] = u.z;
+                }
+                vm[k][j] = g < G ? vp[2 * (g & (G - 1)) + 1] : 0u;
+            }
+        }
+        if (edge) {
+            // Tokens that no row sees count as zero, whatever the page holds there.  A token that some rows see and
+            // others do not may be NaN for the first and must not touch the others: it is taken out of the products
+            // and put back row by row.
+#pragma unroll
+            for (int k = 0; k < TT; ++k) {
+                uint32_t nan_tokens[G] = {};
+                bool any = false;
+                const int in_sight = (there >> k & 1) ? u.kmax - (pos0 + k * kKvBlock) : 0;
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int tok = 2 * t + 8 * j + e;
+                        const uint32_t keep = e ? 0x0000ffffu : 0xffff0000u;
+                        const bool unseen = tok >= in_sight;
+#pragma unroll
+                        for (int w = 0; w < G; ++w) {
+                            const bool bad = ((vs[k][j][w] >> 16 * e) & 0x7c00u) == 0x7c00u;
+                            if (bad && !unseen) nan_tokens[w] |= 1u << tok, any = true;
+                            if (bad || unseen) vs[k][j][w] &= keep;
+                        }
+                        if (unseen || ((vm[k][j] >> 16 * e) & 0x7c00u) == 0x7c00u) vm[k][j] &= keep;
+                    }
+                if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+                    for (int w = 0; w < G; ++w) {   // the quad holds all 16 tokens
+                        nan_tokens[w] |= __shfl_xor_sync(0xffffffffu, nan_tokens[w], 1);
+                        nan_tokens[w] |= __shfl_xor_sync(0xffffffffu, nan_tokens[w], 2);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int seen = seen_by(nt * 8 + 2 * t + e, k);
+                            const uint32_t mask = seen >= 16 ? 0xffffu : seen <= 0 ? 0u : (1u << seen) - 1;
+#pragma unroll
+                            for (int i = 0; i < MT; ++i)
+                                if (nan_tokens[i / 2] & mask) o[nt][i][e] = o[nt][i][2 + e] = __int_as_float(0x7fffffff);
+                        }
+                }
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < G; ++w) {
+            most[w] = __hmax2(as_h2(vs[0][0][w]), as_h2(vs[0][1][w]));
+#pragma unroll
+            for (int k = 1; k < TT; ++k) most[w] = __hmax2(most[w], __hmax2(as_h2(vs[k][0][w]), as_h2(vs[k][1][w])));
+            large |= h2_bits(__hmul2(most[w], unit[w]));
+        }
+        // ---- softmax
+        bool grow = (large & 0x40004000u) != 0;
+        float top[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const float2 f = *reinterpret_cast<const float2*>(&sm.factor[nt][2 * t]);
+#pragma unroll
+            for (int k = 0; k < TT; ++k) {
+                z[k][nt][0] *= f.x, z[k][nt][2] *= f.x;
+                z[k][nt][1] *= f.y, z[k][nt][3] *= f.y;
+                if (edge) {
+                    const int s0 = seen_by(nt * 8 + 2 * t, k), s1 = seen_by(nt * 8 + 2 * t + 1, k);
+                    if (g >= s0) z[k][nt][0] = -INFINITY;
+                    if (g >= s1) z[k][nt][1] = -INFINITY;
+                    if (g + 8 >= s0) z[k][nt][2] = -INFINITY;
+                    if (g + 8 >= s1) z[k][nt][3] = -INFINITY;
+                }
+                const float n0 = fmaxf(z[k][nt][0], z[k][nt][2]), n1 = fmaxf(z[k][nt][1], z[k][nt][3]);
+                top[nt][0] = k ? fmaxf(top[nt][0], n0) : n0;
+                top[nt][1] = k ? fmaxf(top[nt][1], n1) : n1;
+            }
+            grow = grow || top[nt][0] > mx[nt][0] + kSlack || top[nt][1] > mx[nt][1] + kSlack;
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+            float down[G];
+#pragma unroll
+            for (int w = 0; w < G; ++w) {
+                // the largest scale by its bits; an infinity or NaN, and what no fp16 range of values has, asks for nothing
+                const uint32_t x = h2_bits(most[w]), hi = max(x & 0x7fffu, x >> 16 & 0x7fffu), e = __reduce_max_sync(0xffffffffu, hi) >> 10;
+                const __half2 was = unit[w];
+                if (e < 30) unit[w] = __hmin2(was, __half2half2(__ushort_as_half((unsigned short)((30 - e) << 10))));
+                down[w] = power(exponent_of(unit[w]) - exponent_of(was));
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float n0 = top[nt][0], n1 = top[nt][1];
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) {
+                    n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, d));
+                    n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, d));
+                }
+                n0 = fmaxf(n0, mx[nt][0]), n1 = fmaxf(n1, mx[nt][1]);
+                const float r0 = mx[nt][0] == -INFINITY ? 0.f : exp2_approx(mx[nt][0] - n0);
+                const float r1 = mx[nt][1] == -INFINITY ? 0.f : exp2_approx(mx[nt][1] - n1);
+                mx[nt][0] = n0, mx[nt][1] = n1;
+                rescale(nt, r0, r1, down);
+            }
+        }
+        uint32_t b0[TT][NT], b1[TT][NT], r0[TT][NT], r1[TT][NT];   // r: what rounding to fp16 took away, for short contexts
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const float m0 = (mx[nt][0] == -INFINITY ? 0.f : mx[nt][0]) - kShift;
+            const float m1 = (mx[nt][1] == -INFINITY ? 0.f : mx[nt][1]) - kShift;
+#pragma unroll
+            for (int k = 0; k < TT; ++k) {
+                const float w0 = exp2_approx(z[k][nt][0] - m0), w1 = exp2_approx(z[k][nt][1] - m1);
+                const float w2 = exp2_approx(z[k][nt][2] - m0), w3 = exp2_approx(z[k][nt][3] - m1);
+                sum[nt][0] += w0 + w2;
+                sum[nt][1] += w1 + w3;
+                b0[k][nt] = transpose8x8(h2_bits(__floats2half2_rn(w0, w1)));
+                b1[k][nt] = transpose8x8(h2_bits(__floats2half2_rn(w2, w3)));
+                if constexpr (FINE) {
+                    r0[k][nt] = transpose8x8(h2_bits(__floats2half2_rn(w0 - __half2float(__float2half_rn(w0)), w1 - __half2float(__float2half_rn(w1)))));
+                    r1[k][nt] = transpose8x8(h2_bits(__floats2half2_rn(w2 - __half2float(__float2half_rn(w2)), w3 - __half2float(__float2half_rn(w3)))));
+                }
+            }
+        }
+        // ---- weighted values
+#pragma unroll
+        for (int k = 0; k < TT; ++k) {
+            uint32_t vw[2][G];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint8_t* vc = blk0 + k * L::kBlockBytes + L::kVCodes + j * 4 * D + lane * (D / 8);
+                if constexpr (G == 4) *reinterpret_cast<uint4*>(vw[j]) = *reinterpret_cast<const uint4*>(vc);
+                else *reinterpret_cast<uint2*>(vw[j]) = *reinterpret_cast<const uint2*>(vc);
+            }
+            const uint32_t am[4] = {vm[k][0], 0u, vm[k][1], 0u};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                mma(om[nt], am, b0[k][nt], b1[k][nt]);
+                if constexpr (FINE) mma(om[nt], am, r0[k][nt], r1[k][nt]);
+            }
+#pragma unroll
+            for (int w = 0; w < G; ++w) {
+                const uint32_t x0 = vw[0][w], x1 = vw[1][w], y0 = x0 >> 8, y1 = x1 >> 8;
+                const uint32_t even[4] = {x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u};
+                const uint32_t odd[4] = {y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u};
+                const __half2 v0 = __hmul2(as_h2(vs[k][0][w]), unit[w]), v1 = __hmul2(as_h2(vs[k][1][w]), unit[w]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uint32_t c0 = h2_bits(__hmul2(as_h2(b0[k][nt]), v0)), c1 = h2_bits(__hmul2(as_h2(b1[k][nt]), v1));
+                    mma(o[nt][2 * w], even, c0, c1);
+                    mma(o[nt][2 * w + 1], odd, c0, c1);
+                    if constexpr (FINE) {   // P s less its rounded product
+                        const uint32_t d0 = h2_bits(__hfma2(as_h2(r0[k][nt]), v0, __hfma2(as_h2(b0[k][nt]), v0, __hneg2(as_h2(c0)))));
+                        const uint32_t d1 = h2_bits(__hfma2(as_h2(r1[k][nt]), v1, __hfma2(as_h2(b1[k][nt]), v1, __hneg2(as_h2(c1)))));
+                        mma(o[nt][2 * w], even, d0, d1);
+                        mma(o[nt][2 * w + 1], odd, d0, d1);
+                    }
+                }
+            }
+        }
+}
+// A function of its own, on a copy of the sums: in the kernel's loop, as a branch or as a second loop, it made long contexts up to 10 %
+// slower by the registers it took (8 sequences of up to 1087 tokens, 40 heads: 25.2 us as a second loop, 23.8 so, 23.2 without).
+template <int D, int NT>
+__device__ __noinline__ void attend_fine(Sums<D, NT>& x, const Smem<D, NT>& sm, const Unit& u)
+{
+    attend<D, NT, true>(x, sm, u);
+}
+
+// SHORT: the table holds no more than one unit, so that every row tile is fine: no call for it (9.0 us against 10.2: 25 sequences of 5
+// tokens, 12 heads).  The arithmetic is the same.
+template <int D, int NT, bool SHORT>
 __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_split_kernel(KvAttnArgs a, int whole_tiles, int* status)
 {
     using L = KvLayout<D>;
@@ -348,10 +636,11 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
         }
         __syncthreads();
 
-        float o[NT][MT][4];      // sum of P s c, rows of the high nibbles 2^-20, of the low ones 2^-24 of it
-        float om[NT][4];         // sum of P m, row = group
-        float mx[NT][2], sum[NT][2];
-        __half2 unit[G];         // 2^-e of a group, e the exponent of its largest scale so far, -15 at least
+        Sums<D, NT> x;
+        auto &o = x.o;
+        auto &om = x.om;
+        auto &mx = x.mx, &sum = x.sum;
+        auto &unit = x.unit;
 #pragma unroll
         for (int w = 0; w < G; ++w) unit[w] = __half2half2(__ushort_as_half((unsigned short)(30 << 10)));
 #pragma unroll
@@ -362,16 +651,8 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
             mx[nt][0] = mx[nt][1] = -INFINITY;
             sum[nt][0] = sum[nt][1] = 0.f;
         }
-        auto rescale = [&](int nt, float r0, float r1, const float (&down)[G]) {   // rows by r0, r1, groups by down
-            sum[nt][0] *= r0, sum[nt][1] *= r1;
-            om[nt][0] *= r0, om[nt][1] *= r1;
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const float d0 = r0 * down[i / 2], d1 = r1 * down[i / 2];
-                o[nt][i][0] *= d0, o[nt][i][1] *= d1, o[nt][i][2] *= d0, o[nt][i][3] *= d1;
-            }
-        };
-
+        // by what the rows see and not by how wide the table is
+        const bool fine = seg.kmin <= kUnit;
         int pos0 = ((seg.begin - seg.tile_begin) * kWarps + warp) * (kKvBlock * TT);
         for (int left = seg.end - seg.begin; left > 0; --left, pos0 += kUnit) {
             if (alive) {
@@ -381,249 +662,16 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
             }
             const int there = alive ? sm.ok[warp][stage] : 0;
             if (there) {
-                const uint8_t* blk0 = sm.ring[warp][stage];
-                // some row does not see all of these tokens, or a block is not there: it counts as unseen
-                const bool edge = pos0 + TT * kKvBlock > seg.kmin || there != (1 << TT) - 1;
-                auto seen_by = [&](int row, int k) {   // tokens of block k that a row of the tile sees
-                    return (there >> k & 1) ? visible_keys(s, seg.rt * ROWS + row, group) - (pos0 + k * kKvBlock) : 0;
-                };
-                // ---- scores.  keys: one word of codes per group for tokens g and g + 8
-                uint32_t k0[TT][G], k1[TT][G], p0[TT][G], p1[TT][G];
-#pragma unroll
-                for (int k = 0; k < TT; ++k) {
-                    const uint32_t* kc = reinterpret_cast<const uint32_t*>(blk0 + k * L::kBlockBytes + L::kKCodes);
-                    const uint32_t* kp = reinterpret_cast<const uint32_t*>(blk0 + k * L::kBlockBytes + L::kKParams);
-                    if constexpr (G == 4) {
-                        *reinterpret_cast<uint4*>(k0[k]) = *reinterpret_cast<const uint4*>(kc + g * 16 + t * 4);
-                        *reinterpret_cast<uint4*>(k1[k]) = *reinterpret_cast<const uint4*>(kc + (g + 8) * 16 + t * 4);
-                        *reinterpret_cast<uint4*>(p0[k]) = *reinterpret_cast<const uint4*>(kp + g * 4);
-                        *reinterpret_cast<uint4*>(p1[k]) = *reinterpret_cast<const uint4*>(kp + (g + 8) * 4);
-                    } else {
-                        *reinterpret_cast<uint2*>(k0[k]) = *reinterpret_cast<const uint2*>(kc + g * 8 + t * 2);
-                        *reinterpret_cast<uint2*>(k1[k]) = *reinterpret_cast<const uint2*>(kc + (g + 8) * 8 + t * 2);
-                        *reinterpret_cast<uint2*>(p0[k]) = *reinterpret_cast<const uint2*>(kp + g * 2);
-                        *reinterpret_cast<uint2*>(p1[k]) = *reinterpret_cast<const uint2*>(kp + (g + 8) * 2);
-                    }
-                }
-                float z[TT][NT][4];
-                {
-                    // minima of the lane's two groups, as an operand (lanes without a group: zero)
-                    uint32_t qs[NT];
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) qs[nt] = sm.qsum[nt][lane];
-#pragma unroll
-                    for (int k = 0; k < TT; ++k) {
-                        uint32_t am[4] = {0u, 0u, 0u, 0u};
-                        if constexpr (G == 4) {
-                            const bool odd = t & 1;
-                            am[0] = __byte_perm(odd ? p0[k][2] : p0[k][0], odd ? p0[k][3] : p0[k][1], 0x7632);
-                            am[1] = __byte_perm(odd ? p1[k][2] : p1[k][0], odd ? p1[k][3] : p1[k][1], 0x7632);
-                        } else if (!(t & 1)) {
-                            am[0] = __byte_perm(p0[k][0], p0[k][1], 0x7632);
-                            am[1] = __byte_perm(p1[k][0], p1[k][1], 0x7632);
-                        }
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            z[k][nt][0] = z[k][nt][1] = z[k][nt][2] = z[k][nt][3] = 0.f;
-                            mma(z[k][nt], am, qs[nt], 0u);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) z[k][nt][i] *= 0x1p-24f;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int w = 0; w < G; ++w) {
-                    uint2 ql[NT], qh[NT];
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) ql[nt] = sm.qfrag[nt][2 * w][lane], qh[nt] = sm.qfrag[nt][2 * w + 1][lane];
-#pragma unroll
-                    for (int k = 0; k < TT; ++k) {
-                        const uint32_t u = k0[k][w], v = k1[k][w], us = u >> 8, vs = v >> 8;
-                        const uint32_t alow[4] = {u & 0x000f000fu, v & 0x000f000fu, us & 0x000f000fu, vs & 0x000f000fu};
-                        const uint32_t ahigh[4] = {u & 0x00f000f0u, v & 0x00f000f0u, us & 0x00f000f0u, vs & 0x00f000f0u};
-                        const float s0 = __low2float(as_h2(p0[k][w])), s1 = __low2float(as_h2(p1[k][w]));
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma(acc, alow, ql[nt].x, ql[nt].y);
-                            mma(acc, ahigh, qh[nt].x, qh[nt].y);
-                            z[k][nt][0] = fmaf(s0, acc[0], z[k][nt][0]);
-                            z[k][nt][1] = fmaf(s0, acc[1], z[k][nt][1]);
-                            z[k][nt][2] = fmaf(s1, acc[2], z[k][nt][2]);
-                            z[k][nt][3] = fmaf(s1, acc[3], z[k][nt][3]);
-                        }
-                    }
-                }
-                // ---- scales of the values of tokens 2t, 2t+1 (j = 0) and 2t+8, 2t+9 (j = 1), all groups; minima of group g
-                uint32_t vs[TT][2][G], vm[TT][2], large = 0;   // large: bit 14 of an fp16 value, 2 or more
-                __half2 most[G];   // of a group's scales here
-#pragma unroll
-                for (int k = 0; k < TT; ++k) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const uint32_t* vp = reinterpret_cast<const uint32_t*>(blk0 + k * L::kBlockBytes + L::kVParams) + (t + 4 * j) * 2 * G;
-                        if constexpr (G == 4) {
-                            const uint4 u = *reinterpret_cast<const uint4*>(vp), w = *reinterpret_cast<const uint4*>(vp + 4);
-                            vs[k][j][0] = u.x, vs[k][j][1] = u.z, vs[k][j][2] = w.x, vs[k][j][3] = w.z;
-                        } else {
-                            const uint4 u = *reinterpret_cast<const uint4*>(vp);
-                            vs[k][j][0] = u.x, vs[k][j][1] = u.z;
-                        }
-                        vm[k][j] = g < G ? vp[2 * (g & (G - 1)) + 1] : 0u;
-                    }
-                }
-                if (edge) {
-                    // Tokens that no row sees count as zero, whatever the page holds there.  A token that some rows see and
-                    // others do not may be NaN for the first and must not touch the others: it is taken out of the products
-                    // and put back row by row.
-#pragma unroll
-                    for (int k = 0; k < TT; ++k) {
-                        uint32_t nan_tokens[G] = {};
-                        bool any = false;
-                        const int in_sight = (there >> k & 1) ? seg.kmax - (pos0 + k * kKvBlock) : 0;
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int tok = 2 * t + 8 * j + e;
-                                const uint32_t keep = e ? 0x0000ffffu : 0xffff0000u;
-                                const bool unseen = tok >= in_sight;
-#pragma unroll
-                                for (int w = 0; w < G; ++w) {
-                                    const bool bad = ((vs[k][j][w] >> 16 * e) & 0x7c00u) == 0x7c00u;
-                                    if (bad && !unseen) nan_tokens[w] |= 1u << tok, any = true;
-                                    if (bad || unseen) vs[k][j][w] &= keep;
-                                }
-                                if (unseen || ((vm[k][j] >> 16 * e) & 0x7c00u) == 0x7c00u) vm[k][j] &= keep;
-                            }
-                        if (__any_sync(0xffffffffu, any)) {
-#pragma unroll
-                            for (int w = 0; w < G; ++w) {   // the quad holds all 16 tokens
-                                nan_tokens[w] |= __shfl_xor_sync(0xffffffffu, nan_tokens[w], 1);
-                                nan_tokens[w] |= __shfl_xor_sync(0xffffffffu, nan_tokens[w], 2);
-                            }
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    const int seen = seen_by(nt * 8 + 2 * t + e, k);
-                                    const uint32_t mask = seen >= 16 ? 0xffffu : seen <= 0 ? 0u : (1u << seen) - 1;
-#pragma unroll
-                                    for (int i = 0; i < MT; ++i)
-                                        if (nan_tokens[i / 2] & mask) o[nt][i][e] = o[nt][i][2 + e] = __int_as_float(0x7fffffff);
-                                }
-                        }
-                    }
-                }
-#pragma unroll
-                for (int w = 0; w < G; ++w) {
-                    most[w] = __hmax2(as_h2(vs[0][0][w]), as_h2(vs[0][1][w]));
-#pragma unroll
-                    for (int k = 1; k < TT; ++k) most[w] = __hmax2(most[w], __hmax2(as_h2(vs[k][0][w]), as_h2(vs[k][1][w])));
-                    large |= h2_bits(__hmul2(most[w], unit[w]));
-                }
-                // ---- softmax
-                bool grow = (large & 0x40004000u) != 0;
-                float top[NT][2];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const float2 f = *reinterpret_cast<const float2*>(&sm.factor[nt][2 * t]);
-#pragma unroll
-                    for (int k = 0; k < TT; ++k) {
-                        z[k][nt][0] *= f.x, z[k][nt][2] *= f.x;
-                        z[k][nt][1] *= f.y, z[k][nt][3] *= f.y;
-                        if (edge) {
-                            const int s0 = seen_by(nt * 8 + 2 * t, k), s1 = seen_by(nt * 8 + 2 * t + 1, k);
-                            if (g >= s0) z[k][nt][0] = -INFINITY;
-                            if (g >= s1) z[k][nt][1] = -INFINITY;
-                            if (g + 8 >= s0) z[k][nt][2] = -INFINITY;
-                            if (g + 8 >= s1) z[k][nt][3] = -INFINITY;
-                        }
-                        const float n0 = fmaxf(z[k][nt][0], z[k][nt][2]), n1 = fmaxf(z[k][nt][1], z[k][nt][3]);
-                        top[nt][0] = k ? fmaxf(top[nt][0], n0) : n0;
-                        top[nt][1] = k ? fmaxf(top[nt][1], n1) : n1;
-                    }
-                    grow = grow || top[nt][0] > mx[nt][0] + kSlack || top[nt][1] > mx[nt][1] + kSlack;
-                }
-                if (__any_sync(0xffffffffu, grow)) {
-                    float down[G];
-#pragma unroll
-                    for (int w = 0; w < G; ++w) {
-                        // the largest scale by its bits; an infinity or NaN, and what no fp16 range of values has, asks for nothing
-                        const uint32_t x = h2_bits(most[w]), hi = max(x & 0x7fffu, x >> 16 & 0x7fffu), e = __reduce_max_sync(0xffffffffu, hi) >> 10;
-                        const __half2 was = unit[w];
-                        if (e < 30) unit[w] = __hmin2(was, __half2half2(__ushort_as_half((unsigned short)((30 - e) << 10))));
-                        down[w] = power(exponent_of(unit[w]) - exponent_of(was));
-                    }
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float n0 = top[nt][0], n1 = top[nt][1];
-#pragma unroll
-                        for (int d = 4; d < 32; d *= 2) {
-                            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, d));
-                            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, d));
-                        }
-                        n0 = fmaxf(n0, mx[nt][0]), n1 = fmaxf(n1, mx[nt][1]);
-                        const float r0 = mx[nt][0] == -INFINITY ? 0.f : exp2_approx(mx[nt][0] - n0);
-                        const float r1 = mx[nt][1] == -INFINITY ? 0.f : exp2_approx(mx[nt][1] - n1);
-                        mx[nt][0] = n0, mx[nt][1] = n1;
-                        rescale(nt, r0, r1, down);
-                    }
-                }
-                uint32_t b0[TT][NT], b1[TT][NT], r0[TT][NT], r1[TT][NT];   // r: what rounding to fp16 took away, for short contexts
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const float m0 = (mx[nt][0] == -INFINITY ? 0.f : mx[nt][0]) - kShift;
-                    const float m1 = (mx[nt][1] == -INFINITY ? 0.f : mx[nt][1]) - kShift;
-#pragma unroll
-                    for (int k = 0; k < TT; ++k) {
-                        const float w0 = exp2_approx(z[k][nt][0] - m0), w1 = exp2_approx(z[k][nt][1] - m1);
-                        const float w2 = exp2_approx(z[k][nt][2] - m0), w3 = exp2_approx(z[k][nt][3] - m1);
-                        sum[nt][0] += w0 + w2;
-                        sum[nt][1] += w1 + w3;
-                        b0[k][nt] = transpose8x8(h2_bits(__floats2half2_rn(w0, w1)));
-                        b1[k][nt] = transpose8x8(h2_bits(__floats2half2_rn(w2, w3)));
-                        if (FINE) {
-                            r0[k][nt] = transpose8x8(h2_bits(__floats2half2_rn(w0 - __half2float(__float2half_rn(w0)), w1 - __half2float(__float2half_rn(w1)))));
-                            r1[k][nt] = transpose8x8(h2_bits(__floats2half2_rn(w2 - __half2float(__float2half_rn(w2)), w3 - __half2float(__float2half_rn(w3)))));
-                        }
-                    }
-                }
-                // ---- weighted values
-#pragma unroll
-                for (int k = 0; k < TT; ++k) {
-                    uint32_t vw[2][G];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const uint8_t* vc = blk0 + k * L::kBlockBytes + L::kVCodes + j * 4 * D + lane * (D / 8);
-                        if constexpr (G == 4) *reinterpret_cast<uint4*>(vw[j]) = *reinterpret_cast<const uint4*>(vc);
-                        else *reinterpret_cast<uint2*>(vw[j]) = *reinterpret_cast<const uint2*>(vc);
-                    }
-                    const uint32_t am[4] = {vm[k][0], 0u, vm[k][1], 0u};
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma(om[nt], am, b0[k][nt], b1[k][nt]);
-                        if (FINE) mma(om[nt], am, r0[k][nt], r1[k][nt]);
-                    }
-#pragma unroll
-                    for (int w = 0; w < G; ++w) {
-                        const uint32_t x0 = vw[0][w], x1 = vw[1][w], y0 = x0 >> 8, y1 = x1 >> 8;
-                        const uint32_t even[4] = {x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u};
-                        const uint32_t odd[4] = {y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u};
-                        const __half2 v0 = __hmul2(as_h2(vs[k][0][w]), unit[w]), v1 = __hmul2(as_h2(vs[k][1][w]), unit[w]);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            const uint32_t c0 = h2_bits(__hmul2(as_h2(b0[k][nt]), v0)), c1 = h2_bits(__hmul2(as_h2(b1[k][nt]), v1));
-                            mma(o[nt][2 * w], even, c0, c1);
-                            mma(o[nt][2 * w + 1], odd, c0, c1);
-                            if (FINE) {   // P s less its rounded product
-                                const uint32_t d0 = h2_bits(__hfma2(as_h2(r0[k][nt]), v0, __hfma2(as_h2(b0[k][nt]), v0, __hneg2(as_h2(c0)))));
-                                const uint32_t d1 = h2_bits(__hfma2(as_h2(r1[k][nt]), v1, __hfma2(as_h2(b1[k][nt]), v1, __hneg2(as_h2(c1)))));
-                                mma(o[nt][2 * w], even, d0, d1);
-                                mma(o[nt][2 * w + 1], odd, d0, d1);
-                            }
-                        }
-                    }
+                const Unit u{sm.ring[warp][stage], there, pos0, seg.kmin, seg.kmax, s.len - s.qlen + 1, seg.rt * ROWS, group};
+                if constexpr (SHORT) {
+                    attend<D, NT, true>(x, sm, u);
+                } else if (fine) {
+                    Sums<D, NT> copy = x;
+                    const Unit at = u;
+                    attend_fine<D, NT>(copy, sm, at);
+                    x = copy;
+                } else {
+                    attend<D, NT, false>(x, sm, u);
                 }
             }
             __syncwarp();
@@ -825,7 +873,7 @@ int sm_count()
 
 
 // Thread blocks that fit on the device at once (shared memory and registers).
-template <int D, int NT, bool FINE>
+template <int D, int NT, bool SHORT>
 cudaError_t prepare(int* ctas)
 {
     static int cached[64] = {};
@@ -834,10 +882,10 @@ cudaError_t prepare(int* ctas)
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!cached[dev]) {
-        e = cudaFuncSetAttribute(kv_attention_split_kernel<D, NT, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D, NT>));
+        e = cudaFuncSetAttribute(kv_attention_split_kernel<D, NT, SHORT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D, NT>));
         int n = 0;
         if (e == cudaSuccess)
-            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv_attention_split_kernel<D, NT, FINE>, 32 * kWarps, sizeof(Smem<D, NT>));
+            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv_attention_split_kernel<D, NT, SHORT>, 32 * kWarps, sizeof(Smem<D, NT>));
         if (e != cudaSuccess) return e;
         cached[dev] = (n < 1 ? 1 : n) * sm_count();
     }

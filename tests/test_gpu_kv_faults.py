@@ -166,3 +166,58 @@ def test_groups_of_very_different_magnitude(sp):
     want, tol = relative_attention(q, k, v, scale)
     assert np.all(np.abs(got - want) <= tol)
     assert sp.device_status() == 0
+
+
+def ragged(sp, rng, lens, heads, D, page, capacity):
+    """Sequences of given lengths in a cache whose table holds `capacity` tokens of each."""
+    width = -(-max(capacity, *lens) // page)
+    table, at = np.full((len(lens), width), -1, np.int32), 0
+    for b, n in enumerate(lens):
+        pages = -(-n // page)
+        table[b, :pages] = np.arange(at, at + pages)
+        at += pages
+    cache = sp.KvCacheInt4(at, page, heads, D)
+    k, v = ([randn(rng, n, heads, D) for n in lens] for _ in range(2))
+    cu = i32(0, *np.cumsum(lens))
+    sp.kv_append(cache, dev(np.concatenate(k)), dev(np.concatenate(v)), dev(table), i32(*lens), cu_q=cu)
+    return cache, dev(table), i32(*lens), k, v
+
+
+def off_by(got, want):
+    """Errors and the rounding of the exact result to fp16, in the root mean square; what is left in fp32 is a hundredth of it."""
+    return np.linalg.norm(got - want), np.linalg.norm(want.astype(np.float16).astype(np.float64) - want)
+
+
+@pytest.mark.parametrize("D,heads,group", [(128, 12, 1), (64, 7, 1), (128, 2, 8), (64, 1, 16)])
+def test_short_contexts_in_wide_tables(sp, D, heads, group):
+    """Contexts of a few tokens are as exact in a table made for long ones, and beside a long one; and give the same bits."""
+    rng = np.random.default_rng(D + heads)
+    lens = [1 + i % 9 for i in range(40)]
+    cache, table, n, k, v = ragged(sp, rng, lens, heads, D, 16, 0)
+    q = randn(rng, 41, heads * group, D)
+    narrow = sp.kv_attention(dev(q[:40]), cache, table, n)
+    want = np.concatenate([model.attention(q[b:b + 1].astype(np.float64), *held(k[b], v[b]), D ** -0.5)[0] for b in range(40)])
+    for capacity in (129, 600, 40000):
+        wide = torch.full((40, -(-capacity // 16)), -1, dtype=torch.int32, device="cuda")
+        wide[:, :table.shape[1]] = table
+        got = sp.kv_attention(dev(q[:40]), cache, wide, n)
+        err, rounding = off_by(got.cpu().numpy().astype(np.float64), want)
+        assert err <= 1.1 * rounding, capacity
+        assert torch.equal(got, narrow), capacity
+    cache, table, n, k, v = ragged(sp, rng, lens + [5000], heads, D, 16, 0)
+    want = np.concatenate([model.attention(q[b:b + 1].astype(np.float64), *held(k[b], v[b]), D ** -0.5)[0] for b in range(40)])
+    err, rounding = off_by(sp.kv_attention(dev(q), cache, table, n)[:40].cpu().numpy().astype(np.float64), want)
+    assert err <= 1.1 * rounding
+    assert sp.device_status() == 0
+
+
+def test_the_first_rows_of_a_prompt_are_as_exact_as_their_rounding(sp):
+    """A prompt of more than one unit of the context, too few heads for the kernel for many rows: rows that see a few keys."""
+    rng = np.random.default_rng(31)
+    D, heads, n = 128, 6, 200
+    cache, table, lens, k, v = ragged(sp, rng, [n], heads, D, 32, 0)
+    q = randn(rng, n, heads, D)
+    got = sp.kv_attention(dev(q), cache, table, lens).cpu().numpy().astype(np.float64)
+    want = model.attention(q.astype(np.float64), *held(k[0], v[0]), D ** -0.5)[0]
+    err, rounding = off_by(got[:16], want[:16])
+    assert err <= 1.1 * rounding
