@@ -160,6 +160,19 @@ __device__ __forceinline__ uint32_t pack_codes(const float* t)
     return x + __float_as_uint(t[2]) * (1u << S2) + __float_as_uint(t[3]) * (1u << S3) - kOff;
 }
 
+constexpr float kRound = 12582912.f;   // 1.5 2^23: a small number added to it is rounded to even in the sum's last bits
+// The code of x, as kRound + code: the quotient (x - lo) / s rounded to even.  The quotient by the reciprocal, and of the rounded
+// difference, is off by less than 2^-18; next to a border b of two codes it is asked on which side of b s the exact difference lies:
+// b s has 16 bits, d - b s is exact, and what the difference lost is the second term.
+__device__ __noinline__ float border_code(float x, float lo, float s, float inv)
+{
+    const float d = __fsub_rn(x, lo), y = __fmaf_rn(d, inv, kRound), r = __fmaf_rn(d, inv, kRound - y);
+    if (!(fabsf(r) > 0.5f - 0x1p-16f)) return fminf(y, kRound + 15.f);
+    const float b = y - kRound + copysignf(0.5f, r), z = __fsub_rn(d, x), lost = __fadd_rn(__fsub_rn(x, __fsub_rn(d, z)), __fsub_rn(-lo, z));
+    const float side = __fadd_rn(__fsub_rn(d, b * s), lost);
+    return fminf(side > 0.f ? b + 0.5f : side < 0.f ? b - 0.5f : rintf(b), 15.f) + kRound;
+}
+
 // Heads head0, head0 + 32 / (D / 8), .. of one token: `turns` of them for every D/8 lanes, which hold a head's vector.
 template <int D, Kind KIND>
 __device__ __forceinline__ void append_vectors(const KvAppendArgs& a, int tok, int b, int pos, int head, int turns, int* status)
@@ -237,9 +250,7 @@ __device__ __forceinline__ void append_vectors(const KvAppendArgs& a, int tok, i
         __half s = __float2half_rd(span * 0x1.111116p-4f);
         if (15.f * __half2float(s) > span) s = __ushort_as_half((unsigned short)(__half_as_ushort(s) - 1));
         const float sf = __half2float(s), inv = __fdividef(1.f, sf);
-        // The code is the quotient rounded to even: added to 1.5 2^23 it is the sum's last bits.  The quotient by the reciprocal is off by
-        // less than 2^-18; only next to a border of two codes is it divided out.
-        constexpr float kRound = 12582912.f;
+        // kRound + code, by the reciprocal; border_code where that might not decide
         float t[8];
         bool near = false;
 #pragma unroll
@@ -250,7 +261,7 @@ __device__ __forceinline__ void append_vectors(const KvAppendArgs& a, int tok, i
         }
         if (near)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) t[k] = fminf(__fdiv_rn(__fsub_rn(__half2float(x[k / 4][k % 4]), lo), sf), 15.f) + kRound;
+            for (int k = 0; k < 8; ++k) t[k] = border_code(__half2float(x[k / 4][k % 4]), lo, sf, inv);
         __half m = __float2half_rn(lo);
         const bool plain = finite && sf > 0.f;   // a constant group has no codes
         if (!finite) s = m = __ushort_as_half((unsigned short)0x7fff);

@@ -221,3 +221,30 @@ def test_the_first_rows_of_a_prompt_are_as_exact_as_their_rounding(sp):
     want = model.attention(q.astype(np.float64), *held(k[0], v[0]), D ** -0.5)[0]
     err, rounding = off_by(got[:16], want[:16])
     assert err <= 1.1 * rounding
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_codes_next_to_a_border(sp, D):
+    """Values whose difference from the group's minimum does not fit in 32 bits, at and next to the middle between two codes, and groups of
+    ordinary and tiny values: the codes are those of the exact quotient."""
+    rng = np.random.default_rng(D)
+    heads, n = 8, 4000
+    x = (rng.standard_normal((n, heads, D)) * np.repeat([1, 30, 1000, 8000], 2)[:, None]).clip(-60000, 60000).astype(np.float16)
+    x[:, :, 5:12] = (rng.standard_normal((n, heads, 7)) * 1e-5).astype(np.float16)
+    for i in range(1500):   # a range of 15 codes of s, a power of two, that ends k + 1/2 codes below zero
+        s, k = 2.0 ** rng.integers(-8, 10), rng.integers(0, 15)
+        x[i, :, :32] = 0
+        x[i, :, 0], x[i, :, 1] = -(k + 0.5) * s, (14.5 - k) * s
+        x[i, :, 2:32] = (rng.choice([-1, 0, 1], (heads, 30)) * 2.0 ** rng.integers(-24, -8, (heads, 30))).astype(np.float16)
+    cache = sp.KvCacheInt4(-(-n // 64), 64, heads, D)
+    table = torch.arange(-(-n // 64), dtype=torch.int32, device="cuda").view(1, -1)
+    sp.kv_append(cache, dev(x), dev(x), table, i32(n))
+    want = model.entry(x.astype(np.float64)).astype(np.float16)
+    with np.errstate(invalid="ignore"):   # what the quotient of the difference rounded to 32 bits would give: the inputs tell
+        g = x.reshape(n, heads, -1, 32).astype(np.float32)
+        s = model.quantise(x.astype(np.float64))[1].astype(np.float32)
+        rounded = np.clip(np.rint((g - g.min(-1, keepdims=True)) / s), 0, 15)
+        assert (rounded != model.quantise(x.astype(np.float64))[0]).sum() > 10000
+    for got in sp.kv_read(cache, table, i32(n), n_tokens=n):
+        assert np.array_equal(got.cpu().numpy(), want)
+    assert sp.device_status() == 0
