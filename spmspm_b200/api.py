@@ -41,9 +41,22 @@ def _on(device, stream):
         return torch.cuda.device(device)
     if not isinstance(stream, torch.cuda.Stream):
         stream = torch.cuda.ExternalStream(stream.cuda_stream, device=device)
-    if stream.device != torch.device(device):
-        raise SpmmError(f"the stream is {stream.device}'s, the tensors are {device}'s")
+    _same_device(stream, device)
     return torch.cuda.stream(stream)
+
+
+def _same_device(stream, device):
+    if stream.device != device:
+        raise SpmmError(f"the stream is {stream.device}'s, the tensors are {device}'s")
+
+
+def _raw(stream, device):
+    """The handle of a stream given by hand, for the extension's calls."""
+    if stream is None:
+        return None
+    if isinstance(stream, torch.cuda.Stream):
+        _same_device(stream, device)
+    return stream.cuda_stream
 
 
 def _hand_over(t, stream):

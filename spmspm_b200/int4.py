@@ -7,7 +7,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .api import ACT_NONE, SpmmError, _check, _hand_over, _on, _ptr, _stream_ptr
+from .api import ACT_NONE, SpmmError, _check, _hand_over, _on, _ptr, _raw, _stream_ptr
 
 
 @dataclass
@@ -94,4 +94,4 @@ def int4_workspace(W, N):
 def linear_int4(W: Int4Matrix, B, bias=None, residual=None, activation=ACT_NONE, out=None, workspace=None, stream=None):
     """spb_linear_int4: out[N,M] = residual + act(B W^T + bias), summed in fp32 and rounded to fp16 once.  B [N,K] as in
     `linear`; out may be the residual itself, not B.  workspace: int4_workspace(W, N) bytes; a new one by default."""
-    return _lib.ext().linear_int4(W.data, W.M, W.K, W.group, B, bias, residual, activation, out, workspace, None if stream is None else stream.cuda_stream)
+    return _lib.ext().linear_int4(W.data, W.M, W.K, W.group, B, bias, residual, activation, out, workspace, _raw(stream, W.data.device))

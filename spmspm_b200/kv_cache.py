@@ -13,7 +13,7 @@ A page number outside the pool or a token past the table sets bit 8 of `device_s
 import torch
 
 from . import _lib
-from .api import SpmmError
+from .api import SpmmError, _raw
 
 
 class KvCacheInt4:
@@ -50,10 +50,6 @@ class KvCacheInt4:
         return self.kv_heads * 20 * self.head_dim // 16
 
 
-def _raw(stream):
-    return None if stream is None else stream.cuda_stream
-
-
 def kv_append(cache, k, v, page_table, kv_lens, cu_q=None, q=None, cos=None, sin=None, interleaved=False, q_out=None, stream=None):
     """spb_kv_append: write the keys and values [tokens, kv_heads, head_dim] of the new tokens.
 
@@ -62,13 +58,13 @@ def kv_append(cache, k, v, page_table, kv_lens, cu_q=None, q=None, cos=None, sin
     or a new tensor).
     Tokens before the start of the context or past the angles are skipped as a whole; their rows, and those of no sequence, leave q_out as
     it was (a new tensor has no defined value there)."""
-    return _lib.ext().kv_append(cache._handle, k, v, page_table, kv_lens, cu_q, q, cos, sin, interleaved, q_out, _raw(stream))
+    return _lib.ext().kv_append(cache._handle, k, v, page_table, kv_lens, cu_q, q, cos, sin, interleaved, q_out, _raw(stream, cache.pool.device))
 
 
 def kv_read(cache, page_table, kv_lens, cu_q=None, n_tokens=None, k_out=None, v_out=None, stream=None):
     """spb_kv_read: k, v [n_tokens, kv_heads, head_dim] fp16, what the cache holds for the last tokens of every sequence (n_tokens is
     the number of packed rows, cu_q[-1] on the host; it may be left out when k_out is given)."""
-    return _lib.ext().kv_read(cache._handle, page_table, kv_lens, cu_q, n_tokens, k_out, v_out, _raw(stream))
+    return _lib.ext().kv_read(cache._handle, page_table, kv_lens, cu_q, n_tokens, k_out, v_out, _raw(stream, cache.pool.device))
 
 
 def kv_attention_workspace(cache, q_heads, batch, max_q):
@@ -80,6 +76,6 @@ def kv_attention(q, cache, page_table, kv_lens, cu_q=None, max_q=None, scale=Non
     """spb_kv_attention: out [tokens, heads, head_dim] = softmax(scale q K^T) V over the keys of the row's sequence up to its own position.
 
     max_q: an upper bound of the new tokens of one sequence (default: tokens / batch without cu_q, all of them with it); it
-    chooses the kernel only.  scale: 1 / sqrt(head_dim) by default.  out may be q itself.  workspace: kv_attention_workspace() bytes; a new one
+    chooses the kernel only.  With cu_q it should be given: many sequences with few new tokens each are else taken for a prompt.  scale: 1 / sqrt(head_dim) by default.  out may be q itself.  workspace: kv_attention_workspace() bytes; a new one
     by default.  Rows that see no key get zeros, rows that belong to no sequence are left as they were."""
-    return _lib.ext().kv_attention(q, cache._handle, page_table, kv_lens, cu_q, max_q, scale, out, workspace, _raw(stream))
+    return _lib.ext().kv_attention(q, cache._handle, page_table, kv_lens, cu_q, max_q, scale, out, workspace, _raw(stream, cache.pool.device))

@@ -112,5 +112,21 @@ def test_cache(sp, T):
 def test_a_stream_of_another_device_is_refused(sp):
     if torch.cuda.device_count() < 2:
         pytest.skip("one device")
+    s = torch.cuda.Stream(device=1)
+    A = half(1, 64, 128)
+    W, cache = sp.encode_int4(A, 64), sp.KvCacheInt4(1, 16, 2, 64)
+    table, lens, x = torch.zeros((1, 1), dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda"), half(2, 1, 2, 64)
+    for call in (lambda: sp.encode_int4(A, 64, stream=s), lambda: sp.linear_int4(W, half(3, 1, 128), stream=s),
+                 lambda: sp.kv_append(cache, x, x, table, lens, stream=s), lambda: sp.kv_attention(x, cache, table, lens, stream=s)):
+        with pytest.raises(sp.SpmmError, match="stream"):
+            call()
+
+
+def test_the_device_of_a_stream_is_looked_at(sp):
+    """The check itself, against a device that is not the stream's."""
+    s = torch.cuda.Stream()
+    assert api._raw(s, torch.device("cuda", 0)) == s.cuda_stream and api._raw(None, "cpu") is None
     with pytest.raises(sp.SpmmError, match="stream"):
-        sp.encode_int4(half(1, 64, 128), 64, stream=torch.cuda.Stream(device=1))
+        api._raw(s, torch.device("cuda", 1))
+    with pytest.raises(sp.SpmmError, match="stream"):
+        api._on(torch.device("cuda", 1), s)
