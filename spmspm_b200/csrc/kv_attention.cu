@@ -107,18 +107,15 @@ template <int ROWS>
 struct List {
     Seq mine;
     int total;       // units of the list
-    int before = 0;  // of them, those of sequences below `upto`
     bool too_long;   // more than kMostUnits, which only sequences that share rows can bring about: refused
-    __device__ __forceinline__ List(const KvView& c, int group, int tall, int upto = 0)
+    __device__ __forceinline__ List(const KvView& c, int group, int tall)
     {
         const int lane = threadIdx.x & 31;
         long long sum = 0;
         for (int b = lane; b < c.B; b += 32) {
             load_seq<ROWS>(mine, c, b, group, tall);
             sum += mine.total;
-            if (b < upto) before += mine.total;
         }
-        if (upto) before = __reduce_add_sync(0xffffffffu, before);
         total = (int)__reduce_add_sync(0xffffffffu, (unsigned)sum);
         too_long = __reduce_add_sync(0xffffffffu, (unsigned)min((sum + (1 << 20) - 1) >> 20, 1ll << 20)) >= 1u << 11;   // rounded up in each lane
     }
@@ -771,9 +768,11 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(NT)) kv_attention_s
     for (; waited < issued; ++waited) wait_full(bars + 8 * (waited % kStages), (waited / kStages) & 1);
 }
 
-// Adds the parts of the row tiles that were cut between thread blocks, in order.  blockIdx.y: sequence, blockIdx.x: key head and row
-// tile, and row if there are as many thread blocks (`spread`).  With many row tiles each has few parts: a warp takes a row.  With few, a
-// thread block takes a row and its warps share out the parts (one key head, 444 parts: 207 -> 28 us).
+// Adds the parts of the row tiles that were cut between thread blocks, in order.  blockIdx.x: thread block of the split kernel, for the tile
+// that starts in its share and goes on behind it, if there is one; and row if there are as many thread blocks (`spread`).  With many row
+// tiles each has few parts: a warp takes a row.  With few, a thread block takes a row and its warps share out the parts (one key head, 444
+// parts: 207 -> 28 us).  A grid over sequences, heads and row tiles, each of whose warps walked over all lengths, took 47 ms for 1024 single
+// tokens with offsets and no bound, where the attention itself takes 0.4.
 constexpr int kJoinWarps = 8;
 template <int D, int NT>
 __global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvAttnArgs a, int ctas, int spread)
@@ -783,82 +782,85 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvAt
     const KvView& c = a.c;
     const int group = a.q_heads / c.kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     // the lengths are none of the preceding kernel's results, and what wrote them had ended before that kernel let this one start
+    const int row0 = spread ? blockIdx.x % spread : warp, step = spread ? spread : kJoinWarps, c0 = spread ? blockIdx.x / spread : blockIdx.x;
     Seq s;
-    const List<ROWS> list(c, group, a.tall, blockIdx.y);
-    const int total = list.total, begin = list.before;
-    load_seq<ROWS>(s, c, blockIdx.y, group, a.tall);
-    grid_wait();
-    if (total == 0 || list.too_long) return;
-    const Shares shares(total, ctas);
-    const int step = spread ? spread : kJoinWarps, pairs = spread ? gridDim.x / spread : gridDim.x;
-    for (int pair = spread ? blockIdx.x / spread : blockIdx.x; pair < c.kv_heads * s.tiles; pair += pairs) {
-        const int h = pair / s.tiles, rt = pair - h * s.tiles;
-        const int p0 = begin + pair * s.units, p1 = p0 + s.units;
-        const int c0 = shares.of(p0), c1 = shares.of(p1 - 1);
-        if (c0 == c1) continue;
-        const int rows = min(ROWS, s.qlen * group - rt * ROWS);
-        // the first part is the end of its thread block's share, the later ones start theirs (slot 0)
-        auto slot = [&](int i) { return a.ws + (2 * (size_t)i + (i == c0)) * slot_floats<D, ROWS>(); };
-        for (int row = spread ? blockIdx.x % spread : warp; row < rows; row += step) {
-            // four parts at a time, all their loads under way together
-            float m = -INFINITY, acc[V] = {}, w = 0.f;
-            const int stride = spread ? kJoinWarps : 1;
-            for (int i0 = c0 + (spread ? warp : 0); i0 <= c1; i0 += 4 * stride) {
-                float pm[4], pw[4], v[4][V];
+    List<ROWS> list(c, group, a.tall);
+    const Shares shares(list.total, ctas);
+    const int lo = shares.begin(c0), hi = shares.begin(c0 + 1);
+    bool cut = false;
+    int h = 0, rt = 0, c1 = 0;
+    if (!list.too_long && lo < hi && hi < list.total) {
+        list.find(s, c, group, a.tall, hi - 1);
+        const int pair = (hi - 1 - s.begin) / s.units, p0 = s.begin + pair * s.units, p1 = p0 + s.units;
+        cut = p0 >= lo && p1 > hi;
+        h = pair / s.tiles, rt = pair - h * s.tiles;
+        c1 = shares.of(p1 - 1);
+    }
+    if (!cut && blockIdx.x) return;
+    grid_wait();   // one thread block at least: the kernel must not end before what it was launched behind
+    if (!cut) return;
+    const int rows = min(ROWS, s.qlen * group - rt * ROWS);
+    // the first part is the end of its thread block's share, the later ones start theirs (slot 0)
+    auto slot = [&](int i) { return a.ws + (2 * (size_t)i + (i == c0)) * slot_floats<D, ROWS>(); };
+    for (int row = row0; row < rows; row += step) {
+        // four parts at a time, all their loads under way together
+        float m = -INFINITY, acc[V] = {}, w = 0.f;
+        const int stride = spread ? kJoinWarps : 1;
+        for (int i0 = c0 + (spread ? warp : 0); i0 <= c1; i0 += 4 * stride) {
+            float pm[4], pw[4], v[4][V];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int i = min(i0 + j * stride, c1);
-                    const float* p = slot(i);
-                    const bool in = i0 + j * stride <= c1;
-                    pm[j] = in ? p[ROWS * D + row] : -INFINITY;
-                    pw[j] = in ? p[ROWS * D + ROWS + row] : 0.f;
-                    if constexpr (V == 4) *reinterpret_cast<float4*>(v[j]) = *reinterpret_cast<const float4*>(p + row * D + lane * V);
-                    else *reinterpret_cast<float2*>(v[j]) = *reinterpret_cast<const float2*>(p + row * D + lane * V);
+            for (int j = 0; j < 4; ++j) {
+                const int i = min(i0 + j * stride, c1);
+                const float* p = slot(i);
+                const bool in = i0 + j * stride <= c1;
+                pm[j] = in ? p[ROWS * D + row] : -INFINITY;
+                pw[j] = in ? p[ROWS * D + ROWS + row] : 0.f;
+                if constexpr (V == 4) *reinterpret_cast<float4*>(v[j]) = *reinterpret_cast<const float4*>(p + row * D + lane * V);
+                else *reinterpret_cast<float2*>(v[j]) = *reinterpret_cast<const float2*>(p + row * D + lane * V);
+            }
+            const float n = fmaxf(m, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]))), z = n == -INFINITY ? 0.f : n, r = exp2_approx(m - z);
+            m = n;
+            w *= r;
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[k] *= r;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (i0 + j * stride <= c1) {
+                    const float q = exp2_approx(pm[j] - z);
+                    w = fmaf(pw[j], q, w);
+#pragma unroll
+                    for (int k = 0; k < V; ++k) acc[k] = fmaf(v[j][k], q, acc[k]);
                 }
-                const float n = fmaxf(m, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]))), z = n == -INFINITY ? 0.f : n, r = exp2_approx(m - z);
-                m = n;
-                w *= r;
-#pragma unroll
-                for (int k = 0; k < V; ++k) acc[k] *= r;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (i0 + j * stride <= c1) {
-                        const float q = exp2_approx(pm[j] - z);
-                        w = fmaf(pw[j], q, w);
-#pragma unroll
-                        for (int k = 0; k < V; ++k) acc[k] = fmaf(v[j][k], q, acc[k]);
-                    }
-            }
-            const int r = rt * ROWS + row;
-            uint16_t* dst = a.out + ((long long)(s.first + r / group) * a.q_heads + h * group + r % group) * D;
-            if (!spread) {
-                const float inv = w == 0.f ? 0.f : 1.f / w;
-                __half2 y[V / 2];
-#pragma unroll
-                for (int k = 0; k < V / 2; ++k) y[k] = __floats2half2_rn(acc[2 * k] * inv, acc[2 * k + 1] * inv);
-                if constexpr (V == 4) *reinterpret_cast<uint2*>(dst + lane * V) = *reinterpret_cast<uint2*>(y);
-                else *reinterpret_cast<uint32_t*>(dst + lane * V) = *reinterpret_cast<uint32_t*>(y);
-                continue;
-            }
-#pragma unroll
-            for (int k = 0; k < V; ++k) part_sum[warp][lane * V + k] = acc[k];
-            if (lane == 0) part_weight[warp] = w, part_max[warp] = m;
-            __syncthreads();
-            const int ch = threadIdx.x;
-            if (ch < D) {
-                float y = 0.f, all = 0.f, n = part_max[0];
-#pragma unroll
-                for (int i = 1; i < kJoinWarps; ++i) n = fmaxf(n, part_max[i]);
-                const float z = n == -INFINITY ? 0.f : n;
-#pragma unroll
-                for (int i = 0; i < kJoinWarps; ++i) {
-                    const float q = exp2_approx(part_max[i] - z);
-                    y = fmaf(part_sum[i][ch], q, y), all = fmaf(part_weight[i], q, all);
-                }
-                dst[ch] = __half_as_ushort(__float2half_rn(all == 0.f ? 0.f : y / all));
-            }
-            __syncthreads();
         }
+        const int r = rt * ROWS + row;
+        uint16_t* dst = a.out + ((long long)(s.first + r / group) * a.q_heads + h * group + r % group) * D;
+        if (!spread) {
+            const float inv = w == 0.f ? 0.f : 1.f / w;
+            __half2 y[V / 2];
+#pragma unroll
+            for (int k = 0; k < V / 2; ++k) y[k] = __floats2half2_rn(acc[2 * k] * inv, acc[2 * k + 1] * inv);
+            if constexpr (V == 4) *reinterpret_cast<uint2*>(dst + lane * V) = *reinterpret_cast<uint2*>(y);
+            else *reinterpret_cast<uint32_t*>(dst + lane * V) = *reinterpret_cast<uint32_t*>(y);
+            continue;
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) part_sum[warp][lane * V + k] = acc[k];
+        if (lane == 0) part_weight[warp] = w, part_max[warp] = m;
+        __syncthreads();
+        const int ch = threadIdx.x;
+        if (ch < D) {
+            float y = 0.f, all = 0.f, n = part_max[0];
+#pragma unroll
+            for (int i = 1; i < kJoinWarps; ++i) n = fmaxf(n, part_max[i]);
+            const float z = n == -INFINITY ? 0.f : n;
+#pragma unroll
+            for (int i = 0; i < kJoinWarps; ++i) {
+                const float q = exp2_approx(part_max[i] - z);
+                y = fmaf(part_sum[i][ch], q, y), all = fmaf(part_weight[i], q, all);
+            }
+            dst[ch] = __half_as_ushort(__float2half_rn(all == 0.f ? 0.f : y / all));
+        }
+        __syncthreads();
     }
 }
 
@@ -931,8 +933,7 @@ cudaError_t launch(cudaStream_t s, const KvAttnArgs& a, int* status)
     if (e != cudaSuccess || whole) return e;
     const long long rows = (long long)a.max_q * group, pairs = a.c.kv_heads * (tiles > 0 ? tiles : 1);
     const long long spread = pairs * a.c.B * 4 > ctas ? 0 : rows < 1 ? 1 : rows < ROWS ? rows : ROWS;   // five parts and more
-    const long long x = pairs * (spread ? spread : 1), most_x = 0x7fffffff / ROWS * ROWS;
-    cfg.gridDim = dim3((unsigned)(x < most_x ? x : most_x / (spread ? spread : 1) * (spread ? spread : 1)), (unsigned)a.c.B);
+    cfg.gridDim = dim3((unsigned)(ctas * (spread ? spread : 1)));
     cfg.blockDim = dim3(32 * kJoinWarps);
     cfg.dynamicSmemBytes = 0;
     e = cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<D, NT>, a, ctas, (int)spread);

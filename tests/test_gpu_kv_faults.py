@@ -248,3 +248,26 @@ def test_codes_next_to_a_border(sp, D):
     for got in sp.kv_read(cache, table, i32(n), n_tokens=n):
         assert np.array_equal(got.cpu().numpy(), want)
     assert sp.device_status() == 0
+
+
+@pytest.mark.parametrize("heads,group,D", [(2, 4, 64), (3, 1, 128), (1, 20, 64)])
+@pytest.mark.parametrize("batch,most", [(300, 900), (1100, 260), (40, 6000)])
+def test_many_ragged_sequences_with_and_without_a_bound(sp, heads, group, D, batch, most):
+    """Row tiles cut between thread blocks in every way: long and short contexts, sequences without new tokens, few and many parts."""
+    rng = np.random.default_rng(batch + heads + D)
+    lens = [int(n) for n in np.exp(rng.uniform(0, np.log(most), batch))]
+    new = [min(n, int(t)) for n, t in zip(lens, rng.integers(0, 4, batch))]
+    lens[5] = new[5] = 0
+    lens[batch // 2] = most
+    cache, table, n, k, v = ragged(sp, rng, lens, heads, D, 16, 2 * most)
+    q = randn(rng, sum(new), heads * group, D)
+    cu = i32(0, *np.cumsum(new))
+    first = np.cumsum([0] + new)
+    for max_q in (3, None):
+        got = sp.kv_attention(dev(q), cache, table, n, cu_q=cu, max_q=max_q).cpu().numpy().astype(np.float64)
+        for b in [*rng.integers(0, batch, 25), batch // 2, batch - 1, 0]:
+            rows = slice(first[b], first[b + 1])
+            if new[b]:
+                want, tol = model.attention(q[rows].astype(np.float64), *held(k[b], v[b]), D ** -0.5)
+                assert np.all(np.abs(got[rows] - want) <= tol), (b, max_q)
+    assert sp.device_status() == 0
