@@ -371,7 +371,8 @@ int spb_linear_int4(void* stream, const void* packed, int M, int K, int group, c
                      many rows (a sequence with 64 and more of them a key head), keys and values are taken as spb_kv_read returns
                      them, rounded to fp16; elsewhere unrounded.  A row of q that is not finite has no defined result.  out may be q itself.
  *                     workspace: spb_kv_attention_workspace_bytes bytes, 16-byte aligned, need not be cleared; not shared by
- *                     calls that may run at the same time.
+ *                     calls that may run at the same time.  Rows times contexts of 2^31 and more pieces (128 tokens and 8 or 16 rows
+ *                     of a key head) set bit 8 and leave out as it was.
  * k, v and q are fp16 with contiguous channels; token and head strides in elements, multiples of 4; pointers 8-byte aligned
  * (out, q_out, the angle tables and the workspace 16).  The same bits come out for the same call on the same device.
  */

@@ -229,7 +229,7 @@ int spb_kv_attention(void* stream, const void* pool, int num_pages, int page_siz
     a.ws = static_cast<float*>(workspace);
     a.ws_floats = workspace_bytes / 4;
     e = kv_attention_launch((cudaStream_t)stream, head_dim, a, status);
-    if (e != cudaSuccess && e != cudaErrorInvalidValue) set_error("%s: %s", who, cudaGetErrorString(e));
+    if (e != cudaSuccess) set_error("%s: %s", who, cudaGetErrorString(e));
     return (int)e;
 }
 

@@ -80,8 +80,6 @@ __device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<
 __device__ __forceinline__ float power(int exponent) { return __int_as_float((127 + exponent) << 23); }
 __device__ __forceinline__ int exponent_of(__half2 power_of_two) { return (int)(h2_bits(power_of_two) >> 26) - 15; }
 
-constexpr long long kMostUnits = (1ll << 31) - (1ll << 25);   // of a list
-
 // Sequence b of the work list.
 struct Seq {
     int b = 0;
@@ -100,14 +98,14 @@ __device__ __forceinline__ void load_seq(Seq& s, const KvView& c, int b, int gro
     // tokens past the table's width have no page: they are not walked over
     const int held = (int)min((long long)s.len, (long long)c.table_stride * c.page_size);
     s.units = max((held - 1) / kUnit + 1, 1);
-    s.total = c.kv_heads * s.tiles * s.units;
+    s.total = (int)min((long long)c.kv_heads * s.tiles * s.units, 0x7fffffffll);   // as much makes the list too long
 }
 // The list as a warp sees it: its length, and of up to 32 sequences lane b's, so that finding one needs no second look at memory.
 template <int ROWS>
 struct List {
     Seq mine;
     int total;       // units of the list
-    bool too_long;   // more than kMostUnits, which only sequences that share rows can bring about: refused
+    bool too_long;   // 2^31 units or next to it: refused, here, where the lengths are known (a table may be far wider than they need)
     __device__ __forceinline__ List(const KvView& c, int group, int tall)
     {
         const int lane = threadIdx.x & 31;
@@ -912,10 +910,6 @@ cudaError_t launch(cudaStream_t s, const KvAttnArgs& a, int* status)
     // never more thread blocks than units there can be: every table entry used, every packed row in a tile of its own at worst
     const long long tiles = ((long long)a.max_q * group + ROWS - 1) / ROWS;
     const long long most = (long long)a.c.B * a.c.kv_heads * (tiles > 0 ? tiles : 1) * units;
-    if (((long long)a.c.n_tokens * group / ROWS + a.c.B) * a.c.kv_heads * units > kMostUnits) {
-        set_error("kv_attention: too much work for one call (rows times context)");
-        return cudaErrorInvalidValue;
-    }
     if (whole ? most / units < ctas : most < ctas) ctas = (int)(whole ? most / units : most);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

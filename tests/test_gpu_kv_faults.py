@@ -271,3 +271,28 @@ def test_many_ragged_sequences_with_and_without_a_bound(sp, heads, group, D, bat
                 want, tol = model.attention(q[rows].astype(np.float64), *held(k[b], v[b]), D ** -0.5)
                 assert np.all(np.abs(got[rows] - want) <= tol), (b, max_q)
     assert sp.device_status() == 0
+
+
+def test_a_table_far_wider_than_the_contexts(sp):
+    """Room for 2^29 tokens and a few thousand of them: what counts is the contexts."""
+    rng = np.random.default_rng(41)
+    D, heads, group, page = 64, 2, 8, 65536
+    k, v = randn(rng, 900, heads, D), randn(rng, 900, heads, D)
+    cache = sp.KvCacheInt4(1, page, heads, D)
+    narrow = i32(0).view(1, 1)
+    wide = torch.full((1, 8192), -1, dtype=torch.int32, device="cuda")
+    wide[0, 0] = 0
+    sp.kv_append(cache, dev(k), dev(v), wide, i32(900))
+    q = randn(rng, 700, heads * group, D)
+    want, tol = model.attention(q.astype(np.float64), *held(k, v), D ** -0.5)
+    for table in (narrow, wide):
+        got = sp.kv_attention(dev(q), cache, table, i32(900), cu_q=i32(0, 700), max_q=1).cpu().numpy().astype(np.float64)
+        assert np.all(np.abs(got - want) <= tol)
+    # also with the kernel for many rows beside the other
+    cache = sp.KvCacheInt4(1, page, 24, D)
+    k, v, q = (randn(rng, 900, 24, D) for _ in range(3))
+    sp.kv_append(cache, dev(k), dev(v), wide, i32(900))
+    table = wide.repeat(2, 1)
+    args = dict(cu_q=i32(0, 850, 900), max_q=850)
+    assert torch.equal(sp.kv_attention(dev(q), cache, table, i32(900, 50), **args), sp.kv_attention(dev(q), cache, narrow.repeat(2, 1), i32(900, 50), **args))
+    assert sp.device_status() == 0
