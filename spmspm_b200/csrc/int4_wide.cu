@@ -2,10 +2,12 @@
 //
 //   out[n][m] = residual + act(bias + sum_k w[m][k] x[n][k]),   w = s (c - z) rounded to fp16 (the value int4_decode returns)
 //
+// The rounding of w costs accuracy: 2.8e-4 from the exact result where fp32 sums of unrounded weights are 2.1e-4 (int4_stream.cu).
 // Rows of W are the 128-row side of the matrix instruction, rows of x its 32..256-column side.  Codes become fp16 on the way
 // into tensor memory, where the instruction takes its left operand from; x comes as 128-byte-swizzled tiles by tensor copies.
 //
-// Bound: 9216 x 36864, 509 rows: 264 us, 1310 TFLOP/s, 79 % of the library's dense rate, tensor pipe 69 % busy; every 128 rows of W read
+// Bound: 9216 x 36864, 509 rows: 262 us in a burst at 1965 MHz, 1320 TFLOP/s, 79 % of the library's dense rate in a burst; 301 to 315 us kept up
+// under the power cap at 1430 MHz, 1100 to 1150 TFLOP/s, 79 to 82 % of the library's kept up.  Tensor pipe 69 % busy; every 128 rows of W read
 // all of x from L2, 2.8 GB or 10 TB/s, which is near what L2 gives.  With 32 to 64 rows the product is bound by the 8 instructions of a
 // unit, which cost the same 80 cycles for 32 columns as for 128 (16384 x 16384, 40 rows: 52 us, 22 at copy rate).  Scaling a group's sums in
 // fp32 instead of the weights, so that these need no rounding, was built and measured: 405 us and 64 us for these two with groups of

@@ -14,9 +14,9 @@
 //
 // Bound by latency and by the instructions of exact rounding, not by its bytes (4 D in and 1.25 D out per token and head): a warp takes up
 // to eight turns of vectors of one kind of one token, whose place and angles it then finds once, and loads a turn ahead.  Prompts of
-// 7300 tokens, 8 key heads and 32 query heads, half of each turned, with kv_read of them: 63 us (82 when a warp went through the
-// tokens of one head; 7 more without the loads ahead), 31 at copy rate.  64 single tokens, 8 and 64 heads: 6.8 us, launches and
-// the dependent loads that find a token's place.
+// 7300 tokens, 8 key heads and 32 query heads, half of each turned, with kv_read of them: 64.5 us (82 when a warp went through the
+// tokens of one head; 7 more without the loads ahead), 31 at copy rate; issue slots 69 % busy in the append, 57 % in the read, the rest waits
+// for loads.  64 single tokens, 8 and 64 heads: 7.3 us, launches and the dependent loads that find a token's place.
 #include "kv_int4.cuh"
 #include "sm100.cuh"
 
@@ -298,7 +298,7 @@ __device__ __forceinline__ void append_vectors(const KvAppendArgs& a, int tok, i
 struct AppendPlan {
     int kv_turns, kv_warps, q_turns, q_warps;
 };
-// Registers for 8 thread blocks an SM: 7 took 68 us, 9 took 66 where these take 63.
+// Registers for 8 thread blocks an SM: 7 took 68 us, 9 took 66 where these took 63.
 template <int D>
 __global__ void __launch_bounds__(32 * kWarps, 8) kv_append_kernel(KvAppendArgs a, AppendPlan plan, int* status)
 {
