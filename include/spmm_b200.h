@@ -374,7 +374,8 @@ int spb_linear_int4(void* stream, const void* packed, int M, int K, int group, c
  *                     calls that may run at the same time.  Rows times contexts of 2^31 and more pieces (128 tokens and 8 or 16 rows
  *                     of a key head) set bit 8 and leave out as it was.
  * k, v and q are fp16 with contiguous channels; token and head strides in elements, multiples of 4; pointers 8-byte aligned
- * (out, q_out, the angle tables and the workspace 16).  The same bits come out for the same call on the same device.
+ * (out, q_out, the angle tables and the workspace 16).  The same bits come out for the same call on the same device; the width
+ * of the page table is part of the call.
  */
 size_t spb_kv_cache_bytes(int num_pages, int page_size, int kv_heads, int head_dim);
 int spb_kv_append(void* stream, void* pool, int num_pages, int page_size, int kv_heads, int head_dim, const int* page_table,

@@ -28,7 +28,7 @@
 // the end of a row tile.
 //
 // Bound: the cache's bytes when there are enough of them, else the launches, a unit's latency and the join.  One row, 32 query heads on 8,
-// 262139 tokens: 77 us, 4.35 TB/s; 32 sequences of up to 8191 tokens, 64 heads on 8: 65 us, 3.9 TB/s (issue slots 56-57 % busy, tensor pipe
+// 262139 tokens: 79 us, 4.25 TB/s; 32 sequences of up to 8191 tokens, 64 heads on 8: 65 us, 3.9 TB/s (issue slots 56-57 % busy, tensor pipe
 // 22-25 %).  One sequence of 131 tokens: 9.3 us, a third of it launch at most (a linear layer with its launch takes 3.6); the rest is one
 // dependent step after the other: lengths, list, table, the first copy, and two units of 128 tokens in a row on 40 thread blocks.
 #include "kv_int4.cuh"
