@@ -42,6 +42,11 @@ def _on(device, stream):
     if not isinstance(stream, torch.cuda.Stream):
         stream = torch.cuda.ExternalStream(stream.cuda_stream, device=device)
     _same_device(stream, device)
+    if torch.cuda.is_current_stream_capturing():
+        with torch.cuda.stream(stream):
+            captured = torch.cuda.is_current_stream_capturing()
+        if not captured:   # a call beside a capture: nothing can be allocated outside the graph's pool, nor a stream prepared
+            return torch.cuda.device(device)
     return torch.cuda.stream(stream)
 
 

@@ -7,6 +7,7 @@
 #include <torch/csrc/utils/pybind.h>
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
@@ -92,7 +93,14 @@ struct Place {
           caller(c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev)),
           stream(s ? c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(*s), (c10::DeviceIndex)dev) : caller)
     {
-        if (s) given.emplace(stream.unwrap());
+        // beside a capture of the caller's stream nothing can be allocated outside the graph's pool
+        if (s && (!captured(caller) || captured(stream))) given.emplace(stream.unwrap());
+    }
+    static bool captured(c10::cuda::CUDAStream s)
+    {
+        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+        C10_CUDA_CHECK(cudaStreamIsCapturing(s.stream(), &status));
+        return status != cudaStreamCaptureStatusNone;
     }
     void* ptr() const { return stream.stream(); }
     Tensor output(at::IntArrayRef shape, c10::Device dev) const
