@@ -296,3 +296,22 @@ def test_a_table_far_wider_than_the_contexts(sp):
     args = dict(cu_q=i32(0, 850, 900), max_q=850)
     assert torch.equal(sp.kv_attention(dev(q), cache, table, i32(900, 50), **args), sp.kv_attention(dev(q), cache, narrow.repeat(2, 1), i32(900, 50), **args))
     assert sp.device_status() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 3])
+def test_nan_in_the_middle_of_a_context_stays_in_its_group(sp, rows):
+    """A value that is not finite in one group of one token that every row sees, and scales that grow behind it."""
+    rng = np.random.default_rng(51)
+    D, heads, L = 128, 2, 3000
+    k, v = randn(rng, L, heads, D), randn(rng, L, heads, D)
+    v[2000:] *= np.float16(40)
+    bad = v.copy()
+    bad[700, 1, 70] = np.inf
+    q = randn(rng, rows, heads * 4, D)
+    cache, table, lens = cached(sp, k, bad)
+    got = sp.kv_attention(dev(q), cache, table, lens).cpu().numpy().astype(np.float64)
+    want, tol = model.attention(q.astype(np.float64), *held(k, v), D ** -0.5)
+    lost = np.zeros(got.shape, bool)
+    lost[:, 4:, 64:96] = True
+    assert np.isnan(got[lost]).all() and np.all(np.abs(got - want)[~lost] <= tol[~lost])
+    assert sp.device_status() == 0
